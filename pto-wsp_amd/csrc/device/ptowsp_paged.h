@@ -1,0 +1,1139 @@
+// Operators over a paged KV cache held in 8 bits, hand-written for gfx950:
+// block tables and slot maps (plan), quantising writes (store) and causal
+// grouped-query attention (attend).  The host library compiles one entry per
+// combination of types, head size, page size and group.
+#pragma once
+
+#include "ptowsp_paged_args.h"
+
+namespace ptowsp {
+
+typedef long long pg_i64;
+typedef unsigned int pg_u32;
+typedef unsigned long long pg_u64;
+typedef unsigned short pg_u16;
+typedef unsigned char pg_u8;
+typedef pg_u32 pg_u32x2 __attribute__((ext_vector_type(2)));
+typedef pg_u32 pg_u32x4 __attribute__((ext_vector_type(4)));
+typedef float pg_f32x2 __attribute__((ext_vector_type(2)));
+typedef float pg_f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 pg_bf2 __attribute__((ext_vector_type(2)));
+typedef __bf16 pg_bf8 __attribute__((ext_vector_type(8)));
+typedef _Float16 pg_h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 pg_h8 __attribute__((ext_vector_type(8)));
+
+// Types of activations and of cache codes.
+constexpr int kBF16 = 0, kF16 = 1, kF32 = 2;
+constexpr int kE4M3 = 0, kI8 = 1;
+
+constexpr int elem_size(int t) { return t == kF32 ? 4 : 2; }
+
+template <int T>
+__device__ inline float elem_f32(const char* p) {
+    if constexpr (T == kF32) return *reinterpret_cast<const float*>(p);
+    else if constexpr (T == kF16) return static_cast<float>(*reinterpret_cast<const _Float16*>(p));
+    else return __uint_as_float(static_cast<pg_u32>(*reinterpret_cast<const pg_u16*>(p)) << 16);
+}
+template <int T>
+__device__ inline void store_elem(char* p, float x) {
+    if constexpr (T == kF32) *reinterpret_cast<float*>(p) = x;
+    else if constexpr (T == kF16) *reinterpret_cast<_Float16*>(p) = static_cast<_Float16>(x);
+    else *reinterpret_cast<__bf16*>(p) = static_cast<__bf16>(x);
+}
+
+// Sum over the workgroup's threads of `v`, and the sum of those before this
+// one.  One barrier pair; `lds` holds a value per wave.
+template <int THREADS>
+__device__ inline pg_i64 block_scan(pg_i64 v, pg_i64& total, pg_i64* lds) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    pg_i64 x = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const pg_i64 y = __shfl_up(x, d, 64);
+        if (lane >= d) x += y;
+    }
+    if (lane == 63) lds[wave] = x;
+    __syncthreads();
+    pg_i64 before = 0, sum = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) {
+        const pg_i64 y = lds[w];
+        if (w < wave) before += y;
+        sum += y;
+    }
+    __syncthreads();
+    total = sum;
+    return before + x - v;
+}
+
+// ---------------------------------------------------------------------------
+// paged_plan
+//
+// Per request: old and new page counts ceil(length / page), ceil((length +
+// count) / page); exclusive sums over the requests of the counts (its first
+// row) and of the pages that it lacks (its first entry of the free list).  Per
+// row: its request by binary search of the first rows, its page from the table
+// or the free list, its slot.  The row at a page's first offset also writes
+// that page's table entry: a page that is new to a request holds nothing older
+// than its new tokens.  Bound by latency: a few KB move.
+// ---------------------------------------------------------------------------
+
+struct PlanRequest {
+    int start, length, first;  // first row, cached tokens, first entry of the free list
+};
+
+__device__ inline int page_count(pg_u32 tokens, pg_u32 page) { return static_cast<int>((tokens + (page - 1)) / page); }
+
+// The sums, for all requests, in one workgroup; put(b, request, count)
+// receives them.  Returns whether the plan fits; nothing has been put where it
+// does not.  A request's length and count are read by one thread only, before
+// it writes, so that new_lengths may be lengths.
+template <int THREADS, class Put>
+__device__ inline bool plan_requests(const PlanArgs& A, int& total_rows, Put put) {
+    __shared__ pg_i64 lds[THREADS / 64];
+    const pg_i64 per = (A.batch + THREADS - 1) / THREADS, b0 = threadIdx.x * per;
+    const pg_i64 b1 = b0 + per < A.batch ? b0 + per : A.batch;
+    const int used = *A.used, page = A.page;
+    bool bad = used < 0;
+    pg_i64 rows = 0, pages = 0;
+    int length = 0, count = 0;
+    for (pg_i64 b = b0; b < b1; ++b) {
+        length = A.lengths[b * A.s_lengths];
+        count = A.counts[b * A.s_counts];
+        const pg_i64 all = static_cast<pg_i64>(length) + count;
+        const bool wrong = length < 0 || count < 0 || all > 0x7FFFFFFF || all > A.width * page;
+        bad |= wrong;
+        if (wrong) continue;
+        rows += count;
+        pages += page_count(length + count, page) - page_count(length, page);
+    }
+    pg_i64 all_rows, all_pages;
+    const pg_i64 row0 = block_scan<THREADS>(rows, all_rows, lds);
+    const pg_i64 page0 = block_scan<THREADS>(pages, all_pages, lds);
+    bad |= all_rows > A.rows || used + all_pages > A.nfree;
+    if (__syncthreads_or(bad)) {
+        if (threadIdx.x == 0) *A.err = 4;
+        return false;
+    }
+    total_rows = static_cast<int>(all_rows);
+    int row = static_cast<int>(row0), first = used + static_cast<int>(page0);
+    for (pg_i64 b = b0; b < b1; ++b) {
+        if (per > 1) {
+            length = A.lengths[b * A.s_lengths];
+            count = A.counts[b * A.s_counts];
+        }
+        put(b, PlanRequest{row, length, first}, count);
+        A.starts[b * A.s_starts] = row;
+        A.new_lengths[b * A.s_new_lengths] = length + count;
+        row += count;
+        first += page_count(length + count, page) - page_count(length, page);
+    }
+    if (threadIdx.x == 0) {
+        A.starts[A.batch * A.s_starts] = total_rows;
+        *A.new_used = used + static_cast<int>(all_pages);
+    }
+    return true;
+}
+
+// Row r of request b.
+__device__ inline void plan_row(const PlanArgs& A, int r, int b, PlanRequest q) {
+    const int pos = q.length + (r - q.start), page = A.page;
+    const int p = static_cast<int>(static_cast<pg_u32>(pos) / static_cast<pg_u32>(page)), off = pos - p * page;
+    const int old = page_count(q.length, page);
+    int id;
+    if (p >= old) {
+        id = A.free_pages[static_cast<pg_i64>(q.first + (p - old)) * A.s_free];
+        if (off == 0) A.table[b * A.s_table + p * A.s_table_col] = id;
+    } else {
+        id = A.table[b * A.s_table + p * A.s_table_col];
+    }
+    const pg_i64 slot = static_cast<pg_i64>(id) * page + off;
+    const bool fits = id >= 0 && slot <= 0x7FFFFFFF;
+    if (!fits) *A.err = 5;
+    A.slots[r * A.s_slots] = fits ? static_cast<int>(slot) : -1;
+}
+
+// One workgroup for everything: the requests' sums stay in LDS.
+template <int THREADS, int BATCH>
+__device__ inline void plan_one(const PlanArgs& A) {
+    __shared__ int start[BATCH], length[BATCH], first[BATCH];
+    int rows;
+    const bool fits = plan_requests<THREADS>(A, rows, [&](pg_i64 b, PlanRequest q, int) {
+        start[b] = q.start;
+        length[b] = q.length;
+        first[b] = q.first;
+    });
+    if (!fits) return;
+    __syncthreads();
+    const int n = static_cast<int>(A.batch);
+    for (pg_i64 r = threadIdx.x; r < A.rows; r += THREADS) {
+        if (r >= rows) {
+            A.slots[r * A.s_slots] = -1;
+            continue;
+        }
+        int lo = 0, hi = n;  // start[lo] <= r < start[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (start[mid] <= r) lo = mid;
+            else hi = mid;
+        }
+        plan_row(A, static_cast<int>(r), lo, PlanRequest{start[lo], length[lo], first[lo]});
+    }
+}
+
+// Two launches: the sums by one workgroup into the scratch, then the rows by
+// as many workgroups as they need.
+template <int THREADS>
+__device__ inline void plan_sums(const PlanArgs& A) {
+    int* const start = A.scratch + 2;
+    int* const length = start + A.batch;
+    int* const first = length + A.batch;
+    int rows;
+    const bool fits = plan_requests<THREADS>(A, rows, [&](pg_i64 b, PlanRequest q, int) {
+        start[b] = q.start;
+        length[b] = q.length;
+        first[b] = q.first;
+    });
+    if (threadIdx.x == 0) {
+        A.scratch[0] = fits;
+        A.scratch[1] = fits ? rows : 0;
+    }
+}
+
+template <int THREADS>
+__device__ inline void plan_rows(const PlanArgs& A) {
+    if (!A.scratch[0]) return;
+    const int rows = A.scratch[1];
+    const int* const start = A.scratch + 2;
+    const int* const length = start + A.batch;
+    const int* const first = length + A.batch;
+    const pg_i64 r0 = static_cast<pg_i64>(blockIdx.x) * kPlanRows;
+    const pg_i64 end = r0 + kPlanRows < A.rows ? r0 + kPlanRows : A.rows;
+    const int r1 = static_cast<int>(end < rows ? end : rows);  // rows with a token
+    if (r0 < r1) {
+        // The requests of the first and the last row: the whole workgroup probes.
+        int lo[2] = {0, 0}, hi[2] = {static_cast<int>(A.batch), static_cast<int>(A.batch)};
+        const int row[2] = {static_cast<int>(r0), r1 - 1};
+        while (hi[0] - lo[0] > 1 || hi[1] - lo[1] > 1) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int step = (hi[k] - lo[k] + THREADS - 1) / THREADS;
+                const int at = lo[k] + static_cast<int>(threadIdx.x) * step;
+                const int below = __syncthreads_count(at < hi[k] && start[at] <= row[k]);
+                lo[k] += (below - 1) * step;
+                hi[k] = lo[k] + step < hi[k] ? lo[k] + step : hi[k];
+            }
+        }
+        for (int r = static_cast<int>(r0) + static_cast<int>(threadIdx.x); r < r1; r += THREADS) {
+            int l = lo[0], h = hi[1];
+            while (h - l > 1) {
+                const int mid = (l + h) >> 1;
+                if (start[mid] <= r) l = mid;
+                else h = mid;
+            }
+            plan_row(A, r, l, PlanRequest{start[l], length[l], first[l]});
+        }
+    }
+    for (pg_i64 r = (r0 > rows ? r0 : rows) + threadIdx.x; r < end; r += THREADS) A.slots[r * A.s_slots] = -1;
+}
+
+// ---------------------------------------------------------------------------
+// Codes
+// ---------------------------------------------------------------------------
+
+template <int CT>
+constexpr float code_top() {
+    return CT == kI8 ? 127.0f : 448.0f;
+}
+
+// Two codes (bytes 0, 1 or 2, 3 of w) as two bf16 or f16 values: exact, both
+// types hold the 4 significant bits of e4m3 and the 8 of a signed byte.
+template <int CT, bool H, bool HI>
+__device__ inline pg_u32 codes2(pg_u32 w) {
+    if constexpr (CT == kE4M3) {
+        if constexpr (H) return __builtin_bit_cast(pg_u32, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HI));
+        else return __builtin_bit_cast(pg_u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
+    } else {
+        const float a = static_cast<float>(static_cast<signed char>(w >> (HI ? 16 : 0)));
+        const float b = static_cast<float>(static_cast<signed char>(w >> (HI ? 24 : 8)));
+        if constexpr (H) return __builtin_bit_cast(pg_u32, __builtin_amdgcn_cvt_pkrtz(a, b));
+        else return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+    }
+}
+
+// Four numbers, already multiplied by 1 / scale, as codes.
+template <int CT>
+__device__ inline pg_u32 encode4(const float* y) {
+    constexpr float top = code_top<CT>();
+    float z[4];
+    bool nan[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        nan[i] = y[i] != y[i];
+        z[i] = fminf(fmaxf(y[i], -top), top);
+    }
+    pg_u32 w;
+    if constexpr (CT == kI8) {
+        w = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w |= (static_cast<pg_u32>(nan[i] ? 0 : static_cast<int>(rintf(z[i]))) & 0xFFu) << (8 * i);
+    } else {
+        int c = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
+        c = __builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], c, true);
+        w = static_cast<pg_u32>(c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (nan[i]) w = (w & ~(0xFFu << (8 * i))) | 0x7Fu << (8 * i);
+    }
+    return w;
+}
+
+template <int CT>
+__device__ inline float decode1(pg_u32 w, int i) {
+    const pg_u32 byte = (w >> (8 * i)) & 0xFFu;
+    if constexpr (CT == kI8) return static_cast<float>(static_cast<signed char>(byte));
+    else return __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(byte), 0);
+}
+
+// ---------------------------------------------------------------------------
+// paged_store
+//
+// One wave per run of neighbouring rows of a page, head, and keys or values:
+// the largest finite |x| of the run, the scale (kept tokens: at least the old
+// one), the kept codes anew where it grew, the run's codes.  Every quotient is
+// the product with 1 / scale, rounded as float32 values are, so that the codes
+// follow from the inputs bit by bit.  Bound by HBM: x is read once (its second
+// reading hits the caches: a run is at most a page), codes are written once.
+// ---------------------------------------------------------------------------
+
+// Eight elements of x at p.
+template <int T, bool VEC>
+__device__ inline void load8(const char* p, float* x) {
+    if constexpr (VEC && T == kF32) {
+        const pg_f32x4 a = *reinterpret_cast<const pg_f32x4*>(p), b = *reinterpret_cast<const pg_f32x4*>(p + 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = a[i];
+            x[4 + i] = b[i];
+        }
+    } else if constexpr (VEC) {
+        const pg_u32x4 a = *reinterpret_cast<const pg_u32x4*>(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const pg_u32 w = a[i];  // the bit cast takes a value: of a vector's element it reads element 0
+            if constexpr (T == kF16) {
+                const pg_h2 h = __builtin_bit_cast(pg_h2, w);
+                x[2 * i] = static_cast<float>(h[0]);
+                x[2 * i + 1] = static_cast<float>(h[1]);
+            } else {
+                x[2 * i] = __uint_as_float(w << 16);
+                x[2 * i + 1] = __uint_as_float(w & 0xFFFF0000u);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = elem_f32<T>(p + i * elem_size(T));
+    }
+}
+
+template <int D, int PAGE, int T, int CT, bool VEC, int CHUNK>
+__device__ inline void store_rows(const StoreArgs& A) {
+    const int heads = A.heads;
+    constexpr int PARTS = D / 8;  // pieces of eight elements in a row
+    const int lane = threadIdx.x & 63;
+    const pg_i64 item = static_cast<pg_i64>(blockIdx.x) * (blockDim.x >> 6) + (threadIdx.x >> 6);
+    const pg_i64 chunk = item / (2 * heads);
+    const int which = static_cast<int>(item - chunk * (2 * heads)), h = which >> 1, kv = which & 1;
+    const pg_i64 row0 = chunk * CHUNK;
+    if (row0 >= A.rows) return;
+    const pg_i64 slots_end = A.pages * PAGE;
+    auto page_of = [&](pg_i64 r) -> int {  // -1: not stored
+        if (r < 0 || r >= A.rows) return -1;
+        const int s = A.slots[r * A.s_slots];
+        return s < 0 || s >= slots_end ? -1 : s / PAGE;
+    };
+    // The runs that begin among the chunk's rows.
+    pg_u64 leaders;
+    {
+        const pg_i64 r = row0 + lane;
+        const int p = lane < CHUNK ? page_of(r) : -1;
+        if (lane < CHUNK && r < A.rows && A.slots[r * A.s_slots] >= slots_end) *A.err = 6;
+        leaders = __ballot(p >= 0 && page_of(r - 1) != p);
+    }
+    const char* const x = A.x[kv] + h * A.s_x[kv][1] * elem_size(T);
+    while (leaders) {
+        const pg_i64 r0 = row0 + __builtin_ctzll(leaders);
+        leaders &= leaders - 1;
+        const int page = page_of(r0);
+        // Rows of the run, its first offset, and whether its offsets ascend by one.
+        int n = 0, low = PAGE;
+        bool dense = true;
+        for (;;) {
+            const bool in = page_of(r0 + n + lane) == page;
+            const pg_u64 out = ~__ballot(in);
+            const int more = out ? __builtin_ctzll(out) : 64;
+            const int off = lane < more ? A.slots[(r0 + n + lane) * A.s_slots] - page * PAGE : PAGE;
+            const int first = n == 0 ? __shfl(off, 0, 64) : low;
+            dense &= __ballot(lane < more && off != first + n + lane) == 0;
+            int l = off;
+#pragma unroll
+            for (int d = 32; d >= 1; d >>= 1) {
+                const int y = __shfl_xor(l, d, 64);
+                l = y < l ? y : l;
+            }
+            low = l < low ? l : low;
+            n += more;
+            if (more < 64) break;
+        }
+        const char* const xr = x + r0 * A.s_x[kv][0] * elem_size(T);
+        float most = 0.0f;
+        for (int e = lane; e < n * PARTS; e += 64) {
+            const int t = e / PARTS;
+            float y[8];
+            load8<T, VEC>(xr + (t * A.s_x[kv][0] + (e - t * PARTS) * 8) * elem_size(T), y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float a = fabsf(y[i]);
+                if (a < __builtin_inff()) most = fmaxf(most, a);
+            }
+        }
+#pragma unroll
+        for (int d = 32; d >= 1; d >>= 1) most = fmaxf(most, __shfl_xor(most, d, 64));
+        float* const sp = A.scale[kv] + page * A.s_scale[kv][0] + h * A.s_scale[kv][1];
+        const float old = low > 0 ? *sp : 0.0f;
+        const float scale = fmaxf(fmaxf(most / code_top<CT>(), 0x1p-126f), old);
+        const float inverse = 1.0f / scale;
+        char* const cp = A.cache[kv] + page * A.s_cache[kv][0] + h * A.s_cache[kv][1];
+        if (low > 0 && scale > old) {
+            for (int e = lane; e < low * PARTS; e += 64) {
+                const int t = e / PARTS;
+                pg_u32x2* const c = reinterpret_cast<pg_u32x2*>(cp + t * A.s_cache[kv][2] + (e - t * PARTS) * 8);
+                pg_u32x2 w = *c;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    float y[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) y[i] = (decode1<CT>(w[k], i) * old) * inverse;
+                    w[k] = encode4<CT>(y);
+                }
+                *c = w;
+            }
+        }
+        auto put = [&](int t, int part) {
+            float y[8];
+            load8<T, VEC>(xr + (t * A.s_x[kv][0] + part * 8) * elem_size(T), y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = y[i] * inverse;
+            const int off = A.slots[(r0 + t) * A.s_slots] - page * PAGE;
+            *reinterpret_cast<pg_u32x2*>(cp + off * A.s_cache[kv][2] + part * 8) = pg_u32x2{encode4<CT>(y), encode4<CT>(y + 4)};
+        };
+        if (dense) {
+            for (int e = lane; e < n * PARTS; e += 64) put(e / PARTS, e % PARTS);
+        } else {
+            // Rows in order, each piece by the same lane: of several rows at one
+            // offset the last one stays.
+            for (int t = 0; t < n; ++t)
+                for (int part = lane; part < PARTS; part += 64) put(t, part);
+        }
+        if (lane == 0) *sp = scale;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// paged_attention
+//
+// A unit is C tokens of one request times the G query heads of one key head:
+// up to RB = 16 * NT query rows that read the same keys.  A workgroup's four
+// waves take 32 of every 128 tokens each, with a softmax of their own, and are
+// joined through LDS.  All tiles of all units make one line that the
+// workgroups cut into equal pieces, so a long request is shared by many of
+// them; the pieces of a unit that is cut meet in attend_join.
+//
+// Per 32 tokens a wave forms S^T = K q^T and O^T += V^T P^T with
+// v_mfma_f32_16x16x32: both operands' lanes hold what their loads deliver.
+//   K: lane (m, g) of 16 x 4 reads 16 bytes of token m, dims 64j + 16g, which
+//      are two MFMA operands; q is laid out alike.
+//   S: lane (n, g) holds, of query row n, tokens 4g .. 4g + 3 of each 16: the
+//      eight of a lane are the P operand of one MFMA, in that order of tokens.
+//   V: lane (c, g) reads those eight tokens' dims 64j + 4c .. + 3, one dword
+//      each; byte q of them is the operand of dims 64j + 4c + q.
+//   O: lane (n, g) ends up with dims 64j + 16g .. + 15 of query row n.
+// No value crosses lanes but the maxima, and those only when one grows: p is
+// exp2(s - m) for an m that may lag the true maximum by a factor of 2^8.
+// Codes enter the MFMAs as they are, exactly; a page's scales multiply s and p
+// in float32.  q enters exactly too (an f32 as three bf16), p as two bf16
+// parts (2^-17 of it; three for f32 outputs), sums are float32.
+// ---------------------------------------------------------------------------
+
+__device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ inline pg_i64 uniform64(pg_i64 x) {
+    const pg_u32 lo = __builtin_amdgcn_readfirstlane(static_cast<int>(x));
+    const pg_u32 hi = __builtin_amdgcn_readfirstlane(static_cast<int>(x >> 32));
+    return static_cast<pg_i64>(static_cast<pg_u64>(hi) << 32 | lo);
+}
+// Loads that all lanes share, of data that no launch in flight writes.
+template <class T>
+__device__ inline T uniform_load(const T* p) {
+    typedef const T __attribute__((address_space(4)))* constant;
+    return *(constant)(reinterpret_cast<pg_u64>(p));
+}
+
+template <int D_, int PAGE_, int G_, int NT_, int QT_, int CT_, bool WIN_, bool LSE_, bool VEC_>
+struct Attend {
+    static constexpr int D = D_, PAGE = PAGE_, G = G_, NT = NT_, QT = QT_, CT = CT_;
+    static constexpr bool WIN = WIN_, LSE = LSE_, VEC = VEC_;
+    static constexpr int RB = 16 * NT;
+    static constexpr int C = G <= RB ? RB / G : 1;               // tokens of a unit
+    static constexpr int HS = G <= RB ? 1 : (G + RB - 1) / RB;   // units that share a token's heads
+    static constexpr int GH = G <= RB ? G : RB;                  // query heads of a unit
+    static constexpr int NK = (D + 63) / 64, DP = 64 * NK;
+    static constexpr bool H = QT == kF16;                        // K and q as f16
+    static constexpr int QP = QT == kF32 ? 3 : 1;                // parts of q
+    static constexpr int PP = QT == kF32 ? 3 : 2;                // parts of p
+    static constexpr bool PAGED16 = PAGE % 16 == 0;              // 16 aligned tokens lie in one page
+    static constexpr int PART = RB * (2 + DP);                   // floats of a partial result
+    static constexpr int E = 16 * NK * NT;                       // accumulators of a lane
+
+    // One request.
+    struct Request {
+        int row, n, length, first, kt, units;  // first row, rows, tokens; first tile, tiles and units of a key head
+    };
+    __device__ static Request request(const AttendArgs& A, pg_i64 b, bool report) {
+        Request r;
+        const int s0 = A.starts[b * A.s_starts], s1 = A.starts[(b + 1) * A.s_starts];
+        int length = A.lengths[b * A.s_lengths];
+        const pg_i64 most = A.width * PAGE;
+        bool bad = s0 < 0 || s1 < s0 || s1 > A.rows || length < 0 || length > most;
+        if (bad) {
+            if (report) *A.err = 7;
+            r.row = r.n = r.length = r.first = r.kt = r.units = 0;
+            return r;
+        }
+        r.row = s0;
+        r.n = s1 - s0;
+        r.length = length;
+        int lo = 0;
+        if constexpr (WIN) {
+            const pg_i64 w = static_cast<pg_i64>(length) - r.n + 1 - A.window;
+            lo = w > 0 ? static_cast<int>(w) : 0;
+            if (lo > length) lo = length;
+        }
+        r.first = lo / kAttendTile;
+        const int last = static_cast<int>((static_cast<pg_u32>(length) + (kAttendTile - 1)) / kAttendTile);
+        r.kt = last > r.first ? last - r.first : 1;
+        r.units = (r.n + C - 1) / C * HS;
+        return r;
+    }
+
+    struct Raw {
+        pg_u32x4 k[2][NK];
+        pg_u32 v[NK][8];
+        float ks[PAGED16 ? 2 : 8], vs[PAGED16 ? 2 : 8];
+    };
+
+    // One unit of one workgroup's piece.
+    struct Unit {
+        const int* table;  // the request's row
+        int h, n;          // key head; tokens of the unit
+        int p0;            // position of its first token
+        int lo, hi;        // positions that its rows attend to, together
+    };
+
+    // Pages of the 32 tokens from `base` on.  Tokens outside the unit's
+    // positions take the page of a neighbour inside; they are masked.
+    struct Pages {
+        int id[2];
+    };
+    __device__ static int checked(const AttendArgs& A, int id) {
+        if (static_cast<pg_u32>(id) >= static_cast<pg_u64>(A.pages)) {
+            *A.err = 7;
+            return 0;
+        }
+        return id;
+    }
+    __device__ static int inside(const Unit& u, int t) { return t < u.lo ? u.lo : t >= u.hi ? u.hi - 1 : t; }
+    __device__ static void pages(const AttendArgs& A, const Unit& u, int base, Pages& p) {
+        if constexpr (PAGED16) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) p.id[i] = uniform_load(u.table + inside(u, base + 16 * i) / PAGE);
+        } else {
+            p.id[0] = u.table[inside(u, base + (static_cast<int>(threadIdx.x) & 31)) / PAGE];
+        }
+    }
+
+    __device__ static void load(const AttendArgs& A, const Unit& u, int base, const Pages& p, Raw& r) {
+        const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+        if constexpr (PAGED16) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int id = checked(A, p.id[i]), off = (base + 16 * i) % PAGE;
+                r.ks[i] = uniform_load(A.scale[0] + id * A.s_scale[0][0] + u.h * A.s_scale[0][1]);
+                r.vs[i] = uniform_load(A.scale[1] + id * A.s_scale[1][0] + u.h * A.s_scale[1][1]);
+                const char* const kp = A.cache[0] + id * A.s_cache[0][0] + u.h * A.s_cache[0][1] + off * A.s_cache[0][2];
+                const char* const vp = A.cache[1] + id * A.s_cache[1][0] + u.h * A.s_cache[1][1] + off * A.s_cache[1][2];
+                const int ko = m * static_cast<int>(A.s_cache[0][2]) + 16 * g, vt = static_cast<int>(A.s_cache[1][2]);
+#pragma unroll
+                for (int j = 0; j < NK; ++j) {
+                    r.k[i][j] = pg_u32x4{0, 0, 0, 0};
+                    if (D % 64 == 0 || 64 * j + 16 * g < D) r.k[i][j] = *reinterpret_cast<const pg_u32x4*>(kp + ko + 64 * j);
+                }
+#pragma unroll
+                for (int j = 0; j < NK; ++j)
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        r.v[j][4 * i + t] = 0;
+                        if (D % 64 == 0 || 64 * j + 4 * m < D)
+                            r.v[j][4 * i + t] = *reinterpret_cast<const pg_u32*>(vp + (4 * g + t) * vt + 64 * j + 4 * m);
+                    }
+            }
+        } else {
+            // Lane l has looked up token base + l % 32.
+            const int id = checked(A, p.id[0]), off = inside(u, base + (lane & 31)) % PAGE;
+            const float ks = A.scale[0][id * A.s_scale[0][0] + u.h * A.s_scale[0][1]];
+            const float vs = A.scale[1][id * A.s_scale[1][0] + u.h * A.s_scale[1][1]];
+            const char* const kp = A.cache[0] + u.h * A.s_cache[0][1];
+            const char* const vp = A.cache[1] + u.h * A.s_cache[1][1];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const char* const row = kp + __shfl(id, 16 * i + m, 64) * A.s_cache[0][0] + __shfl(off, 16 * i + m, 64) * A.s_cache[0][2];
+#pragma unroll
+                for (int j = 0; j < NK; ++j) {
+                    r.k[i][j] = pg_u32x4{0, 0, 0, 0};
+                    if (D % 64 == 0 || 64 * j + 16 * g < D) r.k[i][j] = *reinterpret_cast<const pg_u32x4*>(row + 64 * j + 16 * g);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+                const int from = (t & 4) * 4 + 4 * g + (t & 3);
+                const char* const row = vp + __shfl(id, from, 64) * A.s_cache[1][0] + __shfl(off, from, 64) * A.s_cache[1][2];
+                r.ks[t] = __shfl(ks, from, 64);
+                r.vs[t] = __shfl(vs, from, 64);
+#pragma unroll
+                for (int j = 0; j < NK; ++j) {
+                    r.v[j][t] = 0;
+                    if (D % 64 == 0 || 64 * j + 4 * m < D) r.v[j][t] = *reinterpret_cast<const pg_u32*>(row + 64 * j + 4 * m);
+                }
+            }
+        }
+    }
+
+    __device__ static pg_f32x4 mma(pg_u32x4 a, pg_u32x4 b, pg_f32x4 c, bool half) {
+        if (half) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(pg_h8, a), __builtin_bit_cast(pg_h8, b), c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pg_bf8, a), __builtin_bit_cast(pg_bf8, b), c, 0, 0, 0);
+    }
+    // Two floats as bf16, and what the rounding left of them.
+    __device__ static pg_u32 take_bf16(float& a, float& b) {
+        const pg_bf2 h = __builtin_convertvector((pg_f32x2{a, b}), pg_bf2);
+        const pg_u32 w = __builtin_bit_cast(pg_u32, h);
+        a = a - __uint_as_float(w << 16);
+        b = b - __uint_as_float(w & 0xFFFF0000u);
+        return w;
+    }
+
+    struct State {
+        pg_u32x4 q[NT][2 * NK][QP];
+        pg_f32x4 o[NT][NK][4];
+        float m[NT], l[NT];
+    };
+
+    __device__ static void load_q(const AttendArgs& A, const Unit& u, int row, int head, State& st) {
+        const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int r = 16 * t + n, i = r / GH, hh = r - i * GH;
+            const bool valid = i < u.n && (HS == 1 || head % G + hh < G);
+            const char* const p = A.q + ((row + i) * A.s_q[0] + (head + hh) * A.s_q[1]) * elem_size(QT);
+#pragma unroll
+            for (int j = 0; j < 2 * NK; ++j) {
+                const int d = 64 * (j >> 1) + 16 * g + 8 * (j & 1);
+                const bool in = valid && d < D;
+                if constexpr (QT == kF32) {
+                    float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+                    if (in) load8<QT, VEC>(p + d * 4, x);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (int k = 0; k < 3; ++k) st.q[t][j][k][e] = take_bf16(x[2 * e], x[2 * e + 1]);
+                } else {
+                    pg_u32x4 w = {0, 0, 0, 0};
+                    if (in) {
+                        if constexpr (VEC) {
+                            w = *reinterpret_cast<const pg_u32x4*>(p + d * 2);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                w[e] = static_cast<pg_u32>(*reinterpret_cast<const pg_u16*>(p + d * 2 + 4 * e)) |
+                                       static_cast<pg_u32>(*reinterpret_cast<const pg_u16*>(p + d * 2 + 4 * e + 2)) << 16;
+                        }
+                    }
+                    st.q[t][j][0] = w;
+                }
+            }
+            st.m[t] = -__builtin_inff();
+            st.l[t] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NK; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) st.o[t][j][e] = pg_f32x4{0, 0, 0, 0};
+        }
+    }
+
+    // O^T += V^T P^T for P's parts in the eight token places of a lane.
+    __device__ static void values(const pg_u32 (&v)[NK][8], const pg_u32x4 (&p)[NT][PP], pg_f32x4 (&o)[NT][NK][4]) {
+#pragma unroll
+        for (int j = 0; j < NK; ++j) {
+            pg_u32x4 a[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const pg_u32 x = v[j][2 * e], y = v[j][2 * e + 1];
+                const pg_u32 w0 = __builtin_amdgcn_perm(y, x, 0x05010400u), w1 = __builtin_amdgcn_perm(y, x, 0x07030602u);
+                a[0][e] = codes2<CT, false, false>(w0);
+                a[1][e] = codes2<CT, false, true>(w0);
+                a[2][e] = codes2<CT, false, false>(w1);
+                a[3][e] = codes2<CT, false, true>(w1);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int k = 0; k < PP; ++k) o[t][j][q] = mma(a[q], p[t][k], o[t][j][q], false);
+        }
+    }
+
+    template <bool MASKED>
+    __device__ static void step(const AttendArgs& A, const Unit& u, int base, Raw& r, State& st) {
+        const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+        float s[NT][8];
+        {
+            pg_f32x4 acc[NT][2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t) acc[t][i] = pg_f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < 2 * NK; ++j) {
+                    const pg_u32 w0 = r.k[i][j >> 1][2 * (j & 1)], w1 = r.k[i][j >> 1][2 * (j & 1) + 1];
+                    const pg_u32x4 a = {codes2<CT, H, false>(w0), codes2<CT, H, true>(w0), codes2<CT, H, false>(w1), codes2<CT, H, true>(w1)};
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int k = 0; k < QP; ++k) acc[t][i] = mma(a, st.q[t][j][k], acc[t][i], H);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float f = r.ks[PAGED16 ? e >> 2 : e] * A.factor;
+#pragma unroll
+                for (int t = 0; t < NT; ++t) s[t][e] = acc[t][e >> 2][e & 3] * f;
+            }
+        }
+        bool part = false;  // some tokens are seen by some rows only
+        pg_u32 seen[NT];    // masked: bit e, the lane's row attends to its token e
+        if constexpr (MASKED) {
+            const int tok = base + 4 * g;  // token of place e: tok + e % 4, 16 further for e >= 4
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const int hi = u.p0 + (16 * t + n) / GH + 1, lo = WIN ? hi - A.window : 0;
+                seen[t] = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int at = tok + (e & 3) + 4 * (e & 4);
+                    const bool in = at < hi && at >= lo && at < u.hi;
+                    seen[t] |= static_cast<pg_u32>(in) << e;
+                    s[t][e] = in ? s[t][e] : -__builtin_inff();
+                }
+            }
+            // What lies outside the unit's positions may be anything.
+            pg_u32 nan = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int at = tok + (e & 3) + 4 * (e & 4);
+                const bool in = at < u.hi && at >= u.lo;
+#pragma unroll
+                for (int j = 0; j < NK; ++j) {
+                    r.v[j][e] = in ? r.v[j][e] : 0;
+                    nan |= ((r.v[j][e] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+                }
+            }
+            if constexpr (CT == kE4M3 && (C > 1 || WIN)) part = __ballot(nan != 0) != 0;
+        }
+        // The maximum, only if some score is far above it.
+        bool grow = false;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            float mx = s[t][0];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[t][e]);
+            grow |= mx > st.m[t] + 8.0f;
+        }
+        if (__ballot(grow)) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                float mx = s[t][0];
+#pragma unroll
+                for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[t][e]);
+                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                const float m = fmaxf(st.m[t], mx);
+                const float a = m == st.m[t] ? 1.0f : __builtin_amdgcn_exp2f(st.m[t] - m);
+                st.m[t] = m;
+                st.l[t] *= a;
+#pragma unroll
+                for (int j = 0; j < NK; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) st.o[t][j][q] *= a;
+            }
+        }
+        pg_u32x4 p[NT][PP];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const float m = st.m[t] == -__builtin_inff() ? 0.0f : st.m[t];
+            float x[8], l = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[e] = __builtin_amdgcn_exp2f(s[t][e] - m);
+                l += x[e];
+                x[e] *= r.vs[PAGED16 ? e >> 2 : e];
+                if (MASKED) x[e] = seen[t] >> e & 1 ? x[e] : 0.0f;
+            }
+            st.l[t] += l;
+#pragma unroll
+            for (int k = 0; k < PP; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[t][k][e] = take_bf16(x[2 * e], x[2 * e + 1]);
+        }
+        if (MASKED && part) {
+            // A NaN among values that some rows do not see: token by token, and
+            // only into the rows that see it (0 * NaN is NaN).
+            for (int at = 0; at < 32; ++at) {
+                const int e = (at & 3) | (at & 16) >> 2;
+                const bool mine = (at & 12) >> 2 == g;
+                pg_u32 v[NK][8];
+#pragma unroll
+                for (int j = 0; j < NK; ++j)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) v[j][k] = mine && k == e ? r.v[j][k] : 0;
+                pg_f32x4 o[NT][NK][4];
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int j = 0; j < NK; ++j)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) o[t][j][q] = pg_f32x4{0, 0, 0, 0};
+                values(v, p, o);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const int hi = u.p0 + (16 * t + n) / GH + 1;
+                    const bool in = base + at < hi && (!WIN || base + at >= hi - A.window);
+#pragma unroll
+                    for (int j = 0; j < NK; ++j)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            if (in) st.o[t][j][q] += o[t][j][q];
+                }
+            }
+        } else {
+            values(r.v, p, st.o);
+        }
+    }
+
+    __device__ static void write_row(const AttendArgs& A, int row, int head, int g, int j, const pg_f32x4 (&o)[4], float f) {
+        // o[q][i]: dim 64j + 16g + 4i + q.
+        const int d = 64 * j + 16 * g;
+        if (D % 64 != 0 && d >= D) return;
+        char* const p = A.out + (row * A.s_out[0] + head * A.s_out[1] + d) * elem_size(QT);
+        float y[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) y[i] = o[i & 3][i >> 2] * f;
+        if constexpr (VEC && QT == kF32) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) *reinterpret_cast<pg_f32x4*>(p + 16 * i) = pg_f32x4{y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]};
+        } else if constexpr (VEC) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                pg_u32x4 w;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float a = y[8 * i + 2 * e], b = y[8 * i + 2 * e + 1];
+                    if constexpr (QT == kF16) w[e] = __builtin_bit_cast(pg_u32, (pg_h2{static_cast<_Float16>(a), static_cast<_Float16>(b)}));
+                    else w[e] = __builtin_bit_cast(pg_u32, __builtin_convertvector((pg_f32x2{a, b}), pg_bf2));
+                }
+                *reinterpret_cast<pg_u32x4*>(p + 16 * i) = w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) store_elem<QT>(p + i * elem_size(QT), y[i]);
+        }
+    }
+
+    struct Shared {
+        pg_f32x4 o[4][NT * NK * 4][64];
+        float m[4][RB], l[4][RB];
+        pg_i64 scan[4];
+        pg_i64 begin[2];  // where the piece starts: request, items before it
+    };
+
+    __device__ static void run(const AttendArgs& A) {
+        __shared__ Shared sh;
+        const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+        const int wave = uniform(threadIdx.x >> 6);
+        const pg_i64 w = blockIdx.x;
+        int* const span = A.spans + w * kSpanInts;
+        // The pieces: per request the items of its units, and their sums.
+        const pg_i64 per = (A.batch + kAttendThreads - 1) / kAttendThreads, b0 = threadIdx.x * per;
+        const pg_i64 b1 = b0 + per < A.batch ? b0 + per : A.batch;
+        pg_i64 sum = 0;
+        for (pg_i64 b = b0; b < b1; ++b) {
+            const Request r = request(A, b, w == 0);
+            sum += static_cast<pg_i64>(A.heads) * r.units * r.kt;
+        }
+        pg_i64 total;
+        pg_i64 before = block_scan<kAttendThreads>(sum, total, sh.scan);
+        total = uniform64(total);
+        const pg_i64 pieces = total < static_cast<pg_i64>(gridDim.x) ? total : static_cast<pg_i64>(gridDim.x);
+        if (w >= pieces) {
+            if (threadIdx.x == 0) span[0] = 0;
+            return;
+        }
+        pg_i64 x = total * w / pieces;
+        const pg_i64 x1 = total * (w + 1) / pieces;
+        if (x >= before && x < before + sum) {
+            pg_i64 at = before;
+            for (pg_i64 b = b0; b < b1; ++b) {
+                const Request r = request(A, b, false);
+                const pg_i64 items = static_cast<pg_i64>(A.heads) * r.units * r.kt;
+                if (x < at + items) {
+                    sh.begin[0] = b;
+                    sh.begin[1] = at;
+                    break;
+                }
+                at += items;
+            }
+        }
+        __syncthreads();
+        pg_i64 b = uniform64(sh.begin[0]), xb = uniform64(sh.begin[1]);
+        int joined = 0;
+        while (x < x1) {
+            Request rq = request(A, b, false);
+            rq.row = uniform(rq.row);
+            rq.n = uniform(rq.n);
+            rq.length = uniform(rq.length);
+            rq.first = uniform(rq.first);
+            rq.kt = uniform(rq.kt);
+            rq.units = uniform(rq.units);
+            const pg_i64 items = static_cast<pg_i64>(A.heads) * rq.units * rq.kt;
+            if (x >= xb + items) {
+                xb += items;
+                ++b;
+                continue;
+            }
+            const pg_i64 unit = (x - xb) / rq.kt;
+            const int t0 = static_cast<int>(x - xb - unit * rq.kt);
+            const int t1 = x1 - x < rq.kt - t0 ? t0 + static_cast<int>(x1 - x) : rq.kt;
+            const int h = static_cast<int>(unit / rq.units), in = static_cast<int>(unit - static_cast<pg_i64>(h) * rq.units);
+            const int tile = in / HS, hs = in - tile * HS;
+            Unit u;
+            u.table = A.table + b * A.s_table;
+            u.h = h;
+            u.n = rq.n - tile * C < C ? rq.n - tile * C : C;
+            u.p0 = rq.length - rq.n + tile * C;
+            u.hi = u.p0 + u.n > 0 ? u.p0 + u.n : 0;
+            u.lo = 0;
+            if (WIN && u.p0 + 1 > A.window) u.lo = u.p0 + 1 - A.window;
+            const int row = rq.row + tile * C, head = h * G + hs * RB;
+            State st;
+            load_q(A, u, row, head, st);
+            piece(A, u, (rq.first + t0) * kAttendTile + 32 * wave, (rq.first + t1) * kAttendTile, st);
+            // The four waves' results.
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                st.l[t] += __shfl_xor(st.l[t], 16, 64);
+                st.l[t] += __shfl_xor(st.l[t], 32, 64);
+                if (g == 0) {
+                    sh.m[wave][16 * t + n] = st.m[t];
+                    sh.l[wave][16 * t + n] = st.l[t];
+                }
+            }
+            __syncthreads();
+            float m[NT], l[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                m[t] = -__builtin_inff();
+#pragma unroll
+                for (int k = 0; k < 4; ++k) m[t] = fmaxf(m[t], sh.m[k][16 * t + n]);
+                l[t] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float mk = sh.m[k][16 * t + n];
+                    l[t] += mk == -__builtin_inff() ? 0.0f : sh.l[k][16 * t + n] * __builtin_amdgcn_exp2f(mk - m[t]);
+                }
+                const float f = st.m[t] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(st.m[t] - m[t]);
+#pragma unroll
+                for (int j = 0; j < NK; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) sh.o[wave][(t * NK + j) * 4 + q][lane] = st.o[t][j][q] * f;
+            }
+            __syncthreads();
+            const bool opens = t0 == 0, closes = t1 == rq.kt;
+            float* const part = A.parts + (2 * w + (opens ? 1 : 0)) * PART;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const int r = 16 * t + n, i = r / GH, hh = r - i * GH;
+                const bool valid = i < u.n && (HS == 1 || hs * RB + hh < G);
+#pragma unroll
+                for (int j = 0; j < NK; ++j) {
+                    if ((t * NK + j) % 4 != wave) continue;
+                    pg_f32x4 o[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        o[q] = sh.o[0][(t * NK + j) * 4 + q][lane];
+#pragma unroll
+                        for (int k = 1; k < 4; ++k) o[q] += sh.o[k][(t * NK + j) * 4 + q][lane];
+                    }
+                    if (!valid) continue;
+                    if (opens && closes) {
+                        write_row(A, row + i, head + hh, g, j, o, l[t] == 0.0f ? 0.0f : 1.0f / l[t]);
+                    } else {
+                        float* const po = part + 2 * RB + r * DP + 64 * j + 16 * g;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) *reinterpret_cast<pg_f32x4*>(po + 4 * e) = pg_f32x4{o[0][e], o[1][e], o[2][e], o[3][e]};
+                    }
+                }
+                if (wave == 0 && g == 0 && valid) {
+                    if (!(opens && closes)) {
+                        part[r] = m[t];
+                        part[RB + r] = l[t];
+                    } else if (LSE) {
+                        A.lse[(row + i) * A.s_lse[0] + (head + hh) * A.s_lse[1]] = lse_of(m[t], l[t]);
+                    }
+                }
+            }
+            if (opens && !closes) {
+                joined = 1;
+                if (threadIdx.x == 0) {
+                    // The workgroup of the unit's last item.
+                    const pg_i64 last = xb + (unit + 1) * rq.kt - 1;
+                    span[1] = row;
+                    span[2] = head;
+                    span[3] = u.n;
+                    span[4] = static_cast<int>(((last + 1) * pieces - 1) / total);
+                    span[5] = hs;
+                }
+            }
+            x += t1 - t0;
+        }
+        if (threadIdx.x == 0) span[0] = joined;
+    }
+
+    __device__ static float lse_of(float m, float l) {
+        return l == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f;
+    }
+
+    // This wave's steps of the tokens from `base` on, below `end`: every
+    // fourth 32.  The next step's pages and bytes are under way during one.
+    __device__ static void piece(const AttendArgs& A, const Unit& u, int base, int end, State& st) {
+        if (end > u.hi) end = u.hi;
+        if (base + 32 <= u.lo) base += (u.lo - base - 31 + kAttendTile - 1) / kAttendTile * kAttendTile;
+        if (base >= end) return;
+        Pages pg;
+        Raw a, b;
+        pages(A, u, base, pg);
+        load(A, u, base, pg, a);
+        pages(A, u, base + kAttendTile, pg);
+        for (;;) {
+            if (base + kAttendTile < end) {
+                load(A, u, base + kAttendTile, pg, b);
+                pages(A, u, base + 2 * kAttendTile, pg);
+            }
+            one(A, u, base, a, st);
+            base += kAttendTile;
+            if (base >= end) return;
+            if (base + kAttendTile < end) {
+                load(A, u, base + kAttendTile, pg, a);
+                pages(A, u, base + 2 * kAttendTile, pg);
+            }
+            one(A, u, base, b, st);
+            base += kAttendTile;
+            if (base >= end) return;
+        }
+    }
+    __device__ static void one(const AttendArgs& A, const Unit& u, int base, Raw& r, State& st) {
+        // Every row of the unit sees every one of the tokens.
+        const bool whole = base + 32 <= u.p0 + 1 && (!WIN || base >= u.p0 + u.n - A.window);
+        if (whole) step<false>(A, u, base, r, st);
+        else step<true>(A, u, base, r, st);
+    }
+
+    // Joins the pieces of the unit that workgroup blockIdx.x left open.
+    __device__ static void join(const AttendArgs& A) {
+        constexpr int THREADS = 256, GROUPS = THREADS / RB;
+        __shared__ float weight[THREADS], top[RB], sums[RB];
+        __shared__ float red[GROUPS][RB];
+        const int* const span = A.spans + static_cast<pg_i64>(blockIdx.x) * kSpanInts;
+        if (!span[0]) return;
+        const int row = span[1], head = span[2], ntok = span[3], last = span[4], hs = span[5];
+        const int np = last - static_cast<int>(blockIdx.x) + 1;
+        const int heads = HS == 1 ? GH : (G - hs * RB < RB ? G - hs * RB : RB), rows = HS == 1 ? ntok * GH : heads;
+        auto part = [&](int k) { return A.parts + (2 * (static_cast<pg_i64>(blockIdx.x) + k) + (k == 0 ? 1 : 0)) * PART; };
+        const int r = threadIdx.x % RB, grp = threadIdx.x / RB;
+        float m = -__builtin_inff();
+        if (r < rows)
+            for (int k = grp; k < np; k += GROUPS) m = fmaxf(m, part(k)[r]);
+        red[grp][r] = m;
+        __syncthreads();
+        if (threadIdx.x < RB) {
+            for (int k = 1; k < GROUPS; ++k) m = fmaxf(m, red[k][r]);
+            top[r] = m;
+            sums[r] = 0.0f;
+        }
+        // Output pieces of four dims; the threads left over share the parts.
+        constexpr int Q = DP / 4;
+        const int pieces = rows * Q;
+        float l = 0.0f;
+        for (int p0 = 0; p0 < pieces; p0 += THREADS) {
+            const int idx = p0 + static_cast<int>(threadIdx.x), pr = idx / Q, d = (idx - pr * Q) * 4;
+            pg_f32x4 o = {0, 0, 0, 0};
+            for (int k0 = 0; k0 < np; k0 += GROUPS) {
+                // Weights of GROUPS parts.
+                __syncthreads();
+                const int k = k0 + grp;
+                float wt = 0.0f;
+                if (k < np && r < rows) {
+                    const float mk = part(k)[r];
+                    wt = mk == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mk - top[r]);
+                    if (p0 == 0) l += wt * part(k)[RB + r];
+                }
+                weight[threadIdx.x] = wt;
+                __syncthreads();
+                if (idx < pieces) {
+                    const int many = np - k0 < GROUPS ? np - k0 : GROUPS;
+                    for (int k2 = 0; k2 < many; ++k2) {
+                        const pg_f32x4 x = *reinterpret_cast<const pg_f32x4*>(part(k0 + k2) + 2 * RB + pr * DP + d);
+                        o += x * weight[k2 * RB + pr];
+                    }
+                }
+            }
+            if (p0 == 0) {
+                red[grp][r] = l;
+                __syncthreads();
+                if (threadIdx.x < RB) {
+                    float s = 0.0f;
+                    for (int k = 0; k < GROUPS; ++k) s += red[k][r];
+                    sums[r] = s;
+                }
+                __syncthreads();
+            }
+            if (idx < pieces && d < D) {
+                const int i = pr / GH, hh = pr - i * GH;
+                const float s = sums[pr], f = s == 0.0f ? 0.0f : 1.0f / s;
+                char* const p = A.out + ((row + i) * A.s_out[0] + (head + hh) * A.s_out[1] + d) * elem_size(QT);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) store_elem<QT>(p + e * elem_size(QT), o[e] * f);
+                if (LSE && d == 0) A.lse[(row + i) * A.s_lse[0] + (head + hh) * A.s_lse[1]] = lse_of(top[pr], s);
+            }
+        }
+    }
+};
+
+}  // namespace ptowsp

@@ -527,6 +527,9 @@ KernelAnalysis analyze_kernel(const KernelDef& k) {
         return a;
     }
 
+    for (const ValueInfo& v : k.values)
+        if (v.dtype == DType::F8E4M3) refuse(k, "values of dtype f8e4m3 are not supported (caches of the paged operators hold them)");
+
     auto val = [&](int id) -> const ValueInfo* {
         if (id <= 0 || id >= n || !a.by_id[id]) refuse(k, "op references undefined value " + std::to_string(id));
         return a.by_id[id];

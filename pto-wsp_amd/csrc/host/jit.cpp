@@ -141,10 +141,10 @@ std::string jit_cache_dir() {
 
 std::vector<char> jit_compile(const std::string& source) {
     hiprtcProgram prog = nullptr;
-    const char* headers[] = {kDeviceHeader, kLaunchHeader, kKernelAbi, kPtoisaBridge, kStdTypes, kStdTypes, kStdTypes, kStdTypes};
-    const char* names[] = {"ptowsp_device.h", "ptowsp_launch.h", "pto/wsp/codegen/abi/kernel_abi.hpp",
+    const char* headers[] = {kDeviceHeader, kLaunchHeader, kPagedHeader, kPagedArgsHeader, kKernelAbi, kPtoisaBridge, kStdTypes, kStdTypes, kStdTypes, kStdTypes};
+    const char* names[] = {"ptowsp_device.h", "ptowsp_launch.h", "ptowsp_paged.h", "ptowsp_paged_args.h", "pto/wsp/codegen/abi/kernel_abi.hpp",
                            "pto/wsp/codegen/abi/ptoisa_bridge.hpp", "cstdint", "cstddef", "stdint.h", "stddef.h"};
-    const int nh = source.rfind(kTuMarker, 0) == 0 ? 8 : 2;
+    const int nh = source.rfind(kTuMarker, 0) == 0 ? 10 : 4;
     if (hiprtcCreateProgram(&prog, source.c_str(), "ptowsp_kernel.hip", nh, headers, names) != HIPRTC_SUCCESS)
         throw CompileError("hiprtcCreateProgram failed");
     const int nopt = static_cast<int>(sizeof(kOptions) / sizeof(kOptions[0]));
@@ -168,23 +168,29 @@ std::vector<char> jit_compile(const std::string& source) {
 namespace {
 // The headers and options are hashed once: they are a hundred times a source.
 std::string source_key(const std::string& source) {
-    static const std::string fixed = hex64(fnv1a_64(options_key() + kDeviceHeader + kLaunchHeader));
+    static const std::string fixed = hex64(fnv1a_64(options_key() + kDeviceHeader + kLaunchHeader + kPagedHeader + kPagedArgsHeader));
     static const std::string tu = hex64(fnv1a_64(std::string(kKernelAbi) + kPtoisaBridge + kStdTypes));
     return hex64(fnv1a_64(source + "\n" + fixed + (source.rfind(kTuMarker, 0) == 0 ? tu : "")));
+}
+// A module is loaded on one GPU: the current one.
+std::string loaded_key(const std::string& key, const std::string& entry) {
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) (void)hipGetLastError();
+    return key + entry + "@" + std::to_string(dev);
 }
 }  // namespace
 
 const JitKernel* jit_loaded(const std::string& source, const std::string& entry) {
-    const std::string key = source_key(source);
+    const std::string key = loaded_key(source_key(source), entry);
     std::lock_guard<std::mutex> lock(g_mu);
-    auto it = g_loaded.find(key + entry);
+    auto it = g_loaded.find(key);
     return it == g_loaded.end() ? nullptr : it->second.get();
 }
 
 const JitKernel& jit_kernel(const std::string& source, const std::string& entry) {
-    const std::string key = source_key(source);
+    const std::string key = source_key(source), loaded = loaded_key(key, entry);
     std::lock_guard<std::mutex> lock(g_mu);
-    auto it = g_loaded.find(key + entry);
+    auto it = g_loaded.find(loaded);
     if (it != g_loaded.end()) return *it->second;
 
     const std::string dir = jit_cache_dir();
@@ -206,7 +212,7 @@ const JitKernel& jit_kernel(const std::string& source, const std::string& entry)
     e = hipModuleGetFunction(&k->function, k->module, entry.c_str());
     if (e != hipSuccess) throw std::runtime_error(std::string("hipModuleGetFunction: ") + hipGetErrorString(e));
     auto& ref = *k;
-    g_loaded.emplace(key + entry, std::move(k));
+    g_loaded.emplace(loaded, std::move(k));
     return ref;
 }
 

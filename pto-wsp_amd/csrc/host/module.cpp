@@ -8,8 +8,8 @@ namespace ptowsp {
 
 namespace {
 
-const char* kDTypeNames[] = {"f16", "bf16", "f32", "f64", "i8", "i16", "i32", "i64", "u8", "u16", "u32", "u64", "bool"};
-const int kDTypeSizes[] = {2, 2, 4, 8, 1, 2, 4, 8, 1, 2, 4, 8, 1};
+const char* kDTypeNames[] = {"f16", "bf16", "f32", "f64", "i8", "i16", "i32", "i64", "u8", "u16", "u32", "u64", "bool", "f8e4m3"};
+const int kDTypeSizes[] = {2, 2, 4, 8, 1, 2, 4, 8, 1, 2, 4, 8, 1, 1};
 
 class Lexer {
 public:
@@ -72,7 +72,7 @@ public:
 
     DType dtype() {
         std::string t = tok();
-        for (int i = 0; i < 13; ++i)
+        for (int i = 0; i < static_cast<int>(sizeof(kDTypeSizes) / sizeof(kDTypeSizes[0])); ++i)
             if (t == kDTypeNames[i]) return static_cast<DType>(i);
         throw CompileError("module text: unknown dtype '" + t + "'");
     }
@@ -251,6 +251,18 @@ std::unique_ptr<SExpr> parse_expr(Lexer& L) {
     }
 }
 
+TensorArg parse_tensor_arg(Lexer& L, const Module& m, const std::string& who) {
+    TensorArg t;
+    t.param = L.str();
+    t.tid = static_cast<int>(L.i64());
+    t.base_rank = static_cast<int>(L.i64());
+    t.view_rank = static_cast<int>(L.i64());
+    const int64_t ni = L.i64();
+    for (int64_t j = 0; j < ni; ++j) t.idx.push_back(parse_index(L));
+    if (t.tid < 0 || t.tid >= static_cast<int>(m.tensors.size())) throw CompileError(who + ": bad tensor id");
+    return t;
+}
+
 std::unique_ptr<Node> parse_node(Lexer& L, const Module& m) {
     auto n = std::make_unique<Node>();
     std::string k = L.tok();
@@ -276,18 +288,7 @@ std::unique_ptr<Node> parse_node(Lexer& L, const Module& m) {
         int64_t ns = L.i64();
         for (int64_t i = 0; i < ns; ++i) n->scalar_args.push_back(parse_arg(L));
         int64_t nt = L.i64();
-        for (int64_t i = 0; i < nt; ++i) {
-            TensorArg t;
-            t.param = L.str();
-            t.tid = static_cast<int>(L.i64());
-            t.base_rank = static_cast<int>(L.i64());
-            t.view_rank = static_cast<int>(L.i64());
-            int64_t ni = L.i64();
-            for (int64_t j = 0; j < ni; ++j) t.idx.push_back(parse_index(L));
-            if (t.tid < 0 || t.tid >= static_cast<int>(m.tensors.size()))
-                throw CompileError("task " + n->kernel + ": bad tensor id");
-            n->tensor_args.push_back(std::move(t));
-        }
+        for (int64_t i = 0; i < nt; ++i) n->tensor_args.push_back(parse_tensor_arg(L, m, "task " + n->kernel));
     } else if (k == "sel") {
         n->kind = NodeKind::Select;
         n->var = L.str();
@@ -325,6 +326,18 @@ std::unique_ptr<Node> parse_node(Lexer& L, const Module& m) {
             case DType::Bool: break;
             default:
                 throw CompileError(std::string("Unsupported dtype for workload codegen: ") + dtype_name(m.tensors[t.tid].dtype));
+        }
+    } else if (k == "oper") {
+        n->kind = NodeKind::Operator;
+        n->op = L.str();
+        const int64_t nt = L.i64();
+        for (int64_t i = 0; i < nt; ++i) n->tensor_args.push_back(parse_tensor_arg(L, m, n->op));
+        const int64_t na = L.i64();
+        for (int64_t i = 0; i < na; ++i) {
+            const std::string key = L.str(), ty = L.tok();
+            if (ty == "i") n->op_ints[key] = L.i64();
+            else if (ty == "d") n->op_floats[key] = L.f64();
+            else throw CompileError(n->op + ": bad attr type '" + ty + "'");
         }
     } else {
         throw CompileError("module text: bad node kind '" + k + "'");

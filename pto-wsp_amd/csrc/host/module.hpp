@@ -20,7 +20,7 @@
 
 namespace ptowsp {
 
-enum class DType : int { F16, BF16, F32, F64, I8, I16, I32, I64, U8, U16, U32, U64, Bool };
+enum class DType : int { F16, BF16, F32, F64, I8, I16, I32, I64, U8, U16, U32, U64, Bool, F8E4M3 };
 
 const char* dtype_name(DType d);
 int dtype_size(DType d);
@@ -112,7 +112,7 @@ struct Axis {
     int64_t max = 0;   // DynTensor: declared upper bound of the extent
 };
 
-enum class NodeKind { Empty, ParallelFor, ForEach, Combine, Sequential, Task, Select, Cond, SlotSet, SlotLoad };
+enum class NodeKind { Empty, ParallelFor, ForEach, Combine, Sequential, Task, Select, Cond, SlotSet, SlotLoad, Operator };
 
 struct Node {
     NodeKind kind = NodeKind::Empty;
@@ -133,6 +133,11 @@ struct Node {
     uint64_t value = 0;
     TensorArg view;
     int64_t row = 0, col = 0;
+    // operator step: its kind (operators.hpp), operands (tensor_args, by name)
+    // and attributes
+    std::string op;
+    std::map<std::string, int64_t> op_ints;
+    std::map<std::string, double> op_floats;
 };
 
 struct Schedule {

@@ -1,0 +1,48 @@
+// Operator steps of a workload (pto_wsp/paged.py): operands checked when a
+// module is compiled, launches made when a run reaches the step.
+#pragma once
+
+#include <cstddef>
+#include <cstdint>
+#include <functional>
+#include <string>
+#include <vector>
+
+#include "module.hpp"
+
+namespace ptowsp {
+
+// Throws CompileError where types, shapes or attributes of an operator step do not fit.
+void check_operator(const Module& m, const Node& n);
+
+// Whether the step writes the operand.
+bool operator_writes(const Node& n, size_t operand);
+
+// One operand at a run: the view's first element on the device.
+struct Operand {
+    char* ptr = nullptr;
+    std::vector<int64_t> shape, stride;  // elements
+    DType dtype = DType::F32;
+};
+
+// What a step needs of the run around it.
+struct OperatorRun {
+    int cus = 1;         // compute units of the device
+    int* err = nullptr;  // the kernels' error flag
+    // Device scratch for the step: `need` bytes, any content.
+    std::function<char*(size_t)> scratch;
+    std::function<void(const std::string& source, const char* entry, int64_t blocks, int threads, const void* args, size_t bytes)> launch;
+};
+
+// Enqueues the step.  Throws std::runtime_error where strides, alignment or
+// overlaps do not fit.
+void run_operator(const Node& n, const std::vector<Operand>& operands, const OperatorRun& run);
+
+// The message of an error flag that an operator's kernel raised, or null.
+const char* operator_error(int flag);
+
+// Sources of the step's kernels for operands laid out one behind the other
+// (for builds without a GPU).
+std::vector<std::pair<std::string, std::string>> operator_sources(const Module& m, const Node& n);
+
+}  // namespace ptowsp

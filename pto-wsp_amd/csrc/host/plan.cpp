@@ -28,12 +28,13 @@ bool chain_is_custom(const Module& m, const Node* n) {
     return n && n->kind == NodeKind::Task && m.kernels[n->kernel_index].custom;
 }
 
-bool has_slot_ops(const Node* n) {
+// Slot and operator steps run between launches: loops around them run on the host.
+bool has_host_steps(const Node* n) {
     if (!n) return false;
-    if (n->kind == NodeKind::SlotSet || n->kind == NodeKind::SlotLoad) return true;
-    if (has_slot_ops(n->body.get())) return true;
+    if (n->kind == NodeKind::SlotSet || n->kind == NodeKind::SlotLoad || n->kind == NodeKind::Operator) return true;
+    if (has_host_steps(n->body.get())) return true;
     for (const auto& k : n->kids)
-        if (has_slot_ops(k.get())) return true;
+        if (has_host_steps(k.get())) return true;
     return false;
 }
 
@@ -58,6 +59,17 @@ bool reads_grid(const Ctx& ctx, const SExpr& e) {
     for (uint64_t id : r.axes) grid |= scope_of(ctx, id) == 2;
     if (r.task_params) throw CompileError("emit_scalar_expr_cpp: task_param() requires task_param_expr callback");
     return grid;
+}
+
+// An operator's views are indexed by constants and host-loop variables.
+void check_host_index(const Ctx& ctx, const Node& n, const IndexExpr& e) {
+    auto bound = [&](const std::string& var) {
+        if (std::find(ctx.host.begin(), ctx.host.end(), var) == ctx.host.end())
+            throw CompileError(n.op + ": loop variable '" + var + "' is not in scope");
+    };
+    if (e.kind == 't') throw CompileError(n.op + ": an operand is not indexed by a tensor's elements");
+    if (e.kind == 'v') bound(e.var);
+    for (const auto& [var, coef] : e.terms) bound(var);
 }
 
 void lower(const Module& m, const std::vector<KernelAnalysis>& ka, const Node* n, Ctx ctx, Plan& plan,
@@ -107,7 +119,7 @@ void lower(const Module& m, const std::vector<KernelAnalysis>& ka, const Node* n
             if (!ctx.inner.empty()) throw CompileError("internal: P() inside an in-kernel loop");
             if (n->axis.kind == AxisKind::DynTensor)
                 throw CompileError("P() over a tensor-bound extent is not supported (use P.seq)");
-            if (has_slot_ops(n->body.get())) {
+            if (has_host_steps(n->body.get())) {
                 PlanItem loop;
                 loop.is_loop = true;
                 loop.loop = LoopSpec{n->var, &n->axis};
@@ -171,9 +183,13 @@ void lower(const Module& m, const std::vector<KernelAnalysis>& ka, const Node* n
             out.push_back(std::move(c));
             return;
         }
+        case NodeKind::Operator:
+            for (const TensorArg& t : n->tensor_args)
+                for (const IndexExpr& e : t.idx) check_host_index(ctx, *n, e);
+            [[fallthrough]];
         case NodeKind::SlotSet:
         case NodeKind::SlotLoad: {
-            if (!ctx.grid.empty()) throw CompileError("internal: a slot step inside a launch grid");
+            if (!ctx.grid.empty()) throw CompileError("internal: a host step inside a launch grid");
             PlanItem c;
             c.ctl = n;
             out.push_back(std::move(c));
@@ -365,6 +381,7 @@ struct Walker {
                 // src/python/pto_codegen.cpp:2248-2253.
                 if (n->slot < slots.size()) slots[n->slot] = n->value;
                 return ready;
+            case NodeKind::Operator: return ready;  // the model knows tasks only
             case NodeKind::SlotLoad: {
                 // src/python/pto_codegen.cpp:2254-2303.
                 const uint64_t v = env.slot_load(*n, vars);

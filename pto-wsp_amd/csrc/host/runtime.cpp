@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <array>
+#include <atomic>
 #include <chrono>
 #include <cstdlib>
 #include <cmath>
@@ -20,11 +21,13 @@
 #include <vector>
 
 #include "../device/ptowsp_launch.h"
+#include "../device/ptowsp_paged_args.h"
 #include "analysis.hpp"
 #include "emit.hpp"
 #include "jit.hpp"
 #include "module.hpp"
 #include "noalloc.hpp"
+#include "operators.hpp"
 #include "plan.hpp"
 #include "ptowsp_hip.h"
 
@@ -38,7 +41,8 @@ void check(hipError_t e, const char* what) {
     if (e != hipSuccess) throw std::runtime_error(std::string(what) + ": " + hipGetErrorString(e));
 }
 
-bool is_device_pointer(const void* p) {
+// device: the GPU that the memory is on.
+bool is_device_pointer(const void* p, int* device = nullptr) {
     hipPointerAttribute_t attr;
     std::memset(&attr, 0, sizeof attr);
     hipError_t e = hipPointerGetAttributes(&attr, p);
@@ -46,7 +50,9 @@ bool is_device_pointer(const void* p) {
         (void)hipGetLastError();
         return false;
     }
-    return attr.type == hipMemoryTypeDevice || attr.type == hipMemoryTypeManaged;
+    if (attr.type != hipMemoryTypeDevice && attr.type != hipMemoryTypeManaged) return false;
+    if (device && attr.type == hipMemoryTypeDevice) *device = attr.device;
+    return true;
 }
 
 struct TensorState {
@@ -57,6 +63,7 @@ struct TensorState {
     size_t bytes = 0;
     bool staged = false;
     bool written = false;
+    int device = -1;           // GPU of a caller's device memory (-1: any)
 };
 
 // The kernels of one launch, by what they were specialized on (a few at most).
@@ -132,7 +139,12 @@ struct ptowsp_program {
     std::string precompiled_source;
     void* scratch = nullptr;  // counters and partials of decode and split-K GEMM launches
     size_t scratch_bytes = 0;
-    std::vector<void*> retired;  // launch scratch outgrown after a captured run
+    std::vector<void*> retired;  // launch scratch outgrown after a captured run, workspaces that graphs hold
+    // Workspace of operator steps.  A captured run's stays with its graph: the
+    // next run takes another.
+    void* op_scratch = nullptr;
+    size_t op_scratch_bytes = 0;
+    bool op_captured = false;
     void* gtile = nullptr;    // tile programs: tiles beyond LDS, one region per workgroup
     size_t gtile_bytes = 0;
     // Task lists of masked launches: pinned host chunks copied into device
@@ -181,6 +193,7 @@ struct ptowsp_program {
             if (c.dev) (void)hipFree(c.dev);
         }
         if (slot_stage) (void)hipHostFree(slot_stage);
+        if (op_scratch) (void)hipFree(op_scratch);
         if (gtile) (void)hipFree(gtile);
         for (void* b : stage_buf)
             if (b) (void)hipFree(b);
@@ -336,6 +349,7 @@ struct RunEnv {
     char* nscratch = nullptr;
     size_t nscratch_limit = 0;
     bool capturing = false;  // the stream is being captured into a graph
+    bool op_captured = false;  // this run has put the operators' workspace into it
     // Bytes of launch scratch that a no-allocation run of the program would
     // have: every run stays below it where it has a choice, so that both
     // entry points run the same kernels.
@@ -1942,12 +1956,102 @@ void run_items(RunEnv& E, const std::vector<PlanItem>& items, hipStream_t stream
     }
 }
 
-// A cond evaluated on the host, a slot set or a slot load
+// Workspace of the run's operator steps, which run one after the other.
+char* operator_scratch(RunEnv& E, const std::string& op, size_t need) {
+    if (E.nscratch) {
+        if (!scratch_fits(E, kScratchCounters * sizeof(int32_t) + need))
+            throw std::runtime_error("ptowsp_hip_launch_noalloc: " + op + " needs " + std::to_string(need) +
+                                     " bytes of scratch, more than the fixed scratch holds");
+        return E.nscratch + kNoAllocHeaderBytes + kScratchCounters * sizeof(int32_t);
+    }
+    ptowsp_program* P = E.P;
+    if (E.capturing) {
+        if (P->op_scratch_bytes < need || (P->op_captured && !E.op_captured))
+            throw std::runtime_error(op + ": a run is captured after a run with the same bindings, each captured one after a run of its own");
+        P->op_captured = E.op_captured = true;
+        return static_cast<char*>(P->op_scratch);
+    }
+    if (P->op_captured || P->op_scratch_bytes < need) {
+        if (P->op_scratch && P->op_captured) {
+            P->retired.push_back(P->op_scratch);
+        } else if (P->op_scratch) {
+            check(hipDeviceSynchronize(), "hipDeviceSynchronize");  // earlier steps of this run may use it
+            check(hipFree(P->op_scratch), "hipFree(operator scratch)");
+        }
+        need = std::max(need, P->op_scratch_bytes);
+        P->op_scratch = nullptr;
+        P->op_scratch_bytes = 0;
+        P->op_captured = false;
+        if (hipMalloc(&P->op_scratch, need) != hipSuccess) {
+            (void)hipGetLastError();
+            ptowsp_program::drain_pool();
+            check(hipMalloc(&P->op_scratch, need), "hipMalloc(operator scratch)");
+        }
+        P->op_scratch_bytes = need;
+    }
+    return static_cast<char*>(P->op_scratch);
+}
+
+// An operator step (operators.hpp): its operands as the host loops' variables
+// place them.
+void enqueue_operator(RunEnv& E, const Node& n, hipStream_t stream, uint64_t& launches) {
+    std::vector<Operand> operands(n.tensor_args.size());
+    int dev = 0;
+    check(hipGetDevice(&dev), "hipGetDevice");
+    for (size_t i = 0; i < operands.size(); ++i) {
+        const TensorArg& t = n.tensor_args[i];
+        const TensorState& T = E.ts[t.tid];
+        const TensorInfo& ti = E.P->m.tensors[t.tid];
+        Operand& o = operands[i];
+        int64_t off = 0;
+        for (size_t d = 0; d < t.idx.size(); ++d) {
+            const int64_t v = eval_index_host(E, t.idx[d], {});
+            if (v < 0 || v >= ti.shape[d])
+                throw std::runtime_error(n.op + ": index " + std::to_string(v) + " of " + t.param + " is outside its tensor");
+            off += v * T.stride[d];
+        }
+        if (T.device >= 0 && T.device != dev)
+            throw std::runtime_error(n.op + ": " + t.param + " is on GPU " + std::to_string(T.device) + ", the current one is " + std::to_string(dev));
+        o.dtype = ti.dtype;
+        o.shape.assign(ti.shape.begin() + static_cast<std::ptrdiff_t>(t.idx.size()), ti.shape.end());
+        o.stride.assign(T.stride.begin() + static_cast<std::ptrdiff_t>(t.idx.size()), T.stride.end());
+        o.ptr = T.dev ? T.dev + off * dtype_size(ti.dtype) : nullptr;
+    }
+    OperatorRun run;
+    static std::atomic<int> cus[64] = {};
+    if (dev < 0 || dev >= 64) throw std::runtime_error(n.op + ": device index out of range");
+    if (!(run.cus = cus[dev].load(std::memory_order_relaxed))) {
+        check(hipDeviceGetAttribute(&run.cus, hipDeviceAttributeMultiprocessorCount, dev), "hipDeviceGetAttribute");
+        cus[dev].store(run.cus, std::memory_order_relaxed);
+    }
+    run.err = E.err ? E.err : E.P->d_err;
+    run.scratch = [&](size_t need) { return operator_scratch(E, n.op, need); };
+    run.launch = [&](const std::string& source, const char* entry, int64_t blocks, int threads, const void* args, size_t bytes) {
+        const JitKernel* jk = E.nscratch ? jit_loaded(source, entry) : &jit_kernel(source, entry);
+        if (!jk) throw std::runtime_error("ptowsp_hip_launch_noalloc: a kernel of " + n.op + " has not been loaded by an ordinary launch");
+        union {
+            LaunchArgs launch;
+            char raw[sizeof(LaunchArgs)];
+        } buffer;
+        static_assert(sizeof(AttendArgs) <= sizeof(LaunchArgs) && sizeof(StoreArgs) <= sizeof(LaunchArgs) && sizeof(PlanArgs) <= sizeof(LaunchArgs));
+        std::memcpy(buffer.raw, args, bytes);
+        void* params[] = {buffer.raw};
+        launch_kernel(E, jk->function, blocks, threads, 0, stream, params, entry);
+        launches += 1;
+    };
+    run_operator(n, operands, run);
+}
+
+// A cond evaluated on the host, a slot set, a slot load or an operator
 // (src/python/pto_codegen.cpp:2248-2303, 2458-2478).
 void run_host_step(RunEnv& E, const PlanItem& it, hipStream_t stream, uint64_t& launches) {
     const Node& n = *it.ctl;
     if (n.kind == NodeKind::Cond) {
         run_items(E, eval_truth(*n.pred, host_env(E, E.host_vars)) ? it.body : it.alt, stream, launches);
+        return;
+    }
+    if (n.kind == NodeKind::Operator) {
+        enqueue_operator(E, n, stream, launches);
         return;
     }
     uint64_t v = n.value;
@@ -2005,7 +2109,7 @@ void resolve_tensors(RunEnv& E, hipStream_t stream) {
         T.written = P->tensor_written[t];
         if (span == 0) continue;
         if (!ptr) throw std::runtime_error("tensor " + std::to_string(t) + " has no data");
-        if (is_device_pointer(ptr)) {
+        if (is_device_pointer(ptr, &T.device)) {
             T.dev = ptr;
             continue;
         }
@@ -2350,6 +2454,19 @@ int launch_impl(ptowsp_program* P, RuntimeContext* ctx, void* hip_stream, ptowsp
     return 0;
 }
 
+// Operator steps of the workload, in program order.
+std::vector<const Node*> operator_nodes(const Module& m) {
+    std::vector<const Node*> out;
+    std::function<void(const Node*)> walk = [&](const Node* n) {
+        if (!n) return;
+        if (n->kind == NodeKind::Operator) out.push_back(n);
+        walk(n->body.get());
+        for (const auto& c : n->kids) walk(c.get());
+    };
+    walk(m.root.get());
+    return out;
+}
+
 int fail(const std::exception& e) {
     g_last_error = e.what();
     return -1;
@@ -2376,6 +2493,11 @@ int ptowsp_hip_compile(const char* module_text, ptowsp_program** out) {
             const KernelAnalysis& a = P->ka[L.kernel];
             for (size_t p = 0; p < L.targs.size(); ++p)
                 if (a.stored[p]) P->tensor_written[L.targs[p]->tid] = true;
+        }
+        for (const Node* n : operator_nodes(P->m)) {
+            check_operator(P->m, *n);
+            for (size_t i = 0; i < n->tensor_args.size(); ++i)
+                if (operator_writes(*n, i)) P->tensor_written[n->tensor_args[i].tid] = true;
         }
         *out = P.release();
         return 0;
@@ -2484,6 +2606,12 @@ int ptowsp_hip_precompile(ptowsp_program* P, int index, int flags, const char** 
             (void)jit_compile(ek.source);
             if (static_cast<int>(li) == index) P->precompiled_source = ek.source;
         }
+        size_t at = P->plan.launches.size();  // operator steps come after the launches
+        for (const Node* n : operator_nodes(P->m))
+            for (const auto& [text, entry] : operator_sources(P->m, *n)) {
+                (void)jit_compile(text);
+                if (static_cast<int>(at++) == index) P->precompiled_source = text;
+            }
         if (source) *source = P->precompiled_source.c_str();
         return 0;
     } catch (const std::exception& e) {
@@ -2585,6 +2713,7 @@ int ptowsp_hip_synchronize(ptowsp_program* P, ptowsp_timing* timing) {
             if (!P->noalloc_run) __atomic_store_n(P->h_err, 0, __ATOMIC_RELAXED);
             throw std::runtime_error(err == 1   ? "an indirect tensor index was out of range (tasks skipped)"
                                      : err == 3 ? "a loop extent read from a tensor exceeded its declared maximum"
+                                     : operator_error(err) ? operator_error(err)
                                                 : "a task's tile fell outside its tensor (tasks skipped)");
         }
         if (timing) *timing = ptowsp_timing{static_cast<double>(dev_ms), P->h2d_ms, d2h};

@@ -52,6 +52,7 @@ from pto_wsp.primitives import (
     slot_set_u64,
     slot_load_u64,
 )
+from pto_wsp.paged import paged_plan, paged_store, paged_attention
 from pto_wsp import scalar_expr
 from pto_wsp.ptoisa_jit import ptoisa, ptoisa_kernel
 
@@ -70,5 +71,5 @@ __all__ = [
     "KernelParam", "extract_kernel_params", "get_direction", "get_inner_type",
     "CompileError", "ExecutionError", "IRBridgeError", "PtoError",
     "parallel_for", "for_each", "select", "cond", "task", "combine", "sequential", "slot_set_u64", "slot_load_u64",
-    "scalar_expr",
+    "paged_plan", "paged_store", "paged_attention", "scalar_expr",
 ]

@@ -19,8 +19,9 @@ INCLUDE = os.path.join(os.path.dirname(ROOT), "include")
 BUILD_DIR = os.path.join(CSRC, "_build")
 LIB_PATH = os.path.join(PKG_DIR, "libptowsp_hip.so")
 
-HOST_SOURCES = ["module.cpp", "scalar.cpp", "analysis.cpp", "plan.cpp", "emit.cpp", "jit.cpp", "runtime.cpp", "noalloc.hip"]
-DEVICE_HEADERS = [("kDeviceHeader", "ptowsp_device.h"), ("kLaunchHeader", "ptowsp_launch.h")]
+HOST_SOURCES = ["module.cpp", "scalar.cpp", "analysis.cpp", "plan.cpp", "emit.cpp", "jit.cpp", "operators.cpp", "runtime.cpp", "noalloc.hip"]
+DEVICE_HEADERS = [("kDeviceHeader", "ptowsp_device.h"), ("kLaunchHeader", "ptowsp_launch.h"), ("kPagedHeader", "ptowsp_paged.h"),
+                  ("kPagedArgsHeader", "ptowsp_paged_args.h")]
 DELIM = "PTOWSP_HDR"
 
 
@@ -60,6 +61,24 @@ def build(verbose: bool = False) -> str:
         print(res.stdout + res.stderr, file=sys.stderr)
     os.replace(tmp, LIB_PATH)
     return LIB_PATH
+
+
+def _operator_workloads():
+    """The paged operators, in types and shapes that between them reach every variant."""
+    from pto_wsp import DType, Tensor, paged_attention, paged_plan, paged_store
+
+    def T(dtype, *shape):
+        return Tensor(data=None, shape=shape, dtype=dtype)
+
+    i32, f32 = DType.I32, DType.F32
+    yield paged_plan(lengths=T(i32, 4), counts=T(i32, 4), page_table=T(i32, 4, 8), free_pages=T(i32, 9), used=T(i32, 1),
+                     new_lengths=T(i32, 4), new_used=T(i32, 1), starts=T(i32, 5), slots=T(i32, 7), page_size=16)
+    for code, dt, heads, group, dim, page, rows, window in (
+            (DType.F8E4M3, DType.BF16, 8, 4, 128, 16, 4, 0), (DType.I8, DType.F16, 2, 7, 80, 8, 64, 9), (DType.I8, f32, 1, 40, 256, 64, 4, 0)):
+        cache = {x + "_cache": T(code, 6, heads, page, dim) for x in "kv"} | {x + "_scale": T(f32, 6, heads) for x in "kv"}
+        yield paged_store(k=T(dt, rows, heads, dim), v=T(dt, rows, heads, dim), slots=T(i32, rows), **cache)
+        yield paged_attention(q=T(dt, rows, heads * group, dim), out=T(dt, rows, heads * group, dim), page_table=T(i32, 4, 3),
+                              lengths=T(i32, 4), starts=T(i32, 5), window=window, lse=T(f32, rows, heads * group) if window else None, **cache)
 
 
 def check_device_templates() -> None:
@@ -132,6 +151,9 @@ def check_device_templates() -> None:
                 topk8[i, t](scores=sc[i][t], out_idx=ti[i][t])
 
     from pto_wsp.ir_bridge import workload_to_codegen_ir
+
+    for w in _operator_workloads():
+        NativeProgram(workload_to_codegen_ir(w, "operator_check").module).precompile(0)
 
     prog = NativeProgram(workload_to_codegen_ir(wl(), "template_check").module)
     for i in range(prog.num_launches()):

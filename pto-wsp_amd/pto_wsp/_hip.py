@@ -80,6 +80,7 @@ _NUMPY_DTYPES = {
     DType.F32: np.float32, DType.F16: np.float16, DType.BF16: np.uint16, DType.F64: np.float64,
     DType.I8: np.int8, DType.I16: np.int16, DType.I32: np.int32, DType.I64: np.int64,
     DType.U8: np.uint8, DType.U16: np.uint16, DType.U32: np.uint32, DType.U64: np.uint64,
+    DType.F8E4M3: np.uint8,  # bit patterns
 }
 
 
@@ -88,7 +89,7 @@ def _torch_dtypes():
         return {}
     return {DType.F32: torch.float32, DType.F16: torch.float16, DType.BF16: torch.bfloat16,
             DType.F64: torch.float64, DType.I8: torch.int8, DType.I16: torch.int16, DType.I32: torch.int32,
-            DType.I64: torch.int64, DType.U8: torch.uint8}
+            DType.I64: torch.int64, DType.U8: torch.uint8, DType.F8E4M3: torch.float8_e4m3fn}
 
 
 def _error() -> str:

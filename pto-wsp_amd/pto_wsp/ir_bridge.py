@@ -115,6 +115,9 @@ class _Collector:
             self.collect(self.body(node))
         elif kind == "slot_load_u64":
             self._register(kw.get("tensor"))
+        elif kind == "operator":
+            for t in kw.get("tensors", {}).values():
+                self._register(t)
 
     def _register(self, t: Any) -> None:
         if not isinstance(t, Tensor):
@@ -204,6 +207,11 @@ class _Writer:
             return f"c {int(v) & 0xFFFFFFFFFFFFFFFF}"
         raise IRBridgeError(f"Unsupported scalar dtype for codegen args: {dtype!r}")
 
+    def tensor_arg(self, name: str, t: Tensor) -> str:
+        tid = self.c.tensor_ids[id(t.base)]
+        idx = [self.index_expr(e) for e in t.index_exprs]
+        return f"{enc(name)} {tid} {len(t.base.shape)} {len(t.shape)} {len(idx)} {' '.join(idx)}".rstrip()
+
     # -- workload tree ----------------------------------------------------
     def node(self, w: Any) -> None:
         if not isinstance(w, Workload):
@@ -247,6 +255,12 @@ class _Writer:
             idx = [self.index_expr(e) for e in t.index_exprs]
             self.emit("slotld", int(kw.get("slot", 0)) & 0xFFFFFFFF, tid, len(t.base.shape), len(t.shape), len(idx),
                       *idx, int(kw.get("row", 0)), int(kw.get("col", 0)))
+        elif kind == "operator":
+            tensors, attrs = kw.get("tensors", {}), kw.get("attrs", {})
+            self.emit("oper", enc(str(kw.get("op"))), len(tensors))
+            for name, t in tensors.items():
+                self.emit(" ", self.tensor_arg(name, t))
+            self.emit(" ", len(attrs), *self.attrs(attrs))
         else:
             raise IRBridgeError(f"workload node kind '{kind}' is not supported by codegen")
 
@@ -276,10 +290,7 @@ class _Writer:
             t = resources.get(pname)
             if not isinstance(t, Tensor):
                 raise IRBridgeError(f"Missing tensor arg for param '{pname}' in task {kernel.name}")
-            tid = self.c.tensor_ids[id(t.base)]
-            idx = [self.index_expr(e) for e in t.index_exprs]
-            tensor_args.append(
-                f"{enc(pname)} {tid} {len(t.base.shape)} {len(t.shape)} {len(idx)} {' '.join(idx)}".rstrip())
+            tensor_args.append(self.tensor_arg(pname, t))
         self.emit("task", enc(kernel.name), len(axis_args), *axis_args, len(scalar_args), *scalar_args,
                   len(tensor_args))
         for ta in tensor_args:

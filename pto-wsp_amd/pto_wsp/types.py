@@ -160,12 +160,15 @@ class DType(Enum):
     U16 = "u16"
     U32 = "u32"
     U64 = "u64"
+    # OCP e4m3 (4 exponent, 3 mantissa bits, no infinities): caches of the paged operators.
+    F8E4M3 = "f8e4m3"
 
 
 DTYPE_NBYTES = {
     DType.F16: 2, DType.BF16: 2, DType.F32: 4, DType.F64: 8,
     DType.I8: 1, DType.I16: 2, DType.I32: 4, DType.I64: 8,
     DType.U8: 1, DType.U16: 2, DType.U32: 4, DType.U64: 8,
+    DType.F8E4M3: 1,
 }
 
 

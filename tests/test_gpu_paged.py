@@ -1,0 +1,671 @@
+"""GPU tests of the operators over an 8-bit paged cache, against plain forms in 64 bits (paged_ref).
+
+Plans and codes are whole numbers and equal theirs; scales are float32 values and equal theirs.
+Attention: with w the softmax's weights, an output is off by at most
+
+    half * |out| + sum(w |v|) * (2 ds + dp + (n / 128 + 64 + D) 2^-24),
+
+its own rounding (half a step: bf16 2^-8, f16 2^-11, f32 2^-24); the scores' error ds = (D + 8) 2^-24
+max(sum |q k|) scale, a float32 dot product's and that of its two products, exponent and exp2, which moves
+numerator and denominator; p's parts (two bf16: 2^-18, three: 2^-24); the float32 sums over steps of 128
+tokens, the 32 inside an MFMA and the joins."""
+
+import numpy as np
+import pytest
+
+import paged_ref as R
+from pto_wsp import (CompileError, Dense, DType, ExecutionError, P, Tensor, paged_attention, paged_plan, paged_store, sequential,
+                     workload)
+
+pytestmark = pytest.mark.gpu
+
+HALF = {"bf16": 2.0 ** -8, "f16": 2.0 ** -11, "f32": 2.0 ** -24}
+PARTS = {"bf16": 2.0 ** -18, "f16": 2.0 ** -18, "f32": 2.0 ** -24}
+
+
+def _torch():
+    import torch
+
+    return torch
+
+
+def _dt(name):
+    torch = _torch()
+    return {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}[name]
+
+
+def T(x):
+    torch = _torch()
+    kinds = {torch.float32: DType.F32, torch.float16: DType.F16, torch.bfloat16: DType.BF16, torch.int32: DType.I32,
+             torch.int8: DType.I8, torch.float8_e4m3fn: DType.F8E4M3}
+    return Tensor(data=x, shape=tuple(x.shape), dtype=kinds[x.dtype])
+
+
+def ints(gpu, x):
+    return _torch().tensor(np.asarray(x), dtype=_torch().int32, device=gpu)
+
+
+def go(w):
+    p = w.compile(target="hip_gfx950")
+    p.execute()
+    p.synchronize()
+    return p
+
+
+def codes_on(gpu, codes, kind):
+    torch = _torch()
+    t = torch.from_numpy(codes.view(np.int8).copy()).to(gpu)
+    return t if kind == "i8" else t.view(torch.float8_e4m3fn)
+
+
+def codes_of(t, kind):
+    torch = _torch()
+    c = t.view(torch.int8).cpu().numpy()
+    return c if kind == "i8" else c.view(np.uint8)
+
+
+def same_codes(a, b, kind):
+    if kind == "i8":
+        return np.array_equal(a, b)
+    nan = (a & 0x7F) == 0x7F
+    return np.array_equal(nan, (b & 0x7F) == 0x7F) and np.array_equal(a[~nan], b[~nan])
+
+
+# ------------------------------------------------------------------------------ plan
+def _plan_case(rng, batch, cmax, lmax, page, spare_rows=3):
+    lengths, counts = rng.integers(0, lmax + 1, batch), rng.integers(0, cmax + 1, batch)
+    held = -(-lengths // page)
+    width = int((-(-(lengths + counts) // page)).max(initial=1)) + 1
+    need = int((-(-(lengths + counts) // page) - held).sum())
+    order = rng.permutation(int(held.sum()) + need + 5)
+    table = np.full((batch, width), -7)
+    table[np.arange(width)[None] < held[:, None]] = order[:int(held.sum())]
+    return lengths, counts, table, order[int(held.sum()):], int(counts.sum()) + spare_rows
+
+
+def _plan_tensors(gpu, lengths, counts, table, free, used, rows):
+    torch = _torch()
+    t = {"lengths": ints(gpu, lengths), "counts": ints(gpu, counts), "page_table": ints(gpu, table), "free_pages": ints(gpu, free),
+         "used": ints(gpu, [used]), "new_lengths": ints(gpu, np.full(len(lengths), -9)), "new_used": ints(gpu, [-9]),
+         "starts": ints(gpu, np.full(len(lengths) + 1, -9)), "slots": torch.full((rows,), -9, dtype=torch.int32, device=gpu)}
+    return t
+
+
+# One workgroup; several requests a thread; two launches by rows and by requests; empty batches.
+@pytest.mark.parametrize("batch,cmax,lmax,page", [(1, 1, 0, 16), (1, 0, 5, 16), (3, 40, 33, 16), (64, 1, 500, 16), (100, 7, 50, 1), (37, 90, 64, 24),
+                                                  (1500, 3, 9, 8), (5, 9000, 100, 64), (4500, 2, 40, 16), (2, 20000, 3, 4096), (0, 1, 1, 16)])
+def test_plan(gpu, batch, cmax, lmax, page):
+    rng = np.random.default_rng(batch * 7 + page)
+    lengths, counts, table, free, rows = _plan_case(rng, batch, cmax, lmax, page)
+    used = 2 if len(free) > 2 else 0
+    free = np.concatenate([[-1] * used, free]).astype(np.int64)
+    t = _plan_tensors(gpu, lengths, counts, table, free, used, rows)
+    go(paged_plan(**{k: T(x) for k, x in t.items()}, page_size=page))
+    want = R.plan(lengths, counts, table, free, used, page, rows)
+    for k, x in want.items():
+        assert np.array_equal(t[k].cpu().numpy(), x), k
+
+
+@pytest.mark.parametrize("batch", [9, 5000])
+def test_plan_in_place_and_strided(gpu, batch):
+    torch = _torch()
+    rng = np.random.default_rng(batch)
+    lengths, counts, table, free, rows = _plan_case(rng, batch, 3, 40, 8)
+    t = _plan_tensors(gpu, lengths, counts, table, free, 0, rows)
+    wide = torch.full((rows, 3), 5, dtype=torch.int32, device=gpu)
+    t["slots"] = wide[:, 1]
+    t["page_table"] = torch.full((t["page_table"].shape[1], batch), 3, dtype=torch.int32, device=gpu).t().copy_(t["page_table"])
+    w = {k: T(x) for k, x in t.items()}
+    w["new_lengths"], w["new_used"] = w["lengths"], w["used"]
+    prog = go(paged_plan(**w, page_size=8))
+    want = R.plan(lengths, counts, table, free, 0, 8, rows)
+    got = dict(t, new_lengths=t["lengths"], new_used=t["used"])
+    for k, x in want.items():
+        assert np.array_equal(got[k].cpu().numpy(), x), k
+    assert bool((wide[:, 0] == 5).all()) and bool((wide[:, 2] == 5).all())
+    # The next step of the same requests, the lengths where the first one left them.
+    counts2 = np.minimum(counts, 1)
+    t["counts"].copy_(ints(gpu, counts2))
+    left = len(free) - int(want["new_used"][0])
+    if (-(-(want["new_lengths"] + counts2) // 8) - -(-want["new_lengths"] // 8)).sum() <= left and \
+            (want["new_lengths"] + counts2).max() <= 8 * table.shape[1]:
+        prog.execute()
+        prog.synchronize()
+        again = R.plan(want["new_lengths"], counts2, want["page_table"], free, int(want["new_used"][0]), 8, rows)
+        for k, x in again.items():
+            assert np.array_equal(got[k].cpu().numpy(), x), k
+
+
+@pytest.mark.parametrize("batch", [6, 4800])
+@pytest.mark.parametrize("what", ["length", "count", "width", "free", "rows", "used"])
+def test_plan_that_does_not_fit_writes_nothing(gpu, batch, what):
+    rng = np.random.default_rng(3)
+    lengths, counts, table, free, rows = _plan_case(rng, batch, 9, 30, 8)
+    counts[0] = 9
+    rows += 9
+    used = 0
+    if what == "length":
+        lengths[batch - 1] = -1
+    elif what == "count":
+        counts[batch // 2] = -5
+    elif what == "width":
+        lengths[batch // 2] = 8 * table.shape[1]
+        counts[batch // 2] = 1
+        rows += 1
+    elif what == "free":
+        used = len(free)
+        lengths[0], counts[0] = 0, 9
+    elif what == "rows":
+        rows = int(counts.sum()) - 1
+    else:
+        used = -1
+    t = _plan_tensors(gpu, lengths, counts, table, free, used, rows)
+    before = {k: x.clone() for k, x in t.items()}
+    prog = paged_plan(**{k: T(x) for k, x in t.items()}, page_size=8).compile(target="hip_gfx950")
+    prog.execute()
+    with pytest.raises(ExecutionError, match="nothing was written"):
+        prog.synchronize()
+    for k, x in t.items():
+        assert bool((x == before[k]).all()), k
+
+
+# ------------------------------------------------------------------------------ store
+def _store_case(rng, kind, H, D, page, pieces, pages):
+    """pieces: (first offset, tokens) of requests, each over pages of its own; then a few rows left out."""
+    order, slots, at = rng.permutation(pages), [], 0
+    for first, n in pieces:
+        need = -(-(first + n) // page)
+        own = order[at:at + need]
+        at += need
+        pos = first + np.arange(n)
+        slots += list(own[pos // page] * page + pos % page)
+    slots = np.array(slots + [-1, -5])
+    codes = {}
+    for x in "kv":
+        codes[x] = rng.integers(-127, 128, (pages, H, page, D)).astype(np.int8)
+        if kind == "e4m3":
+            codes[x] = codes[x].view(np.uint8)
+            codes[x][(codes[x] & 0x7F) == 0x7F] = 0
+    scale = {x: (0.01 * np.exp(rng.standard_normal((pages, H)))).astype(np.float32) for x in "kv"}
+    return slots, codes, scale
+
+
+def _check_store(gpu, dt, kind, x, slots, codes, scale, layout="plain"):
+    torch = _torch()
+    t = {}
+    for n in "kv":
+        if layout == "plain":
+            t[n] = torch.from_numpy(x[n]).to(gpu).to(_dt(dt))
+            c = codes_on(gpu, codes[n], kind)
+            s = torch.from_numpy(scale[n]).to(gpu)
+        t[n + "_cache"], t[n + "_scale"] = (c, s) if layout == "plain" else (None, None)
+    if layout == "fused":
+        # One tensor of keys and values by token, one of [k | v] rows, one of scales by head.
+        Tn, H, D = x["k"].shape
+        pages, _, page, _ = codes["k"].shape
+        pool = torch.zeros((pages, page, 2, H, D), dtype=torch.int8, device=gpu)
+        rows = torch.zeros((Tn, 2 * H + 1, D + 3), dtype=_dt(dt), device=gpu)
+        sc = torch.zeros((2, H, pages), dtype=torch.float32, device=gpu)
+        for i, n in enumerate("kv"):
+            c = pool[:, :, i].permute(0, 2, 1, 3)
+            c.copy_(codes_on(gpu, codes[n], "i8"))
+            t[n + "_cache"] = c if kind == "i8" else c.view(torch.float8_e4m3fn)
+            t[n + "_scale"] = sc[i].t()
+            t[n + "_scale"].copy_(torch.from_numpy(scale[n]))
+            t[n] = rows[:, i * H:(i + 1) * H, 1:D + 1]
+            t[n].copy_(torch.from_numpy(x[n]))
+    t["slots"] = ints(gpu, slots)
+    go(paged_store(**{k: T(v) for k, v in t.items()}))
+    for n in "kv":
+        want_codes, want_scale = R.store(t[n].cpu().to(torch.float64).numpy(), slots, codes[n], scale[n], kind)
+        assert np.array_equal(t[n + "_scale"].cpu().numpy(), want_scale), n
+        assert same_codes(codes_of(t[n + "_cache"].contiguous(), kind), want_codes, kind), n
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "i8"])
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("H,D,page,pieces", [(1, 16, 16, [(0, 1)]), (2, 128, 16, [(5, 1), (15, 1), (0, 1), (3, 40)]),
+                                             (3, 80, 24, [(23, 2), (7, 100), (1, 5)]), (2, 256, 1, [(0, 9)]), (1, 64, 128, [(100, 300), (0, 128)])])
+def test_store(gpu, dt, kind, H, D, page, pieces):
+    rng = np.random.default_rng(H * 1000 + D + page)
+    slots, codes, scale = _store_case(rng, kind, H, D, page, pieces, sum(-(-(a + n) // page) for a, n in pieces) + 2)
+    x = {n: (rng.standard_normal((len(slots), H, D)) * np.exp(rng.standard_normal((1, H, 1)))).astype(np.float32) for n in "kv"}
+    _check_store(gpu, dt, kind, x, slots, codes, scale)
+
+
+def test_store_many_rows(gpu):
+    """Enough rows that a wave takes a page's worth of them."""
+    rng = np.random.default_rng(5)
+    pieces = [(int(a), int(n)) for a, n in zip(rng.integers(0, 16, 40), rng.integers(1, 120, 40))]
+    slots, codes, scale = _store_case(rng, "e4m3", 8, 64, 16, pieces, sum(-(-(a + n) // 16) for a, n in pieces) + 2)
+    assert len(slots) * 8 * 2 > 16384
+    x = {n: rng.standard_normal((len(slots), 8, 64)).astype(np.float32) for n in "kv"}
+    _check_store(gpu, "bf16", "e4m3", x, slots, codes, scale)
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "i8"])
+def test_store_strided(gpu, kind):
+    rng = np.random.default_rng(6)
+    slots, codes, scale = _store_case(rng, kind, 3, 48, 16, [(4, 30), (0, 2)], 6)
+    x = {n: rng.standard_normal((len(slots), 3, 48)).astype(np.float32) for n in "kv"}
+    _check_store(gpu, "f32", kind, x, slots, codes, scale, "fused")
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "i8"])
+def test_store_odd_rows(gpu, kind):
+    """Rows out of order, the same slot twice (the later row stays), gaps, numbers at the ends of the range."""
+    rng = np.random.default_rng(7)
+    _, codes, scale = _store_case(rng, kind, 2, 32, 16, [(0, 16)] * 6, 8)
+    slots = np.array([5, 5, -1, 16 + 9, 16 + 7, 16 + 9, 16 + 8, 32, 33, 35, 48 + 15, 64 + 3, -1, 80, 96 + 2, 112])
+    x = {n: rng.standard_normal((len(slots), 2, 32)).astype(np.float32) for n in "kv"}
+    x["k"][7:10] = 0.0                      # a fresh page of zeros
+    x["k"][10] = 0.0                        # zeros into a page that keeps tokens
+    x["k"][11, 0, :4] = [np.inf, -np.inf, np.nan, 1.0]
+    x["v"][13, :, 0] = 3.0e38               # the largest numbers, and ones far below the smallest scale
+    x["v"][14] *= np.float32(1e-44)
+    x["v"][15] = np.nan
+    _check_store(gpu, "f32", kind, x, slots, codes, scale)
+
+
+def test_store_slots_outside_the_cache(gpu):
+    torch = _torch()
+    rng = np.random.default_rng(8)
+    slots, codes, scale = _store_case(rng, "i8", 2, 32, 16, [(0, 20)], 4)
+    bad = slots.copy()
+    bad[3], bad[19] = 4 * 16, 2 ** 31 - 1
+    x = rng.standard_normal((len(slots), 2, 32)).astype(np.float32)
+    t = {"slots": ints(gpu, bad)}
+    for n in "kv":
+        t[n], t[n + "_cache"], t[n + "_scale"] = torch.from_numpy(x).to(gpu), codes_on(gpu, codes[n], "i8"), torch.from_numpy(scale[n]).to(gpu)
+    prog = paged_store(**{k: T(v) for k, v in t.items()}).compile(target="hip_gfx950")
+    prog.execute()
+    with pytest.raises(ExecutionError, match="outside the cache"):
+        prog.synchronize()
+
+
+# ------------------------------------------------------------------------------ attention
+def _attend_case(rng, dt, kind, H, G, D, page, lengths, counts, spare_rows=2, poison=True):
+    """Inputs as numpy arrays; what no row may see is filled with NaN codes and scales, or large ones."""
+    torch = _torch()
+    lengths, counts = np.asarray(lengths), np.asarray(counts)
+    need = -(-lengths // page)
+    pages = int(need.sum()) + 3
+    order = rng.permutation(pages)
+    table = np.zeros((len(lengths), max(1, int(need.max(initial=0)) + 1)), np.int64)
+    at, codes, scale = 0, {}, {}
+    for x in "kv":
+        raw = rng.standard_normal((pages, H, page, D)) * 40
+        codes[x] = R.encode(raw, kind)
+        scale[x] = (0.03 * np.exp(0.5 * rng.standard_normal((pages, H)))).astype(np.float32)
+    live = np.zeros((pages, page), bool)
+    for b, n in enumerate(need):
+        table[b, :n] = order[at:at + n]
+        live[order[at:at + n]] = (np.arange(n * page) < lengths[b]).reshape(n, page)
+        at += n
+        if poison and n < table.shape[1]:
+            table[b, n:] = 10 ** 6  # never looked up
+    if poison:
+        for x in "kv":
+            codes[x] = np.where(live[:, None, :, None], codes[x], 0x7F).astype(codes[x].dtype)
+            scale[x] = np.where(live.any(1)[:, None], scale[x], np.nan).astype(np.float32)
+    starts = np.concatenate([[0], np.cumsum(counts)])
+    rows = int(starts[-1]) + spare_rows
+    q = torch.from_numpy(rng.standard_normal((rows, H * G, D)).astype(np.float32)).to(_dt(dt))
+    return {"q": q, "codes": codes, "scale": scale, "table": table, "lengths": lengths, "starts": starts, "kind": kind, "dt": dt}
+
+
+def _attend_tensors(gpu, c, layout="plain"):
+    torch = _torch()
+    t = {"q": c["q"].to(gpu), "page_table": ints(gpu, c["table"]), "lengths": ints(gpu, c["lengths"]), "starts": ints(gpu, c["starts"])}
+    for x in "kv":
+        t[x + "_cache"], t[x + "_scale"] = codes_on(gpu, c["codes"][x], c["kind"]), torch.from_numpy(c["scale"][x]).to(gpu)
+    t["out"] = torch.full_like(t["q"], 7.0)
+    t["lse"] = torch.full(t["q"].shape[:2], 7.0, device=gpu)
+    if layout == "fused":
+        P_, H, page, D = t["k_cache"].shape
+        pool = torch.zeros((P_, page, 2, H, D), dtype=torch.int8, device=gpu)
+        for i, x in enumerate("kv"):
+            y = pool[:, :, i].permute(0, 2, 1, 3)
+            y.copy_(t[x + "_cache"].view(torch.int8))
+            t[x + "_cache"] = y if c["kind"] == "i8" else y.view(torch.float8_e4m3fn)
+            t[x + "_scale"] = t[x + "_scale"].t().contiguous().t()
+        rows, HQ, _ = t["q"].shape
+        q = torch.zeros((rows, HQ + 1, D + 1), dtype=t["q"].dtype, device=gpu)[:, 1:, 1:]
+        t["q"] = q.copy_(t["q"])
+        t["out"] = torch.full((HQ, rows, 2 * D), 7.0, dtype=q.dtype, device=gpu)[:, :, :D].permute(1, 0, 2)
+        t["lse"] = torch.full((HQ, rows), 7.0, device=gpu).t()
+        wide = torch.full((t["page_table"].shape[0], t["page_table"].shape[1] + 3), -1, dtype=torch.int32, device=gpu)
+        wide[:, 1:-2] = t["page_table"]
+        t["page_table"] = wide[:, 1:-2]
+    return t
+
+
+def _tolerances(c, ref, window=0, scale=None):
+    out, lse, spread, swing = ref
+    D, n = out.shape[-1], int(max(c["lengths"].max(initial=0), 1))
+    ds = (D + 8) * 2.0 ** -24 * np.maximum(swing, 1.0)
+    sums = (n / 128 + 64 + D) * 2.0 ** -24
+    tol = HALF[c["dt"]] * np.abs(out) + spread * (2 * ds[..., None] + PARTS[c["dt"]] + sums)
+    tol = tol * (1 + 2 * HALF[c["dt"]]) + (2.0 ** -25 if c["dt"] == "f16" else 2.0 ** -140)
+    return tol, 2 * ds + sums + 2.0 ** -23 * np.abs(np.where(np.isfinite(lse), lse, 0.0))
+
+
+def _reference(c, scale, window):
+    k, v = (R.decode(c["codes"][x], c["kind"]) for x in "kv")
+    return R.attend(c["q"].double().numpy(), k, v, c["scale"]["k"].astype(np.float64), c["scale"]["v"].astype(np.float64), c["table"], c["lengths"],
+                    c["starts"], scale, window)
+
+
+def _check_attend(c, t, ref, lse=True):
+    n = int(c["starts"][-1])
+    out, got = ref[0][:n], t["out"].double().cpu().numpy()
+    tol, ltol = _tolerances(c, tuple(x[:n] for x in ref))
+    assert np.array_equal(np.isnan(got[:n]), np.isnan(out))
+    off = np.abs(got[:n] - out)
+    assert (np.isnan(out) | (off <= tol)).all(), f"off by {np.nanmax(off / tol):.3g} of the tolerance"
+    assert (got[n:] == 7.0).all()
+    if lse:
+        a, b = t["lse"].double().cpu().numpy(), ref[1][:n]
+        assert np.array_equal(np.isinf(a[:n]), np.isinf(b))
+        fine = np.isfinite(b)
+        assert (np.abs(a[:n] - b)[fine] <= ltol[fine]).all()
+        assert (a[n:] == 7.0).all()
+
+
+def _attend(gpu, c, window=0, scale=None, layout="plain", lse=True):
+    D = c["q"].shape[-1]
+    t = _attend_tensors(gpu, c, layout)
+    w = {k: T(x) for k, x in t.items() if lse or k != "lse"}
+    prog = go(paged_attention(**w, window=window, scale=scale))
+    ref = _reference(c, scale if scale is not None else 1.0 / np.sqrt(D), window)
+    _check_attend(c, t, ref, lse)
+    return prog, t, ref
+
+
+SHAPES = [
+    # H, G, D, page, lengths, counts: single tokens; lengths of one, of a step less one, of several tiles
+    (1, 1, 64, 16, [1], [1]),
+    (2, 4, 128, 16, [1, 31, 33, 127, 129, 700], [1] * 6),
+    (2, 7, 80, 8, [5, 260, 17], [1, 1, 1]),
+    (1, 16, 256, 64, [300, 64], [1, 1]),
+    (1, 40, 64, 32, [130, 3], [1, 1]),
+    (3, 2, 16, 1, [40, 9], [1, 1]),
+    (2, 5, 96, 24, [100, 47], [1, 1]),
+    # several new tokens, prompts, idle requests, a request without tokens
+    (2, 4, 128, 16, [9, 200, 0, 64], [9, 5, 0, 64]),
+    (1, 8, 64, 16, [150, 40, 500], [150, 0, 33]),
+    (2, 3, 48, 128, [200, 129], [130, 129]),
+    (1, 24, 128, 16, [70, 20], [40, 3]),
+]
+
+
+@pytest.mark.parametrize("dt,kind", [("bf16", "e4m3"), ("f16", "i8"), ("f32", "e4m3"), ("bf16", "i8"), ("f32", "i8"), ("f16", "e4m3")])
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+def test_attention(gpu, shape, dt, kind):
+    H, G, D, page, lengths, counts = SHAPES[shape]
+    _attend(gpu, _attend_case(np.random.default_rng(shape), dt, kind, H, G, D, page, lengths, counts))
+
+
+@pytest.mark.parametrize("window", [1, 7, 32, 130, 10000])
+@pytest.mark.parametrize("G,page,lengths,counts", [(4, 16, [1, 300, 129], [1, 1, 1]), (2, 8, [200, 90], [150, 3]), (1, 32, [260], [260])])
+def test_attention_window(gpu, window, G, page, lengths, counts):
+    c = _attend_case(np.random.default_rng(window), "bf16", "e4m3", 2, G, 64, page, lengths, counts)
+    # Pages behind every window have been given away.
+    for b, (n, m) in enumerate(zip(lengths, counts)):
+        c["table"][b, :max(0, n - m + 1 - window) // page] = -1
+    live = c["table"].copy()
+    t = _attend_tensors(gpu, c)
+    go(paged_attention(**{k: T(x) for k, x in t.items()}, window=window))
+    c["table"] = np.where(live < 0, 0, live)
+    _check_attend(c, t, _reference(c, 1.0 / 8.0, window))
+
+
+def test_attention_rows_without_positions(gpu):
+    """More rows than tokens: the first ones lie before position 0."""
+    c = _attend_case(np.random.default_rng(1), "bf16", "e4m3", 2, 4, 64, 16, [0, 3, 20], [2, 6, 1])
+    _attend(gpu, c)
+
+
+@pytest.mark.parametrize("layout", ["plain", "fused"])
+@pytest.mark.parametrize("dt,kind", [("bf16", "e4m3"), ("f32", "i8")])
+def test_attention_layouts(gpu, layout, dt, kind):
+    c = _attend_case(np.random.default_rng(2), dt, kind, 3, 2, 64, 16, [77, 140], [1, 30])
+    _attend(gpu, c, scale=0.2, layout=layout)
+    _attend(gpu, c, scale=0.2, layout=layout, lse=False)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_attention_long_and_few(gpu, dt):
+    """One request that every workgroup shares."""
+    c = _attend_case(np.random.default_rng(3), dt, "e4m3", 1, 4, 64, 16, [40000], [1])
+    _attend(gpu, c)
+
+
+def test_attention_many_short(gpu):
+    """More units than workgroups."""
+    rng = np.random.default_rng(4)
+    lengths = rng.integers(1, 60, 400)
+    _attend(gpu, _attend_case(rng, "bf16", "i8", 4, 2, 32, 16, lengths, [1] * 400))
+
+
+def test_attention_large_scores(gpu):
+    """Scores that grow along the context by far more than exp holds."""
+    c = _attend_case(np.random.default_rng(5), "f32", "e4m3", 1, 2, 64, 16, [400], [3], poison=False)
+    c["scale"]["k"][c["table"][0, :25]] *= np.linspace(0.1, 30, 25)[:, None].astype(np.float32)
+    _attend(gpu, c, scale=3.0)
+
+
+def test_attention_small_scales(gpu):
+    """Scales down to 2^-126: nothing is lost between codes and outputs."""
+    c = _attend_case(np.random.default_rng(6), "f32", "i8", 2, 2, 64, 16, [90, 40], [1, 4])
+    c["scale"]["v"][c["table"][0, 1]] = 1e-30
+    c["scale"]["v"][c["table"][1, 0]] = 1e20
+    _attend(gpu, c)
+
+
+def test_attention_nan_reaches_only_the_rows_that_see_it(gpu):
+    c = _attend_case(np.random.default_rng(7), "bf16", "e4m3", 2, 2, 64, 16, [60, 30], [40, 1])
+    page, off = divmod(45, 16)
+    c["codes"]["v"][c["table"][0, page], 1, off, 5] = 0x7F
+    c["codes"]["k"][c["table"][0, page], 0, off + 1, 3] = 0xFF
+    _, t, ref = _attend(gpu, c, lse=False)
+    assert np.isnan(ref[0][:40]).any() and not np.isnan(ref[0][:25]).any()
+    c["q"][3] = float("nan")
+    _attend(gpu, c, lse=False)
+
+
+@pytest.mark.parametrize("what", ["starts", "length", "page", "negative page", "order"])
+def test_attention_inputs_out_of_range(gpu, what):
+    c = _attend_case(np.random.default_rng(8), "bf16", "e4m3", 2, 2, 64, 16, [60, 30, 20], [4, 1, 2])
+    t = _attend_tensors(gpu, c)
+    if what == "starts":
+        t["starts"][3] = 1000
+    elif what == "order":
+        t["starts"][1] = 6
+    elif what == "length":
+        t["lengths"][1] = 16 * t["page_table"].shape[1] + 1
+    else:
+        t["page_table"][0, 1] = 10 ** 6 if what == "page" else -1
+    prog = paged_attention(**{k: T(x) for k, x in t.items()}).compile(target="hip_gfx950")
+    prog.execute()
+    with pytest.raises(ExecutionError, match="out of range"):
+        prog.synchronize()
+    # The program is whole again afterwards.
+    t["starts"].copy_(ints(gpu, c["starts"]))
+    t["lengths"].copy_(ints(gpu, c["lengths"]))
+    t["page_table"].copy_(ints(gpu, c["table"]))
+    prog.execute()
+    prog.synchronize()
+    _check_attend(c, t, _reference(c, 1.0 / 8.0, 0))
+
+
+# ------------------------------------------------------------------------------ together
+def _step_case(gpu, layers, kind, dt, H, G, D, page, lengths, counts, seed):
+    """A serving step of several layers: plan, then store and attention per layer, over a cache that an
+    earlier step of `lengths` tokens has filled."""
+    torch = _torch()
+    rng = np.random.default_rng(seed)
+    lengths, counts = np.asarray(lengths), np.asarray(counts)
+    held = -(-lengths // page)
+    width = int((-(-(lengths + counts) // page)).max()) + 1
+    pages = int((-(-(lengths + counts) // page)).sum()) + 4
+    order = rng.permutation(pages)
+    table = np.full((len(lengths), width), -1)
+    table[np.arange(width)[None] < held[:, None]] = order[:int(held.sum())]
+    rows = int(counts.sum()) + 3
+    t = _plan_tensors(gpu, lengths, counts, table, order[int(held.sum()):], 0, rows)
+    codes = {x: R.encode(rng.standard_normal((layers, pages, H, page, D)) * 40, kind) for x in "kv"}
+    scale = {x: (0.03 * np.exp(0.3 * rng.standard_normal((layers, pages, H)))).astype(np.float32) for x in "kv"}
+    for x in "kv":
+        t[x + "_cache"], t[x + "_scale"] = codes_on(gpu, codes[x], kind), torch.from_numpy(scale[x]).to(gpu)
+        t[x] = torch.from_numpy(rng.standard_normal((layers, rows, H, D)).astype(np.float32)).to(gpu).to(_dt(dt))
+    t["q"] = torch.from_numpy(rng.standard_normal((layers, rows, H * G, D)).astype(np.float32)).to(gpu).to(_dt(dt))
+    t["out"] = torch.full_like(t["q"], 7.0)
+    return t, codes, scale, (lengths, counts, table, order[int(held.sum()):])
+
+
+def _step_workload(t, layers, page):
+    w = {k: T(x) for k, x in t.items()}
+
+    @workload
+    def step():
+        paged_plan(page_size=page, **{k: w[k] for k in ("lengths", "counts", "page_table", "free_pages", "used", "new_lengths", "new_used", "starts", "slots")})
+        for layer in P.seq(Dense[layers](), name="layer"):
+            cache = {k: w[k][layer] for k in ("k_cache", "v_cache", "k_scale", "v_scale")}
+            paged_store(k=w["k"][layer], v=w["v"][layer], slots=w["slots"], **cache)
+            paged_attention(q=w["q"][layer], out=w["out"][layer], page_table=w["page_table"], lengths=w["new_lengths"], starts=w["starts"], **cache)
+
+    return step()
+
+
+def _check_step(t, layers, kind, dt, page, codes, scale, plan):
+    torch = _torch()
+    lengths, counts, table, free = plan
+    rows = t["slots"].shape[0]
+    want = R.plan(lengths, counts, table, free, 0, page, rows)
+    for k, x in want.items():
+        assert np.array_equal(t[k].cpu().numpy(), x), k
+    for layer in range(layers):
+        c = {"q": t["q"][layer].cpu(), "codes": {}, "scale": {}, "table": want["page_table"], "lengths": want["new_lengths"], "starts": want["starts"],
+             "kind": kind, "dt": dt}
+        for x in "kv":
+            c["codes"][x], c["scale"][x] = R.store(t[x][layer].cpu().to(torch.float64).numpy(), want["slots"], codes[x][layer], scale[x][layer], kind)
+            assert same_codes(codes_of(t[x + "_cache"][layer], kind), c["codes"][x], kind)
+            assert np.array_equal(t[x + "_scale"][layer].cpu().numpy(), c["scale"][x])
+        _check_attend(c, {"out": t["out"][layer]}, _reference(c, 1.0 / np.sqrt(t["q"].shape[-1]), 0), lse=False)
+
+
+@pytest.mark.parametrize("kind,dt", [("e4m3", "bf16"), ("i8", "f32")])
+def test_step(gpu, kind, dt):
+    t, codes, scale, plan = _step_case(gpu, 2, kind, dt, 2, 4, 64, 16, [0, 31, 100, 5, 16], [20, 1, 1, 0, 40], 1)
+    prog = go(_step_workload(t, 2, 16))
+    assert prog.stats.launches >= 5
+    _check_step(t, 2, kind, dt, 16, codes, scale, plan)
+
+
+def _restore(t, first):
+    for k, x in first.items():
+        t[k].copy_(x)
+
+
+@pytest.mark.parametrize("counts", [[1, 1, 1], [40, 1, 0]])
+def test_step_captured(gpu, counts):
+    """Captured twice and replayed beside eager runs: every graph keeps a workspace of its own."""
+    torch = _torch()
+    t, codes, scale, plan = _step_case(gpu, 2, "e4m3", "bf16", 2, 4, 64, 16, [60, 700, 16], counts, 2)
+    first = {k: x.clone() for k, x in t.items()}
+    prog = _step_workload(t, 2, 16).compile(target="hip_gfx950")
+    streams, graphs = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for s in streams:
+        with torch.cuda.stream(s):
+            prog.execute()
+            prog.synchronize()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            prog.execute()
+        prog.synchronize()
+        graphs.append(g)
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=streams[0]):
+            try:
+                prog.execute()
+            finally:
+                torch.zeros(1, device=gpu).add_(1)  # the capture holds something
+    torch.cuda.synchronize()
+    for i in range(3):
+        for g in graphs:
+            _restore(t, first)
+            g.replay()
+            torch.cuda.synchronize()
+            _check_step(t, 2, "e4m3", "bf16", 16, codes, scale, plan)
+        _restore(t, first)
+        torch.cuda.synchronize()
+        prog.execute()
+        prog.synchronize()
+        _check_step(t, 2, "e4m3", "bf16", 16, codes, scale, plan)
+
+
+def test_step_on_another_stream(gpu):
+    torch = _torch()
+    t, codes, scale, plan = _step_case(gpu, 1, "i8", "f16", 2, 2, 64, 8, [10, 300], [3, 1], 3)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        prog = go(_step_workload(t, 1, 8))
+    assert prog.stats.launches >= 3
+    _check_step(t, 1, "i8", "f16", 8, codes, scale, plan)
+
+
+def test_step_host_tensors(gpu):
+    """numpy arrays are staged through the device."""
+    t, codes, scale, plan = _step_case(gpu, 1, "i8", "f32", 1, 2, 32, 16, [10, 50], [3, 1], 4)
+    host = {k: x.cpu().numpy() for k, x in t.items()}
+    kinds = {np.dtype(np.int32): DType.I32, np.dtype(np.float32): DType.F32, np.dtype(np.int8): DType.I8}
+    w = {k: Tensor(data=x, shape=x.shape, dtype=kinds[x.dtype]) for k, x in host.items()}
+    layer = {k: w[k][0] for k in ("k_cache", "v_cache", "k_scale", "v_scale")}
+    go(sequential(paged_plan(page_size=16, **{k: w[k] for k in ("lengths", "counts", "page_table", "free_pages", "used", "new_lengths", "new_used", "starts",
+                                                                "slots")}),
+                  paged_store(k=w["k"][0], v=w["v"][0], slots=w["slots"], **layer),
+                  paged_attention(q=w["q"][0], out=w["out"][0], page_table=w["page_table"], lengths=w["new_lengths"], starts=w["starts"], **layer)))
+    torch = _torch()
+    _check_step({k: torch.from_numpy(x) for k, x in host.items()}, 1, "i8", "f32", 16, codes, scale, plan)
+
+
+def test_two_programs_at_once(gpu):
+    """Runs of two programs in flight together on two streams."""
+    torch = _torch()
+    cs = [_attend_case(np.random.default_rng(20 + i), "bf16", "e4m3", 2, 4, 64, 16, [3000 + i, 40], [1, 2]) for i in range(2)]
+    ts = [_attend_tensors(gpu, c) for c in cs]
+    progs = [paged_attention(**{k: T(x) for k, x in t.items()}).compile(target="hip_gfx950") for t in ts]
+    streams = [torch.cuda.Stream() for _ in cs]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for p, s in zip(progs, streams):
+            with torch.cuda.stream(s):
+                p.execute()
+        for p in progs:
+            p.synchronize()
+    for c, t in zip(cs, ts):
+        _check_attend(c, t, _reference(c, 1.0 / 8.0, 0))
+
+
+def test_refusals_at_execute(gpu):
+    torch = _torch()
+    c = _attend_case(np.random.default_rng(30), "bf16", "e4m3", 2, 2, 64, 16, [60], [4])
+    t = _attend_tensors(gpu, c)
+
+    def attempt(**other):
+        paged_attention(**{k: T(x) for k, x in dict(t, **other).items()}).compile(target="hip_gfx950").execute()
+
+    with pytest.raises(RuntimeError, match="out is written and lies where q does"):
+        attempt(out=t["q"])
+    with pytest.raises(RuntimeError, match="stride 0"):
+        attempt(out=t["out"][:1].expand_as(t["out"]))
+    with pytest.raises(RuntimeError, match="must have stride 1"):
+        attempt(q=t["q"].transpose(1, 2).contiguous().transpose(1, 2))
+    odd = torch.zeros(t["k_cache"].numel() + 8, dtype=torch.int8, device=gpu)[8:].view(torch.float8_e4m3fn).view(t["k_cache"].shape)
+    with pytest.raises(RuntimeError, match="aligned to 16 bytes"):
+        attempt(k_cache=odd)
+    with pytest.raises(CompileError, match="differ in type"):
+        attempt(v_cache=t["v_cache"].view(torch.int8))
