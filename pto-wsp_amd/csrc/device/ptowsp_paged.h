@@ -21,6 +21,7 @@ typedef __bf16 pg_bf2 __attribute__((ext_vector_type(2)));
 typedef __bf16 pg_bf8 __attribute__((ext_vector_type(8)));
 typedef _Float16 pg_h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 pg_h8 __attribute__((ext_vector_type(8)));
+typedef float pg_f32x16 __attribute__((ext_vector_type(16)));
 
 // Types of activations and of cache codes.
 constexpr int kBF16 = 0, kF16 = 1, kF32 = 2;
@@ -478,8 +479,9 @@ __device__ inline T uniform_load(const T* p) {
     return *(constant)(reinterpret_cast<pg_u64>(p));
 }
 
-template <int D_, int PAGE_, int G_, int NT_, int QT_, int CT_, bool WIN_, bool LSE_, bool VEC_>
+template <int D_, int PAGE_, int G_, int NT_, int QT_, int CT_, bool WIN_, bool LSE_, bool VEC_, bool PROMPT_ = false>
 struct Attend {
+    static constexpr bool PROMPT = PROMPT_;
     static constexpr int D = D_, PAGE = PAGE_, G = G_, NT = NT_, QT = QT_, CT = CT_;
     static constexpr bool WIN = WIN_, LSE = LSE_, VEC = VEC_;
     static constexpr int RB = 16 * NT;
@@ -503,9 +505,9 @@ struct Attend {
         const int s0 = A.starts[b * A.s_starts], s1 = A.starts[(b + 1) * A.s_starts];
         int length = A.lengths[b * A.s_lengths];
         const pg_i64 most = A.width * PAGE;
-        bool bad = s0 < 0 || s1 < s0 || s1 > A.rows || length < 0 || length > most;
-        if (bad) {
-            if (report) *A.err = 7;
+        const bool bad = s0 < 0 || s1 < s0 || s1 > A.rows || length < 0 || length > most;
+        if (bad && report) *A.err = 7;
+        if (bad || (PROMPT ? s1 - s0 <= A.few : s1 - s0 > A.few)) {
             r.row = r.n = r.length = r.first = r.kt = r.units = 0;
             return r;
         }
@@ -701,9 +703,108 @@ struct Attend {
         }
     }
 
-    template <bool MASKED>
-    __device__ static void step(const AttendArgs& A, const Unit& u, int base, Raw& r, State& st) {
+    // p of the scores, and its products with the values.
+    __device__ static void weigh(const Raw& r, const float (&s)[NT][8], State& st) {
+        pg_u32x4 p[NT][PP];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const float m = st.m[t] == -__builtin_inff() ? 0.0f : st.m[t];
+            float x[8], l = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[e] = __builtin_amdgcn_exp2f(s[t][e] - m);
+                l += x[e];
+                x[e] *= r.vs[PAGED16 ? e >> 2 : e];
+            }
+            st.l[t] += l;
+#pragma unroll
+            for (int k = 0; k < PP; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[t][k][e] = take_bf16(x[2 * e], x[2 * e + 1]);
+        }
+        values(r.v, p, st.o);
+    }
+
+    // For a branch that is hardly ever taken: what it computes of these is not
+    // moved ahead of it, where it would take registers from every step.
+    __device__ static void apart(Raw& r, float (&s)[NT][8]) {
+#pragma unroll
+        for (int j = 0; j < NK; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) asm volatile("" : "+v"(r.v[j][e]));
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) asm volatile("" : "+v"(s[t][e]));
+    }
+
+    // Scores and values of a step that some row does not see whole.  What lies
+    // outside the unit's positions may be anything; a NaN among values that some
+    // rows see and others do not (0 * NaN is NaN) goes into those rows' sums here
+    // and is 0 afterwards: ones at the NaNs times ones at the rows that see them.
+    __device__ static void mask(const AttendArgs& A, const Unit& u, int base, Raw& r, float (&s)[NT][8], State& st) {
         const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+        const int tok = base + 4 * g;  // token of place e: tok + e % 4, 16 further for e >= 4
+        pg_u32 seen[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int hi = u.p0 + (16 * t + n) / GH + 1, lo = WIN ? hi - A.window : 0;
+            seen[t] = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int at = tok + (e & 3) + 4 * (e & 4);
+                const bool in = at < hi && at >= lo && at < u.hi;
+                seen[t] |= static_cast<pg_u32>(in) << e;
+                s[t][e] = in ? s[t][e] : -__builtin_inff();
+            }
+        }
+        pg_u32 nan = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int at = tok + (e & 3) + 4 * (e & 4);
+            const bool in = at < u.hi && at >= u.lo;
+#pragma unroll
+            for (int j = 0; j < NK; ++j) {
+                r.v[j][e] = in ? r.v[j][e] : 0;
+                nan |= ((r.v[j][e] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+            }
+        }
+        if constexpr (CT == kE4M3 && (C > 1 || WIN)) {
+            if (__ballot(nan != 0) == 0) return;
+            apart(r, s);
+#pragma unroll
+            for (int j = 0; j < NK; ++j) {
+                pg_u32 ones[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const pg_u32 at = (((r.v[j][e] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) >> 7;
+                    ones[e] = at * 0x38u;  // the code of 1
+                    r.v[j][e] &= ~(at * 0xFFu);
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    pg_u32x4 a;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const pg_u32 w = __builtin_amdgcn_perm(ones[2 * e + 1], ones[2 * e], q < 2 ? 0x05010400u : 0x07030602u);
+                        a[e] = q & 1 ? codes2<CT, false, true>(w) : codes2<CT, false, false>(w);
+                    }
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        pg_u32x4 p;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) p[e] = (seen[t] >> (2 * e) & 1) * 0x3F80u | (seen[t] >> (2 * e + 1) & 1) * 0x3F800000u;
+                        const pg_f32x4 hit = mma(a, p, pg_f32x4{0, 0, 0, 0}, false);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (hit[i] > 0.0f) st.o[t][j][q][i] = __builtin_nanf("");
+                    }
+                }
+            }
+        }
+    }
+
+    __device__ static void step(const AttendArgs& A, const Unit& u, int base, Raw& r, State& st) {
         float s[NT][8];
         {
             pg_f32x4 acc[NT][2];
@@ -728,36 +829,8 @@ struct Attend {
                 for (int t = 0; t < NT; ++t) s[t][e] = acc[t][e >> 2][e & 3] * f;
             }
         }
-        bool part = false;  // some tokens are seen by some rows only
-        pg_u32 seen[NT];    // masked: bit e, the lane's row attends to its token e
-        if constexpr (MASKED) {
-            const int tok = base + 4 * g;  // token of place e: tok + e % 4, 16 further for e >= 4
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const int hi = u.p0 + (16 * t + n) / GH + 1, lo = WIN ? hi - A.window : 0;
-                seen[t] = 0;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int at = tok + (e & 3) + 4 * (e & 4);
-                    const bool in = at < hi && at >= lo && at < u.hi;
-                    seen[t] |= static_cast<pg_u32>(in) << e;
-                    s[t][e] = in ? s[t][e] : -__builtin_inff();
-                }
-            }
-            // What lies outside the unit's positions may be anything.
-            pg_u32 nan = 0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int at = tok + (e & 3) + 4 * (e & 4);
-                const bool in = at < u.hi && at >= u.lo;
-#pragma unroll
-                for (int j = 0; j < NK; ++j) {
-                    r.v[j][e] = in ? r.v[j][e] : 0;
-                    nan |= ((r.v[j][e] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
-                }
-            }
-            if constexpr (CT == kE4M3 && (C > 1 || WIN)) part = __ballot(nan != 0) != 0;
-        }
+        // Every row of the unit sees every one of the tokens, or not.
+        if (!(base + 32 <= u.p0 + 1 && (!WIN || base >= u.p0 + u.n - A.window))) mask(A, u, base, r, s, st);
         // The maximum, only if some score is far above it.
         bool grow = false;
 #pragma unroll
@@ -785,57 +858,7 @@ struct Attend {
                     for (int q = 0; q < 4; ++q) st.o[t][j][q] *= a;
             }
         }
-        pg_u32x4 p[NT][PP];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const float m = st.m[t] == -__builtin_inff() ? 0.0f : st.m[t];
-            float x[8], l = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x[e] = __builtin_amdgcn_exp2f(s[t][e] - m);
-                l += x[e];
-                x[e] *= r.vs[PAGED16 ? e >> 2 : e];
-                if (MASKED) x[e] = seen[t] >> e & 1 ? x[e] : 0.0f;
-            }
-            st.l[t] += l;
-#pragma unroll
-            for (int k = 0; k < PP; ++k)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) p[t][k][e] = take_bf16(x[2 * e], x[2 * e + 1]);
-        }
-        if (MASKED && part) {
-            // A NaN among values that some rows do not see: token by token, and
-            // only into the rows that see it (0 * NaN is NaN).
-            for (int at = 0; at < 32; ++at) {
-                const int e = (at & 3) | (at & 16) >> 2;
-                const bool mine = (at & 12) >> 2 == g;
-                pg_u32 v[NK][8];
-#pragma unroll
-                for (int j = 0; j < NK; ++j)
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) v[j][k] = mine && k == e ? r.v[j][k] : 0;
-                pg_f32x4 o[NT][NK][4];
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int j = 0; j < NK; ++j)
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) o[t][j][q] = pg_f32x4{0, 0, 0, 0};
-                values(v, p, o);
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const int hi = u.p0 + (16 * t + n) / GH + 1;
-                    const bool in = base + at < hi && (!WIN || base + at >= hi - A.window);
-#pragma unroll
-                    for (int j = 0; j < NK; ++j)
-#pragma unroll
-                        for (int q = 0; q < 4; ++q)
-                            if (in) st.o[t][j][q] += o[t][j][q];
-                }
-            }
-        } else {
-            values(r.v, p, st.o);
-        }
+        weigh(r, s, st);
     }
 
     __device__ static void write_row(const AttendArgs& A, int row, int head, int g, int j, const pg_f32x4 (&o)[4], float f) {
@@ -944,7 +967,7 @@ struct Attend {
             const int row = rq.row + tile * C, head = h * G + hs * RB;
             State st;
             load_q(A, u, row, head, st);
-            piece(A, u, (rq.first + t0) * kAttendTile + 32 * wave, (rq.first + t1) * kAttendTile, st);
+            piece<kAttendTile>(A, u, (rq.first + t0) * kAttendTile + 32 * wave, (rq.first + t1) * kAttendTile, st);
             // The four waves' results.
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
@@ -1030,39 +1053,629 @@ struct Attend {
         return l == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f;
     }
 
-    // This wave's steps of the tokens from `base` on, below `end`: every
-    // fourth 32.  The next step's pages and bytes are under way during one.
+    // This wave's steps of 32 tokens from `base` on, STRIDE tokens apart, below
+    // `end`.  The next step's pages and bytes are under way during one.
+    template <int STRIDE>
     __device__ static void piece(const AttendArgs& A, const Unit& u, int base, int end, State& st) {
         if (end > u.hi) end = u.hi;
-        if (base + 32 <= u.lo) base += (u.lo - base - 31 + kAttendTile - 1) / kAttendTile * kAttendTile;
+        if (base + 32 <= u.lo) base += (u.lo - base - 32 + STRIDE) / STRIDE * STRIDE;
         if (base >= end) return;
         Pages pg;
         Raw a, b;
         pages(A, u, base, pg);
         load(A, u, base, pg, a);
-        pages(A, u, base + kAttendTile, pg);
+        pages(A, u, base + STRIDE, pg);
         for (;;) {
-            if (base + kAttendTile < end) {
-                load(A, u, base + kAttendTile, pg, b);
-                pages(A, u, base + 2 * kAttendTile, pg);
+            if (base + STRIDE < end) {
+                load(A, u, base + STRIDE, pg, b);
+                pages(A, u, base + 2 * STRIDE, pg);
             }
-            one(A, u, base, a, st);
-            base += kAttendTile;
+            step(A, u, base, a, st);
+            base += STRIDE;
             if (base >= end) return;
-            if (base + kAttendTile < end) {
-                load(A, u, base + kAttendTile, pg, a);
-                pages(A, u, base + 2 * kAttendTile, pg);
+            if (base + STRIDE < end) {
+                load(A, u, base + STRIDE, pg, a);
+                pages(A, u, base + 2 * STRIDE, pg);
             }
-            one(A, u, base, b, st);
-            base += kAttendTile;
+            step(A, u, base, b, st);
+            base += STRIDE;
             if (base >= end) return;
         }
     }
-    __device__ static void one(const AttendArgs& A, const Unit& u, int base, Raw& r, State& st) {
-        // Every row of the unit sees every one of the tokens.
-        const bool whole = base + 32 <= u.p0 + 1 && (!WIN || base >= u.p0 + u.n - A.window);
-        if (whole) step<false>(A, u, base, r, st);
-        else step<true>(A, u, base, r, st);
+    // ---- prompts ----
+    // A unit is 4 * C tokens, C for each wave of a workgroup: the waves read the
+    // same keys at about the same time, each for rows of its own, and need not
+    // meet.  attend_units lists the units, the longest first, those beyond a
+    // compute unit's share of the work in several pieces; a unit's last piece to
+    // end joins them.
+    static constexpr int kUnitTokens = 4 * C;
+
+    struct Span {
+        int lo, hi;  // tokens of a unit's keys, lo a multiple of 32
+    };
+    __device__ static Span span_of(const AttendArgs& A, const Request& rq, int tile) {
+        const int p0 = rq.length - rq.n + tile * kUnitTokens;
+        const int n = rq.n - tile * kUnitTokens < kUnitTokens ? rq.n - tile * kUnitTokens : kUnitTokens;
+        Span s;
+        s.hi = p0 + n > 0 ? p0 + n : 0;
+        s.lo = WIN && p0 + 1 > A.window ? (p0 + 1 - A.window) / 32 * 32 : 0;
+        return s;
+    }
+
+    // units: {entries, partial results}, then entries {request, tile, piece << 16
+    // | pieces, first partial result}; behind the room for them a counter for each partial result.
+    template <int THREADS>
+    __device__ static void list_units(const AttendArgs& A, int room, int counters) {
+        constexpr int BUCKETS = 128;
+        __shared__ pg_i64 lds[THREADS / 64];
+        __shared__ int many[BUCKETS], slots;
+        __shared__ pg_u64 work;
+        const pg_i64 per = (A.batch + THREADS - 1) / THREADS, b0 = threadIdx.x * per;
+        const pg_i64 b1 = b0 + per < A.batch ? b0 + per : A.batch;
+        if (threadIdx.x < BUCKETS) many[threadIdx.x] = 0;
+        if (threadIdx.x == 0) {
+            slots = 0;
+            work = 0;
+        }
+        int* const count = A.units + 2 + room * kUnitInts;
+        for (int i = threadIdx.x; i < counters; i += THREADS) count[i] = 0;
+        __shared__ pg_i64 before[THREADS];
+        pg_i64 units = 0, total;
+        for (pg_i64 b = b0; b < b1; ++b) units += (request(A, b, false).n + kUnitTokens - 1) / kUnitTokens;
+        before[threadIdx.x] = block_scan<THREADS>(units, total, lds);
+        __syncthreads();
+        // Three passes over the units, spread over the threads: the work, the
+        // sizes, the places.
+        int limit = 0x7FFFFFFF;
+#pragma unroll 1
+        for (int pass = 0; pass < 3; ++pass) {
+            pg_u64 sum = 0;
+            for (pg_i64 i = threadIdx.x; i < total; i += THREADS) {
+                int lo = 0, hi = THREADS;  // before[lo] <= i < before[hi]
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1;
+                    if (before[mid] <= i) lo = mid;
+                    else hi = mid;
+                }
+                pg_i64 b = lo * per, at = before[lo];
+                Request rq = request(A, b, false);
+                for (;;) {
+                    const int tiles = (rq.n + kUnitTokens - 1) / kUnitTokens;
+                    if (i < at + tiles) break;
+                    at += tiles;
+                    rq = request(A, ++b, false);
+                }
+                const int tile = static_cast<int>(i - at);
+                const Span s = span_of(A, rq, tile);
+                const int steps = s.hi > s.lo ? (s.hi - s.lo + 31) / 32 : 1;
+                sum += static_cast<pg_u64>(steps);
+                if (pass == 0) continue;
+                const int pieces = (steps + limit - 1) / limit, size = steps < limit ? steps : limit;
+                const int bucket = BUCKETS - 1 - static_cast<int>(static_cast<pg_i64>(size) * (BUCKETS - 1) / limit);
+                const int place = atomicAdd(&many[bucket], pieces * HS);
+                if (pass == 1) continue;
+                for (int hs = 0; hs < HS; ++hs) {
+                    const int slot = pieces > 1 ? atomicAdd(&slots, pieces) : 0;
+                    for (int k = 0; k < pieces; ++k) {
+                        int* const e = A.units + 2 + static_cast<pg_i64>(place + hs * pieces + k) * kUnitInts;
+                        e[0] = static_cast<int>(b);
+                        e[1] = tile * HS + hs;
+                        e[2] = k << 16 | pieces;
+                        e[3] = slot;
+                    }
+                }
+            }
+            if (pass == 0) atomicAdd(&work, sum);
+            __syncthreads();
+            if (pass == 0) {
+                const pg_u64 share = (work * HS * A.heads * 9 / 8 + A.cus - 1) / A.cus;
+                limit = share < 16 ? 16 : share > 0x7FFFFFF ? 0x7FFFFFF : static_cast<int>(share);
+            } else if (pass == 1) {
+                // Places of the buckets, longest units first.
+                int first = 0;
+                if (threadIdx.x < BUCKETS)
+                    for (int k = 0; k < static_cast<int>(threadIdx.x); ++k) first += many[k];
+                if (threadIdx.x == BUCKETS - 1) A.units[0] = first + many[BUCKETS - 1];
+                __syncthreads();
+                if (threadIdx.x < BUCKETS) many[threadIdx.x] = first;
+            }
+            __syncthreads();
+        }
+    }
+
+    // A piece of a unit, as one wave of a workgroup sees it.
+    struct Part {
+        int b, h, tile, hs, piece, pieces, slot;
+        int base, end;   // tokens of the piece
+        int row, head;   // of the wave's rows
+        Request rq;
+        Unit u;
+    };
+    // False: no such entry.
+    __device__ static bool part_of(const AttendArgs& A, Part& p) {
+        const int wave = uniform(threadIdx.x >> 6);
+        const int entry = static_cast<int>(blockIdx.x / A.heads);
+        p.h = static_cast<int>(blockIdx.x) - entry * A.heads;
+        if (entry >= A.units[0]) return false;
+        const int* const e = A.units + 2 + static_cast<pg_i64>(entry) * kUnitInts;
+        const int code = uniform(e[1]), kp = uniform(e[2]);
+        p.b = uniform(e[0]);
+        p.slot = uniform(e[3]);
+        p.piece = static_cast<int>(static_cast<pg_u32>(kp) >> 16);
+        p.pieces = kp & 0xFFFF;
+        p.tile = code / HS;
+        p.hs = code - p.tile * HS;
+        p.rq = request(A, p.b, true);
+        p.rq.row = uniform(p.rq.row);
+        p.rq.n = uniform(p.rq.n);
+        p.rq.length = uniform(p.rq.length);
+        const Span s = span_of(A, p.rq, p.tile);
+        const int steps = s.hi > s.lo ? (s.hi - s.lo + 31) / 32 : 1;
+        p.base = s.lo + 32 * static_cast<int>(static_cast<pg_i64>(steps) * p.piece / p.pieces);
+        p.end = s.lo + 32 * static_cast<int>(static_cast<pg_i64>(steps) * (p.piece + 1) / p.pieces);
+        if (p.end > s.hi) p.end = s.hi;
+        const int first = p.tile * kUnitTokens + wave * C;
+        p.row = p.rq.row + first;
+        p.head = p.h * G + p.hs * RB;
+        p.u.table = A.table + p.b * A.s_table;
+        p.u.h = p.h;
+        p.u.n = p.rq.n - first < C ? p.rq.n - first : C;
+        p.u.p0 = p.rq.length - p.rq.n + first;
+        p.u.hi = p.u.n > 0 && p.u.p0 + p.u.n > 0 ? p.u.p0 + p.u.n : 0;
+        p.u.lo = WIN && p.u.p0 + 1 > A.window ? p.u.p0 + 1 - A.window : 0;
+        return true;
+    }
+    __device__ static float* part_sums(const AttendArgs& A, const Part& p, int piece) {
+        const int wave = uniform(threadIdx.x >> 6);
+        return A.unit_parts + ((static_cast<pg_i64>(p.slot + piece) * A.heads + p.h) * 4 + wave) * PART;
+    }
+
+    // Place of a unit's row (token, head of the group) in a partial result.
+    __device__ static int place_of(int i, int hh) { return HS == 1 ? i * G + hh : hh % RB; }
+
+    // The steps of a wave's rows, by itself, 16 * NT rows at a time.  The piece
+    // is one of W's, whose units may be wider.
+    template <class W>
+    __device__ static void rows(const AttendArgs& A, const typename W::Part& p) {
+        const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+        const int heads = W::HS == 1 ? G : (G - p.hs * W::RB < W::RB ? G - p.hs * W::RB : W::RB);
+#pragma unroll 1
+        for (int i0 = 0; i0 < p.u.n; i0 += C)
+#pragma unroll 1
+            for (int h0 = 0; h0 < heads; h0 += GH) {
+                Unit u;
+                u.table = p.u.table;
+                u.h = p.h;
+                u.n = p.u.n - i0 < C ? p.u.n - i0 : C;
+                u.p0 = p.u.p0 + i0;
+                u.hi = u.p0 + u.n > 0 ? u.p0 + u.n : 0;
+                u.lo = WIN && u.p0 + 1 > A.window ? u.p0 + 1 - A.window : 0;
+                const int row = p.row + i0, head = p.head + h0;
+                State st;
+                load_q(A, u, row, head, st);
+                piece<32>(A, u, p.base, p.end, st);
+                float* const part = W::part_sums(A, p, p.piece);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    st.l[t] += __shfl_xor(st.l[t], 16, 64);
+                    st.l[t] += __shfl_xor(st.l[t], 32, 64);
+                    const int r = 16 * t + n, i = r / GH, hh = r - i * GH;
+                    if (i >= u.n || h0 + hh >= heads) continue;
+                    if (p.pieces == 1) {
+                        const float f = st.l[t] == 0.0f ? 0.0f : 1.0f / st.l[t];
+#pragma unroll
+                        for (int j = 0; j < NK; ++j) write_row(A, row + i, head + hh, g, j, st.o[t][j], f);
+                        if (LSE && g == 0) A.lse[(row + i) * A.s_lse[0] + (head + hh) * A.s_lse[1]] = lse_of(st.m[t], st.l[t]);
+                    } else {
+                        const int at = W::place_of(i0 + i, h0 + hh);
+                        if (g == 0) {
+                            part[at] = st.m[t];
+                            part[W::RB + at] = st.l[t];
+                        }
+#pragma unroll
+                        for (int j = 0; j < NK; ++j)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                *reinterpret_cast<pg_f32x4*>(part + 2 * W::RB + at * DP + 64 * j + 16 * g + 4 * k) =
+                                    pg_f32x4{st.o[t][j][0][k], st.o[t][j][1][k], st.o[t][j][2][k], st.o[t][j][3][k]};
+                    }
+                }
+            }
+    }
+
+    // The last piece of a unit to end joins all of them.
+    __device__ static void join_pieces(const AttendArgs& A, int room, const Part& p) {
+        const int lane = threadIdx.x & 63;
+        __shared__ int arrived;
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            int* const count = A.units + 2 + room * kUnitInts + p.slot * A.heads + p.h;
+            arrived = __hip_atomic_fetch_add(count, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
+        if (arrived != p.pieces - 1 || p.u.n <= 0) return;
+        __threadfence();
+        const pg_i64 next = static_cast<pg_i64>(A.heads) * 4 * PART;
+        const float* const part = part_sums(A, p, 0);
+        for (int r = 0; r < RB; ++r) {
+            const int i = r / GH, hh = r - i * GH;
+            if (i >= p.u.n || i >= C || (HS > 1 && p.hs * RB + hh >= G)) continue;
+            float m = -__builtin_inff(), l = 0.0f;
+            for (int k = 0; k < p.pieces; ++k) m = fmaxf(m, part[k * next + r]);
+            float o[NK];
+#pragma unroll
+            for (int j = 0; j < NK; ++j) o[j] = 0.0f;
+            for (int k = 0; k < p.pieces; ++k) {
+                const float mk = part[k * next + r], w = mk == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mk - m);
+                l += w * part[k * next + RB + r];
+#pragma unroll
+                for (int j = 0; j < NK; ++j) o[j] += w * part[k * next + 2 * RB + r * DP + 64 * j + lane];
+            }
+            const float f = l == 0.0f ? 0.0f : 1.0f / l;
+            char* const q = A.out + ((p.row + i) * A.s_out[0] + (p.head + hh) * A.s_out[1]) * elem_size(QT);
+#pragma unroll
+            for (int j = 0; j < NK; ++j)
+                if (64 * j + lane < D) store_elem<QT>(q + (64 * j + lane) * elem_size(QT), o[j] * f);
+            if (LSE && lane == 0) A.lse[(p.row + i) * A.s_lse[0] + (p.head + hh) * A.s_lse[1]] = lse_of(m, l);
+        }
+    }
+
+    // ---- prompts, tile by tile ----
+    // The four waves convert a tile of 64 tokens once, 16 each, into LDS: keys
+    // as rows of bf16 (f16 for f16 queries), values as columns of f16, both in
+    // the order in which v_mfma_f32_32x32x16 takes them, two tiles in turn with
+    // one barrier a tile.  A wave has 32 query rows: lane (n, h) of 32 x 2 holds
+    // of row n tokens 8k + 4h .. + 3 of the scores, which are the P operand.
+    // p enters as f16: between 2^10 and 2^14 at a row's maximum (kLift, kLag), so
+    // that no p that matters is subnormal; in one part for bf16 outputs (2^-12 of
+    // it, and as much of each value), in two for f16 ones.  Values are relative
+    // to a base that follows the pages' scales; where those spread too far for
+    // f16, or a NaN lies among values that some rows do not see, the waves do the
+    // piece over with bf16 parts (rows).
+    static constexpr bool TILES = PROMPT && NT == 2 && PAGED16 && D <= 128 && QT != kF32;
+    static constexpr int kTile = 64, kChunks = DP / 8;  // tokens; 16-byte pieces of a key
+    static constexpr float kLift = 10.0f, kLag = 4.0f;
+    static constexpr int TP = QT == kF16 ? 2 : 1;       // parts of p
+
+    struct Tiles {
+        pg_u32x4 k[2][kTile * kChunks], v[2][DP * 8];
+        float ks[2][4];
+        int bad[2];
+    };
+    // Where a 16-byte piece lies, so that neither the waves' writes nor the
+    // MFMAs' reads meet in a bank more often than their size asks.
+    __device__ static int key_at(int token, int chunk) {
+        if constexpr (kChunks == 16) return token * 16 + (chunk ^ (token & 15));
+        else return token * 8 + (chunk ^ (token >> 1 & 7));
+    }
+    __device__ static int value_at(int d, int chunk) { return d * 8 + (chunk ^ (d >> 1 & 7) ^ (d >> 4 & 1)); }
+
+    struct Stage {
+        pg_u32x4 k[kChunks / 8];
+        pg_u32 v[8];
+        float ks[4], vs[4];
+        int base;
+    };
+    struct Ids {
+        int id[4];
+    };
+    // Positions that the unit's rows attend to, together.
+    struct Reach {
+        int lo, hi;
+    };
+    __device__ static void tile_pages(const Part& p, const Reach& r, int base, Ids& ids) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            int t = base + 16 * i;
+            t = t < r.lo ? r.lo : t >= r.hi ? r.hi - 1 : t;
+            ids.id[i] = uniform_load(p.u.table + t / PAGE);
+        }
+    }
+    __device__ static void tile_load(const AttendArgs& A, const Part& p, int base, const Ids& ids, Stage& s) {
+        const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+        s.base = base;
+        int mine = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int id = checked(A, ids.id[i]);
+            s.ks[i] = uniform_load(A.scale[0] + id * A.s_scale[0][0] + p.h * A.s_scale[0][1]);
+            s.vs[i] = uniform_load(A.scale[1] + id * A.s_scale[1][0] + p.h * A.s_scale[1][1]);
+            if (i == wave) mine = id;
+        }
+        const int off = (base + 16 * wave) % PAGE;
+        const char* const kp = A.cache[0] + mine * A.s_cache[0][0] + p.h * A.s_cache[0][1] + off * A.s_cache[0][2];
+        const char* const vp = A.cache[1] + mine * A.s_cache[1][0] + p.h * A.s_cache[1][1] + off * A.s_cache[1][2];
+        const int kd = (lane & 3) * (DP / 4), ko = (lane >> 2) * static_cast<int>(A.s_cache[0][2]) + kd;
+#pragma unroll
+        for (int j = 0; j < kChunks / 8; ++j) {
+            s.k[j] = pg_u32x4{0, 0, 0, 0};
+            if (D % 64 == 0 || kd + 16 * j < D) s.k[j] = *reinterpret_cast<const pg_u32x4*>(kp + ko + 16 * j);
+        }
+        const int vd = 4 * (lane & (DP / 4 - 1)), h = lane / (DP / 4), vt = static_cast<int>(A.s_cache[1][2]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            s.v[i] = 0;
+            if (h < 2 && (D % 64 == 0 || vd < D)) s.v[i] = *reinterpret_cast<const pg_u32*>(vp + (4 * h + (i & 3) + 2 * (i & 4)) * vt + vd);
+        }
+    }
+
+    __device__ static void tile_write(const Part& p, const Reach& r, const Stage& s, float inv, bool edge, Tiles& T, int buf) {
+        const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+        const int token = 16 * wave + (lane >> 2);
+#pragma unroll
+        for (int j = 0; j < kChunks / 8; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const pg_u32 w0 = s.k[j][2 * i], w1 = s.k[j][2 * i + 1];
+                T.k[buf][key_at(token, (lane & 3) * (kChunks / 4) + 2 * j + i)] =
+                    pg_u32x4{codes2<CT, H, false>(w0), codes2<CT, H, true>(w0), codes2<CT, H, false>(w1), codes2<CT, H, true>(w1)};
+            }
+        const int d = 4 * (lane & (DP / 4 - 1)), h = lane / (DP / 4);
+        pg_u32 v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = s.v[i];
+        if (edge) {
+            // What lies outside the unit's positions may be anything.
+            pg_u32 nan = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int at = s.base + 16 * wave + 4 * h + (i & 3) + 2 * (i & 4);
+                v[i] = at >= r.lo && at < r.hi ? v[i] : 0;
+                nan |= ((v[i] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+            }
+            if (CT == kE4M3 && nan) T.bad[buf] = 1;
+        }
+        if (DP == 64 && h >= 2) return;
+        // Relative scale of the values, exact for f16 outputs (p takes it there).
+        const _Float16 w = static_cast<_Float16>((wave == 0 ? s.vs[0] : wave == 1 ? s.vs[1] : wave == 2 ? s.vs[2] : s.vs[3]) * inv);
+        pg_u32x4 out[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const pg_u32 a = __builtin_amdgcn_perm(v[2 * e + 1], v[2 * e], 0x05010400u), b = __builtin_amdgcn_perm(v[2 * e + 1], v[2 * e], 0x07030602u);
+            const pg_u32 c[4] = {codes2<CT, true, false>(a), codes2<CT, true, true>(a), codes2<CT, true, false>(b), codes2<CT, true, true>(b)};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const pg_u32 x = c[q];
+                out[q][e] = TP == 1 ? __builtin_bit_cast(pg_u32, __builtin_bit_cast(pg_h2, x) * pg_h2{w, w}) : x;
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) T.v[buf][value_at(d + q, 2 * wave + h)] = out[q];
+    }
+
+    __device__ static pg_f32x16 mma32(pg_u32x4 a, pg_u32x4 b, pg_f32x16 c, bool half) {
+        if (half) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(pg_h8, a), __builtin_bit_cast(pg_h8, b), c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(pg_bf8, a), __builtin_bit_cast(pg_bf8, b), c, 0, 0, 0);
+    }
+
+    // False where the piece is to be done over.
+    __device__ static bool tiles(const AttendArgs& A, const Part& p) {
+        __shared__ Tiles T;
+        constexpr int KS = DP / 16, DT = DP / 32;
+        const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
+        const int row_i = n / GH, row_h = n - row_i * GH;
+        const bool valid = row_i < p.u.n && row_i < C && (HS == 1 || p.hs * RB + row_h < G);
+        // The lane's row attends to positions lo .. hi - 1; all the unit's rows to
+        // those of every tile between `from` and `till`.
+        const int hi = p.u.p0 + row_i + 1 < p.end ? p.u.p0 + row_i + 1 : p.end;
+        const int lo = WIN ? p.u.p0 + row_i + 1 - A.window : 0;
+        const int first = p.rq.length - p.rq.n + p.tile * kUnitTokens;  // position of the unit's first row
+        const int ntok = p.rq.n - p.tile * kUnitTokens < kUnitTokens ? p.rq.n - p.tile * kUnitTokens : kUnitTokens;
+        const int till = first + 1 < p.end ? first + 1 : p.end, from = WIN ? first + ntok - A.window : 0;
+        Reach reach;
+        reach.hi = first + ntok < p.end ? first + ntok : p.end;
+        reach.lo = WIN && first + 1 > A.window ? first + 1 - A.window : 0;
+        pg_u32x4 q[KS];
+        const char* const qp = A.q + ((p.row + row_i) * A.s_q[0] + (p.head + row_h) * A.s_q[1]) * 2;
+#pragma unroll
+        for (int j = 0; j < KS; ++j) {
+            const int d = 16 * j + 8 * h;
+            pg_u32x4 w = {0, 0, 0, 0};
+            if (valid && (D % 64 == 0 || d < D)) {
+                if constexpr (VEC) {
+                    w = *reinterpret_cast<const pg_u32x4*>(qp + d * 2);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        w[e] = static_cast<pg_u32>(*reinterpret_cast<const pg_u16*>(qp + d * 2 + 4 * e)) |
+                               static_cast<pg_u32>(*reinterpret_cast<const pg_u16*>(qp + d * 2 + 4 * e + 2)) << 16;
+                }
+            }
+            q[j] = w;
+        }
+        pg_f32x16 o[DT];
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
+        float m = -__builtin_inff(), l = 0.0f;
+        float unit = 1.0f, next = 1.0f;  // base of the sums, and of the tile that is converted next
+        bool done = true;
+        if (reach.hi > p.base) {
+            Ids ids;
+            Stage s;
+            // Whether the tile's values suit f16 relative to a base, which moves if need be.
+            auto settle = [&]() -> bool {
+                const float top = fmaxf(fmaxf(s.vs[0], s.vs[1]), fmaxf(s.vs[2], s.vs[3]));
+                const float low = fminf(fminf(s.vs[0], s.vs[1]), fminf(s.vs[2], s.vs[3]));
+                if (!(top <= next * 2.0f && low >= next * 0.125f)) {
+                    next = top;
+                    return top <= 0x1p40f && top >= 0x1p-40f && low >= top * 0.125f;
+                }
+                return true;
+            };
+            auto edge_of = [&](int base) { return base + kTile > till || base < from; };
+            tile_pages(p, reach, p.base, ids);
+            tile_load(A, p, p.base, ids, s);
+            tile_pages(p, reach, p.base + kTile, ids);
+            if (threadIdx.x < 2) T.bad[threadIdx.x] = 0;
+            __syncthreads();
+            done = settle();
+            if (done) {
+                tile_write(p, reach, s, 1.0f / next, edge_of(p.base), T, 0);
+                float ks[4], vs[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    ks[i] = s.ks[i];
+                    vs[i] = s.vs[i];
+                }
+                if (p.base + kTile < reach.hi) {
+                    tile_load(A, p, p.base + kTile, ids, s);
+                    tile_pages(p, reach, p.base + 2 * kTile, ids);
+                }
+                __syncthreads();
+                int buf = 0;
+                for (int base = p.base;; base += kTile, buf ^= 1) {
+                    const bool edge = edge_of(base), more = base + kTile < reach.hi;
+                    if (CT == kE4M3 && edge && (C > 1 || WIN || ntok > 1) && uniform(T.bad[buf])) {
+                        done = false;
+                        break;
+                    }
+                    if (next != unit) {
+                        const float f = unit / next;
+#pragma unroll
+                        for (int t = 0; t < DT; ++t) o[t] *= f;
+                        unit = next;
+                    }
+                    // Scores of the two halves of the tile.
+                    float x[2][16];
+#pragma unroll
+                    for (int a = 0; a < 2; ++a) {
+                        pg_f32x16 acc;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
+#pragma unroll
+                        for (int j = 0; j < KS; ++j) acc = mma32(T.k[buf][key_at(32 * a + n, 2 * j + h)], q[j], acc, H);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) x[a][i] = acc[i] * (ks[2 * a + (i >> 3)] * A.factor);
+                    }
+                    if (edge) {
+#pragma unroll
+                        for (int a = 0; a < 2; ++a)
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const int at = base + 32 * a + 8 * (i >> 2) + 4 * h + (i & 3);
+                                x[a][i] = at < hi && at >= lo ? x[a][i] : -__builtin_inff();
+                            }
+                    }
+                    float mx = x[0][0];
+#pragma unroll
+                    for (int a = 0; a < 2; ++a)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[a][i]);
+                    if (__ballot(mx > m + (kLift + kLag))) {
+                        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                        const float to = fmaxf(m, mx - kLift), f = to == m ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+                        m = to;
+                        l *= f;
+#pragma unroll
+                        for (int t = 0; t < DT; ++t) o[t] *= f;
+                    }
+                    const float ms = m == -__builtin_inff() ? 0.0f : m;
+                    float sum = 0.0f;
+                    pg_u32x4 pk[4][TP];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float w = TP == 1 ? 1.0f : vs[k] / unit;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float y0 = __builtin_amdgcn_exp2f(x[k >> 1][8 * (k & 1) + 2 * e] - ms);
+                            float y1 = __builtin_amdgcn_exp2f(x[k >> 1][8 * (k & 1) + 2 * e + 1] - ms);
+                            sum += y0 + y1;
+                            if (TP > 1) {
+                                y0 *= w;
+                                y1 *= w;
+                                // One value each for both parts: a conversion that takes in
+                                // the product rounds the exact one, another the float32 one.
+                                asm("" : "+v"(y0), "+v"(y1));
+                            }
+                            pg_h2 c = {static_cast<_Float16>(y0), static_cast<_Float16>(y1)};
+                            pk[k][0][e] = __builtin_bit_cast(pg_u32, c);
+                            if constexpr (TP > 1) {
+                                c = pg_h2{static_cast<_Float16>(y0 - static_cast<float>(c[0])), static_cast<_Float16>(y1 - static_cast<float>(c[1]))};
+                                pk[k][TP - 1][e] = __builtin_bit_cast(pg_u32, c);
+                            }
+                        }
+                    }
+                    l += sum;
+                    // The next tile, into the other buffer: its last readers have passed the barrier.
+                    if (more) {
+                        done = settle();
+                        if (!done) break;
+                        tile_write(p, reach, s, 1.0f / next, edge_of(base + kTile), T, buf ^ 1);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            ks[i] = s.ks[i];
+                            vs[i] = s.vs[i];
+                        }
+                        if (base + 2 * kTile < reach.hi) {
+                            tile_load(A, p, base + 2 * kTile, ids, s);
+                            tile_pages(p, reach, base + 3 * kTile, ids);
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+#pragma unroll
+                        for (int t = 0; t < DT; ++t)
+#pragma unroll
+                            for (int z = 0; z < TP; ++z) o[t] = mma32(T.v[buf][value_at(32 * t + n, 2 * k + h)], pk[k][z], o[t], true);
+                    if (!more) break;
+                    __syncthreads();
+                }
+            }
+        }
+        if (!done) return false;
+        l += __shfl_xor(l, 32, 64);
+        if (!valid) return true;
+        const int at = p.row + row_i, head = p.head + row_h;
+        if (p.pieces == 1) {
+            const float f = l == 0.0f ? 0.0f : unit / l;
+            char* const op = A.out + (at * A.s_out[0] + head * A.s_out[1]) * 2;
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int d = 32 * t + 8 * i + 4 * h;
+                    if (D % 64 != 0 && d >= D) continue;
+                    if constexpr (VEC) {
+                        pg_u32x2 w;
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float a = o[t][4 * i + 2 * e] * f, b = o[t][4 * i + 2 * e + 1] * f;
+                            if constexpr (QT == kF16) w[e] = __builtin_bit_cast(pg_u32, (pg_h2{static_cast<_Float16>(a), static_cast<_Float16>(b)}));
+                            else w[e] = __builtin_bit_cast(pg_u32, __builtin_convertvector((pg_f32x2{a, b}), pg_bf2));
+                        }
+                        *reinterpret_cast<pg_u32x2*>(op + d * 2) = w;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) store_elem<QT>(op + (d + e) * 2, o[t][4 * i + e] * f);
+                    }
+                }
+            if (LSE && h == 0) A.lse[at * A.s_lse[0] + head * A.s_lse[1]] = lse_of(m, l);
+        } else {
+            float* const part = part_sums(A, p, p.piece);
+            if (h == 0) {
+                part[n] = m;
+                part[RB + n] = l;
+            }
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<pg_f32x4*>(part + 2 * RB + n * DP + 32 * t + 8 * i + 4 * h) =
+                        pg_f32x4{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]} * unit;
+        }
+        return true;
+    }
+
+    __device__ static void prompt(const AttendArgs& A, int room) {
+        Part p;
+        if (!part_of(A, p)) return;
+        bool done = false;
+        if constexpr (TILES) done = tiles(A, p);
+        if (!done) Attend<D, PAGE, G, 1, QT, CT, WIN, LSE, VEC, true>::template rows<Attend>(A, p);
+        if (p.pieces > 1) join_pieces(A, room, p);
     }
 
     // Joins the pieces of the unit that workgroup blockIdx.x left open.

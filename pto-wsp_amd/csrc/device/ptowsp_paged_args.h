@@ -7,6 +7,7 @@ namespace ptowsp {
 constexpr int kPlanRows = 1024;     // rows of a workgroup of paged_plan's second launch
 constexpr int kAttendThreads = 256, kAttendTile = 128;  // a workgroup of paged_attention, and tokens of its tile
 constexpr int kSpanInts = 8;        // AttendArgs::spans of a workgroup
+constexpr int kUnitInts = 4;        // AttendArgs::units of an entry
 
 struct PlanArgs {
     const int* lengths;
@@ -59,6 +60,12 @@ struct AttendArgs {
     int* err;      // 7: starts, lengths or a page out of range
     int* spans;    // per workgroup: where the unit that it leaves open is joined
     float* parts;  // partial results, two per workgroup
+    // Prompts: the list of their units, and partial results of those that are cut.
+    int* units;
+    float* unit_parts;
+    int room, counters;  // entries and counters that `units` has room for
+    int cus;             // workgroups that run at once
+    int few;       // requests of at most so many rows are left to the kernel for few rows
 };
 
 }  // namespace ptowsp

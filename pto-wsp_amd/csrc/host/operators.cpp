@@ -237,13 +237,35 @@ struct AttendShape {
     int D, page, G, NT, type, code;
     bool window, lse, vec;
 };
-std::string attend_source(const AttendShape& s) {
+std::string attend_type(const AttendShape& s, int nt, bool prompt) {
     auto num = [](int v) { return std::to_string(v); };
-    const std::string t = "ptowsp::Attend<" + num(s.D) + ", " + num(s.page) + ", " + num(s.G) + ", " + num(s.NT) + ", " + num(s.type) + ", " + num(s.code) + ", " +
-                          flag(s.window) + ", " + flag(s.lse) + ", " + flag(s.vec) + ">";
+    return "ptowsp::Attend<" + num(s.D) + ", " + num(s.page) + ", " + num(s.G) + ", " + num(nt) + ", " + num(s.type) + ", " + num(s.code) + ", " +
+           flag(s.window) + ", " + flag(s.lse) + ", " + flag(s.vec) + ", " + flag(prompt) + ">";
+}
+std::string attend_source(const AttendShape& s) {
+    const std::string t = attend_type(s, s.NT, false);
     return entry_source("extern \"C\" __global__ __launch_bounds__(256, 2) void ptowsp_paged_attention(ptowsp::AttendArgs A) { " + t + "::run(A); }\n" +
                         "extern \"C\" __global__ __launch_bounds__(256) void ptowsp_paged_attention_join(ptowsp::AttendArgs A) { " + t + "::join(A); }\n");
 }
+// Prompts: 16 * nt query rows a wave, `waves` waves on a SIMD.
+struct PromptShape {
+    int nt, waves;
+};
+PromptShape prompt_shape(const AttendShape& s) {
+    return s.type != 2 && s.D <= 128 && s.page % 16 == 0 ? PromptShape{2, 2} : PromptShape{1, 2};
+}
+std::string prompt_source(const AttendShape& s) {
+    const PromptShape p = prompt_shape(s);
+    const std::string t = attend_type(s, p.nt, true);
+    return entry_source("extern \"C\" __global__ __launch_bounds__(1024) void ptowsp_paged_attention_units(ptowsp::AttendArgs A) { " + t + "::list_units<1024>(A, A.room, A.counters); }\n" +
+                        "extern \"C\" __global__ __launch_bounds__(256, " + std::to_string(p.waves) + ") void ptowsp_paged_attention_prompt(ptowsp::AttendArgs A) { " + t +
+                        "::prompt(A, A.room); }\n");
+}
+
+// Query rows of a request and key head up to which its keys are streamed by
+// all compute units alike (the kernel for few rows), and beyond which rows
+// share them.
+constexpr int kFewRows = 64;
 
 // 16 query rows at a time, or 32 where a request's rows of a key head are more
 // than 16 and the accumulators leave room.
@@ -284,16 +306,43 @@ void run_attend(const Node& n, const std::vector<Operand>& o, const OperatorRun&
     s.NT = attend_nt(rows, batch, s.G, D);
     s.type = type_id(q.dtype), s.code = code_id(o[1].dtype);
     s.window = A.window > 0, s.lse = lse, s.vec = vectors(q) && vectors(out);
+    // Requests of more tokens than a few go to the kernel for prompts, launched
+    // if there can be one while every other request has a token.
+    const int few = std::max(1, kFewRows / s.G);
+    const bool prompts = rows - batch >= few;
+    A.few = prompts ? few : 0x7FFFFFFF;
+    if (prompts) s.NT = s.G > 16 && D <= 128 ? 2 : 1;
     const int rb = 16 * s.NT, dp = (s.D + 63) / 64 * 64;
     const int64_t blocks = 2 * static_cast<int64_t>(run.cus);
-    const size_t span_bytes = (static_cast<size_t>(blocks) * kSpanInts * sizeof(int) + 255) / 256 * 256;
-    const size_t part_bytes = static_cast<size_t>(2 * blocks) * static_cast<size_t>(rb) * static_cast<size_t>(2 + dp) * sizeof(float);
-    char* const scratch = run.scratch(span_bytes + part_bytes);
+    auto whole = [](int64_t bytes) { return (static_cast<size_t>(bytes) + 255) / 256 * 256; };
+    const size_t span_bytes = whole(blocks * kSpanInts * 4);
+    size_t need = span_bytes + whole(2 * blocks * rb * (2 + dp) * 4);
+    PromptShape p{};
+    int64_t entries = 0;
+    size_t unit_bytes = 0;
+    if (prompts) {
+        // Units, pieces and partial results as list_units makes them, at most.
+        p = prompt_shape(s);
+        const int prb = 16 * p.nt, c = s.G <= prb ? prb / s.G : 1, hs = s.G <= prb ? 1 : (s.G + prb - 1) / prb;
+        A.cus = run.cus * p.waves;
+        entries = hs * (rows / (4 * c) + std::min(batch, rows / (A.few + 1))) + A.cus + 1;
+        if (entries > (int64_t(1) << 24)) stop(n, "too many rows for one call");
+        A.room = static_cast<int>(entries), A.counters = 2 * A.cus;
+        unit_bytes = whole((2 + entries * kUnitInts + A.counters) * 4);
+        need = std::max(need, unit_bytes + whole(int64_t(2) * A.cus * 4 * prb * (2 + dp) * 4));
+    }
+    char* const scratch = run.scratch(need);
     A.spans = reinterpret_cast<int*>(scratch);
     A.parts = reinterpret_cast<float*>(scratch + span_bytes);
     const std::string source = attend_source(s);
     run.launch(source, "ptowsp_paged_attention", blocks, 256, &A, sizeof A);
     run.launch(source, "ptowsp_paged_attention_join", blocks, 256, &A, sizeof A);
+    if (!prompts) return;
+    A.units = reinterpret_cast<int*>(scratch);
+    A.unit_parts = reinterpret_cast<float*>(scratch + unit_bytes);
+    const std::string more = prompt_source(s);
+    run.launch(more, "ptowsp_paged_attention_units", 1, 1024, &A, sizeof A);
+    run.launch(more, "ptowsp_paged_attention_prompt", entries * heads, 256, &A, sizeof A);
 }
 
 }  // namespace
@@ -383,9 +432,8 @@ std::vector<std::pair<std::string, std::string>> operator_sources(const Module& 
         return {{store_source(D, page, type_id(s.dtype[0]), code, true, store_chunk(s.of("k")[0], c[1], c[2])), "ptowsp_paged_store"}};
     const auto& q = s.of("q");
     const int G = static_cast<int>(q[1] / c[1]);
-    return {{attend_source({D, page, G, attend_nt(q[0], s.of("lengths")[0], G, D), type_id(s.dtype[0]), code, attr(n, "window") > 0,
-                            !s.of("lse").empty(), true}),
-             "ptowsp_paged_attention"}};
+    const AttendShape t{D, page, G, attend_nt(q[0], s.of("lengths")[0], G, D), type_id(s.dtype[0]), code, attr(n, "window") > 0, !s.of("lse").empty(), true};
+    return {{attend_source(t), "ptowsp_paged_attention"}, {prompt_source(t), "ptowsp_paged_attention_prompt"}};
 }
 
 }  // namespace ptowsp

@@ -92,13 +92,13 @@ def store(x, slots, codes, scale, kind):
 
 
 def attend(q, k, v, k_scale, v_scale, table, lengths, starts, scale, window=0):
-    """q [T, HQ, D], k, v [P, H, page, D] as numbers, all float64: out, lse, and the bound of the error
-    of an evaluation with float32 scores and sums, in units described in tolerance()."""
+    """q [T, HQ, D], k, v [P, H, page, D] as numbers, all float64: out, lse, and what bounds an evaluation's
+    error: sum(w |v|), the largest sum(|q k|) scale, sum(|v|)."""
     T, HQ, D = q.shape
     P, H, page, _ = k.shape
     G = HQ // H
     out, lse = np.full((T, HQ, D), np.nan), np.full((T, HQ), np.nan)
-    spread, swing = np.zeros((T, HQ, D)), np.zeros((T, HQ))
+    spread, swing, bulk = np.zeros((T, HQ, D)), np.zeros((T, HQ)), np.zeros((T, HQ, D))
     for b in range(len(lengths)):
         n, L = starts[b + 1] - starts[b], int(lengths[b])
         pages = table[b, :-(-L // page)]
@@ -118,5 +118,6 @@ def attend(q, k, v, k_scale, v_scale, table, lengths, starts, scale, window=0):
                 out[r, h] = e @ vt / e.sum()
                 lse[r, h] = m + np.log(e.sum())
                 spread[r, h] = e @ np.abs(vt) / e.sum()
+                bulk[r, h] = np.abs(vt).sum(0)
                 swing[r, h] = (np.abs(kt) @ np.abs(q[r, h])).max() * abs(scale)
-    return out, lse, spread, swing
+    return out, lse, spread, swing, bulk

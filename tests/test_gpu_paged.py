@@ -7,8 +7,10 @@ Attention: with w the softmax's weights, an output is off by at most
 
 its own rounding (half a step: bf16 2^-8, f16 2^-11, f32 2^-24); the scores' error ds = (D + 8) 2^-24
 max(sum |q k|) scale, a float32 dot product's and that of its two products, exponent and exp2, which moves
-numerator and denominator; p's parts (two bf16: 2^-18, three: 2^-24); the float32 sums over steps of 128
-tokens, the 32 inside an MFMA and the joins."""
+numerator and denominator; p's parts (two bf16: 2^-18, three: 2^-24; in prompts one f16 for bf16 outputs, times values and scales
+as f16: 3 2^-12); the float32 sums over
+steps of 128 tokens, the 32 inside an MFMA and the joins.  f16 parts below 2^-14 are off by 2^-25: a row's largest p
+is 2^10 or more there and a value's scale an eighth of the sums' unit or more, so by sum |v| 2^-32 in all."""
 
 import numpy as np
 import pytest
@@ -21,6 +23,7 @@ pytestmark = pytest.mark.gpu
 
 HALF = {"bf16": 2.0 ** -8, "f16": 2.0 ** -11, "f32": 2.0 ** -24}
 PARTS = {"bf16": 2.0 ** -18, "f16": 2.0 ** -18, "f32": 2.0 ** -24}
+PROMPT = {"bf16": 3 * 2.0 ** -12, "f16": 2.0 ** -18, "f32": 2.0 ** -24}
 
 
 def _torch():
@@ -341,11 +344,12 @@ def _attend_tensors(gpu, c, layout="plain"):
 
 
 def _tolerances(c, ref, window=0, scale=None):
-    out, lse, spread, swing = ref
+    out, lse, spread, swing, bulk = ref
     D, n = out.shape[-1], int(max(c["lengths"].max(initial=0), 1))
+    parts = (PROMPT if len(out) - len(c["lengths"]) >= 1 else PARTS)[c["dt"]]
     ds = (D + 8) * 2.0 ** -24 * np.maximum(swing, 1.0)
     sums = (n / 128 + 64 + D) * 2.0 ** -24
-    tol = HALF[c["dt"]] * np.abs(out) + spread * (2 * ds[..., None] + PARTS[c["dt"]] + sums)
+    tol = HALF[c["dt"]] * np.abs(out) + spread * (2 * ds[..., None] + parts + sums) + bulk * 2.0 ** -32
     tol = tol * (1 + 2 * HALF[c["dt"]]) + (2.0 ** -25 if c["dt"] == "f16" else 2.0 ** -140)
     return tol, 2 * ds + sums + 2.0 ** -23 * np.abs(np.where(np.isfinite(lse), lse, 0.0))
 
@@ -362,7 +366,8 @@ def _check_attend(c, t, ref, lse=True):
     tol, ltol = _tolerances(c, tuple(x[:n] for x in ref))
     assert np.array_equal(np.isnan(got[:n]), np.isnan(out))
     off = np.abs(got[:n] - out)
-    assert (np.isnan(out) | (off <= tol)).all(), f"off by {np.nanmax(off / tol):.3g} of the tolerance"
+    fine = bool((np.isnan(out) | (off <= tol)).all())
+    assert fine, f"off by {np.nanmax(off / tol):.3g} of the tolerance"
     assert (got[n:] == 7.0).all()
     if lse:
         a, b = t["lse"].double().cpu().numpy(), ref[1][:n]
@@ -446,6 +451,39 @@ def test_attention_many_short(gpu):
     rng = np.random.default_rng(4)
     lengths = rng.integers(1, 60, 400)
     _attend(gpu, _attend_case(rng, "bf16", "i8", 4, 2, 32, 16, lengths, [1] * 400))
+
+
+# Prompts beside single tokens: whole waves and odd ends, groups that do not divide the rows of a wave,
+# more query heads than rows, contexts long enough that a unit is cut into pieces.
+PROMPTS = [
+    (2, 4, 128, 16, [300, 70, 513], [300, 1, 200]),
+    (1, 5, 64, 16, [90, 2000], [77, 100]),
+    (2, 7, 80, 8, [150, 33], [90, 33]),
+    (1, 40, 32, 24, [60], [25]),
+    (1, 4, 128, 16, [9000, 40], [130, 17]),
+    (3, 1, 256, 64, [200, 90, 5], [180, 0, 5]),
+    (1, 100, 64, 1, [70, 30], [9, 30]),
+]
+
+
+@pytest.mark.parametrize("dt,kind", [("bf16", "e4m3"), ("f16", "i8"), ("f32", "e4m3")])
+@pytest.mark.parametrize("shape", range(len(PROMPTS)))
+def test_attention_prompts(gpu, shape, dt, kind):
+    H, G, D, page, lengths, counts = PROMPTS[shape]
+    _attend(gpu, _attend_case(np.random.default_rng(50 + shape), dt, kind, H, G, D, page, lengths, counts))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("page", [16, 8])
+def test_attention_prompt_scales(gpu, dt, page):
+    """Value scales that differ by more than f16 holds, from page to page and within 32 tokens."""
+    rng = np.random.default_rng(60)
+    c = _attend_case(rng, dt, "e4m3", 1, 4, 64, page, [700], [120], poison=False)
+    exps = np.repeat(rng.choice([-90.0, -38.0, -7.0, 0.0, 3.0], 700 // (4 * page) + 1), 4)[:-(-700 // page)] + rng.choice([0.0, 0.0, 9.0, 20.0], -(-700 // page))
+    if dt == "f16":
+        exps = np.minimum(exps - 3, 3)
+    c["scale"]["v"][c["table"][0, :len(exps)], 0] = 2.0 ** exps
+    _attend(gpu, c)
 
 
 def test_attention_large_scores(gpu):
