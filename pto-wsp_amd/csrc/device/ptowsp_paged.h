@@ -463,7 +463,7 @@ __device__ inline void store_rows(const StoreArgs& A) {
 // exp2(s - m) for an m that may lag the true maximum by a factor of 2^8.
 // Codes enter the MFMAs as they are, exactly; a page's scales multiply s and p
 // in float32.  q enters exactly too (an f32 as three bf16), p as two bf16
-// parts (2^-17 of it; three for f32 outputs), sums are float32.
+// parts (2^-16 of it; three for f32 outputs), sums are float32.
 // ---------------------------------------------------------------------------
 
 __device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -897,11 +897,10 @@ struct Attend {
         pg_i64 begin[2];  // where the piece starts: request, items before it
     };
 
-    __device__ static void run(const AttendArgs& A) {
-        __shared__ Shared sh;
+    __device__ static void run(const AttendArgs& A, int workgroup, Shared& sh) {
         const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
         const int wave = uniform(threadIdx.x >> 6);
-        const pg_i64 w = blockIdx.x;
+        const pg_i64 w = workgroup;
         int* const span = A.spans + w * kSpanInts;
         // The pieces: per request the items of its units, and their sums.
         const pg_i64 per = (A.batch + kAttendThreads - 1) / kAttendThreads, b0 = threadIdx.x * per;
@@ -914,7 +913,7 @@ struct Attend {
         pg_i64 total;
         pg_i64 before = block_scan<kAttendThreads>(sum, total, sh.scan);
         total = uniform64(total);
-        const pg_i64 pieces = total < static_cast<pg_i64>(gridDim.x) ? total : static_cast<pg_i64>(gridDim.x);
+        const pg_i64 pieces = total < A.blocks ? total : A.blocks;
         if (w >= pieces) {
             if (threadIdx.x == 0) span[0] = 0;
             return;
@@ -1102,10 +1101,11 @@ struct Attend {
         return s;
     }
 
-    // units: {entries, partial results}, then entries {request, tile, piece << 16
-    // | pieces, first partial result}; behind the room for them a counter for each partial result.
+    // units: {entries, pieces to be done over}, then entries {request, tile, piece
+    // << 16 | pieces, first partial result}; behind the room for them a counter for
+    // each partial result (zeroed here), and the pieces to be done over.
     template <int THREADS>
-    __device__ static void list_units(const AttendArgs& A, int room, int counters) {
+    __device__ static void list_units(const AttendArgs& A) {
         constexpr int BUCKETS = 128;
         __shared__ pg_i64 lds[THREADS / 64];
         __shared__ int many[BUCKETS], slots;
@@ -1116,9 +1116,10 @@ struct Attend {
         if (threadIdx.x == 0) {
             slots = 0;
             work = 0;
+            A.units[1] = 0;
         }
-        int* const count = A.units + 2 + room * kUnitInts;
-        for (int i = threadIdx.x; i < counters; i += THREADS) count[i] = 0;
+        int* const count = A.units + 2 + A.room * kUnitInts;
+        for (int i = threadIdx.x; i < A.counters; i += THREADS) count[i] = 0;
         __shared__ pg_i64 before[THREADS];
         pg_i64 units = 0, total;
         for (pg_i64 b = b0; b < b1; ++b) units += (request(A, b, false).n + kUnitTokens - 1) / kUnitTokens;
@@ -1127,27 +1128,35 @@ struct Attend {
         // Three passes over the units, spread over the threads: the work, the
         // sizes, the places.
         int limit = 0x7FFFFFFF;
+        struct Listed {
+            int b, tile, steps;
+        };
+        auto find = [&](pg_i64 i) {
+            int lo = 0, hi = THREADS;  // before[lo] <= i < before[hi]
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (before[mid] <= i) lo = mid;
+                else hi = mid;
+            }
+            pg_i64 b = lo * per, at = before[lo];
+            Request rq = request(A, b, false);
+            for (;;) {
+                const int tiles = (rq.n + kUnitTokens - 1) / kUnitTokens;
+                if (i < at + tiles) break;
+                at += tiles;
+                rq = request(A, ++b, false);
+            }
+            const Span s = span_of(A, rq, static_cast<int>(i - at));
+            return Listed{static_cast<int>(b), static_cast<int>(i - at), s.hi > s.lo ? (s.hi - s.lo + 31) / 32 : 1};
+        };
+        Listed own{};  // this thread's first unit
+        if (threadIdx.x < total) own = find(threadIdx.x);
 #pragma unroll 1
         for (int pass = 0; pass < 3; ++pass) {
             pg_u64 sum = 0;
             for (pg_i64 i = threadIdx.x; i < total; i += THREADS) {
-                int lo = 0, hi = THREADS;  // before[lo] <= i < before[hi]
-                while (hi - lo > 1) {
-                    const int mid = (lo + hi) >> 1;
-                    if (before[mid] <= i) lo = mid;
-                    else hi = mid;
-                }
-                pg_i64 b = lo * per, at = before[lo];
-                Request rq = request(A, b, false);
-                for (;;) {
-                    const int tiles = (rq.n + kUnitTokens - 1) / kUnitTokens;
-                    if (i < at + tiles) break;
-                    at += tiles;
-                    rq = request(A, ++b, false);
-                }
-                const int tile = static_cast<int>(i - at);
-                const Span s = span_of(A, rq, tile);
-                const int steps = s.hi > s.lo ? (s.hi - s.lo + 31) / 32 : 1;
+                const Listed unit = i < THREADS ? own : find(i);
+                const int tile = unit.tile, steps = unit.steps;
                 sum += static_cast<pg_u64>(steps);
                 if (pass == 0) continue;
                 const int pieces = (steps + limit - 1) / limit, size = steps < limit ? steps : limit;
@@ -1158,7 +1167,7 @@ struct Attend {
                     const int slot = pieces > 1 ? atomicAdd(&slots, pieces) : 0;
                     for (int k = 0; k < pieces; ++k) {
                         int* const e = A.units + 2 + static_cast<pg_i64>(place + hs * pieces + k) * kUnitInts;
-                        e[0] = static_cast<int>(b);
+                        e[0] = unit.b;
                         e[1] = tile * HS + hs;
                         e[2] = k << 16 | pieces;
                         e[3] = slot;
@@ -1191,12 +1200,9 @@ struct Attend {
         Request rq;
         Unit u;
     };
-    // False: no such entry.
-    __device__ static bool part_of(const AttendArgs& A, Part& p) {
+    __device__ static void part_of(const AttendArgs& A, int entry, int h, Part& p) {
         const int wave = uniform(threadIdx.x >> 6);
-        const int entry = static_cast<int>(blockIdx.x / A.heads);
-        p.h = static_cast<int>(blockIdx.x) - entry * A.heads;
-        if (entry >= A.units[0]) return false;
+        p.h = h;
         const int* const e = A.units + 2 + static_cast<pg_i64>(entry) * kUnitInts;
         const int code = uniform(e[1]), kp = uniform(e[2]);
         p.b = uniform(e[0]);
@@ -1223,7 +1229,6 @@ struct Attend {
         p.u.p0 = p.rq.length - p.rq.n + first;
         p.u.hi = p.u.n > 0 && p.u.p0 + p.u.n > 0 ? p.u.p0 + p.u.n : 0;
         p.u.lo = WIN && p.u.p0 + 1 > A.window ? p.u.p0 + 1 - A.window : 0;
-        return true;
     }
     __device__ static float* part_sums(const AttendArgs& A, const Part& p, int piece) {
         const int wave = uniform(threadIdx.x >> 6);
@@ -1284,40 +1289,61 @@ struct Attend {
     }
 
     // The last piece of a unit to end joins all of them.
-    __device__ static void join_pieces(const AttendArgs& A, int room, const Part& p) {
+    __device__ static void join_pieces(const AttendArgs& A, const Part& p) {
         const int lane = threadIdx.x & 63;
         __shared__ int arrived;
         __threadfence();
         __syncthreads();
         if (threadIdx.x == 0) {
-            int* const count = A.units + 2 + room * kUnitInts + p.slot * A.heads + p.h;
+            int* const count = A.units + 2 + A.room * kUnitInts + p.slot * A.heads + p.h;
             arrived = __hip_atomic_fetch_add(count, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
         }
         __syncthreads();
         if (arrived != p.pieces - 1 || p.u.n <= 0) return;
         __threadfence();
+        // Lane r < RB weighs row r; the lanes share the rows' numbers, four each.
+        constexpr int LANES = DP / 4, AT_ONCE = 64 / LANES, TURNS = RB / AT_ONCE;
         const pg_i64 next = static_cast<pg_i64>(A.heads) * 4 * PART;
         const float* const part = part_sums(A, p, 0);
-        for (int r = 0; r < RB; ++r) {
-            const int i = r / GH, hh = r - i * GH;
-            if (i >= p.u.n || i >= C || (HS > 1 && p.hs * RB + hh >= G)) continue;
-            float m = -__builtin_inff(), l = 0.0f;
+        const int sub = lane / LANES, d = 4 * (lane - sub * LANES), r = lane & (RB - 1);
+        float m = -__builtin_inff(), l = 0.0f;
+        auto valid = [&](int row) {
+            const int i = row / GH, hh = row - i * GH;
+            return i < p.u.n && i < C && (HS == 1 || p.hs * RB + hh < G);
+        };
+        if (valid(r))
             for (int k = 0; k < p.pieces; ++k) m = fmaxf(m, part[k * next + r]);
-            float o[NK];
+        pg_f32x4 o[TURNS];
 #pragma unroll
-            for (int j = 0; j < NK; ++j) o[j] = 0.0f;
-            for (int k = 0; k < p.pieces; ++k) {
-                const float mk = part[k * next + r], w = mk == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mk - m);
+        for (int t = 0; t < TURNS; ++t) o[t] = pg_f32x4{0, 0, 0, 0};
+        for (int k = 0; k < p.pieces; ++k) {
+            float w = 0.0f;
+            if (valid(r)) {
+                const float mk = part[k * next + r];
+                w = mk == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mk - m);
                 l += w * part[k * next + RB + r];
-#pragma unroll
-                for (int j = 0; j < NK; ++j) o[j] += w * part[k * next + 2 * RB + r * DP + 64 * j + lane];
             }
-            const float f = l == 0.0f ? 0.0f : 1.0f / l;
-            char* const q = A.out + ((p.row + i) * A.s_out[0] + (p.head + hh) * A.s_out[1]) * elem_size(QT);
 #pragma unroll
-            for (int j = 0; j < NK; ++j)
-                if (64 * j + lane < D) store_elem<QT>(q + (64 * j + lane) * elem_size(QT), o[j] * f);
-            if (LSE && lane == 0) A.lse[(p.row + i) * A.s_lse[0] + (p.head + hh) * A.s_lse[1]] = lse_of(m, l);
+            for (int t = 0; t < TURNS; ++t) {
+                const int row = t * AT_ONCE + sub;
+                const float f = __shfl(w, row, 64);
+                if (valid(row)) o[t] += f * *reinterpret_cast<const pg_f32x4*>(part + k * next + 2 * RB + row * DP + d);
+            }
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int t = 0; t < TURNS; ++t) {
+            const int row = t * AT_ONCE + sub;
+            const float f = __shfl(inv, row, 64);
+            if (!valid(row) || d >= D) continue;
+            const int i = row / GH, hh = row - i * GH;
+            char* const q = A.out + ((p.row + i) * A.s_out[0] + (p.head + hh) * A.s_out[1] + d) * elem_size(QT);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) store_elem<QT>(q + e * elem_size(QT), o[t][e] * f);
+        }
+        if (LSE && lane < RB && valid(r)) {
+            const int i = r / GH, hh = r - i * GH;
+            A.lse[(p.row + i) * A.s_lse[0] + (p.head + hh) * A.s_lse[1]] = lse_of(m, l);
         }
     }
 
@@ -1328,64 +1354,60 @@ struct Attend {
     // one barrier a tile.  A wave has 32 query rows: lane (n, h) of 32 x 2 holds
     // of row n tokens 8k + 4h .. + 3 of the scores, which are the P operand.
     // p enters as f16: between 2^10 and 2^14 at a row's maximum (kLift, kLag), so
-    // that no p that matters is subnormal; in one part for bf16 outputs (2^-12 of
-    // it, and as much of each value), in two for f16 ones.  Values are relative
-    // to a base that follows the pages' scales; where those spread too far for
-    // f16, or a NaN lies among values that some rows do not see, the waves do the
-    // piece over with bf16 parts (rows).
+    // that no p that matters is subnormal; in one part for bf16 outputs (2^-11 of
+    // it, as much again of each value and of its scale), in two for f16 ones.
+    // Values are relative to a base that follows the pages' scales (kLow, kHigh:
+    // as f16 values, no code of theirs is too large or loses more than one of a
+    // scale's 2^8; f16 outputs have the scales in p); where those spread too far
+    // for f16, or a NaN lies among values that some rows do not
+    // see, the waves do the piece over with bf16 parts (rows).
     static constexpr bool TILES = PROMPT && NT == 2 && PAGED16 && D <= 128 && QT != kF32;
     static constexpr int kTile = 64, kChunks = DP / 8;  // tokens; 16-byte pieces of a key
     static constexpr float kLift = 10.0f, kLag = 4.0f;
     static constexpr int TP = QT == kF16 ? 2 : 1;       // parts of p
+    static constexpr float kLow = TP == 1 ? 0x1p-8f : 0x1p-5f, kHigh = TP == 1 ? 0x1p6f : 2.0f, kStart = TP == 1 ? 0x1p-4f : 1.0f;
 
+    // LDS: {keys, values} of one tile, then of the next.  A key is a row of
+    // kChunks 16-byte pieces, a value's dimension one of 8 (64 tokens); a piece
+    // lies where the exclusive or of its number and a function of its row says, so
+    // that neither the waves' writes nor the MFMAs' reads meet in a bank more
+    // often than their size asks, and a lane's addresses differ in few bits.
+    static constexpr int kRow = 2 * DP, kPart = kTile * kRow, kBuffer = 2 * kPart;
     struct Tiles {
-        pg_u32x4 k[2][kTile * kChunks], v[2][DP * 8];
-        float ks[2][4];
+        alignas(1024) char bytes[2 * kBuffer];
+        float ks[4][4], vs[4][4];  // scales of four tiles in turn, one for each 16 tokens
         int bad[2];
     };
-    // Where a 16-byte piece lies, so that neither the waves' writes nor the
-    // MFMAs' reads meet in a bank more often than their size asks.
-    __device__ static int key_at(int token, int chunk) {
-        if constexpr (kChunks == 16) return token * 16 + (chunk ^ (token & 15));
-        else return token * 8 + (chunk ^ (token >> 1 & 7));
-    }
-    __device__ static int value_at(int d, int chunk) { return d * 8 + (chunk ^ (d >> 1 & 7) ^ (d >> 4 & 1)); }
+    __device__ static int key_bits(int token) { return kChunks == 16 ? token & 15 : token >> 1 & 7; }
+    __device__ static int value_bits(int d) { return (d >> 1 & 7) ^ (d >> 4 & 1); }
 
     struct Stage {
         pg_u32x4 k[kChunks / 8];
         pg_u32 v[8];
-        float ks[4], vs[4];
-        int base;
-    };
-    struct Ids {
-        int id[4];
     };
     // Positions that the unit's rows attend to, together.
     struct Reach {
         int lo, hi;
     };
-    __device__ static void tile_pages(const Part& p, const Reach& r, int base, Ids& ids) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            int t = base + 16 * i;
-            t = t < r.lo ? r.lo : t >= r.hi ? r.hi - 1 : t;
-            ids.id[i] = uniform_load(p.u.table + t / PAGE);
-        }
+    // Loads that all lanes share, as vector loads: they return in order, where
+    // scalar ones make every wait for LDS wait for them too.
+    template <class T>
+    __device__ static T shared_load(const T* p) {
+        int zero = 0;
+        asm volatile("" : "+v"(zero));
+        return p[zero];
     }
-    __device__ static void tile_load(const AttendArgs& A, const Part& p, int base, const Ids& ids, Stage& s) {
-        const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-        s.base = base;
-        int mine = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int id = checked(A, ids.id[i]);
-            s.ks[i] = uniform_load(A.scale[0] + id * A.s_scale[0][0] + p.h * A.s_scale[0][1]);
-            s.vs[i] = uniform_load(A.scale[1] + id * A.s_scale[1][0] + p.h * A.s_scale[1][1]);
-            if (i == wave) mine = id;
-        }
-        const int off = (base + 16 * wave) % PAGE;
-        const char* const kp = A.cache[0] + mine * A.s_cache[0][0] + p.h * A.s_cache[0][1] + off * A.s_cache[0][2];
-        const char* const vp = A.cache[1] + mine * A.s_cache[1][0] + p.h * A.s_cache[1][1] + off * A.s_cache[1][2];
+    // The page of this wave's 16 tokens of the tile at `base`.
+    __device__ static int tile_page(const AttendArgs& A, const Part& p, const Reach& r, int base) {
+        int t = base + 16 * uniform(threadIdx.x >> 6);
+        t = t < r.lo ? r.lo : t >= r.hi ? r.hi - 1 : t;
+        return shared_load(p.u.table + static_cast<pg_u32>(t) / PAGE);
+    }
+    __device__ static void tile_load(const AttendArgs& A, const Part& p, int base, int id, Stage& s) {
+        const int lane = threadIdx.x & 63;
+        const int off = static_cast<int>(static_cast<pg_u32>(base + 16 * uniform(threadIdx.x >> 6)) % PAGE);
+        const char* const kp = A.cache[0] + id * A.s_cache[0][0] + p.h * A.s_cache[0][1] + off * A.s_cache[0][2];
+        const char* const vp = A.cache[1] + id * A.s_cache[1][0] + p.h * A.s_cache[1][1] + off * A.s_cache[1][2];
         const int kd = (lane & 3) * (DP / 4), ko = (lane >> 2) * static_cast<int>(A.s_cache[0][2]) + kd;
 #pragma unroll
         for (int j = 0; j < kChunks / 8; ++j) {
@@ -1400,17 +1422,17 @@ struct Attend {
         }
     }
 
-    __device__ static void tile_write(const Part& p, const Reach& r, const Stage& s, float inv, bool edge, Tiles& T, int buf) {
+    // w: the values' scale relative to the base (f16 outputs: p takes it).
+    __device__ static void tile_write(const Reach& r, const Stage& s, int base, float w, bool edge, Tiles& T, int buf) {
         const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
         const int token = 16 * wave + (lane >> 2);
+        const int ko = buf * kBuffer + token * kRow + (((lane & 3) * (kChunks / 4)) ^ key_bits(token)) * 16;
 #pragma unroll
-        for (int j = 0; j < kChunks / 8; ++j)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const pg_u32 w0 = s.k[j][2 * i], w1 = s.k[j][2 * i + 1];
-                T.k[buf][key_at(token, (lane & 3) * (kChunks / 4) + 2 * j + i)] =
-                    pg_u32x4{codes2<CT, H, false>(w0), codes2<CT, H, true>(w0), codes2<CT, H, false>(w1), codes2<CT, H, true>(w1)};
-            }
+        for (int i = 0; i < kChunks / 4; ++i) {
+            const pg_u32 w0 = s.k[i >> 1][2 * (i & 1)], w1 = s.k[i >> 1][2 * (i & 1) + 1];
+            *reinterpret_cast<pg_u32x4*>(T.bytes + (ko ^ 16 * i)) =
+                pg_u32x4{codes2<CT, H, false>(w0), codes2<CT, H, true>(w0), codes2<CT, H, false>(w1), codes2<CT, H, true>(w1)};
+        }
         const int d = 4 * (lane & (DP / 4 - 1)), h = lane / (DP / 4);
         pg_u32 v[8];
 #pragma unroll
@@ -1420,28 +1442,26 @@ struct Attend {
             pg_u32 nan = 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int at = s.base + 16 * wave + 4 * h + (i & 3) + 2 * (i & 4);
+                const int at = base + 16 * wave + 4 * h + (i & 3) + 2 * (i & 4);
                 v[i] = at >= r.lo && at < r.hi ? v[i] : 0;
                 nan |= ((v[i] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
             }
             if (CT == kE4M3 && nan) T.bad[buf] = 1;
         }
         if (DP == 64 && h >= 2) return;
-        // Relative scale of the values, exact for f16 outputs (p takes it there).
-        const _Float16 w = static_cast<_Float16>((wave == 0 ? s.vs[0] : wave == 1 ? s.vs[1] : wave == 2 ? s.vs[2] : s.vs[3]) * inv);
-        pg_u32x4 out[4];
+        const _Float16 wh = static_cast<_Float16>(w);
+        const int vo = buf * kBuffer + kPart + d * 128 + ((2 * wave + h) ^ value_bits(d)) * 16;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const pg_u32 a = __builtin_amdgcn_perm(v[2 * e + 1], v[2 * e], 0x05010400u), b = __builtin_amdgcn_perm(v[2 * e + 1], v[2 * e], 0x07030602u);
-            const pg_u32 c[4] = {codes2<CT, true, false>(a), codes2<CT, true, true>(a), codes2<CT, true, false>(b), codes2<CT, true, true>(b)};
+        for (int q = 0; q < 4; ++q) {
+            pg_u32x4 out;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const pg_u32 x = c[q];
-                out[q][e] = TP == 1 ? __builtin_bit_cast(pg_u32, __builtin_bit_cast(pg_h2, x) * pg_h2{w, w}) : x;
+            for (int e = 0; e < 4; ++e) {
+                const pg_u32 a = __builtin_amdgcn_perm(v[2 * e + 1], v[2 * e], q < 2 ? 0x05010400u : 0x07030602u);
+                const pg_u32 x = q & 1 ? codes2<CT, true, true>(a) : codes2<CT, true, false>(a);
+                out[e] = TP == 1 ? __builtin_bit_cast(pg_u32, __builtin_bit_cast(pg_h2, x) * pg_h2{wh, wh}) : x;
             }
+            *reinterpret_cast<pg_u32x4*>(T.bytes + (vo ^ 16 * (q >> 1)) + 128 * q) = out;
         }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) T.v[buf][value_at(d + q, 2 * wave + h)] = out[q];
     }
 
     __device__ static pg_f32x16 mma32(pg_u32x4 a, pg_u32x4 b, pg_f32x16 c, bool half) {
@@ -1450,10 +1470,9 @@ struct Attend {
     }
 
     // False where the piece is to be done over.
-    __device__ static bool tiles(const AttendArgs& A, const Part& p) {
-        __shared__ Tiles T;
+    __device__ static bool tiles(const AttendArgs& A, const Part& p, Tiles& T) {
         constexpr int KS = DP / 16, DT = DP / 32;
-        const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
+        const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5, wave = uniform(threadIdx.x >> 6);
         const int row_i = n / GH, row_h = n - row_i * GH;
         const bool valid = row_i < p.u.n && row_i < C && (HS == 1 || p.hs * RB + row_h < G);
         // The lane's row attends to positions lo .. hi - 1; all the unit's rows to
@@ -1466,6 +1485,9 @@ struct Attend {
         Reach reach;
         reach.hi = first + ntok < p.end ? first + ntok : p.end;
         reach.lo = WIN && first + 1 > A.window ? first + 1 - A.window : 0;
+        // q, with the sign of `factor`: scores are products with scales >= 0.
+        const pg_u32 flip = A.factor < 0.0f ? 0x80008000u : 0u;
+        const float factor = fabsf(A.factor);
         pg_u32x4 q[KS];
         const char* const qp = A.q + ((p.row + row_i) * A.s_q[0] + (p.head + row_h) * A.s_q[1]) * 2;
 #pragma unroll
@@ -1482,7 +1504,7 @@ struct Attend {
                                static_cast<pg_u32>(*reinterpret_cast<const pg_u16*>(qp + d * 2 + 4 * e + 2)) << 16;
                 }
             }
-            q[j] = w;
+            q[j] = w ^ flip;
         }
         pg_f32x16 o[DT];
 #pragma unroll
@@ -1493,133 +1515,162 @@ struct Attend {
         float unit = 1.0f, next = 1.0f;  // base of the sums, and of the tile that is converted next
         bool done = true;
         if (reach.hi > p.base) {
-            Ids ids;
-            Stage s;
-            // Whether the tile's values suit f16 relative to a base, which moves if need be.
-            auto settle = [&]() -> bool {
-                const float top = fmaxf(fmaxf(s.vs[0], s.vs[1]), fmaxf(s.vs[2], s.vs[3]));
-                const float low = fminf(fminf(s.vs[0], s.vs[1]), fminf(s.vs[2], s.vs[3]));
-                if (!(top <= next * 2.0f && low >= next * 0.125f)) {
-                    next = top;
-                    return top <= 0x1p40f && top >= 0x1p-40f && low >= top * 0.125f;
+            float ks, vs;  // of this wave's tokens two tiles ahead
+            auto scales = [&](int id) {
+                ks = shared_load(A.scale[0] + id * A.s_scale[0][0] + p.h * A.s_scale[0][1]);
+                vs = shared_load(A.scale[1] + id * A.s_scale[1][0] + p.h * A.s_scale[1][1]);
+            };
+            auto post = [&](int slot) {
+                if (lane == 0) {
+                    T.ks[slot][wave] = ks;
+                    T.vs[slot][wave] = vs;
+                }
+            };
+            auto four = [&](const float* v) { return *reinterpret_cast<const pg_f32x4*>(v); };
+            auto frag = [&](int at) { return *reinterpret_cast<const pg_u32x4*>(T.bytes + at); };
+            // Whether a tile's values suit f16 relative to a base, which moves if need be.
+            float inv = 1.0f;  // 1 / next
+            auto settle = [&](const pg_f32x4 v) -> bool {
+                const float top = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), low = fminf(fminf(v[0], v[1]), fminf(v[2], v[3]));
+                if (__ballot(!(top <= next * kHigh && low >= next * kLow))) {
+                    next = top * kStart;
+                    inv = 1.0f / next;
+                    return __ballot(!(next <= 0x1p36f && next >= 0x1p-36f && low >= next * kLow)) == 0;
                 }
                 return true;
             };
             auto edge_of = [&](int base) { return base + kTile > till || base < from; };
-            tile_pages(p, reach, p.base, ids);
-            tile_load(A, p, p.base, ids, s);
-            tile_pages(p, reach, p.base + kTile, ids);
+            Stage s;
+            // Two tiles' scales and the first one's bytes, then the second's.
+            int id = checked(A, uniform(tile_page(A, p, reach, p.base)));
+            tile_load(A, p, p.base, id, s);
+            scales(id);
             if (threadIdx.x < 2) T.bad[threadIdx.x] = 0;
+            post(0);
+            id = checked(A, uniform(tile_page(A, p, reach, p.base + kTile)));
+            scales(id);
+            post(1);
+            int id2 = checked(A, uniform(tile_page(A, p, reach, p.base + 2 * kTile))), id3 = tile_page(A, p, reach, p.base + 3 * kTile);
             __syncthreads();
-            done = settle();
+            done = settle(four(T.vs[0]));
+            if (done) tile_write(reach, s, p.base, T.vs[0][wave] * inv, edge_of(p.base), T, 0);
             if (done) {
-                tile_write(p, reach, s, 1.0f / next, edge_of(p.base), T, 0);
-                float ks[4], vs[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    ks[i] = s.ks[i];
-                    vs[i] = s.vs[i];
-                }
-                if (p.base + kTile < reach.hi) {
-                    tile_load(A, p, p.base + kTile, ids, s);
-                    tile_pages(p, reach, p.base + 2 * kTile, ids);
-                }
+                if (p.base + kTile < reach.hi) tile_load(A, p, p.base + kTile, id, s);
+                scales(id2);
                 __syncthreads();
-                int buf = 0;
-                for (int base = p.base;; base += kTile, buf ^= 1) {
+                int buf = 0, slot = 0;
+                // Where the lane's first pieces of a key and a value lie.
+                const int k0 = n * kRow + (h ^ key_bits(n)) * 16, v0 = kPart + n * 128 + (h ^ value_bits(n)) * 16;
+                for (int base = p.base;; base += kTile, buf ^= 1, slot = (slot + 1) & 3) {
                     const bool edge = edge_of(base), more = base + kTile < reach.hi;
-                    if (CT == kE4M3 && edge && (C > 1 || WIN || ntok > 1) && uniform(T.bad[buf])) {
+                    if (CT == kE4M3 && edge && uniform(T.bad[buf])) {
                         done = false;
                         break;
                     }
-                    if (next != unit) {
+                    if (__ballot(next != unit)) {
                         const float f = unit / next;
 #pragma unroll
                         for (int t = 0; t < DT; ++t) o[t] *= f;
                         unit = next;
                     }
-                    // Scores of the two halves of the tile.
-                    float x[2][16];
+                    // Scores of the two halves of the tile, their keys read half a tile ahead.
+                    const int kb = k0 + buf * kBuffer, vb = v0 + buf * kBuffer;
+                    pg_f32x16 x[2];
+                    pg_u32x4 kf[KS], vf[DT];
 #pragma unroll
-                    for (int a = 0; a < 2; ++a) {
-                        pg_f32x16 acc;
+                    for (int j = 0; j < KS; ++j) kf[j] = frag(kb ^ 32 * j);
+                    pg_f32x4 f = four(T.ks[slot]) * factor;
+                    const pg_f32x4 vnext = four(T.vs[(slot + 1) & 3]);
+                    const float wnext = T.vs[(slot + 1) & 3][wave];
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
+                    for (int a = 0; a < 2; ++a)
 #pragma unroll
-                        for (int j = 0; j < KS; ++j) acc = mma32(T.k[buf][key_at(32 * a + n, 2 * j + h)], q[j], acc, H);
+                        for (int j = 0; j < KS; ++j) {
+                            pg_f32x16 zero;
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) x[a][i] = acc[i] * (ks[2 * a + (i >> 3)] * A.factor);
-                    }
+                            for (int i = 0; i < 16; ++i) zero[i] = 0.0f;
+                            x[a] = mma32(kf[j], q[j], j ? x[a] : zero, H);
+                            if (a == 0) kf[j] = frag((kb ^ 32 * j) + 32 * kRow);
+                        }
+#pragma unroll
+                    for (int t = 0; t < DT; ++t) vf[t] = frag(vb + 4096 * t);
+                    float mx[4];
                     if (edge) {
 #pragma unroll
                         for (int a = 0; a < 2; ++a)
 #pragma unroll
                             for (int i = 0; i < 16; ++i) {
                                 const int at = base + 32 * a + 8 * (i >> 2) + 4 * h + (i & 3);
-                                x[a][i] = at < hi && at >= lo ? x[a][i] : -__builtin_inff();
+                                x[a][i] = at < hi && at >= lo ? x[a][i] * f[2 * a + (i >> 3)] : -__builtin_inff();
                             }
+                        f = pg_f32x4{1.0f, 1.0f, 1.0f, 1.0f};
                     }
-                    float mx = x[0][0];
-#pragma unroll
-                    for (int a = 0; a < 2; ++a)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[a][i]);
-                    if (__ballot(mx > m + (kLift + kLag))) {
-                        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-                        const float to = fmaxf(m, mx - kLift), f = to == m ? 1.0f : __builtin_amdgcn_exp2f(m - to);
-                        m = to;
-                        l *= f;
-#pragma unroll
-                        for (int t = 0; t < DT; ++t) o[t] *= f;
-                    }
-                    const float ms = m == -__builtin_inff() ? 0.0f : m;
-                    float sum = 0.0f;
-                    pg_u32x4 pk[4][TP];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const float w = TP == 1 ? 1.0f : vs[k] / unit;
+                        mx[k] = x[k >> 1][8 * (k & 1)];
+#pragma unroll
+                        for (int i = 1; i < 8; ++i) mx[k] = fmaxf(mx[k], x[k >> 1][8 * (k & 1) + i]);
+                    }
+                    float peak = fmaxf(fmaxf(mx[0] * f[0], mx[1] * f[1]), fmaxf(mx[2] * f[2], mx[3] * f[3]));
+                    if (__ballot(peak > m + (kLift + kLag))) {
+                        peak = fmaxf(peak, __shfl_xor(peak, 32, 64));
+                        const float to = fmaxf(m, peak - kLift), g = to == m ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+                        m = to;
+                        l *= g;
+#pragma unroll
+                        for (int t = 0; t < DT; ++t) o[t] *= g;
+                    }
+                    const float ms = m == -__builtin_inff() ? 0.0f : m;
+                    // The next tile, into the other buffer: its last readers have passed the barrier.
+                    if (more) {
+                        done = settle(vnext);
+                        if (!done) break;
+                        tile_write(reach, s, base + kTile, wnext * inv, edge_of(base + kTile), T, buf ^ 1);
+                        post((slot + 2) & 3);
+                        const int ahead = checked(A, uniform(id3));  // loaded before the bytes: no wait for them
+                        if (base + 2 * kTile < reach.hi) tile_load(A, p, base + 2 * kTile, id2, s);
+                        id2 = ahead;
+                        scales(id2);
+                        id3 = tile_page(A, p, reach, base + 4 * kTile);
+                    }
+                    pg_f32x4 w;
+                    if constexpr (TP > 1) w = four(T.vs[slot]) / unit;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        pg_u32x4 pk[TP];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            float y0 = __builtin_amdgcn_exp2f(x[k >> 1][8 * (k & 1) + 2 * e] - ms);
-                            float y1 = __builtin_amdgcn_exp2f(x[k >> 1][8 * (k & 1) + 2 * e + 1] - ms);
-                            sum += y0 + y1;
-                            if (TP > 1) {
-                                y0 *= w;
-                                y1 *= w;
+                            pg_f32x2 y;
+#pragma unroll
+                            for (int z = 0; z < 2; ++z) y[z] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[k >> 1][8 * (k & 1) + 2 * e + z], f[k], -ms));
+                            if constexpr (TP > 1) {
+                                l += y[0] + y[1];
+                                float y0 = y[0] * w[k], y1 = y[1] * w[k];
                                 // One value each for both parts: a conversion that takes in
                                 // the product rounds the exact one, another the float32 one.
                                 asm("" : "+v"(y0), "+v"(y1));
+                                const pg_h2 c = __builtin_convertvector((pg_f32x2{y0, y1}), pg_h2);
+                                pk[0][e] = __builtin_bit_cast(pg_u32, c);
+                                pk[TP - 1][e] = __builtin_bit_cast(
+                                    pg_u32, __builtin_convertvector((pg_f32x2{y0 - static_cast<float>(c[0]), y1 - static_cast<float>(c[1])}), pg_h2));
+                            } else {
+                                const pg_h2 c = __builtin_convertvector(y, pg_h2);
+                                pk[0][e] = __builtin_bit_cast(pg_u32, c);
+                                // The sum of the weights as they are used, so that their rounding cancels in part.
+                                if constexpr (LSE) l += y[0] + y[1];
+                                else l = __builtin_amdgcn_fdot2(c, pg_h2{static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)}, l, false);
                             }
-                            pg_h2 c = {static_cast<_Float16>(y0), static_cast<_Float16>(y1)};
-                            pk[k][0][e] = __builtin_bit_cast(pg_u32, c);
-                            if constexpr (TP > 1) {
-                                c = pg_h2{static_cast<_Float16>(y0 - static_cast<float>(c[0])), static_cast<_Float16>(y1 - static_cast<float>(c[1]))};
-                                pk[k][TP - 1][e] = __builtin_bit_cast(pg_u32, c);
-                            }
                         }
-                    }
-                    l += sum;
-                    // The next tile, into the other buffer: its last readers have passed the barrier.
-                    if (more) {
-                        done = settle();
-                        if (!done) break;
-                        tile_write(p, reach, s, 1.0f / next, edge_of(base + kTile), T, buf ^ 1);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            ks[i] = s.ks[i];
-                            vs[i] = s.vs[i];
-                        }
-                        if (base + 2 * kTile < reach.hi) {
-                            tile_load(A, p, base + 2 * kTile, ids, s);
-                            tile_pages(p, reach, base + 3 * kTile, ids);
-                        }
-                    }
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
 #pragma unroll
                         for (int t = 0; t < DT; ++t)
 #pragma unroll
-                            for (int z = 0; z < TP; ++z) o[t] = mma32(T.v[buf][value_at(32 * t + n, 2 * k + h)], pk[k][z], o[t], true);
+                            for (int z = 0; z < TP; ++z) o[t] = mma32(vf[t], pk[z], o[t], true);
+                        if (k < 3) {
+#pragma unroll
+                            for (int t = 0; t < DT; ++t) vf[t] = frag((vb ^ 32 * (k + 1)) + 4096 * t);
+                        }
+                    }
                     if (!more) break;
                     __syncthreads();
                 }
@@ -1669,13 +1720,52 @@ struct Attend {
         return true;
     }
 
-    __device__ static void prompt(const AttendArgs& A, int room) {
+    // Narrow: the kernel for 16 rows a wave.
+    using Narrow = Attend<D, PAGE, G, 1, QT, CT, WIN, LSE, VEC, true>;
+    __device__ static int* over(const AttendArgs& A) { return A.units + 2 + A.room * kUnitInts + A.counters; }
+
+    __device__ static void prompt(const AttendArgs& A, Tiles& T) {
+        const int entry = static_cast<int>(blockIdx.x / A.heads), h = static_cast<int>(blockIdx.x) - entry * A.heads;
+        if (entry >= A.units[0]) return;
         Part p;
-        if (!part_of(A, p)) return;
-        bool done = false;
-        if constexpr (TILES) done = tiles(A, p);
-        if (!done) Attend<D, PAGE, G, 1, QT, CT, WIN, LSE, VEC, true>::template rows<Attend>(A, p);
-        if (p.pieces > 1) join_pieces(A, room, p);
+        part_of(A, entry, h, p);
+        if constexpr (TILES) {
+            if (!tiles(A, p, T)) {
+                if (threadIdx.x == 0) over(A)[atomicAdd(A.units + 1, 1)] = static_cast<int>(blockIdx.x);
+                return;
+            }
+        } else {
+            Narrow::template rows<Attend>(A, p);
+        }
+        if (p.pieces > 1) join_pieces(A, p);
+    }
+
+    // Prompts by the first workgroups, single tokens and few (F: the type for
+    // those) by the last `blocks`.
+    template <class F>
+    __device__ static void both(const AttendArgs& A) {
+        constexpr size_t few = sizeof(typename F::Shared), mine = TILES ? sizeof(Tiles) : 0;
+        __shared__ __attribute__((aligned(1024))) char lds[few > mine ? few : mine];
+        const int units = static_cast<int>(gridDim.x) - A.blocks;
+        if (static_cast<int>(blockIdx.x) < units) prompt(A, *reinterpret_cast<Tiles*>(lds));
+        else F::run(A, static_cast<int>(blockIdx.x) - units, *reinterpret_cast<typename F::Shared*>(lds));
+    }
+
+    // What remains: units that the workgroups for few rows left open, and pieces
+    // to be done over.
+    template <class F>
+    __device__ static void finish(const AttendArgs& A) {
+        F::join(A);
+        if constexpr (TILES) {
+            const int many = uniform(A.units[1]);
+            for (int i = blockIdx.x; i < many; i += gridDim.x) {
+                const int at = uniform(over(A)[i]), entry = at / A.heads;
+                Part p;
+                part_of(A, entry, at - entry * A.heads, p);
+                Narrow::template rows<Attend>(A, p);
+                if (p.pieces > 1) join_pieces(A, p);
+            }
+        }
     }
 
     // Joins the pieces of the unit that workgroup blockIdx.x left open.

@@ -58,6 +58,7 @@ struct AttendArgs {
     int window;    // 0: none
     float factor;  // scale * log2(e)
     int* err;      // 7: starts, lengths or a page out of range
+    int blocks;    // workgroups for few rows
     int* spans;    // per workgroup: where the unit that it leaves open is joined
     float* parts;  // partial results, two per workgroup
     // Prompts: the list of their units, and partial results of those that are cut.

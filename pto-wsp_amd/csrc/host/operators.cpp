@@ -242,24 +242,25 @@ std::string attend_type(const AttendShape& s, int nt, bool prompt) {
     return "ptowsp::Attend<" + num(s.D) + ", " + num(s.page) + ", " + num(s.G) + ", " + num(nt) + ", " + num(s.type) + ", " + num(s.code) + ", " +
            flag(s.window) + ", " + flag(s.lse) + ", " + flag(s.vec) + ", " + flag(prompt) + ">";
 }
-std::string attend_source(const AttendShape& s) {
-    const std::string t = attend_type(s, s.NT, false);
-    return entry_source("extern \"C\" __global__ __launch_bounds__(256, 2) void ptowsp_paged_attention(ptowsp::AttendArgs A) { " + t + "::run(A); }\n" +
-                        "extern \"C\" __global__ __launch_bounds__(256) void ptowsp_paged_attention_join(ptowsp::AttendArgs A) { " + t + "::join(A); }\n");
-}
+// Waves on a SIMD that the registers allow.
+int attend_waves(int64_t D) { return D > 128 ? 1 : 2; }
 // Prompts: 16 * nt query rows a wave, `waves` waves on a SIMD.
 struct PromptShape {
     int nt, waves;
 };
 PromptShape prompt_shape(const AttendShape& s) {
-    return s.type != 2 && s.D <= 128 && s.page % 16 == 0 ? PromptShape{2, 2} : PromptShape{1, 2};
+    return s.type != 2 && s.D <= 128 && s.page % 16 == 0 ? PromptShape{2, 2} : PromptShape{1, attend_waves(s.D)};
 }
-std::string prompt_source(const AttendShape& s) {
-    const PromptShape p = prompt_shape(s);
-    const std::string t = attend_type(s, p.nt, true);
-    return entry_source("extern \"C\" __global__ __launch_bounds__(1024) void ptowsp_paged_attention_units(ptowsp::AttendArgs A) { " + t + "::list_units<1024>(A, A.room, A.counters); }\n" +
-                        "extern \"C\" __global__ __launch_bounds__(256, " + std::to_string(p.waves) + ") void ptowsp_paged_attention_prompt(ptowsp::AttendArgs A) { " + t +
-                        "::prompt(A, A.room); }\n");
+std::string attend_source(const AttendShape& s, bool prompts) {
+    const std::string t = attend_type(s, s.NT, false), w = std::to_string(attend_waves(s.D));
+    auto entry = [](const char* bounds, const char* name, const std::string& body) {
+        return std::string("extern \"C\" __global__ __launch_bounds__(") + bounds + ") void ptowsp_paged_attention" + name + "(ptowsp::AttendArgs A) { " + body + "; }\n";
+    };
+    const std::string bounds = "256, " + w;
+    if (!prompts) return entry_source(entry(bounds.c_str(), "", "__shared__ " + t + "::Shared lds; " + t + "::run(A, blockIdx.x, lds)") + entry("256", "_join", t + "::join(A)"));
+    const std::string u = attend_type(s, prompt_shape(s).nt, true);
+    return entry_source(entry("1024", "_units", u + "::list_units<1024>(A)") + entry(bounds.c_str(), "_prompts", u + "::both<" + t + ">(A)") +
+                        entry(bounds.c_str(), "_finish", u + "::finish<" + t + ">(A)"));
 }
 
 // Query rows of a request and key head up to which its keys are streamed by
@@ -313,36 +314,37 @@ void run_attend(const Node& n, const std::vector<Operand>& o, const OperatorRun&
     A.few = prompts ? few : 0x7FFFFFFF;
     if (prompts) s.NT = s.G > 16 && D <= 128 ? 2 : 1;
     const int rb = 16 * s.NT, dp = (s.D + 63) / 64 * 64;
-    const int64_t blocks = 2 * static_cast<int64_t>(run.cus);
+    const int64_t blocks = attend_waves(D) * static_cast<int64_t>(run.cus);
     auto whole = [](int64_t bytes) { return (static_cast<size_t>(bytes) + 255) / 256 * 256; };
-    const size_t span_bytes = whole(blocks * kSpanInts * 4);
-    size_t need = span_bytes + whole(2 * blocks * rb * (2 + dp) * 4);
-    PromptShape p{};
+    const size_t span_bytes = whole(blocks * kSpanInts * 4), few_bytes = span_bytes + whole(2 * blocks * rb * (2 + dp) * 4);
+    size_t unit_bytes = 0, need = few_bytes;
     int64_t entries = 0;
-    size_t unit_bytes = 0;
     if (prompts) {
         // Units, pieces and partial results as list_units makes them, at most.
-        p = prompt_shape(s);
+        const PromptShape p = prompt_shape(s);
         const int prb = 16 * p.nt, c = s.G <= prb ? prb / s.G : 1, hs = s.G <= prb ? 1 : (s.G + prb - 1) / prb;
         A.cus = run.cus * p.waves;
-        entries = hs * (rows / (4 * c) + std::min(batch, rows / (A.few + 1))) + A.cus + 1;
-        if (entries > (int64_t(1) << 24)) stop(n, "too many rows for one call");
+        entries = hs * (rows / (4 * c) + std::min(batch, rows / (A.few + 1))) + A.cus / heads + 1;
+        if (entries * heads >= (int64_t(1) << 24)) stop(n, "too many rows for one call");
         A.room = static_cast<int>(entries), A.counters = 2 * A.cus;
-        unit_bytes = whole((2 + entries * kUnitInts + A.counters) * 4);
-        need = std::max(need, unit_bytes + whole(int64_t(2) * A.cus * 4 * prb * (2 + dp) * 4));
+        unit_bytes = whole((2 + entries * (kUnitInts + heads) + A.counters) * 4);
+        need += unit_bytes + whole(int64_t(2) * A.cus * 4 * prb * (2 + dp) * 4);
     }
     char* const scratch = run.scratch(need);
     A.spans = reinterpret_cast<int*>(scratch);
     A.parts = reinterpret_cast<float*>(scratch + span_bytes);
-    const std::string source = attend_source(s);
-    run.launch(source, "ptowsp_paged_attention", blocks, 256, &A, sizeof A);
-    run.launch(source, "ptowsp_paged_attention_join", blocks, 256, &A, sizeof A);
-    if (!prompts) return;
-    A.units = reinterpret_cast<int*>(scratch);
-    A.unit_parts = reinterpret_cast<float*>(scratch + unit_bytes);
-    const std::string more = prompt_source(s);
-    run.launch(more, "ptowsp_paged_attention_units", 1, 1024, &A, sizeof A);
-    run.launch(more, "ptowsp_paged_attention_prompt", entries * heads, 256, &A, sizeof A);
+    A.units = reinterpret_cast<int*>(scratch + few_bytes);
+    A.unit_parts = reinterpret_cast<float*>(scratch + few_bytes + unit_bytes);
+    A.blocks = static_cast<int>(blocks);
+    const std::string source = attend_source(s, prompts);
+    if (prompts) {
+        run.launch(source, "ptowsp_paged_attention_units", 1, 1024, &A, sizeof A);
+        run.launch(source, "ptowsp_paged_attention_prompts", entries * heads + blocks, 256, &A, sizeof A);
+        run.launch(source, "ptowsp_paged_attention_finish", blocks, 256, &A, sizeof A);
+    } else {
+        run.launch(source, "ptowsp_paged_attention", blocks, 256, &A, sizeof A);
+        run.launch(source, "ptowsp_paged_attention_join", blocks, 256, &A, sizeof A);
+    }
 }
 
 }  // namespace
@@ -433,7 +435,7 @@ std::vector<std::pair<std::string, std::string>> operator_sources(const Module& 
     const auto& q = s.of("q");
     const int G = static_cast<int>(q[1] / c[1]);
     const AttendShape t{D, page, G, attend_nt(q[0], s.of("lengths")[0], G, D), type_id(s.dtype[0]), code, attr(n, "window") > 0, !s.of("lse").empty(), true};
-    return {{attend_source(t), "ptowsp_paged_attention"}, {prompt_source(t), "ptowsp_paged_attention_prompt"}};
+    return {{attend_source(t, false), "ptowsp_paged_attention"}, {attend_source(t, true), "ptowsp_paged_attention_prompts"}};
 }
 
 }  // namespace ptowsp
