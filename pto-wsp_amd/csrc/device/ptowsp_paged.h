@@ -1422,46 +1422,43 @@ struct Attend {
         }
     }
 
-    // w: the values' scale relative to the base (f16 outputs: p takes it).
-    __device__ static void tile_write(const Reach& r, const Stage& s, int base, float w, bool edge, Tiles& T, int buf) {
-        const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-        const int token = 16 * wave + (lane >> 2);
-        const int ko = buf * kBuffer + token * kRow + (((lane & 3) * (kChunks / 4)) ^ key_bits(token)) * 16;
+    // A tile that some row does not see whole: what lies outside the unit's
+    // positions may be anything.
+    __device__ static void tile_edge(const Reach& r, Stage& s, int base, Tiles& T, int buf) {
+        const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane / (DP / 4);
+        pg_u32 nan = 0;
 #pragma unroll
-        for (int i = 0; i < kChunks / 4; ++i) {
+        for (int i = 0; i < 8; ++i) {
+            const int at = base + 16 * wave + 4 * h + (i & 3) + 2 * (i & 4);
+            s.v[i] = at >= r.lo && at < r.hi ? s.v[i] : 0;
+            nan |= ((s.v[i] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+        }
+        if (CT == kE4M3 && nan) T.bad[buf] = 1;
+    }
+
+    // The conversion of a wave's tokens, in kWrites steps of one LDS write each.
+    // w: the values' scale relative to the base (f16 outputs: p takes it).
+    static constexpr int kWrites = kChunks / 4 + 4;
+    __device__ static void tile_write(const Stage& s, _Float16 w, Tiles& T, int buf, int step) {
+        const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+        if (step < kChunks / 4) {
+            const int token = 16 * wave + (lane >> 2), i = step;
+            const int ko = buf * kBuffer + token * kRow + (((lane & 3) * (kChunks / 4)) ^ key_bits(token)) * 16;
             const pg_u32 w0 = s.k[i >> 1][2 * (i & 1)], w1 = s.k[i >> 1][2 * (i & 1) + 1];
             *reinterpret_cast<pg_u32x4*>(T.bytes + (ko ^ 16 * i)) =
                 pg_u32x4{codes2<CT, H, false>(w0), codes2<CT, H, true>(w0), codes2<CT, H, false>(w1), codes2<CT, H, true>(w1)};
+            return;
         }
-        const int d = 4 * (lane & (DP / 4 - 1)), h = lane / (DP / 4);
-        pg_u32 v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = s.v[i];
-        if (edge) {
-            // What lies outside the unit's positions may be anything.
-            pg_u32 nan = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int at = base + 16 * wave + 4 * h + (i & 3) + 2 * (i & 4);
-                v[i] = at >= r.lo && at < r.hi ? v[i] : 0;
-                nan |= ((v[i] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
-            }
-            if (CT == kE4M3 && nan) T.bad[buf] = 1;
-        }
-        if (DP == 64 && h >= 2) return;
-        const _Float16 wh = static_cast<_Float16>(w);
+        const int d = 4 * (lane & (DP / 4 - 1)), h = lane / (DP / 4), q = step - kChunks / 4;
         const int vo = buf * kBuffer + kPart + d * 128 + ((2 * wave + h) ^ value_bits(d)) * 16;
+        pg_u32x4 out;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            pg_u32x4 out;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const pg_u32 a = __builtin_amdgcn_perm(v[2 * e + 1], v[2 * e], q < 2 ? 0x05010400u : 0x07030602u);
-                const pg_u32 x = q & 1 ? codes2<CT, true, true>(a) : codes2<CT, true, false>(a);
-                out[e] = TP == 1 ? __builtin_bit_cast(pg_u32, __builtin_bit_cast(pg_h2, x) * pg_h2{wh, wh}) : x;
-            }
-            *reinterpret_cast<pg_u32x4*>(T.bytes + (vo ^ 16 * (q >> 1)) + 128 * q) = out;
+        for (int e = 0; e < 4; ++e) {
+            const pg_u32 a = __builtin_amdgcn_perm(s.v[2 * e + 1], s.v[2 * e], q < 2 ? 0x05010400u : 0x07030602u);
+            const pg_u32 x = q & 1 ? codes2<CT, true, true>(a) : codes2<CT, true, false>(a);
+            out[e] = TP == 1 ? __builtin_bit_cast(pg_u32, __builtin_bit_cast(pg_h2, x) * pg_h2{w, w}) : x;
         }
+        if (DP == 128 || h < 2) *reinterpret_cast<pg_u32x4*>(T.bytes + (vo ^ 16 * (q >> 1)) + 128 * q) = out;
     }
 
     __device__ static pg_f32x16 mma32(pg_u32x4 a, pg_u32x4 b, pg_f32x16 c, bool half) {
@@ -1553,7 +1550,12 @@ struct Attend {
             int id2 = checked(A, uniform(tile_page(A, p, reach, p.base + 2 * kTile))), id3 = tile_page(A, p, reach, p.base + 3 * kTile);
             __syncthreads();
             done = settle(four(T.vs[0]));
-            if (done) tile_write(reach, s, p.base, T.vs[0][wave] * inv, edge_of(p.base), T, 0);
+            if (edge_of(p.base)) tile_edge(reach, s, p.base, T, 0);
+            if (done) {
+                const _Float16 w = static_cast<_Float16>(T.vs[0][wave] * inv);
+#pragma unroll
+                for (int i = 0; i < kWrites; ++i) tile_write(s, w, T, 0, i);
+            }
             if (done) {
                 if (p.base + kTile < reach.hi) tile_load(A, p, p.base + kTile, id, s);
                 scales(id2);
@@ -1573,15 +1575,23 @@ struct Attend {
                         for (int t = 0; t < DT; ++t) o[t] *= f;
                         unit = next;
                     }
-                    // Scores of the two halves of the tile, their keys read half a tile ahead.
+                    const float wnext = T.vs[(slot + 1) & 3][wave];
+                    if (more) {
+                        done = settle(four(T.vs[(slot + 1) & 3]));
+                        if (!done) break;
+                        if (edge_of(base + kTile)) tile_edge(reach, s, base + kTile, T, buf ^ 1);
+                    }
+                    // Scores of the two halves of the tile, their keys read half a tile
+                    // ahead; beside the MFMAs the next tile's conversion into the other
+                    // buffer, whose last readers have passed the barrier (after the last
+                    // tile: of anything).  The order is kept as it stands here.
                     const int kb = k0 + buf * kBuffer, vb = v0 + buf * kBuffer;
+                    const _Float16 wh = static_cast<_Float16>(wnext * inv);
                     pg_f32x16 x[2];
                     pg_u32x4 kf[KS], vf[DT];
 #pragma unroll
                     for (int j = 0; j < KS; ++j) kf[j] = frag(kb ^ 32 * j);
                     pg_f32x4 f = four(T.ks[slot]) * factor;
-                    const pg_f32x4 vnext = four(T.vs[(slot + 1) & 3]);
-                    const float wnext = T.vs[(slot + 1) & 3][wave];
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int a = 0; a < 2; ++a)
@@ -1592,10 +1602,11 @@ struct Attend {
                             for (int i = 0; i < 16; ++i) zero[i] = 0.0f;
                             x[a] = mma32(kf[j], q[j], j ? x[a] : zero, H);
                             if (a == 0) kf[j] = frag((kb ^ 32 * j) + 32 * kRow);
-                        }
+                            else if (j < DT) vf[j] = frag(vb + 4096 * j);
 #pragma unroll
-                    for (int t = 0; t < DT; ++t) vf[t] = frag(vb + 4096 * t);
-                    float mx[4];
+                            for (int i = (a * KS + j) * kWrites / (2 * KS); i < (a * KS + j + 1) * kWrites / (2 * KS); ++i) tile_write(s, wh, T, buf ^ 1, i);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
                     if (edge) {
 #pragma unroll
                         for (int a = 0; a < 2; ++a)
@@ -1606,6 +1617,7 @@ struct Attend {
                             }
                         f = pg_f32x4{1.0f, 1.0f, 1.0f, 1.0f};
                     }
+                    float mx[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         mx[k] = x[k >> 1][8 * (k & 1)];
@@ -1622,11 +1634,7 @@ struct Attend {
                         for (int t = 0; t < DT; ++t) o[t] *= g;
                     }
                     const float ms = m == -__builtin_inff() ? 0.0f : m;
-                    // The next tile, into the other buffer: its last readers have passed the barrier.
                     if (more) {
-                        done = settle(vnext);
-                        if (!done) break;
-                        tile_write(reach, s, base + kTile, wnext * inv, edge_of(base + kTile), T, buf ^ 1);
                         post((slot + 2) & 3);
                         const int ahead = checked(A, uniform(id3));  // loaded before the bytes: no wait for them
                         if (base + 2 * kTile < reach.hi) tile_load(A, p, base + 2 * kTile, id2, s);
@@ -1636,41 +1644,46 @@ struct Attend {
                     }
                     pg_f32x4 w;
                     if constexpr (TP > 1) w = four(T.vs[slot]) / unit;
+                    // p of the next 16 tokens beside the MFMAs of these.
+                    pg_u32x4 pk[2][TP];
+                    auto weigh_two = [&](int k, int e) {
+                        pg_f32x2 y;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        pg_u32x4 pk[TP];
+                        for (int z = 0; z < 2; ++z) y[z] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[k >> 1][8 * (k & 1) + 2 * e + z], f[k], -ms));
+                        if constexpr (TP > 1) {
+                            l += y[0] + y[1];
+                            float y0 = y[0] * w[k], y1 = y[1] * w[k];
+                            // One value each for both parts: a conversion that takes in
+                            // the product rounds the exact one, another the float32 one.
+                            asm("" : "+v"(y0), "+v"(y1));
+                            const pg_h2 c = __builtin_convertvector((pg_f32x2{y0, y1}), pg_h2);
+                            pk[k & 1][0][e] = __builtin_bit_cast(pg_u32, c);
+                            pk[k & 1][TP - 1][e] = __builtin_bit_cast(
+                                pg_u32, __builtin_convertvector((pg_f32x2{y0 - static_cast<float>(c[0]), y1 - static_cast<float>(c[1])}), pg_h2));
+                        } else {
+                            const pg_h2 c = __builtin_convertvector(y, pg_h2);
+                            pk[k & 1][0][e] = __builtin_bit_cast(pg_u32, c);
+                            // The sum of the weights as they are used, so that their rounding cancels in part.
+                            if constexpr (LSE) l += y[0] + y[1];
+                            else l = __builtin_amdgcn_fdot2(c, pg_h2{static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)}, l, false);
+                        }
+                    };
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            pg_f32x2 y;
+                    for (int e = 0; e < 4; ++e) weigh_two(0, e);
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                            for (int z = 0; z < 2; ++z) y[z] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[k >> 1][8 * (k & 1) + 2 * e + z], f[k], -ms));
-                            if constexpr (TP > 1) {
-                                l += y[0] + y[1];
-                                float y0 = y[0] * w[k], y1 = y[1] * w[k];
-                                // One value each for both parts: a conversion that takes in
-                                // the product rounds the exact one, another the float32 one.
-                                asm("" : "+v"(y0), "+v"(y1));
-                                const pg_h2 c = __builtin_convertvector((pg_f32x2{y0, y1}), pg_h2);
-                                pk[0][e] = __builtin_bit_cast(pg_u32, c);
-                                pk[TP - 1][e] = __builtin_bit_cast(
-                                    pg_u32, __builtin_convertvector((pg_f32x2{y0 - static_cast<float>(c[0]), y1 - static_cast<float>(c[1])}), pg_h2));
-                            } else {
-                                const pg_h2 c = __builtin_convertvector(y, pg_h2);
-                                pk[0][e] = __builtin_bit_cast(pg_u32, c);
-                                // The sum of the weights as they are used, so that their rounding cancels in part.
-                                if constexpr (LSE) l += y[0] + y[1];
-                                else l = __builtin_amdgcn_fdot2(c, pg_h2{static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)}, l, false);
+                    for (int k = 0; k < 4; ++k)
+#pragma unroll
+                        for (int t = 0; t < DT; ++t) {
+#pragma unroll
+                            for (int z = 0; z < TP; ++z) o[t] = mma32(vf[t], pk[k & 1][z], o[t], true);
+                            if (k < 3) {
+                                vf[t] = frag((vb ^ 32 * (k + 1)) + 4096 * t);
+#pragma unroll
+                                for (int e = t * 4 / DT; e < (t + 1) * 4 / DT; ++e) weigh_two(k + 1, e);
                             }
+                            __builtin_amdgcn_sched_barrier(0);
                         }
-#pragma unroll
-                        for (int t = 0; t < DT; ++t)
-#pragma unroll
-                            for (int z = 0; z < TP; ++z) o[t] = mma32(vf[t], pk[z], o[t], true);
-                        if (k < 3) {
-#pragma unroll
-                            for (int t = 0; t < DT; ++t) vf[t] = frag((vb ^ 32 * (k + 1)) + 4096 * t);
-                        }
-                    }
                     if (!more) break;
                     __syncthreads();
                 }
