@@ -262,22 +262,26 @@ __device__ inline pg_u32 codes2(pg_u32 w) {
     }
 }
 
-// Four numbers, already multiplied by 1 / scale, as codes.
-template <int CT>
+// Four numbers, already multiplied by 1 / scale, as codes.  INSIDE: none is NaN,
+// and none beyond the largest code by more than a few roundings of float32,
+// which round away again.
+template <int CT, bool INSIDE>
 __device__ inline pg_u32 encode4(const float* y) {
     constexpr float top = code_top<CT>();
     float z[4];
     bool nan[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        nan[i] = y[i] != y[i];
-        z[i] = fminf(fmaxf(y[i], -top), top);
+        nan[i] = !INSIDE && y[i] != y[i];
+        z[i] = INSIDE ? y[i] : fminf(fmaxf(y[i], -top), top);
     }
     pg_u32 w;
     if constexpr (CT == kI8) {
-        w = 0;
+        // 1.5 * 2^23 more: rounded to a whole number whose byte is the lowest.
+        pg_u32 c[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w |= (static_cast<pg_u32>(nan[i] ? 0 : static_cast<int>(rintf(z[i]))) & 0xFFu) << (8 * i);
+        for (int i = 0; i < 4; ++i) c[i] = __float_as_uint((nan[i] ? 0.0f : z[i]) + 0x1.8p23f);
+        w = __builtin_amdgcn_perm(__builtin_amdgcn_perm(c[3], c[2], 0x0C0C0400u), __builtin_amdgcn_perm(c[1], c[0], 0x0C0C0400u), 0x05040100u);
     } else {
         int c = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
         c = __builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], c, true);
@@ -303,49 +307,86 @@ __device__ inline float decode1(pg_u32 w, int i) {
 // the largest finite |x| of the run, the scale (kept tokens: at least the old
 // one), the kept codes anew where it grew, the run's codes.  Every quotient is
 // the product with 1 / scale, rounded as float32 values are, so that the codes
-// follow from the inputs bit by bit.  Bound by HBM: x is read once (its second
-// reading hits the caches: a run is at most a page), codes are written once.
+// follow from the inputs bit by bit.  Infinities and NaN are met only where the
+// run's largest bits say so; their runs are read a second time.
 // ---------------------------------------------------------------------------
 
-// Eight elements of x at p.
+typedef unsigned short pg_us2 __attribute__((ext_vector_type(2)));
+template <bool V>
+struct Flag {
+    static constexpr bool value = V;
+};
+
+// Eight elements of x at p, as they are.
+template <int T>
+struct Eight {
+    pg_u32 w[T == kF32 ? 8 : 4];
+};
 template <int T, bool VEC>
-__device__ inline void load8(const char* p, float* x) {
-    if constexpr (VEC && T == kF32) {
-        const pg_f32x4 a = *reinterpret_cast<const pg_f32x4*>(p), b = *reinterpret_cast<const pg_f32x4*>(p + 16);
+__device__ inline void load8(const char* p, Eight<T>& x) {
+    constexpr int N = T == kF32 ? 8 : 4;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[i] = a[i];
-            x[4 + i] = b[i];
-        }
-    } else if constexpr (VEC) {
-        const pg_u32x4 a = *reinterpret_cast<const pg_u32x4*>(p);
+    for (int i = 0; i < N; i += 4) {
+        if constexpr (VEC) {
+            const pg_u32x4 a = *reinterpret_cast<const pg_u32x4*>(p + 4 * i);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const pg_u32 w = a[i];  // the bit cast takes a value: of a vector's element it reads element 0
-            if constexpr (T == kF16) {
-                const pg_h2 h = __builtin_bit_cast(pg_h2, w);
-                x[2 * i] = static_cast<float>(h[0]);
-                x[2 * i + 1] = static_cast<float>(h[1]);
-            } else {
-                x[2 * i] = __uint_as_float(w << 16);
-                x[2 * i + 1] = __uint_as_float(w & 0xFFFF0000u);
+            for (int k = 0; k < 4; ++k) x.w[i + k] = a[k];
+        } else {
+#pragma unroll
+            for (int k = i; k < i + 4; ++k) {
+                if constexpr (T == kF32) {
+                    x.w[k] = *reinterpret_cast<const pg_u32*>(p + 4 * k);
+                } else {
+                    x.w[k] = static_cast<pg_u32>(*reinterpret_cast<const pg_u16*>(p + 4 * k)) |
+                             static_cast<pg_u32>(*reinterpret_cast<const pg_u16*>(p + 4 * k + 2)) << 16;
+                }
             }
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = elem_f32<T>(p + i * elem_size(T));
     }
+}
+template <int T>
+__device__ inline void values8(const Eight<T>& x, float* y) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if constexpr (T == kF32) {
+            y[i] = __uint_as_float(x.w[i]);
+        } else if constexpr (T == kF16) {
+            const pg_u32 w = x.w[i >> 1];
+            y[i] = static_cast<float>(__builtin_bit_cast(pg_h2, w)[i & 1]);
+        } else {
+            y[i] = __uint_as_float(i & 1 ? x.w[i >> 1] & 0xFFFF0000u : x.w[i >> 1] << 16);
+        }
+    }
+}
+// The largest |x| as bits without sign, which are ordered as the numbers are,
+// NaN above infinity; of 16-bit types two at once.
+template <int T>
+__device__ inline pg_u32 most8(const Eight<T>& x, pg_u32 most) {
+#pragma unroll
+    for (int i = 0; i < (T == kF32 ? 8 : 4); ++i) {
+        if constexpr (T == kF32) {
+            const pg_u32 a = x.w[i] & 0x7FFFFFFFu;
+            most = a > most ? a : most;
+        } else {
+            const pg_u32 a = x.w[i] & 0x7FFF7FFFu;
+            most = __builtin_bit_cast(pg_u32, __builtin_elementwise_max(__builtin_bit_cast(pg_us2, a), __builtin_bit_cast(pg_us2, most)));
+        }
+    }
+    return most;
 }
 
 template <int D, int PAGE, int T, int CT, bool VEC, int CHUNK>
 __device__ inline void store_rows(const StoreArgs& A) {
     const int heads = A.heads;
     constexpr int PARTS = D / 8;  // pieces of eight elements in a row
+    // Pieces that a lane holds: a page's, of 64 registers at most.
+    constexpr int NEED = (PAGE * PARTS + 63) / 64, ROUNDS = NEED < 8 ? NEED : 8;
     const int lane = threadIdx.x & 63;
-    const pg_i64 item = static_cast<pg_i64>(blockIdx.x) * (blockDim.x >> 6) + (threadIdx.x >> 6);
-    const pg_i64 chunk = item / (2 * heads);
-    const int which = static_cast<int>(item - chunk * (2 * heads)), h = which >> 1, kv = which & 1;
-    const pg_i64 row0 = chunk * CHUNK;
+    // Fewer than 2^24 workgroups of four waves.
+    const pg_u32 item = blockIdx.x * (blockDim.x >> 6) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const pg_u32 chunk = item / static_cast<pg_u32>(2 * heads);
+    const int which = static_cast<int>(item - chunk * static_cast<pg_u32>(2 * heads)), h = which >> 1, kv = which & 1;
+    const pg_i64 row0 = static_cast<pg_i64>(chunk) * CHUNK;
     if (row0 >= A.rows) return;
     const pg_i64 slots_end = A.pages * PAGE;
     auto page_of = [&](pg_i64 r) -> int {  // -1: not stored
@@ -374,32 +415,70 @@ __device__ inline void store_rows(const StoreArgs& A) {
             const pg_u64 out = ~__ballot(in);
             const int more = out ? __builtin_ctzll(out) : 64;
             const int off = lane < more ? A.slots[(r0 + n + lane) * A.s_slots] - page * PAGE : PAGE;
-            const int first = n == 0 ? __shfl(off, 0, 64) : low;
-            dense &= __ballot(lane < more && off != first + n + lane) == 0;
-            int l = off;
+            if (n == 0) low = __builtin_amdgcn_readfirstlane(off);
+            dense = dense && __ballot(lane < more && off != low + n + lane) == 0;
+            if (!dense) {
+                int l = off;
 #pragma unroll
-            for (int d = 32; d >= 1; d >>= 1) {
-                const int y = __shfl_xor(l, d, 64);
-                l = y < l ? y : l;
+                for (int d = 32; d >= 1; d >>= 1) {
+                    const int y = __shfl_xor(l, d, 64);
+                    l = y < l ? y : l;
+                }
+                low = l < low ? l : low;
             }
-            low = l < low ? l : low;
             n += more;
             if (more < 64) break;
         }
         const char* const xr = x + r0 * A.s_x[kv][0] * elem_size(T);
-        float most = 0.0f;
-        for (int e = lane; e < n * PARTS; e += 64) {
-            const int t = e / PARTS;
-            float y[8];
-            load8<T, VEC>(xr + (t * A.s_x[kv][0] + (e - t * PARTS) * 8) * elem_size(T), y);
+        auto from = [&](int t, int part) { return xr + (t * A.s_x[kv][0] + part * 8) * elem_size(T); };
+        // The run's first pieces stay in registers, all their loads in flight at
+        // once; what is longer (or not in order) is read a second time.
+        Eight<T> held[ROUNDS];
+        const char* const own = from(lane / PARTS, lane % PARTS);
+        pg_u32 bits = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float a = fabsf(y[i]);
-                if (a < __builtin_inff()) most = fmaxf(most, a);
-            }
+        for (int k = 0; k < ROUNDS; ++k) {
+            const int e = lane + 64 * k;
+            held[k] = {};
+            if (e < n * PARTS) load8<T, VEC>(64 % PARTS == 0 ? own + k * (64 / PARTS) * A.s_x[kv][0] * elem_size(T) : from(e / PARTS, e % PARTS), held[k]);
         }
 #pragma unroll
-        for (int d = 32; d >= 1; d >>= 1) most = fmaxf(most, __shfl_xor(most, d, 64));
+        for (int k = 0; k < ROUNDS; ++k) bits = most8<T>(held[k], bits);
+        for (int e = lane + 64 * ROUNDS; e < n * PARTS; e += 64) {
+            Eight<T> x8;
+            load8<T, VEC>(from(e / PARTS, e % PARTS), x8);
+            bits = most8<T>(x8, bits);
+        }
+        if constexpr (T != kF32) bits = (bits & 0xFFFFu) > bits >> 16 ? bits & 0xFFFFu : bits >> 16;
+#pragma unroll
+        for (int d = 32; d >= 1; d >>= 1) {
+            const pg_u32 y = static_cast<pg_u32>(__shfl_xor(static_cast<int>(bits), d, 64));
+            bits = y > bits ? y : bits;
+        }
+        constexpr pg_u32 kInf = T == kF32 ? 0x7F800000u : T == kF16 ? 0x7C00u : 0x7F80u;
+        const bool finite = __builtin_amdgcn_readfirstlane(bits) < kInf;
+        float most = 0.0f;
+        if (finite) {
+            Eight<T> x8 = {};
+            float y[8];
+            x8.w[0] = bits;
+            values8<T>(x8, y);
+            most = y[0];
+        } else {
+            for (int e = lane; e < n * PARTS; e += 64) {
+                Eight<T> x8;
+                float y[8];
+                load8<T, VEC>(from(e / PARTS, e % PARTS), x8);
+                values8<T>(x8, y);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float a = fabsf(y[i]);
+                    if (a < __builtin_inff()) most = fmaxf(most, a);
+                }
+            }
+#pragma unroll
+            for (int d = 32; d >= 1; d >>= 1) most = fmaxf(most, __shfl_xor(most, d, 64));
+        }
         float* const sp = A.scale[kv] + page * A.s_scale[kv][0] + h * A.s_scale[kv][1];
         const float old = low > 0 ? *sp : 0.0f;
         const float scale = fmaxf(fmaxf(most / code_top<CT>(), 0x1p-126f), old);
@@ -415,26 +494,39 @@ __device__ inline void store_rows(const StoreArgs& A) {
                     float y[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) y[i] = (decode1<CT>(w[k], i) * old) * inverse;
-                    w[k] = encode4<CT>(y);
+                    w[k] = encode4<CT, false>(y);
                 }
                 *c = w;
             }
         }
-        auto put = [&](int t, int part) {
+        auto code = [&](auto inside, const Eight<T>& x8, char* to) {
+            constexpr bool INSIDE = decltype(inside)::value;
             float y[8];
-            load8<T, VEC>(xr + (t * A.s_x[kv][0] + part * 8) * elem_size(T), y);
+            values8<T>(x8, y);
 #pragma unroll
             for (int i = 0; i < 8; ++i) y[i] = y[i] * inverse;
-            const int off = A.slots[(r0 + t) * A.s_slots] - page * PAGE;
-            *reinterpret_cast<pg_u32x2*>(cp + off * A.s_cache[kv][2] + part * 8) = pg_u32x2{encode4<CT>(y), encode4<CT>(y + 4)};
+            *reinterpret_cast<pg_u32x2*>(to) = pg_u32x2{encode4<CT, INSIDE>(y), encode4<CT, INSIDE>(y + 4)};
         };
-        if (dense) {
-            for (int e = lane; e < n * PARTS; e += 64) put(e / PARTS, e % PARTS);
+        auto put = [&](int t, int part, int off) {
+            Eight<T> x8;
+            load8<T, VEC>(from(t, part), x8);
+            code(Flag<false>(), x8, cp + off * A.s_cache[kv][2] + part * 8);
+        };
+        if (dense && finite) {
+            char* const to = cp + (low + lane / PARTS) * A.s_cache[kv][2] + lane % PARTS * 8;
+#pragma unroll
+            for (int k = 0; k < ROUNDS; ++k) {
+                const int e = lane + 64 * k;
+                if (e < n * PARTS)
+                    code(Flag<true>(), held[k],
+                         64 % PARTS == 0 ? to + k * (64 / PARTS) * A.s_cache[kv][2] : cp + (low + e / PARTS) * A.s_cache[kv][2] + e % PARTS * 8);
+            }
+            for (int e = lane + 64 * ROUNDS; e < n * PARTS; e += 64) put(e / PARTS, e % PARTS, low + e / PARTS);
         } else {
             // Rows in order, each piece by the same lane: of several rows at one
             // offset the last one stays.
             for (int t = 0; t < n; ++t)
-                for (int part = lane; part < PARTS; part += 64) put(t, part);
+                for (int part = lane; part < PARTS; part += 64) put(t, part, A.slots[(r0 + t) * A.s_slots] - page * PAGE);
         }
         if (lane == 0) *sp = scale;
     }
@@ -651,7 +743,11 @@ struct Attend {
                 const bool in = valid && d < D;
                 if constexpr (QT == kF32) {
                     float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-                    if (in) load8<QT, VEC>(p + d * 4, x);
+                    if (in) {
+                        Eight<QT> x8;
+                        load8<QT, VEC>(p + d * 4, x8);
+                        values8<QT>(x8, x);
+                    }
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -1181,11 +1277,9 @@ struct Attend {
                 limit = share < 16 ? 16 : share > 0x7FFFFFF ? 0x7FFFFFF : static_cast<int>(share);
             } else if (pass == 1) {
                 // Places of the buckets, longest units first.
-                int first = 0;
-                if (threadIdx.x < BUCKETS)
-                    for (int k = 0; k < static_cast<int>(threadIdx.x); ++k) first += many[k];
-                if (threadIdx.x == BUCKETS - 1) A.units[0] = first + many[BUCKETS - 1];
-                __syncthreads();
+                pg_i64 entries;
+                const int first = static_cast<int>(block_scan<THREADS>(threadIdx.x < BUCKETS ? many[threadIdx.x] : 0, entries, lds));
+                if (threadIdx.x == 0) A.units[0] = static_cast<int>(entries);
                 if (threadIdx.x < BUCKETS) many[threadIdx.x] = first;
             }
             __syncthreads();
