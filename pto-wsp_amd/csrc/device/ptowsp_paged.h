@@ -255,10 +255,14 @@ __device__ inline pg_u32 codes2(pg_u32 w) {
         if constexpr (H) return __builtin_bit_cast(pg_u32, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HI));
         else return __builtin_bit_cast(pg_u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
     } else {
+        if constexpr (H) {
+            // The f16 of bits 0x6400 + u is 1024 + u; u is the code + 128.
+            const pg_u32 x = __builtin_amdgcn_perm(0x64646464u, w ^ 0x80808080u, HI ? 0x04030402u : 0x04010400u);
+            return __builtin_bit_cast(pg_u32, __builtin_bit_cast(pg_h2, x) - pg_h2{static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)});
+        }
         const float a = static_cast<float>(static_cast<signed char>(w >> (HI ? 16 : 0)));
         const float b = static_cast<float>(static_cast<signed char>(w >> (HI ? 24 : 8)));
-        if constexpr (H) return __builtin_bit_cast(pg_u32, __builtin_amdgcn_cvt_pkrtz(a, b));
-        else return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+        return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
     }
 }
 
@@ -631,15 +635,30 @@ struct Attend {
         int h, n;          // key head; tokens of the unit
         int p0;            // position of its first token
         int lo, hi;        // positions that its rows attend to, together
+        const char* cache[2];  // the key head's first page, keys and values, and their scales
+        const float* scale[2];
+        __device__ void aim(const AttendArgs& A, int head) {
+            h = head;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                cache[i] = A.cache[i] + h * A.s_cache[i][1];
+                scale[i] = A.scale[i] + h * A.s_scale[i][1];
+            }
+        }
     };
+    // Elements before page `id`: the host has checked that a page's stride has 32 bits.
+    __device__ static pg_i64 pages_on(int id, long long stride) {
+        return static_cast<pg_i64>(static_cast<pg_u64>(static_cast<pg_u32>(id)) * static_cast<pg_u32>(stride));
+    }
 
     // Pages of the 32 tokens from `base` on.  Tokens outside the unit's
     // positions take the page of a neighbour inside; they are masked.
+    static constexpr int IDS = PAGE % 32 == 0 ? 1 : 2;
     struct Pages {
-        int id[2];
+        int id[IDS];
     };
     __device__ static int checked(const AttendArgs& A, int id) {
-        if (static_cast<pg_u32>(id) >= static_cast<pg_u64>(A.pages)) {
+        if (static_cast<pg_u32>(id) >= static_cast<pg_u32>(A.pages)) {
             *A.err = 7;
             return 0;
         }
@@ -649,7 +668,7 @@ struct Attend {
     __device__ static void pages(const AttendArgs& A, const Unit& u, int base, Pages& p) {
         if constexpr (PAGED16) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) p.id[i] = uniform_load(u.table + inside(u, base + 16 * i) / PAGE);
+            for (int i = 0; i < IDS; ++i) p.id[i] = uniform_load(u.table + inside(u, base + 16 * i) / PAGE);
         } else {
             p.id[0] = u.table[inside(u, base + (static_cast<int>(threadIdx.x) & 31)) / PAGE];
         }
@@ -658,13 +677,22 @@ struct Attend {
     __device__ static void load(const AttendArgs& A, const Unit& u, int base, const Pages& p, Raw& r) {
         const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
         if constexpr (PAGED16) {
+            const char* page[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int id = checked(A, p.id[i]), off = (base + 16 * i) % PAGE;
-                r.ks[i] = uniform_load(A.scale[0] + id * A.s_scale[0][0] + u.h * A.s_scale[0][1]);
-                r.vs[i] = uniform_load(A.scale[1] + id * A.s_scale[1][0] + u.h * A.s_scale[1][1]);
-                const char* const kp = A.cache[0] + id * A.s_cache[0][0] + u.h * A.s_cache[0][1] + off * A.s_cache[0][2];
-                const char* const vp = A.cache[1] + id * A.s_cache[1][0] + u.h * A.s_cache[1][1] + off * A.s_cache[1][2];
+                const int off = (base + 16 * i) % PAGE;
+                if (i < IDS) {
+                    const int id = checked(A, p.id[i]);
+                    r.ks[i] = uniform_load(u.scale[0] + pages_on(id, A.s_scale[0][0]));
+                    r.vs[i] = uniform_load(u.scale[1] + pages_on(id, A.s_scale[1][0]));
+                    page[0] = u.cache[0] + pages_on(id, A.s_cache[0][0]);
+                    page[1] = u.cache[1] + pages_on(id, A.s_cache[1][0]);
+                } else {
+                    r.ks[i] = r.ks[0];
+                    r.vs[i] = r.vs[0];
+                }
+                const char* const kp = page[0] + off * static_cast<int>(A.s_cache[0][2]);
+                const char* const vp = page[1] + off * static_cast<int>(A.s_cache[1][2]);
                 const int ko = m * static_cast<int>(A.s_cache[0][2]) + 16 * g, vt = static_cast<int>(A.s_cache[1][2]);
 #pragma unroll
                 for (int j = 0; j < NK; ++j) {
@@ -683,13 +711,11 @@ struct Attend {
         } else {
             // Lane l has looked up token base + l % 32.
             const int id = checked(A, p.id[0]), off = inside(u, base + (lane & 31)) % PAGE;
-            const float ks = A.scale[0][id * A.s_scale[0][0] + u.h * A.s_scale[0][1]];
-            const float vs = A.scale[1][id * A.s_scale[1][0] + u.h * A.s_scale[1][1]];
-            const char* const kp = A.cache[0] + u.h * A.s_cache[0][1];
-            const char* const vp = A.cache[1] + u.h * A.s_cache[1][1];
+            const float ks = u.scale[0][pages_on(id, A.s_scale[0][0])];
+            const float vs = u.scale[1][pages_on(id, A.s_scale[1][0])];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const char* const row = kp + __shfl(id, 16 * i + m, 64) * A.s_cache[0][0] + __shfl(off, 16 * i + m, 64) * A.s_cache[0][2];
+                const char* const row = u.cache[0] + pages_on(__shfl(id, 16 * i + m, 64), A.s_cache[0][0]) + __shfl(off, 16 * i + m, 64) * static_cast<int>(A.s_cache[0][2]);
 #pragma unroll
                 for (int j = 0; j < NK; ++j) {
                     r.k[i][j] = pg_u32x4{0, 0, 0, 0};
@@ -699,7 +725,7 @@ struct Attend {
 #pragma unroll
             for (int t = 0; t < 8; ++t) {
                 const int from = (t & 4) * 4 + 4 * g + (t & 3);
-                const char* const row = vp + __shfl(id, from, 64) * A.s_cache[1][0] + __shfl(off, from, 64) * A.s_cache[1][2];
+                const char* const row = u.cache[1] + pages_on(__shfl(id, from, 64), A.s_cache[1][0]) + __shfl(off, from, 64) * static_cast<int>(A.s_cache[1][2]);
                 r.ks[t] = __shfl(ks, from, 64);
                 r.vs[t] = __shfl(vs, from, 64);
 #pragma unroll
@@ -1053,7 +1079,7 @@ struct Attend {
             const int tile = in / HS, hs = in - tile * HS;
             Unit u;
             u.table = A.table + b * A.s_table;
-            u.h = h;
+            u.aim(A, h);
             u.n = rq.n - tile * C < C ? rq.n - tile * C : C;
             u.p0 = rq.length - rq.n + tile * C;
             u.hi = u.p0 + u.n > 0 ? u.p0 + u.n : 0;
@@ -1344,7 +1370,7 @@ struct Attend {
             for (int h0 = 0; h0 < heads; h0 += GH) {
                 Unit u;
                 u.table = p.u.table;
-                u.h = p.h;
+                u.aim(A, p.h);
                 u.n = p.u.n - i0 < C ? p.u.n - i0 : C;
                 u.p0 = p.u.p0 + i0;
                 u.hi = u.p0 + u.n > 0 ? u.p0 + u.n : 0;

@@ -184,6 +184,7 @@ void cache_strides(const Node& n, const Operand& codes, const Operand& scales, l
     for (int d = 0; d < 3; ++d)
         if (codes.stride[d] % 16) stop(n, std::string(who) + "'s strides must be multiples of 16");
     if (reinterpret_cast<uintptr_t>(codes.ptr) % 16) stop(n, std::string(who) + " must be aligned to 16 bytes");
+    if (codes.shape[0] > 1 && (codes.stride[0] >> 32 || scales.stride[0] >> 32)) stop(n, std::string(who) + "'s pages lie too far apart");
     if (codes.stride[2] > (int64_t(1) << 26)) stop(n, std::string(who) + "'s tokens lie too far apart");
     for (int d = 0; d < 3; ++d) s_cache[d] = codes.stride[d];
     for (int d = 0; d < 2; ++d) s_scale[d] = scales.stride[d];
@@ -296,7 +297,7 @@ void run_attend(const Node& n, const std::vector<Operand>& o, const OperatorRun&
         A.lse = reinterpret_cast<float*>(o[9].ptr);
         for (int d = 0; d < 2; ++d) A.s_lse[d] = o[9].stride[d];
     }
-    A.batch = batch, A.width = o[5].shape[1], A.pages = o[1].shape[0], A.rows = rows;
+    A.batch = batch, A.width = o[5].shape[1], A.pages = std::min<int64_t>(o[1].shape[0], int64_t(1) << 31), A.rows = rows;
     A.heads = static_cast<int>(heads);
     A.window = static_cast<int>(std::min<int64_t>(attr(n, "window"), 0x7FFFFFFF));
     A.factor = static_cast<float>(n.op_floats.at("scale") * 1.4426950408889634);
