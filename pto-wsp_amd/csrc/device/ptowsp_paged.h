@@ -668,7 +668,7 @@ struct Attend {
     __device__ static void pages(const AttendArgs& A, const Unit& u, int base, Pages& p) {
         if constexpr (PAGED16) {
 #pragma unroll
-            for (int i = 0; i < IDS; ++i) p.id[i] = uniform_load(u.table + inside(u, base + 16 * i) / PAGE);
+            for (int i = 0; i < IDS; ++i) p.id[i] = shared_load(u.table + inside(u, base + 16 * i) / PAGE);
         } else {
             p.id[0] = u.table[inside(u, base + (static_cast<int>(threadIdx.x) & 31)) / PAGE];
         }
@@ -682,9 +682,9 @@ struct Attend {
             for (int i = 0; i < 2; ++i) {
                 const int off = (base + 16 * i) % PAGE;
                 if (i < IDS) {
-                    const int id = checked(A, p.id[i]);
-                    r.ks[i] = uniform_load(u.scale[0] + pages_on(id, A.s_scale[0][0]));
-                    r.vs[i] = uniform_load(u.scale[1] + pages_on(id, A.s_scale[1][0]));
+                    const int id = checked(A, uniform(p.id[i]));
+                    r.ks[i] = shared_load(u.scale[0] + pages_on(id, A.s_scale[0][0]));
+                    r.vs[i] = shared_load(u.scale[1] + pages_on(id, A.s_scale[1][0]));
                     page[0] = u.cache[0] + pages_on(id, A.s_cache[0][0]);
                     page[1] = u.cache[1] + pages_on(id, A.s_cache[1][0]);
                 } else {
@@ -1181,22 +1181,26 @@ struct Attend {
         if (end > u.hi) end = u.hi;
         if (base + 32 <= u.lo) base += (u.lo - base - 32 + STRIDE) / STRIDE * STRIDE;
         if (base >= end) return;
-        Pages pg;
+        // Page numbers are on their way before the bytes of the step ahead, so that
+        // waiting for them is not waiting for those.
+        Pages pg, ahead;
         Raw a, b;
         pages(A, u, base, pg);
+        pages(A, u, base + STRIDE, ahead);
         load(A, u, base, pg, a);
-        pages(A, u, base + STRIDE, pg);
         for (;;) {
             if (base + STRIDE < end) {
+                pg = ahead;
+                pages(A, u, base + 2 * STRIDE, ahead);
                 load(A, u, base + STRIDE, pg, b);
-                pages(A, u, base + 2 * STRIDE, pg);
             }
             step(A, u, base, a, st);
             base += STRIDE;
             if (base >= end) return;
             if (base + STRIDE < end) {
+                pg = ahead;
+                pages(A, u, base + 2 * STRIDE, ahead);
                 load(A, u, base + STRIDE, pg, a);
-                pages(A, u, base + 2 * STRIDE, pg);
             }
             step(A, u, base, b, st);
             base += STRIDE;
