@@ -1254,6 +1254,7 @@ struct Attend {
         // Three passes over the units, spread over the threads: the work, the
         // sizes, the places.
         int limit = 0x7FFFFFFF;
+        float per_step = 0.0f;
         struct Listed {
             int b, tile, steps;
         };
@@ -1286,7 +1287,7 @@ struct Attend {
                 sum += static_cast<pg_u64>(steps);
                 if (pass == 0) continue;
                 const int pieces = (steps + limit - 1) / limit, size = steps < limit ? steps : limit;
-                const int bucket = BUCKETS - 1 - static_cast<int>(static_cast<pg_i64>(size) * (BUCKETS - 1) / limit);
+                const int bucket = BUCKETS - 1 - static_cast<int>(static_cast<float>(size) * per_step);
                 const int place = atomicAdd(&many[bucket], pieces * HS);
                 if (pass == 1) continue;
                 for (int hs = 0; hs < HS; ++hs) {
@@ -1303,8 +1304,9 @@ struct Attend {
             if (pass == 0) atomicAdd(&work, sum);
             __syncthreads();
             if (pass == 0) {
-                const pg_u64 share = (work * HS * A.heads * 9 / 8 + A.cus - 1) / A.cus;
-                limit = share < 16 ? 16 : share > 0x7FFFFFF ? 0x7FFFFFF : static_cast<int>(share);
+                const float share = static_cast<float>(work) * (1.125f * HS * A.heads / A.cus);
+                limit = share < 16.0f ? 16 : share > 0x7FFFF00 ? 0x7FFFF00 : static_cast<int>(share) + 1;
+                per_step = (BUCKETS - 1) / (static_cast<float>(limit) * 1.0001f);  // below BUCKETS - 1 for a whole one
             } else if (pass == 1) {
                 // Places of the buckets, longest units first.
                 pg_i64 entries;
