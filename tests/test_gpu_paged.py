@@ -493,6 +493,14 @@ def test_attention_large_scores(gpu):
     _attend(gpu, c, scale=3.0)
 
 
+@pytest.mark.parametrize("dt,kind", [("bf16", "e4m3"), ("f16", "i8"), ("f32", "i8")])
+@pytest.mark.parametrize("scale", [-0.3, 0.0])
+@pytest.mark.parametrize("page,counts", [(16, [1, 2]), (8, [1, 2]), (16, [70, 1]), (8, [70, 1])])
+def test_attention_negative_scale(gpu, page, counts, scale, dt, kind):
+    """The largest score is then the smallest product; at 0 all weights are alike."""
+    _attend(gpu, _attend_case(np.random.default_rng(61), dt, kind, 2, 4, 128, page, [150, 260], counts), scale=scale)
+
+
 def test_attention_small_scales(gpu):
     """Scales down to 2^-126: nothing is lost between codes and outputs."""
     c = _attend_case(np.random.default_rng(6), "f32", "i8", 2, 2, 64, 16, [90, 40], [1, 4])
