@@ -270,6 +270,29 @@ def test_store_odd_rows(gpu, kind):
     _check_store(gpu, "f32", kind, x, slots, codes, scale)
 
 
+@pytest.mark.parametrize("kind", ["e4m3", "i8"])
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("n", [1, 16, 200])
+def test_store_not_finite(gpu, dt, kind, n):
+    """NaN and infinities in whole runs, of few and of many rows; the type's largest and smallest numbers beside them."""
+    rng = np.random.default_rng(9)
+    D, H = 128, 24 if n > 100 else 4
+    pieces = [(0, n), (3, n), (0, n), (0, n), (5, n)]
+    slots, codes, scale = _store_case(rng, kind, H, D, 16, pieces, sum(-(-(a + b) // 16) for a, b in pieces) + 2)
+    x = {c: rng.standard_normal((len(slots), H, D)).astype(np.float32) for c in "kv"}
+    top, least = {"bf16": (3.3895313892515355e38, 2.0 ** -133), "f16": (65504.0, 2.0 ** -24), "f32": (3.4028234663852886e38, 2.0 ** -149)}[dt]
+    x["k"][0, 0, :3] = [np.nan, np.inf, -np.inf]
+    x["k"][0, 1, 126:] = [1.0, -np.inf]
+    x["v"][n - 1, 0, 1::2] = np.nan
+    x["k"][n] = np.nan
+    x["v"][n, :, 5] = -np.inf
+    x["k"][2 * n, 0, 0], x["k"][2 * n, 1, 1], x["v"][2 * n, 0, 127] = top, -top, -top
+    x["v"][3 * n:4 * n] = least
+    x["k"][3 * n:4 * n, :, ::2] = -least
+    x["k"][4 * n:5 * n] = -np.abs(x["k"][4 * n:5 * n])
+    _check_store(gpu, dt, kind, x, slots, codes, scale)
+
+
 def test_store_slots_outside_the_cache(gpu):
     torch = _torch()
     rng = np.random.default_rng(8)

@@ -154,7 +154,14 @@ def test_operands_at_execute():
     odd.data = np.zeros((6, 2, 16, 72), np.uint8)[..., :64]
     far = T(E4M3, 6, 2, 16, 64)
     far.data = np.lib.stride_tricks.as_strided(np.zeros(64, np.uint8), (6, 2, 16, 64), (64, 64, 1 << 27, 1))
-    for w, match in ((attend(k_cache=k), "must have stride 1"), (attend(q=q, out=q), "lies where q does"), (attend(q=wide), "must have stride 1"),
+    apart = T(E4M3, 2, 2, 16, 64)
+    apart.data = np.lib.stride_tricks.as_strided(np.zeros(64, np.uint8), (2, 2, 16, 64), (1 << 32, 1024, 64, 1))
+    two = cache(pages=2, k_cache=apart)
+    sparse = T(F32, 6, 2)
+    sparse.data = np.lib.stride_tricks.as_strided(np.zeros(64, np.float32), (6, 2), (1 << 34, 4))
+    for w, match in ((attend(c=two), "pages lie too far apart"), (store(c=two), "pages lie too far apart"),
+                     (attend(v_scale=sparse), "pages lie too far apart"),
+                     (attend(k_cache=k), "must have stride 1"), (attend(q=q, out=q), "lies where q does"), (attend(q=wide), "must have stride 1"),
                      (attend(k_cache=odd), "multiples of 16"), (store(k_cache=odd), "multiples of 16"), (attend(v_cache=far), "too far apart")):
         with hip_stub.program(w) as once:
             with pytest.raises(RuntimeError, match=match):
