@@ -595,6 +595,7 @@ struct Attend {
     // One request.
     struct Request {
         int row, n, length, first, kt, units;  // first row, rows, tokens; first tile, tiles and units of a key head
+        bool bad;
     };
     __device__ static Request request(const AttendArgs& A, pg_i64 b, bool report) {
         Request r;
@@ -603,6 +604,7 @@ struct Attend {
         const pg_i64 most = A.width * PAGE;
         const bool bad = s0 < 0 || s1 < s0 || s1 > A.rows || length < 0 || length > most;
         if (bad && report) *A.err = 7;
+        r.bad = bad;
         if (bad || (PROMPT ? s1 - s0 <= A.few : s1 - s0 > A.few)) {
             r.row = r.n = r.length = r.first = r.kt = r.units = 0;
             return r;
@@ -1248,9 +1250,24 @@ struct Attend {
         for (int i = threadIdx.x; i < A.counters; i += THREADS) count[i] = 0;
         __shared__ pg_i64 before[THREADS];
         pg_i64 units = 0, total;
-        for (pg_i64 b = b0; b < b1; ++b) units += (request(A, b, false).n + kUnitTokens - 1) / kUnitTokens;
-        before[threadIdx.x] = block_scan<THREADS>(units, total, lds);
+        // With a request out of range the rest may add up to more rows than there
+        // are, and than the list has room for: the list stays empty then.
+        constexpr pg_i64 kBad = pg_i64(1) << 40;
+        bool bad = false;
+        for (pg_i64 b = b0; b < b1; ++b) {
+            const Request rq = request(A, b, false);
+            bad |= rq.bad;
+            units += (rq.n + kUnitTokens - 1) / kUnitTokens;
+        }
+        before[threadIdx.x] = block_scan<THREADS>(bad ? kBad : units, total, lds);
         __syncthreads();
+        if (total >= kBad) {
+            if (threadIdx.x == 0) {
+                A.units[0] = 0;
+                *A.err = 7;
+            }
+            return;
+        }
         // Three passes over the units, spread over the threads: the work, the
         // sizes, the places.
         int limit = 0x7FFFFFFF;

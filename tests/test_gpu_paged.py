@@ -568,6 +568,26 @@ def test_attention_inputs_out_of_range(gpu, what):
     _check_attend(c, t, _reference(c, 1.0 / 8.0, 0))
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_attention_starts_up_and_down(gpu, dt):
+    """Requests that are in range one by one, with far more rows together than there are: none of their prompts is run."""
+    c = _attend_case(np.random.default_rng(9), dt, "e4m3", 2, 2, 64, 16, [120] * 40, [20] * 40)
+    t = _attend_tensors(gpu, c)
+    rows = t["q"].shape[0]
+    t["lengths"].fill_(120)
+    t["starts"].copy_(ints(gpu, np.arange(41) % 2 * rows))
+    t["page_table"].copy_(ints(gpu, c["table"]))
+    prog = paged_attention(**{k: T(x) for k, x in t.items()}).compile(target="hip_gfx950")
+    prog.execute()
+    with pytest.raises(ExecutionError, match="out of range"):
+        prog.synchronize()
+    assert bool((t["out"] == 7.0).all())
+    t["starts"].copy_(ints(gpu, c["starts"]))
+    prog.execute()
+    prog.synchronize()
+    _check_attend(c, t, _reference(c, 1.0 / 8.0, 0))
+
+
 # ------------------------------------------------------------------------------ together
 def _step_case(gpu, layers, kind, dt, H, G, D, page, lengths, counts, seed):
     """A serving step of several layers: plan, then store and attention per layer, over a cache that an
