@@ -8,6 +8,7 @@ constexpr int kPlanRows = 1024;     // rows of a workgroup of paged_plan's secon
 constexpr int kAttendThreads = 256, kAttendTile = 128;  // a workgroup of paged_attention, and tokens of its tile
 constexpr int kSpanInts = 8;        // AttendArgs::spans of a workgroup
 constexpr int kUnitInts = 4;        // AttendArgs::units of an entry
+constexpr int kUnitHead = 4;        // AttendArgs::units before the entries
 
 struct PlanArgs {
     const int* lengths;

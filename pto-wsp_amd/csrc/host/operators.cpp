@@ -328,7 +328,7 @@ void run_attend(const Node& n, const std::vector<Operand>& o, const OperatorRun&
         entries = hs * (rows / (4 * c) + std::min(batch, rows / (A.few + 1))) + A.cus / heads + 1;
         if (entries * heads >= (int64_t(1) << 24)) stop(n, "too many rows for one call");
         A.room = static_cast<int>(entries), A.counters = 2 * A.cus;
-        unit_bytes = whole((2 + entries * (kUnitInts + heads) + A.counters) * 4);
+        unit_bytes = whole((kUnitHead + entries * (kUnitInts + heads) + A.counters + A.cus / heads + 1) * 4);
         need += unit_bytes + whole(int64_t(2) * A.cus * 4 * prb * (2 + dp) * 4);
     }
     char* const scratch = run.scratch(need);
