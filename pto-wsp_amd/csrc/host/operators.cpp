@@ -140,8 +140,10 @@ std::string entry_source(const std::string& entries) { return "#include \"ptowsp
 
 // ---- paged_plan ----
 // One workgroup does it all while its LDS holds the requests' sums and the
-// rows are few; otherwise one sums and as many as needed write the rows.
-constexpr int64_t kPlanOneRows = 16384;
+// rows are few; otherwise one sums and as many as needed write the rows.  64
+// requests, one launch or two: 1024 rows 6.6 us and 12.9, 6144 rows 11.7 and 12.6,
+// 8192 rows 14.2 and 12.6.
+constexpr int64_t kPlanOneRows = 6144;
 
 std::string plan_source() {
     const std::string t = std::to_string(kPlanThreads);
@@ -205,7 +207,10 @@ std::string store_source(int D, int page, int type, int code, bool vec, int chun
 
 // Rows of a wave: one while the waves are few (every row of a decode step has
 // a page of its own), a page's worth otherwise (a prompt's rows of a page go
-// together, and waves without a first row end at once).
+// together, and waves without a first row end at once).  8 heads of 128 in bf16,
+// one row a wave or a page's: 64 single tokens 5.2 us and 27.9, 1024 13.6 and 27.6,
+// 4096 51.5 and 45.9; a prompt of 256 tokens 6.1 and 6.8, of 1024 10.4 and 7.2, of
+// 2048 16.1 and 7.4.
 int store_chunk(int64_t rows, int64_t heads, int64_t page) { return rows * heads * 2 <= 16384 ? 1 : static_cast<int>(std::min<int64_t>(page, 64)); }
 
 void run_store(const Node& n, const std::vector<Operand>& o, const OperatorRun& run) {
@@ -243,7 +248,8 @@ std::string attend_type(const AttendShape& s, int nt, bool prompt) {
     return "ptowsp::Attend<" + num(s.D) + ", " + num(s.page) + ", " + num(s.G) + ", " + num(nt) + ", " + num(s.type) + ", " + num(s.code) + ", " +
            flag(s.window) + ", " + flag(s.lse) + ", " + flag(s.vec) + ", " + flag(prompt) + ">";
 }
-// Waves on a SIMD that the registers allow.
+// Waves on a SIMD that the registers allow: 32 requests over 4096 tokens of head
+// size 256 take 101 us with one and 197, spilling, with two.
 int attend_waves(int64_t D) { return D > 128 ? 1 : 2; }
 // Prompts: 16 * nt query rows a wave, `waves` waves on a SIMD.
 struct PromptShape {
@@ -266,14 +272,23 @@ std::string attend_source(const AttendShape& s, bool prompts) {
 
 // Query rows of a request and key head up to which its keys are streamed by
 // all compute units alike (the kernel for few rows), and beyond which rows
-// share them.
+// share them; and query rows of a call up to which none are shared, since they
+// give the prompt kernel too few workgroups.  Groups of 4 x 8 key heads of 128 in
+// bf16, few rows or prompts: 64 requests of 8 tokens 39 us and 60, of 16 tokens (64
+// rows) 66 and 63, of 32 tokens 120 and 69; one prompt of 256 tokens (8192 rows in
+// the call) 43 and 58, of 1024 98 and 94; two of 64 tokens over 16384 99 and 145, of
+// 128 169 and 148.
 constexpr int kFewRows = 64;
+constexpr int64_t kFewInAll = 8192;
 
-// 16 query rows at a time, or 32 where a request's rows of a key head are more
-// than 16 and the accumulators leave room.
-int attend_nt(int64_t rows, int64_t batch, int64_t G, int64_t D) {
+// 16 query rows at a time, or 32 where many read the same keys and the registers
+// suffice (not for float32: 32 query heads 54 us, with 32 at a time 87).  bf16, 16
+// requests over 2048 tokens: 32 rows of a key head 34 us, with 32 at a time 39; 64
+// rows 48 and 46 (two requests over 16384 tokens 43 and 62); 128 rows 82 and 58; 32
+// query heads of single tokens over 4096 52 and 43.
+int attend_nt(int64_t rows, int64_t batch, int64_t G, int64_t D, int type) {
     const int64_t each = G * std::max<int64_t>(1, (rows + batch - 1) / std::max<int64_t>(1, batch));
-    return each > 16 && D <= 128 ? 2 : 1;
+    return type != 2 && D <= 128 && (G > 16 || each > 64) ? 2 : 1;
 }
 
 void run_attend(const Node& n, const std::vector<Operand>& o, const OperatorRun& run) {
@@ -305,15 +320,16 @@ void run_attend(const Node& n, const std::vector<Operand>& o, const OperatorRun&
     if (rows == 0 || batch == 0) return;
     AttendShape s;
     s.D = static_cast<int>(D), s.page = static_cast<int>(page), s.G = static_cast<int>(q.shape[1] / heads);
-    s.NT = attend_nt(rows, batch, s.G, D);
-    s.type = type_id(q.dtype), s.code = code_id(o[1].dtype);
+    s.type = type_id(q.dtype);
+    s.NT = attend_nt(rows, batch, s.G, D, s.type);
+    s.code = code_id(o[1].dtype);
     s.window = A.window > 0, s.lse = lse, s.vec = vectors(q) && vectors(out);
     // Requests of more tokens than a few go to the kernel for prompts, launched
     // if there can be one while every other request has a token.
     const int few = std::max(1, kFewRows / s.G);
-    const bool prompts = rows - batch >= few;
+    const bool prompts = rows - batch >= few && rows * q.shape[1] > kFewInAll;
     A.few = prompts ? few : 0x7FFFFFFF;
-    if (prompts) s.NT = s.G > 16 && D <= 128 ? 2 : 1;
+    if (prompts) s.NT = attend_nt(batch, batch, s.G, D, s.type);
     const int rb = 16 * s.NT, dp = (s.D + 63) / 64 * 64;
     const int64_t blocks = attend_waves(D) * static_cast<int64_t>(run.cus);
     auto whole = [](int64_t bytes) { return (static_cast<size_t>(bytes) + 255) / 256 * 256; };
@@ -435,7 +451,7 @@ std::vector<std::pair<std::string, std::string>> operator_sources(const Module& 
         return {{store_source(D, page, type_id(s.dtype[0]), code, true, store_chunk(s.of("k")[0], c[1], c[2])), "ptowsp_paged_store"}};
     const auto& q = s.of("q");
     const int G = static_cast<int>(q[1] / c[1]);
-    const AttendShape t{D, page, G, attend_nt(q[0], s.of("lengths")[0], G, D), type_id(s.dtype[0]), code, attr(n, "window") > 0, !s.of("lse").empty(), true};
+    const AttendShape t{D, page, G, attend_nt(q[0], s.of("lengths")[0], G, D, type_id(s.dtype[0])), type_id(s.dtype[0]), code, attr(n, "window") > 0, !s.of("lse").empty(), true};
     return {{attend_source(t, false), "ptowsp_paged_attention"}, {attend_source(t, true), "ptowsp_paged_attention_prompts"}};
 }
 

@@ -12,6 +12,8 @@ in numerator and sum, times values and scales as f16: 4 2^-11); the float32 sums
 inside an MFMA and the joins.  f16 parts below 2^-14 are off by 2^-25: a row's largest p is 2^10 or more there,
 and a value's scale 2^-5 of the sums' unit or more where p has it, so by sum |v| 2^-30 in all."""
 
+import sys
+
 import numpy as np
 import pytest
 
@@ -310,7 +312,18 @@ def test_store_slots_outside_the_cache(gpu):
 
 
 # ------------------------------------------------------------------------------ attention
-def _attend_case(rng, dt, kind, H, G, D, page, lengths, counts, spare_rows=2, poison=True):
+# Rows behind the last request.  A call of more than 8192 query rows, these among them, may run its long
+# requests in the kernel for prompts.
+_behind = {"few": lambda heads: 2, "many": lambda heads: 8192 // heads + 1}
+_rows_behind = _behind["few"]
+
+
+@pytest.fixture(params=["few", "many"])
+def rows_behind(request, monkeypatch):
+    monkeypatch.setattr(sys.modules[__name__], "_rows_behind", _behind[request.param])
+
+
+def _attend_case(rng, dt, kind, H, G, D, page, lengths, counts, poison=True):
     """Inputs as numpy arrays; what no row may see is filled with NaN codes and scales, or large ones."""
     torch = _torch()
     lengths, counts = np.asarray(lengths), np.asarray(counts)
@@ -335,7 +348,7 @@ def _attend_case(rng, dt, kind, H, G, D, page, lengths, counts, spare_rows=2, po
             codes[x] = np.where(live[:, None, :, None], codes[x], 0x7F).astype(codes[x].dtype)
             scale[x] = np.where(live.any(1)[:, None], scale[x], np.nan).astype(np.float32)
     starts = np.concatenate([[0], np.cumsum(counts)])
-    rows = int(starts[-1]) + spare_rows
+    rows = int(starts[-1]) + _rows_behind(H * G)
     q = torch.from_numpy(rng.standard_normal((rows, H * G, D)).astype(np.float32)).to(_dt(dt))
     return {"q": q, "codes": codes, "scale": scale, "table": table, "lengths": lengths, "starts": starts, "kind": kind, "dt": dt}
 
@@ -434,6 +447,7 @@ def test_attention(gpu, shape, dt, kind):
     _attend(gpu, _attend_case(np.random.default_rng(shape), dt, kind, H, G, D, page, lengths, counts))
 
 
+@pytest.mark.usefixtures("rows_behind")
 @pytest.mark.parametrize("window", [1, 7, 32, 130, 10000])
 @pytest.mark.parametrize("G,page,lengths,counts", [(4, 16, [1, 300, 129], [1, 1, 1]), (2, 8, [200, 90], [150, 3]), (1, 32, [260], [260])])
 def test_attention_window(gpu, window, G, page, lengths, counts):
@@ -448,12 +462,14 @@ def test_attention_window(gpu, window, G, page, lengths, counts):
     _check_attend(c, t, _reference(c, 1.0 / 8.0, window))
 
 
+@pytest.mark.usefixtures("rows_behind")
 def test_attention_rows_without_positions(gpu):
     """More rows than tokens: the first ones lie before position 0."""
     c = _attend_case(np.random.default_rng(1), "bf16", "e4m3", 2, 4, 64, 16, [0, 3, 20], [2, 6, 1])
     _attend(gpu, c)
 
 
+@pytest.mark.usefixtures("rows_behind")
 @pytest.mark.parametrize("layout", ["plain", "fused"])
 @pytest.mark.parametrize("dt,kind", [("bf16", "e4m3"), ("f32", "i8")])
 def test_attention_layouts(gpu, layout, dt, kind):
@@ -489,6 +505,7 @@ PROMPTS = [
 ]
 
 
+@pytest.mark.usefixtures("rows_behind")
 @pytest.mark.parametrize("dt,kind", [("bf16", "e4m3"), ("f16", "i8"), ("f32", "e4m3")])
 @pytest.mark.parametrize("shape", range(len(PROMPTS)))
 def test_attention_prompts(gpu, shape, dt, kind):
@@ -496,6 +513,7 @@ def test_attention_prompts(gpu, shape, dt, kind):
     _attend(gpu, _attend_case(np.random.default_rng(50 + shape), dt, kind, H, G, D, page, lengths, counts))
 
 
+@pytest.mark.usefixtures("rows_behind")
 @pytest.mark.parametrize("dt", ["bf16", "f16"])
 @pytest.mark.parametrize("page", [16, 8])
 def test_attention_prompt_scales(gpu, dt, page):
@@ -516,6 +534,7 @@ def test_attention_large_scores(gpu):
     _attend(gpu, c, scale=3.0)
 
 
+@pytest.mark.usefixtures("rows_behind")
 @pytest.mark.parametrize("dt,kind", [("bf16", "e4m3"), ("f16", "i8"), ("f32", "i8")])
 @pytest.mark.parametrize("scale", [-0.3, 0.0])
 @pytest.mark.parametrize("page,counts", [(16, [1, 2]), (8, [1, 2]), (16, [70, 1]), (8, [70, 1])])
@@ -532,6 +551,7 @@ def test_attention_small_scales(gpu):
     _attend(gpu, c)
 
 
+@pytest.mark.usefixtures("rows_behind")
 def test_attention_nan_reaches_only_the_rows_that_see_it(gpu):
     c = _attend_case(np.random.default_rng(7), "bf16", "e4m3", 2, 2, 64, 16, [60, 30], [40, 1])
     page, off = divmod(45, 16)
@@ -543,12 +563,13 @@ def test_attention_nan_reaches_only_the_rows_that_see_it(gpu):
     _attend(gpu, c, lse=False)
 
 
+@pytest.mark.usefixtures("rows_behind")
 @pytest.mark.parametrize("what", ["starts", "length", "page", "negative page", "order"])
 def test_attention_inputs_out_of_range(gpu, what):
     c = _attend_case(np.random.default_rng(8), "bf16", "e4m3", 2, 2, 64, 16, [60, 30, 20], [4, 1, 2])
     t = _attend_tensors(gpu, c)
     if what == "starts":
-        t["starts"][3] = 1000
+        t["starts"][3] = max(1000, t["q"].shape[0] + 1)  # beyond the rows of either size
     elif what == "order":
         t["starts"][1] = 6
     elif what == "length":
@@ -569,8 +590,9 @@ def test_attention_inputs_out_of_range(gpu, what):
 
 
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
-def test_attention_starts_up_and_down(gpu, dt):
+def test_attention_starts_up_and_down(gpu, dt, monkeypatch):
     """Requests that are in range one by one, with far more rows together than there are: none of their prompts is run."""
+    monkeypatch.setattr(sys.modules[__name__], "_rows_behind", _behind["many"])
     c = _attend_case(np.random.default_rng(9), dt, "e4m3", 2, 2, 64, 16, [120] * 40, [20] * 40)
     t = _attend_tensors(gpu, c)
     rows = t["q"].shape[0]
@@ -601,7 +623,7 @@ def _step_case(gpu, layers, kind, dt, H, G, D, page, lengths, counts, seed):
     order = rng.permutation(pages)
     table = np.full((len(lengths), width), -1)
     table[np.arange(width)[None] < held[:, None]] = order[:int(held.sum())]
-    rows = int(counts.sum()) + 3
+    rows = int(counts.sum()) + 1 + _rows_behind(H * G)
     t = _plan_tensors(gpu, lengths, counts, table, order[int(held.sum()):], 0, rows)
     codes = {x: R.encode(rng.standard_normal((layers, pages, H, page, D)) * 40, kind) for x in "kv"}
     scale = {x: (0.03 * np.exp(0.3 * rng.standard_normal((layers, pages, H)))).astype(np.float32) for x in "kv"}
@@ -644,6 +666,7 @@ def _check_step(t, layers, kind, dt, page, codes, scale, plan):
         _check_attend(c, {"out": t["out"][layer]}, _reference(c, 1.0 / np.sqrt(t["q"].shape[-1]), 0), lse=False)
 
 
+@pytest.mark.usefixtures("rows_behind")
 @pytest.mark.parametrize("kind,dt", [("e4m3", "bf16"), ("i8", "f32")])
 def test_step(gpu, kind, dt):
     t, codes, scale, plan = _step_case(gpu, 2, kind, dt, 2, 4, 64, 16, [0, 31, 100, 5, 16], [20, 1, 1, 0, 40], 1)
@@ -657,6 +680,7 @@ def _restore(t, first):
         t[k].copy_(x)
 
 
+@pytest.mark.usefixtures("rows_behind")
 @pytest.mark.parametrize("counts", [[1, 1, 1], [40, 1, 0]])
 def test_step_captured(gpu, counts):
     """Captured twice and replayed beside eager runs: every graph keeps a workspace of its own."""

@@ -129,12 +129,20 @@ def _entries(launches):
 
 
 def test_launches_of_a_plan():
-    for batch, rows, want in ((4096, 16384, ["plan"]), (4097, 4, ["plan_sums", "plan_rows"]), (1, 16385, ["plan_sums", "plan_rows"]), (5000, 0, ["plan_sums"])):
+    for batch, rows, want in ((4096, 6144, ["plan"]), (4097, 4, ["plan_sums", "plan_rows"]), (1, 6145, ["plan_sums", "plan_rows"]), (5000, 0, ["plan_sums"])):
         with hip_stub.program(plan(batch, 8, rows)) as once:
             launches = once()
             assert _entries(launches) == want
             if len(launches) == 2:
                 assert launches[1].blocks == -(-rows // 1024)
+
+
+def test_launches_of_attention():
+    """The kernel for prompts only where a request may have more than 64 rows a key head, of a call of more than 8192."""
+    few, prompts = ["attention", "attention_join"], ["attention_units", "attention_prompts", "attention_finish"]
+    for rows, batch, G, want in ((1024, 3, 4, few), (1025, 3, 4, prompts), (1040, 1025, 4, few), (1041, 1025, 4, prompts), (64, 1, 64, few), (65, 1, 64, prompts)):
+        with hip_stub.program(attend(rows=rows, batch=batch, G=G)) as once:
+            assert _entries(once()) == want
 
 
 def test_empty_calls_launch_nothing():
