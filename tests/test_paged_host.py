@@ -77,6 +77,9 @@ def attend(rows=5, heads=2, G=4, D=64, batch=3, dt=BF16, c=None, **other):
     (lambda: attend(page_table=T(I32, 2, 4)), "2 rows for 3 requests"),
     (lambda: attend(page_table=T(I32, 3, 1 << 28)), "2\\^31 tokens"),
     (lambda: attend(window=-1), "a negative window"),
+    (lambda: attend(dt=F32, window=9, c=cache(page=8)), "multiple of 16 tokens"),
+    (lambda: attend(dt=F32, window=9, c=cache(page=16)), None),
+    (lambda: attend(dt=F32, c=cache(page=8)), None),
     (lambda: attend(scale=float("inf")), "non-finite"),
     (lambda: attend(q=T(BF16, 5, 8)), "rank 3 is needed"),
 ])
