@@ -629,11 +629,36 @@ struct Attend {
         return r;
     }
 
+    static constexpr int SC = PAGED16 ? 2 : 1;
     struct Raw {
         pg_u32x4 k[2][NK];
         pg_u32 v[NK][8];
-        float ks[PAGED16 ? 2 : 8], vs[PAGED16 ? 2 : 8];
+        float ks[SC], vs[SC];  // scales: of each 16 tokens; over odd pages of token base + lane % 32
     };
+    // This lane's number, for what is computed from it where it is used: the
+    // compiler would compute that ahead of the loops over tokens and carry it
+    // through them, beyond the registers that there are.
+    __device__ static int own_lane() {
+        pg_u32 all = ~0u;
+        asm volatile("" : "+s"(all));
+        return static_cast<int>(__builtin_amdgcn_mbcnt_hi(all, __builtin_amdgcn_mbcnt_lo(all, 0)));
+    }
+    // x of lane `first` + `more`: 4 * first in a register, the constant in the instruction.
+    __device__ static int of_lane(int first4, int more, int x) { return __builtin_amdgcn_ds_bpermute(first4 + 4 * more, x); }
+    // The four lanes n + 16 g of a query row joined, in each of them.
+    template <class Op>
+    __device__ static float over_groups(float x, Op op) {
+        const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+        const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
+    }
+    // The scales of the tokens in this lane's places.
+    __device__ static void scales_of(const float (&s)[SC], float (&f)[8]) {
+        const int first4 = PAGED16 ? 0 : own_lane() & 48;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = PAGED16 ? s[e >> 2] : __int_as_float(of_lane(first4, 4 * (e & 4) + (e & 3), __float_as_int(s[0])));
+    }
 
     // One unit of one workgroup's piece.
     struct Unit {
@@ -664,11 +689,26 @@ struct Attend {
         int id[IDS];
     };
     __device__ static int checked(const AttendArgs& A, int id) {
-        if (static_cast<pg_u32>(id) >= static_cast<pg_u32>(A.pages)) {
-            *A.err = 7;
-            return 0;
-        }
-        return id;
+        const bool out = static_cast<pg_u32>(id) >= static_cast<pg_u32>(A.pages);
+        if (__ballot(out)) *A.err = 7;
+        return out ? 0 : id;
+    }
+
+    // First dims of a lane's piece j of a key (16 dims) and of a value (4).  Where
+    // the head size ends inside 64 dims, pieces behind it repeat the row's last
+    // one: q is 0 there, a NaN is in the scores either way, and those dims of the
+    // output are not written.  So no load stands under a branch that only some
+    // lanes take.  The compiler may put copies and spills of other values at the
+    // end of such a branch before it gives the other lanes their turn, which then
+    // go on with what the register or the spill slot held before: 7 rows over int8
+    // pages of 8 tokens, head size 80, lost rows 4 to 6 that way, on some runs.
+    __device__ static int key_dim(int j, int g) {
+        const int d = 64 * j + 16 * g;
+        return D % 64 != 0 && j == NK - 1 && d > D - 16 ? D - 16 : d;
+    }
+    __device__ static int value_dim(int j, int m) {
+        const int d = 64 * j + 4 * m;
+        return D % 64 != 0 && j == NK - 1 && d > D - 4 ? D - 4 : d;
     }
     __device__ static int inside(const Unit& u, int t) { return t < u.lo ? u.lo : t >= u.hi ? u.hi - 1 : t; }
     __device__ static void pages(const AttendArgs& A, const Unit& u, int base, Pages& p) {
@@ -681,7 +721,7 @@ struct Attend {
     }
 
     __device__ static void load(const AttendArgs& A, const Unit& u, int base, const Pages& p, Raw& r) {
-        const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+        const int lane = D % 64 != 0 ? own_lane() : threadIdx.x & 63, m = lane & 15, g = lane >> 4;
         if constexpr (PAGED16) {
             const char* page[2];
 #pragma unroll
@@ -699,46 +739,32 @@ struct Attend {
                 }
                 const char* const kp = page[0] + off * static_cast<int>(A.s_cache[0][2]);
                 const char* const vp = page[1] + off * static_cast<int>(A.s_cache[1][2]);
-                const int ko = m * static_cast<int>(A.s_cache[0][2]) + 16 * g, vt = static_cast<int>(A.s_cache[1][2]);
+                const int ko = m * static_cast<int>(A.s_cache[0][2]), vt = static_cast<int>(A.s_cache[1][2]);
 #pragma unroll
-                for (int j = 0; j < NK; ++j) {
-                    r.k[i][j] = pg_u32x4{0, 0, 0, 0};
-                    if (D % 64 == 0 || 64 * j + 16 * g < D) r.k[i][j] = *reinterpret_cast<const pg_u32x4*>(kp + ko + 64 * j);
-                }
+                for (int j = 0; j < NK; ++j) r.k[i][j] = *reinterpret_cast<const pg_u32x4*>(kp + ko + key_dim(j, g));
 #pragma unroll
                 for (int j = 0; j < NK; ++j)
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        r.v[j][4 * i + t] = 0;
-                        if (D % 64 == 0 || 64 * j + 4 * m < D)
-                            r.v[j][4 * i + t] = *reinterpret_cast<const pg_u32*>(vp + (4 * g + t) * vt + 64 * j + 4 * m);
-                    }
+                    for (int t = 0; t < 4; ++t) r.v[j][4 * i + t] = *reinterpret_cast<const pg_u32*>(vp + (4 * g + t) * vt + value_dim(j, m));
             }
         } else {
             // Lane l has looked up token base + l % 32.
             const int id = checked(A, p.id[0]), off = inside(u, base + (lane & 31)) % PAGE;
-            const float ks = u.scale[0][pages_on(id, A.s_scale[0][0])];
-            const float vs = u.scale[1][pages_on(id, A.s_scale[1][0])];
+            const int own = own_lane(), m4 = 4 * (own & 15), g4 = own & 48;
+            r.ks[0] = u.scale[0][pages_on(id, A.s_scale[0][0])];
+            r.vs[0] = u.scale[1][pages_on(id, A.s_scale[1][0])];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const char* const row = u.cache[0] + pages_on(__shfl(id, 16 * i + m, 64), A.s_cache[0][0]) + __shfl(off, 16 * i + m, 64) * static_cast<int>(A.s_cache[0][2]);
+                const char* const row = u.cache[0] + pages_on(of_lane(m4, 16 * i, id), A.s_cache[0][0]) + of_lane(m4, 16 * i, off) * static_cast<int>(A.s_cache[0][2]);
 #pragma unroll
-                for (int j = 0; j < NK; ++j) {
-                    r.k[i][j] = pg_u32x4{0, 0, 0, 0};
-                    if (D % 64 == 0 || 64 * j + 16 * g < D) r.k[i][j] = *reinterpret_cast<const pg_u32x4*>(row + 64 * j + 16 * g);
-                }
+                for (int j = 0; j < NK; ++j) r.k[i][j] = *reinterpret_cast<const pg_u32x4*>(row + key_dim(j, g));
             }
 #pragma unroll
             for (int t = 0; t < 8; ++t) {
-                const int from = (t & 4) * 4 + 4 * g + (t & 3);
-                const char* const row = u.cache[1] + pages_on(__shfl(id, from, 64), A.s_cache[1][0]) + __shfl(off, from, 64) * static_cast<int>(A.s_cache[1][2]);
-                r.ks[t] = __shfl(ks, from, 64);
-                r.vs[t] = __shfl(vs, from, 64);
+                const int more = (t & 4) * 4 + (t & 3);
+                const char* const row = u.cache[1] + pages_on(of_lane(g4, more, id), A.s_cache[1][0]) + of_lane(g4, more, off) * static_cast<int>(A.s_cache[1][2]);
 #pragma unroll
-                for (int j = 0; j < NK; ++j) {
-                    r.v[j][t] = 0;
-                    if (D % 64 == 0 || 64 * j + 4 * m < D) r.v[j][t] = *reinterpret_cast<const pg_u32*>(row + 64 * j + 4 * m);
-                }
+                for (int j = 0; j < NK; ++j) r.v[j][t] = *reinterpret_cast<const pg_u32*>(row + value_dim(j, m));
             }
         }
     }
@@ -763,40 +789,31 @@ struct Attend {
     };
 
     __device__ static void load_q(const AttendArgs& A, const Unit& u, int row, int head, State& st) {
-        const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+        const int lane = own_lane(), n = lane & 15, g = lane >> 4;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
+            // Places without a row or a dim read the unit's first row, or a dim inside, and are 0.
             const int r = 16 * t + n, i = r / GH, hh = r - i * GH;
             const bool valid = i < u.n && (HS == 1 || head % G + hh < G);
-            const char* const p = A.q + ((row + i) * A.s_q[0] + (head + hh) * A.s_q[1]) * elem_size(QT);
+            const char* const p = A.q + ((row + (valid ? i : 0)) * A.s_q[0] + (head + (valid ? hh : 0)) * A.s_q[1]) * elem_size(QT);
 #pragma unroll
             for (int j = 0; j < 2 * NK; ++j) {
                 const int d = 64 * (j >> 1) + 16 * g + 8 * (j & 1);
-                const bool in = valid && d < D;
+                const bool in = valid && (D % 64 == 0 || d < D);
+                Eight<QT> x8;
+                load8<QT, VEC>(p + (D % 64 != 0 && d >= D ? D - 8 : d) * elem_size(QT), x8);
                 if constexpr (QT == kF32) {
-                    float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-                    if (in) {
-                        Eight<QT> x8;
-                        load8<QT, VEC>(p + d * 4, x8);
-                        values8<QT>(x8, x);
-                    }
+                    float x[8];
+                    values8<QT>(x8, x);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = in ? x[e] : 0.0f;
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
 #pragma unroll
                         for (int k = 0; k < 3; ++k) st.q[t][j][k][e] = take_bf16(x[2 * e], x[2 * e + 1]);
                 } else {
-                    pg_u32x4 w = {0, 0, 0, 0};
-                    if (in) {
-                        if constexpr (VEC) {
-                            w = *reinterpret_cast<const pg_u32x4*>(p + d * 2);
-                        } else {
 #pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                w[e] = static_cast<pg_u32>(*reinterpret_cast<const pg_u16*>(p + d * 2 + 4 * e)) |
-                                       static_cast<pg_u32>(*reinterpret_cast<const pg_u16*>(p + d * 2 + 4 * e + 2)) << 16;
-                        }
-                    }
-                    st.q[t][j][0] = w;
+                    for (int e = 0; e < 4; ++e) st.q[t][j][0][e] = in ? x8.w[e] : 0;
                 }
             }
             st.m[t] = -__builtin_inff();
@@ -808,6 +825,13 @@ struct Attend {
         }
     }
 
+    // Four codes, kept in one register: the compiler would carry their bytes from
+    // the loads through the loop in one each.
+    __device__ static pg_u32 whole(pg_u32 w) {
+        asm("" : "+v"(w));
+        return w;
+    }
+
     // O^T += V^T P^T for P's parts in the eight token places of a lane.
     __device__ static void values(const pg_u32 (&v)[NK][8], const pg_u32x4 (&p)[NT][PP], pg_f32x4 (&o)[NT][NK][4]) {
 #pragma unroll
@@ -815,7 +839,7 @@ struct Attend {
             pg_u32x4 a[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const pg_u32 x = v[j][2 * e], y = v[j][2 * e + 1];
+                const pg_u32 x = whole(v[j][2 * e]), y = whole(v[j][2 * e + 1]);
                 const pg_u32 w0 = __builtin_amdgcn_perm(y, x, 0x05010400u), w1 = __builtin_amdgcn_perm(y, x, 0x07030602u);
                 a[0][e] = codes2<CT, false, false>(w0);
                 a[1][e] = codes2<CT, false, true>(w0);
@@ -834,6 +858,8 @@ struct Attend {
     // p of the scores, and its products with the values.
     __device__ static void weigh(const Raw& r, const float (&s)[NT][8], State& st) {
         pg_u32x4 p[NT][PP];
+        float vs[8];
+        scales_of(r.vs, vs);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const float m = st.m[t] == -__builtin_inff() ? 0.0f : st.m[t];
@@ -842,7 +868,7 @@ struct Attend {
             for (int e = 0; e < 8; ++e) {
                 x[e] = __builtin_amdgcn_exp2f(s[t][e] - m);
                 l += x[e];
-                x[e] *= r.vs[PAGED16 ? e >> 2 : e];
+                x[e] *= vs[e];
             }
             st.l[t] += l;
 #pragma unroll
@@ -871,7 +897,7 @@ struct Attend {
     // rows see and others do not (0 * NaN is NaN) goes into those rows' sums here
     // and is 0 afterwards: ones at the NaNs times ones at the rows that see them.
     __device__ static void mask(const AttendArgs& A, const Unit& u, int base, Raw& r, float (&s)[NT][8], State& st) {
-        const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+        const int lane = own_lane(), n = lane & 15, g = lane >> 4;
         const int tok = base + 4 * g;  // token of place e: tok + e % 4, 16 further for e >= 4
         pg_u32 seen[NT];
 #pragma unroll
@@ -920,8 +946,10 @@ struct Attend {
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
                         pg_u32x4 p;
+                        pg_u32 at = seen[t];
+                        asm volatile("" : "+v"(at));  // p is made where it is used
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) p[e] = (seen[t] >> (2 * e) & 1) * 0x3F80u | (seen[t] >> (2 * e + 1) & 1) * 0x3F800000u;
+                        for (int e = 0; e < 4; ++e) p[e] = (at >> (2 * e) & 1) * 0x3F80u | (at >> (2 * e + 1) & 1) * 0x3F800000u;
                         const pg_f32x4 hit = mma(a, p, pg_f32x4{0, 0, 0, 0}, false);
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
@@ -942,7 +970,7 @@ struct Attend {
                 for (int t = 0; t < NT; ++t) acc[t][i] = pg_f32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int j = 0; j < 2 * NK; ++j) {
-                    const pg_u32 w0 = r.k[i][j >> 1][2 * (j & 1)], w1 = r.k[i][j >> 1][2 * (j & 1) + 1];
+                    const pg_u32 w0 = whole(r.k[i][j >> 1][2 * (j & 1)]), w1 = whole(r.k[i][j >> 1][2 * (j & 1) + 1]);
                     const pg_u32x4 a = {codes2<CT, H, false>(w0), codes2<CT, H, true>(w0), codes2<CT, H, false>(w1), codes2<CT, H, true>(w1)};
 #pragma unroll
                     for (int t = 0; t < NT; ++t)
@@ -950,9 +978,11 @@ struct Attend {
                         for (int k = 0; k < QP; ++k) acc[t][i] = mma(a, st.q[t][j][k], acc[t][i], H);
                 }
             }
+            float ks[8];
+            scales_of(r.ks, ks);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float f = r.ks[PAGED16 ? e >> 2 : e] * A.factor;
+                const float f = ks[e] * A.factor;
 #pragma unroll
                 for (int t = 0; t < NT; ++t) s[t][e] = acc[t][e >> 2][e & 3] * f;
             }
@@ -974,8 +1004,7 @@ struct Attend {
                 float mx = s[t][0];
 #pragma unroll
                 for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[t][e]);
-                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                mx = over_groups(mx, [](float a, float b) { return fmaxf(a, b); });
                 const float m = fmaxf(st.m[t], mx);
                 const float a = m == st.m[t] ? 1.0f : __builtin_amdgcn_exp2f(st.m[t] - m);
                 st.m[t] = m;
@@ -1026,7 +1055,6 @@ struct Attend {
     };
 
     __device__ static void run(const AttendArgs& A, int workgroup, Shared& sh) {
-        const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
         const int wave = uniform(threadIdx.x >> 6);
         const pg_i64 w = workgroup;
         int* const span = A.spans + w * kSpanInts;
@@ -1096,10 +1124,10 @@ struct Attend {
             load_q(A, u, row, head, st);
             piece<kAttendTile>(A, u, (rq.first + t0) * kAttendTile + 32 * wave, (rq.first + t1) * kAttendTile, st);
             // The four waves' results.
+            const int lane = own_lane(), n = lane & 15, g = lane >> 4;
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                st.l[t] += __shfl_xor(st.l[t], 16, 64);
-                st.l[t] += __shfl_xor(st.l[t], 32, 64);
+                st.l[t] = over_groups(st.l[t], [](float a, float b) { return a + b; });
                 if (g == 0) {
                     sh.m[wave][16 * t + n] = st.m[t];
                     sh.l[wave][16 * t + n] = st.l[t];
@@ -1397,7 +1425,6 @@ struct Attend {
     // is one of W's, whose units may be wider.
     template <class W>
     __device__ static void rows(const AttendArgs& A, const typename W::Part& p) {
-        const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
         const int heads = W::HS == 1 ? G : (G - p.hs * W::RB < W::RB ? G - p.hs * W::RB : W::RB);
 #pragma unroll 1
         for (int i0 = 0; i0 < p.u.n; i0 += C)
@@ -1414,11 +1441,11 @@ struct Attend {
                 State st;
                 load_q(A, u, row, head, st);
                 piece<32>(A, u, p.base, p.end, st);
+                const int lane = own_lane(), n = lane & 15, g = lane >> 4;
                 float* const part = W::part_sums(A, p, p.piece);
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    st.l[t] += __shfl_xor(st.l[t], 16, 64);
-                    st.l[t] += __shfl_xor(st.l[t], 32, 64);
+                    st.l[t] = over_groups(st.l[t], [](float a, float b) { return a + b; });
                     const int r = 16 * t + n, i = r / GH, hh = r - i * GH;
                     if (i >= u.n || h0 + hh >= heads) continue;
                     if (p.pieces == 1) {
@@ -1554,29 +1581,29 @@ struct Attend {
         t = t < r.lo ? r.lo : t >= r.hi ? r.hi - 1 : t;
         return shared_load(p.u.table + static_cast<pg_u32>(t) / PAGE);
     }
+    // Pieces behind the head size repeat the last one, as in load().
     __device__ static void tile_load(const AttendArgs& A, const Part& p, int base, int id, Stage& s) {
         const int lane = threadIdx.x & 63;
         const int off = static_cast<int>(static_cast<pg_u32>(base + 16 * uniform(threadIdx.x >> 6)) % PAGE);
         const char* const kp = A.cache[0] + id * A.s_cache[0][0] + p.h * A.s_cache[0][1] + off * A.s_cache[0][2];
         const char* const vp = A.cache[1] + id * A.s_cache[1][0] + p.h * A.s_cache[1][1] + off * A.s_cache[1][2];
-        const int kd = (lane & 3) * (DP / 4), ko = (lane >> 2) * static_cast<int>(A.s_cache[0][2]) + kd;
+        const int kd = (lane & 3) * (DP / 4), ko = (lane >> 2) * static_cast<int>(A.s_cache[0][2]);
 #pragma unroll
-        for (int j = 0; j < kChunks / 8; ++j) {
-            s.k[j] = pg_u32x4{0, 0, 0, 0};
-            if (D % 64 == 0 || kd + 16 * j < D) s.k[j] = *reinterpret_cast<const pg_u32x4*>(kp + ko + 16 * j);
-        }
-        const int vd = 4 * (lane & (DP / 4 - 1)), h = lane / (DP / 4), vt = static_cast<int>(A.s_cache[1][2]);
+        for (int j = 0; j < kChunks / 8; ++j)
+            s.k[j] = *reinterpret_cast<const pg_u32x4*>(kp + ko + (D % 64 != 0 && kd + 16 * j > D - 16 ? D - 16 : kd + 16 * j));
+        const int vd = 4 * (lane & (DP / 4 - 1)), h = value_half(lane), vt = static_cast<int>(A.s_cache[1][2]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            s.v[i] = 0;
-            if (h < 2 && (D % 64 == 0 || vd < D)) s.v[i] = *reinterpret_cast<const pg_u32*>(vp + (4 * h + (i & 3) + 2 * (i & 4)) * vt + vd);
-        }
+        for (int i = 0; i < 8; ++i)
+            s.v[i] = *reinterpret_cast<const pg_u32*>(vp + (4 * h + (i & 3) + 2 * (i & 4)) * vt + (D % 64 != 0 && vd > D - 4 ? D - 4 : vd));
     }
+    // Which half of the tokens a lane's values are of; up to head size 64 the
+    // upper lanes repeat the lower ones'.
+    __device__ static int value_half(int lane) { return lane / (DP / 4) & 1; }
 
     // A tile that some row does not see whole: what lies outside the unit's
     // positions may be anything.
     __device__ static void tile_edge(const Reach& r, Stage& s, int base, Tiles& T, int buf) {
-        const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane / (DP / 4);
+        const int wave = uniform(threadIdx.x >> 6), h = value_half(own_lane());
         pg_u32 nan = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -1622,7 +1649,8 @@ struct Attend {
         constexpr int KS = DP / 16, DT = DP / 32;
         const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5, wave = uniform(threadIdx.x >> 6);
         const int row_i = n / GH, row_h = n - row_i * GH;
-        const bool valid = row_i < p.u.n && row_i < C && (HS == 1 || p.hs * RB + row_h < G);
+        const auto has_row = [&](int i, int hh) { return i < p.u.n && i < C && (HS == 1 || p.hs * RB + hh < G); };
+        const bool valid = has_row(row_i, row_h);
         // The lane's row attends to positions lo .. hi - 1; all the unit's rows to
         // those of every tile between `from` and `till`.
         const int hi = p.u.p0 + row_i + 1 < p.end ? p.u.p0 + row_i + 1 : p.end;
@@ -1637,22 +1665,17 @@ struct Attend {
         const pg_u32 flip = A.factor < 0.0f ? 0x80008000u : 0u;
         const float factor = fabsf(A.factor);
         pg_u32x4 q[KS];
-        const char* const qp = A.q + ((p.row + row_i) * A.s_q[0] + (p.head + row_h) * A.s_q[1]) * 2;
+        // Places without a row or a dim read the unit's first row, or a dim inside, and are 0.
+        const char* const qp = A.q + (static_cast<pg_i64>(valid ? p.row + row_i : p.rq.row + p.tile * kUnitTokens) * A.s_q[0] +
+                                      (p.head + (valid ? row_h : 0)) * A.s_q[1]) * 2;
 #pragma unroll
         for (int j = 0; j < KS; ++j) {
             const int d = 16 * j + 8 * h;
-            pg_u32x4 w = {0, 0, 0, 0};
-            if (valid && (D % 64 == 0 || d < D)) {
-                if constexpr (VEC) {
-                    w = *reinterpret_cast<const pg_u32x4*>(qp + d * 2);
-                } else {
+            const bool in = valid && (D % 64 == 0 || d < D);
+            Eight<QT> x8;
+            load8<QT, VEC>(qp + (D % 64 != 0 && d >= D ? D - 8 : d) * 2, x8);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        w[e] = static_cast<pg_u32>(*reinterpret_cast<const pg_u16*>(qp + d * 2 + 4 * e)) |
-                               static_cast<pg_u32>(*reinterpret_cast<const pg_u16*>(qp + d * 2 + 4 * e + 2)) << 16;
-                }
-            }
-            q[j] = w ^ flip;
+            for (int e = 0; e < 4; ++e) q[j][e] = (in ? x8.w[e] : 0) ^ flip;
         }
         pg_f32x16 o[DT];
 #pragma unroll
@@ -1842,8 +1865,9 @@ struct Attend {
         }
         if (!done) return false;
         l += __shfl_xor(l, 32, 64);
-        if (!valid) return true;
-        const int at = p.row + row_i, head = p.head + row_h;
+        const int out_lane = own_lane(), out_n = out_lane & 31, out_h = out_lane >> 5, out_i = out_n / GH, out_hh = out_n - out_i * GH;
+        if (!has_row(out_i, out_hh)) return true;
+        const int at = p.row + out_i, head = p.head + out_hh;
         if (p.pieces == 1) {
             const float f = l == 0.0f ? 0.0f : unit / l;
             char* const op = A.out + (at * A.s_out[0] + head * A.s_out[1]) * 2;
@@ -1851,7 +1875,7 @@ struct Attend {
             for (int t = 0; t < DT; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int d = 32 * t + 8 * i + 4 * h;
+                    const int d = 32 * t + 8 * i + 4 * out_h;
                     if (D % 64 != 0 && d >= D) continue;
                     if constexpr (VEC) {
                         pg_u32x2 w;
@@ -1867,18 +1891,18 @@ struct Attend {
                         for (int e = 0; e < 4; ++e) store_elem<QT>(op + (d + e) * 2, o[t][4 * i + e] * f);
                     }
                 }
-            if (LSE && h == 0) A.lse[at * A.s_lse[0] + head * A.s_lse[1]] = lse_of(m, l);
+            if (LSE && out_h == 0) A.lse[at * A.s_lse[0] + head * A.s_lse[1]] = lse_of(m, l);
         } else {
             float* const part = part_sums(A, p, p.piece);
-            if (h == 0) {
-                part[n] = m;
-                part[RB + n] = l;
+            if (out_h == 0) {
+                part[out_n] = m;
+                part[RB + out_n] = l;
             }
 #pragma unroll
             for (int t = 0; t < DT; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    *reinterpret_cast<pg_f32x4*>(part + 2 * RB + n * DP + 32 * t + 8 * i + 4 * h) =
+                    *reinterpret_cast<pg_f32x4*>(part + 2 * RB + out_n * DP + 32 * t + 8 * i + 4 * out_h) =
                         pg_f32x4{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]} * unit;
         }
         return true;

@@ -1,0 +1,92 @@
+"""GPU tests of paged_attention over head sizes, groups and pages that fill no registers evenly, and of its
+prompts, against the plain form in 64 bits (paged_ref).
+
+Each row is held to the error of the kernel that it runs in (test_gpu_paged derives them): weights as two bf16 parts
+(three for float32), or, for a prompt in tiles, as one f16 (two for f16 outputs).  A call gives the same bits
+every time: no sum is taken in an order that changes."""
+
+import numpy as np
+import pytest
+
+import paged_ref as R
+import test_gpu_paged as G
+from pto_wsp import paged_attention
+
+pytestmark = pytest.mark.gpu
+
+
+def tolerance(c, ref):
+    """Of each output, and of each lse."""
+    out, lse, spread, swing, bulk = ref
+    rows, heads, D = out.shape
+    group, page = heads // c["codes"]["k"].shape[1], c["codes"]["k"].shape[2]
+    counts, few = np.diff(c["starts"]), max(1, 64 // group)
+    prompts = c["q"].shape[0] - len(counts) >= few and c["q"].shape[0] * heads > 8192
+    tiled = np.repeat(counts > few, counts) & bool(prompts and c["dt"] != "f32" and D <= 128 and page % 16 == 0)
+    parts = np.where(tiled, G.PROMPT[c["dt"]], G.PARTS[c["dt"]])[:, None, None]
+    n = int(max(c["lengths"].max(initial=0), 1))
+    ds = (D + 8) * 2.0 ** -24 * np.maximum(swing, 1.0)
+    sums = (n / 128 + 64 + D) * 2.0 ** -24
+    tol = G.HALF[c["dt"]] * np.abs(out) + spread * (2 * ds[..., None] + parts + sums) + bulk * np.where(tiled, 2.0 ** -30, 0.0)[:, None, None]
+    tol = tol * (1 + 2 * G.HALF[c["dt"]]) + (2.0 ** -25 if c["dt"] == "f16" else 2.0 ** -140)
+    return tol, 2 * ds + sums + 2.0 ** -23 * np.abs(np.where(np.isfinite(lse), lse, 0.0))
+
+
+def check(c, t, ref):
+    n = int(c["starts"][-1])
+    ref = tuple(x[:n] for x in ref)
+    tol, ltol = tolerance(c, ref)
+    got, lse = t["out"].double().cpu().numpy(), t["lse"].double().cpu().numpy()
+    assert np.array_equal(np.isnan(got[:n]), np.isnan(ref[0]))
+    off = np.abs(got[:n] - ref[0])
+    bad = ~(np.isnan(ref[0]) | (off <= tol))
+    assert not bad.any(), f"off by {np.nanmax(off / tol):.3g} of the tolerance, first at {np.argwhere(bad)[0]}, heads {np.unique(np.argwhere(bad)[:, 1])}"
+    assert (got[n:] == 7.0).all() and (lse[n:] == 7.0).all()
+    assert np.array_equal(np.isinf(lse[:n]), np.isinf(ref[1]))
+    fine = np.isfinite(ref[1])
+    assert (np.abs(lse[:n] - ref[1])[fine] <= ltol[fine]).all()
+
+
+def attend(gpu, monkeypatch, dt, kind, H, group, D, page, lengths, counts, window, many, seed, change=None):
+    """A call with lse, three times, and one without."""
+    torch = G._torch()
+    monkeypatch.setattr(G, "_rows_behind", G._behind["many" if many else "few"])
+    c = G._attend_case(np.random.default_rng(seed), dt, kind, H, group, D, page, lengths, counts, poison=not window)
+    if change:
+        change(c)
+    t = G._attend_tensors(gpu, c)
+    w = {k: G.T(x) for k, x in t.items()}
+    prog = paged_attention(**w, window=window).compile(target="hip_gfx950")
+    first, ref = None, G._reference(c, 1.0 / np.sqrt(D), window)
+    for _ in range(3):
+        t["out"].fill_(7.0), t["lse"].fill_(7.0)
+        prog.execute()
+        prog.synchronize()
+        check(c, t, ref)
+        now = t["out"].clone(), t["lse"].clone()
+        first = first or now
+        assert all(torch.equal(a.nan_to_num(nan=3.0), b.nan_to_num(nan=3.0)) for a, b in zip(first, now))
+    t["out"].fill_(7.0)
+    G.go(paged_attention(**{k: x for k, x in w.items() if k != "lse"}, window=window))
+    check(c, t, ref)
+    return prog
+
+
+FEW = ([700, 60, 311, 200], [3, 1, 2, 2])
+MIXED = ([260, 60, 140, 33], [190, 1, 2, 33])
+
+
+@pytest.mark.parametrize("dt,kind,group,D,page,window,many", [
+    ("bf16", "i8", 7, 240, 8, 250, False), ("f16", "i8", 40, 240, 8, 90, False), ("bf16", "e4m3", 4, 176, 16, 0, False),
+    ("f32", "e4m3", 24, 176, 24, 0, False), ("f16", "e4m3", 40, 112, 24, 0, False), ("f32", "i8", 5, 144, 64, 90, False),
+    ("bf16", "i8", 24, 112, 64, 0, False), ("f32", "i8", 16, 96, 8, 0, False), ("f16", "i8", 3, 208, 1, 0, False),
+    ("f32", "i8", 2, 128, 8, 0, False), ("f32", "e4m3", 7, 256, 8, 0, False), ("f32", "i8", 6, 256, 24, 0, False),
+    ("f32", "e4m3", 4, 128, 24, 0, False), ("bf16", "e4m3", 24, 128, 16, 90, False),
+    ("bf16", "i8", 12, 208, 1, 0, True), ("f32", "e4m3", 12, 208, 8, 0, True), ("f16", "i8", 2, 144, 8, 0, True),
+    ("bf16", "i8", 40, 96, 24, 90, True), ("f32", "i8", 40, 144, 64, 0, True), ("bf16", "e4m3", 5, 240, 16, 90, True),
+    ("bf16", "i8", 1, 112, 16, 90, True), ("f16", "e4m3", 24, 96, 16, 90, True), ("f32", "i8", 4, 256, 16, 90, True),
+    ("f16", "i8", 7, 80, 32, 0, True), ("bf16", "e4m3", 3, 48, 16, 40, True),
+])
+def test_head_sizes(gpu, monkeypatch, dt, kind, group, D, page, window, many):
+    """Single tokens and a few, and (many) prompts beside them."""
+    attend(gpu, monkeypatch, dt, kind, 2, group, D, page, *(MIXED if many else FEW), window, many, D + group)
