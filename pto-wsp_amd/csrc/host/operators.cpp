@@ -401,10 +401,6 @@ void check_operator(const Module& m, const Node& n) {
         if (!s.of("lse").empty()) s.want("lse", {q[0], q[1]});
         if (q[0] > (int64_t(1) << 31) - 1 || B > (1 << 24)) refuse(n, "too many rows or requests");
         if (attr(n, "window") < 0) refuse(n, "a negative window");
-        // Rows 4 to 6 of 7 query heads came out wrong or unwritten there (int8, head
-        // size 80, 8-token pages); why is not known.
-        if (attr(n, "window") > 0 && s.dtype[0] == DType::F32 && c[2] % 16)
-            refuse(n, "float32 queries with a window need pages of a multiple of 16 tokens");
         auto it = n.op_floats.find("scale");
         if (it == n.op_floats.end() || !std::isfinite(it->second)) refuse(n, "missing attribute scale");
     }

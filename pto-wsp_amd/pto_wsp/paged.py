@@ -87,9 +87,9 @@ def paged_attention(*, q: Tensor, k_cache: Tensor, v_cache: Tensor, k_scale: Ten
     among them; its rows ``starts[b] .. starts[b + 1] - 1`` are its last tokens, one or many.  A row at
     position p attends to the positions 0 .. p, or to the last ``window`` of those.  ``out`` (as q) is
     softmax(scale * q k^T) v, 0 for a row without positions; ``lse [T, G * H]`` (F32) the logarithm of the
-    softmax's sum, -inf there.  ``scale`` defaults to 1 / sqrt(D) and may be negative;
-    scales of the cache are not.  F32 queries with a window need pages of a multiple of 16 tokens.  Rows behind the last request, and what
-    lies in the cache beyond a request's tokens, are left alone.
+    softmax's sum, -inf there.  ``scale`` defaults to 1 / sqrt(D) and may be negative; scales of the cache
+    are not.  Rows behind the last request, and what lies in the cache beyond a request's tokens, are left
+    alone.
     """
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1]) if isinstance(q, Tensor) and q.shape and q.shape[-1] > 0 else 1.0

@@ -90,3 +90,19 @@ MIXED = ([260, 60, 140, 33], [190, 1, 2, 33])
 def test_head_sizes(gpu, monkeypatch, dt, kind, group, D, page, window, many):
     """Single tokens and a few, and (many) prompts beside them."""
     attend(gpu, monkeypatch, dt, kind, 2, group, D, page, *(MIXED if many else FEW), window, many, D + group)
+
+
+@pytest.mark.parametrize("kind", ["i8", "e4m3"])
+@pytest.mark.parametrize("group,D,page,window,many", [
+    (7, 80, 8, 250, False), (7, 80, 8, 250, True), (4, 128, 24, 33, False), (5, 256, 8, 500, False), (5, 256, 8, 33, True), (3, 96, 24, 250, True),
+    (1, 16, 40, 250, False), (24, 64, 1, 100, False),
+])
+def test_float32_windows_over_odd_pages(gpu, monkeypatch, kind, group, D, page, window, many):
+    attend(gpu, monkeypatch, "f32", kind, 2, group, D, page, *(MIXED if many else FEW), window, many, D + group)
+
+
+def test_float32_window_of_single_tokens(gpu, monkeypatch):
+    """7 heads of 80 over 8-token pages, 37 requests of one to three tokens."""
+    rng = np.random.default_rng(11)
+    counts = rng.integers(1, 4, 37)
+    attend(gpu, monkeypatch, "f32", "i8", 2, 7, 80, 8, np.maximum(counts, rng.integers(1, 5001, 37)), counts, 1500, False, 12)

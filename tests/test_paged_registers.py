@@ -60,6 +60,14 @@ def test_no_register_is_spilled(tmp_path, monkeypatch, dt, code, D, page, G, win
     _check(tmp_path, monkeypatch, dt, code, D, page, G, window, lse, prompts)
 
 
+@pytest.mark.parametrize("code", ["i8", "e4m3"])
+@pytest.mark.parametrize("page", [8, 16, 24])
+@pytest.mark.parametrize("D", [80, 128, 256])
+@pytest.mark.parametrize("window", [9, 0])
+def test_float32(tmp_path, monkeypatch, code, D, page, window):
+    _check(tmp_path, monkeypatch, "f32", code, D, page, 7, window, D == 80, page == 24 and window > 0)
+
+
 def test_the_search_finds_them():
     code = [(0, "s_and_saveexec_b64 s[2:3], vcc", None), (4, "s_cbranch_execz 2", 16), (8, "global_load_dword v1, v[2:3], off", None),
             (16, "s_mov_b32 s5, s6", None), (20, "scratch_store_dword off, v9, off", None), (28, "s_or_b64 exec, exec, s[2:3]", None)]
