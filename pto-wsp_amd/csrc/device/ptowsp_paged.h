@@ -681,6 +681,8 @@ struct Attend {
     __device__ static pg_i64 pages_on(int id, long long stride) {
         return static_cast<pg_i64>(static_cast<pg_u64>(static_cast<pg_u32>(id)) * static_cast<pg_u32>(stride));
     }
+    // Elements before token `off` of a page, up to 4095 strides of 2^26; 16 of them have 32 bits.
+    __device__ static pg_i64 token_at(int off, long long stride) { return static_cast<pg_i64>(off) * static_cast<int>(stride); }
 
     // Pages of the 32 tokens from `base` on.  Tokens outside the unit's
     // positions take the page of a neighbour inside; they are masked.
@@ -737,8 +739,8 @@ struct Attend {
                     r.ks[i] = r.ks[0];
                     r.vs[i] = r.vs[0];
                 }
-                const char* const kp = page[0] + off * static_cast<int>(A.s_cache[0][2]);
-                const char* const vp = page[1] + off * static_cast<int>(A.s_cache[1][2]);
+                const char* const kp = page[0] + token_at(off, A.s_cache[0][2]);
+                const char* const vp = page[1] + token_at(off, A.s_cache[1][2]);
                 const int ko = m * static_cast<int>(A.s_cache[0][2]), vt = static_cast<int>(A.s_cache[1][2]);
 #pragma unroll
                 for (int j = 0; j < NK; ++j) r.k[i][j] = *reinterpret_cast<const pg_u32x4*>(kp + ko + key_dim(j, g));
@@ -755,14 +757,14 @@ struct Attend {
             r.vs[0] = u.scale[1][pages_on(id, A.s_scale[1][0])];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const char* const row = u.cache[0] + pages_on(of_lane(m4, 16 * i, id), A.s_cache[0][0]) + of_lane(m4, 16 * i, off) * static_cast<int>(A.s_cache[0][2]);
+                const char* const row = u.cache[0] + pages_on(of_lane(m4, 16 * i, id), A.s_cache[0][0]) + token_at(of_lane(m4, 16 * i, off), A.s_cache[0][2]);
 #pragma unroll
                 for (int j = 0; j < NK; ++j) r.k[i][j] = *reinterpret_cast<const pg_u32x4*>(row + key_dim(j, g));
             }
 #pragma unroll
             for (int t = 0; t < 8; ++t) {
                 const int more = (t & 4) * 4 + (t & 3);
-                const char* const row = u.cache[1] + pages_on(of_lane(g4, more, id), A.s_cache[1][0]) + of_lane(g4, more, off) * static_cast<int>(A.s_cache[1][2]);
+                const char* const row = u.cache[1] + pages_on(of_lane(g4, more, id), A.s_cache[1][0]) + token_at(of_lane(g4, more, off), A.s_cache[1][2]);
 #pragma unroll
                 for (int j = 0; j < NK; ++j) r.v[j][t] = *reinterpret_cast<const pg_u32*>(row + value_dim(j, m));
             }

@@ -106,3 +106,22 @@ def test_float32_window_of_single_tokens(gpu, monkeypatch):
     rng = np.random.default_rng(11)
     counts = rng.integers(1, 4, 37)
     attend(gpu, monkeypatch, "f32", "i8", 2, 7, 80, 8, np.maximum(counts, rng.integers(1, 5001, 37)), counts, 1500, False, 12)
+
+
+@pytest.mark.parametrize("page", [64, 40])
+@pytest.mark.parametrize("dt,many", [("bf16", False), ("bf16", True), ("f32", True)])
+def test_tokens_far_apart(gpu, monkeypatch, dt, many, page):
+    """Pages whose last tokens lie beyond 2^31 bytes from their first ones: two pages of one head, keys and values
+    between each other's rows."""
+    torch = G._torch()
+    monkeypatch.setattr(G, "_rows_behind", G._behind["many" if many else "few"])
+    D, step = 64, (1 << 31) // (page - 3) // 16 * 16
+    c = G._attend_case(np.random.default_rng(page), dt, "e4m3", 1, 4, D, page, [2 * page - 3], [70 if many else 2], poison=False)
+    t = G._attend_tensors(gpu, c)
+    assert t["k_cache"].shape[0] == 5 and (page - 1) * step >= 1 << 31 and step <= 1 << 26
+    pool = torch.zeros(page * step, dtype=torch.int8, device=gpu)
+    for i, x in enumerate(("k_cache", "v_cache")):
+        far = torch.as_strided(pool, (5, 1, page, D), (2 * D, 2 * D, step, 1), i * D)
+        t[x] = far.copy_(t[x].view(torch.int8)).view(t[x].dtype)
+    G.go(paged_attention(**{k: G.T(x) for k, x in t.items()}))
+    check(c, t, G._reference(c, 0.125, 0))
