@@ -364,6 +364,84 @@ void run_attend(const Node& n, const std::vector<Operand>& o, const OperatorRun&
     }
 }
 
+// ---- operands that share memory ----
+// Multiples x of `step` bytes, lo <= x <= hi.
+struct Term {
+    int64_t step, lo, hi;
+};
+
+// Whether base + the sum of the terms can lie between `above` and `below`, both
+// exclusive.  Terms by descending step: each is left with the few multiples that
+// the smaller ones can make up for.  Strides that leave it many run out of `tries`
+// and count as a hit.
+bool reaches(const std::vector<Term>& t, size_t k, int64_t base, int64_t above, int64_t below, int& tries) {
+    if (--tries < 0) return true;
+    if (k == t.size()) return base > above && base < below;
+    int64_t least = 0, most = 0;  // of the terms behind this one
+    for (size_t i = k + 1; i < t.size(); ++i) least += t[i].step * t[i].lo, most += t[i].step * t[i].hi;
+    auto floor_div = [](int64_t a, int64_t b) { return a / b - (a % b < 0); };
+    const int64_t lo = std::max(t[k].lo, floor_div(above - base - most, t[k].step) + 1);
+    const int64_t hi = std::min(t[k].hi, -floor_div(-(below - base - least), t[k].step) - 1);
+    for (int64_t x = lo; x <= hi; ++x)
+        if (reaches(t, k + 1, base + t[k].step * x, above, below, tries)) return true;
+    return false;
+}
+bool reaches(std::vector<Term> t, int64_t base, int64_t above, int64_t below) {
+    std::sort(t.begin(), t.end(), [](const Term& a, const Term& b) { return a.step > b.step; });
+    std::vector<Term> merged;
+    for (const Term& x : t) {
+        if (!merged.empty() && merged.back().step == x.step) merged.back().lo += x.lo, merged.back().hi += x.hi;
+        else merged.push_back(x);
+    }
+    int tries = 1 << 16;
+    return reaches(merged, 0, base, above, below, tries);
+}
+
+int64_t extent(const Operand& o) {  // bytes from the first element to the end of the last
+    int64_t e = 1;
+    for (size_t d = 0; d < o.shape.size(); ++d) {
+        if (o.shape[d] == 0) return 0;
+        e += (o.shape[d] - 1) * o.stride[d];
+    }
+    return e * dtype_size(o.dtype);
+}
+
+// Whether some byte belongs to an element of each.
+bool meet(const Operand& a, const Operand& b) {
+    const int64_t ea = extent(a), eb = extent(b), base = b.ptr - a.ptr;
+    if (!ea || !eb || base >= ea || base <= -eb) return false;
+    std::vector<Term> t;
+    for (const Operand* o : {&a, &b})
+        for (size_t d = 0; d < o->shape.size(); ++d)
+            if (o->shape[d] > 1 && o->stride[d] > 0) {
+                const int64_t step = o->stride[d] * dtype_size(o->dtype), n = o->shape[d] - 1;
+                t.push_back(o == &a ? Term{step, -n, 0} : Term{step, 0, n});
+            }
+    return reaches(std::move(t), base, -static_cast<int64_t>(dtype_size(b.dtype)), dtype_size(a.dtype));
+}
+
+// Whether two elements of an operand share memory.
+bool folds(const Operand& o) {
+    std::vector<std::pair<int64_t, int64_t>> dims;  // stride, last index
+    if (!extent(o)) return false;
+    for (size_t d = 0; d < o.shape.size(); ++d)
+        if (o.shape[d] > 1) dims.push_back({o.stride[d], o.shape[d] - 1});
+    std::sort(dims.begin(), dims.end());
+    int64_t reach = 0;
+    bool nested = true;  // every dimension steps over the smaller ones
+    for (const auto& [stride, last] : dims) {
+        nested &= stride > reach;
+        reach += stride * last;
+    }
+    for (size_t first = 0; !nested && first < dims.size(); ++first) {
+        // Two that differ in dimension `first` and those of smaller strides.
+        std::vector<Term> t{{dims[first].first, 1, dims[first].second}};
+        for (size_t d = 0; d < first; ++d) t.push_back({dims[d].first, -dims[d].second, dims[d].second});
+        if (reaches(std::move(t), 0, -1, 1)) return true;
+    }
+    return false;
+}
+
 }  // namespace
 
 void check_operator(const Module& m, const Node& n) {
@@ -414,17 +492,30 @@ bool operator_writes(const Node& n, size_t operand) {
 }
 
 void run_operator(const Node& n, const std::vector<Operand>& operands, const OperatorRun& run) {
-    // Written operands: no two elements at one address, none the start of another operand.
+    // Written operands: no two elements at one address, none where another operand
+    // lies; of staged tensors the whole is copied back, so no two written ones have
+    // host memory between each other.
     for (size_t i = 0; i < operands.size(); ++i) {
         const Operand& w = operands[i];
         if (!operator_writes(n, i) || !w.ptr) continue;
+        const std::string& a = n.tensor_args[i].param;
         for (size_t d = 0; d < w.shape.size(); ++d)
-            if (w.shape[d] > 1 && w.stride[d] == 0) stop(n, n.tensor_args[i].param + " is written and has stride 0");
+            if (w.shape[d] > 1 && w.stride[d] == 0) stop(n, a + " is written and has stride 0");
+        if (folds(w)) stop(n, a + " is written and has elements that share memory");
         for (size_t j = 0; j < operands.size(); ++j) {
-            const std::string &a = n.tensor_args[i].param, &b = n.tensor_args[j].param;
-            if (i == j || operands[j].ptr != w.ptr) continue;
-            if ((a == "new_lengths" && b == "lengths") || (a == "new_used" && b == "used")) continue;  // read before they are written
-            stop(n, a + " is written and lies where " + b + " does");
+            const Operand& o = operands[j];
+            const std::string& b = n.tensor_args[j].param;
+            if (i == j || !o.ptr) continue;
+            if (w.tensor != o.tensor && w.host_bytes && o.host_bytes) {
+                if (operator_writes(n, j) && w.host < o.host + o.host_bytes && o.host < w.host + w.host_bytes)
+                    stop(n, a + " and " + b + " are written and share host memory (device memory may be shared row by row)");
+                continue;
+            }
+            // Read by the thread that writes the same element, before it does.
+            const bool in_place = (a == "new_lengths" && b == "lengths") || (a == "new_used" && b == "used");
+            if (in_place && o.ptr == w.ptr && (w.shape[0] < 2 || o.stride[0] == w.stride[0])) continue;
+            if (o.ptr == w.ptr || (meet(w, o) && run.allocated(w.ptr, static_cast<size_t>(extent(w))) && run.allocated(o.ptr, static_cast<size_t>(extent(o)))))
+                stop(n, a + " is written and lies where " + b + " does");
         }
     }
     if (n.op == "paged_plan") run_plan(n, operands, run);

@@ -23,12 +23,18 @@ struct Operand {
     char* ptr = nullptr;
     std::vector<int64_t> shape, stride;  // elements
     DType dtype = DType::F32;
+    int tensor = 0;              // the tensor that it is a view of, and
+    const char* host = nullptr;  // the host memory of a tensor that is staged
+    size_t host_bytes = 0;
 };
 
 // What a step needs of the run around it.
 struct OperatorRun {
     int cus = 1;         // compute units of the device
     int* err = nullptr;  // the kernels' error flag
+    // Whether so many bytes lie in one allocation: operands whose memory the runtime
+    // does not know are not compared.
+    std::function<bool(const char*, size_t)> allocated;
     // Device scratch for the step: `need` bytes, any content.
     std::function<char*(size_t)> scratch;
     std::function<void(const std::string& source, const char* entry, int64_t blocks, int threads, const void* args, size_t bytes)> launch;

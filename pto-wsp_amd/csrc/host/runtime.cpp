@@ -2016,6 +2016,9 @@ void enqueue_operator(RunEnv& E, const Node& n, hipStream_t stream, uint64_t& la
         o.shape.assign(ti.shape.begin() + static_cast<std::ptrdiff_t>(t.idx.size()), ti.shape.end());
         o.stride.assign(T.stride.begin() + static_cast<std::ptrdiff_t>(t.idx.size()), T.stride.end());
         o.ptr = T.dev ? T.dev + off * dtype_size(ti.dtype) : nullptr;
+        o.tensor = t.tid;
+        o.host = T.host;
+        o.host_bytes = T.staged ? T.bytes : 0;
     }
     OperatorRun run;
     static std::atomic<int> cus[64] = {};
@@ -2025,6 +2028,15 @@ void enqueue_operator(RunEnv& E, const Node& n, hipStream_t stream, uint64_t& la
         cus[dev].store(run.cus, std::memory_order_relaxed);
     }
     run.err = E.err ? E.err : E.P->d_err;
+    run.allocated = [](const char* p, size_t bytes) {
+        hipDeviceptr_t base = nullptr;
+        size_t size = 0;
+        if (hipMemGetAddressRange(&base, &size, const_cast<char*>(p)) != hipSuccess) {
+            (void)hipGetLastError();
+            return false;
+        }
+        return bytes <= size && static_cast<size_t>(p - static_cast<const char*>(base)) <= size - bytes;
+    };
     run.scratch = [&](size_t need) { return operator_scratch(E, n.op, need); };
     run.launch = [&](const std::string& source, const char* entry, int64_t blocks, int threads, const void* args, size_t bytes) {
         const JitKernel* jk = E.nscratch ? jit_loaded(source, entry) : &jit_kernel(source, entry);

@@ -16,8 +16,9 @@ indexed by constants and loop variables (``K[layer]``).  Loops around an operato
 order.  A compiled program may be captured into a HIP graph after a run with the same bindings; run it
 once more before it is captured again, since every captured run keeps its workspace.
 
-Wrong types, shapes and attributes raise ``CompileError`` from ``compile()``, wrong strides, devices or
-overlaps ``RuntimeError`` from ``execute()``; lengths, slots and page numbers are read on the device, and
+Wrong types, shapes and attributes raise ``CompileError`` from ``compile()``, wrong strides or devices
+``RuntimeError`` from ``execute()``, as does a written operand of which a byte is another operand's or its own
+again (keys and values may lie between each other's rows); lengths, slots and page numbers are read on the device, and
 ``synchronize()`` raises ``ExecutionError`` for the ones out of range.  The cycle model has no tasks here.
 """
 
@@ -51,7 +52,7 @@ def paged_plan(*, lengths: Tensor, counts: Tensor, page_table: Tensor, free_page
     pages of the cached tokens; the pages that a request lacks are appended to its row, taken in order of
     requests from ``free_pages[F]``, whose first ``used[1]`` entries are gone.  Writes
 
-    * ``new_lengths[B]`` = lengths + counts and ``new_used[1]`` (each may be the tensor it comes from);
+    * ``new_lengths[B]`` = lengths + counts and ``new_used[1]`` (each may be where it comes from, with the same stride);
     * ``starts[B + 1]``: request b has the rows ``starts[b] .. starts[b + 1] - 1``;
     * ``slots[T]``: page * page_size + offset of each row's token, -1 behind the last row.
 

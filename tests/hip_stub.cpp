@@ -80,6 +80,15 @@ hipError_t hipMemset(void* p, int v, size_t n) { return std::memset(p, v, n), hi
 hipError_t hipMemcpy(void* d, const void* s, size_t n, hipMemcpyKind) { return std::memcpy(d, s, n), hipSuccess; }
 hipError_t hipMemcpyAsync(void* d, const void* s, size_t n, hipMemcpyKind, hipStream_t) { return std::memcpy(d, s, n), hipSuccess; }
 hipError_t hipPointerGetAttributes(hipPointerAttribute_t* a, const void*) { return a->type = hipMemoryTypeDevice, hipSuccess; }
+// Memory that stub_allocation() names is one allocation; other memory is not known.
+static char* g_alloc = nullptr;
+static size_t g_alloc_bytes = 0;
+void stub_allocation(void* p, uint64_t bytes) { g_alloc = static_cast<char*>(p), g_alloc_bytes = bytes; }
+hipError_t hipMemGetAddressRange(hipDeviceptr_t* base, size_t* size, hipDeviceptr_t p) {
+    const char* at = static_cast<char*>(p);
+    if (!g_alloc || at < g_alloc || at >= g_alloc + g_alloc_bytes) return hipErrorNotFound;
+    return *base = g_alloc, *size = g_alloc_bytes, hipSuccess;
+}
 hipError_t hipModuleLoadData(hipModule_t* m, const void*) { return *m = nullptr, uncaptured(); }
 hipError_t hipModuleGetFunction(hipFunction_t* f, hipModule_t, const char* name) {
     *f = reinterpret_cast<hipFunction_t>(new std::string(name));

@@ -10,7 +10,7 @@ import pytest
 
 import paged_ref as R
 import test_gpu_paged as G
-from pto_wsp import paged_attention
+from pto_wsp import DType, Tensor, paged_attention, paged_store
 
 pytestmark = pytest.mark.gpu
 
@@ -125,3 +125,27 @@ def test_tokens_far_apart(gpu, monkeypatch, dt, many, page):
         t[x] = far.copy_(t[x].view(torch.int8)).view(t[x].dtype)
     G.go(paged_attention(**{k: G.T(x) for k, x in t.items()}))
     check(c, t, G._reference(c, 0.125, 0))
+
+
+def test_operands_that_share_memory(gpu):
+    """Parts of one torch tensor, and host arrays that are copied back whole."""
+    torch = G._torch()
+    c = G._attend_case(np.random.default_rng(1), "bf16", "e4m3", 2, 2, 64, 16, [60], [4])
+    t = G._attend_tensors(gpu, c)
+    rows = t["q"].shape[0]
+    both = torch.zeros((rows + 1, 4, 64), dtype=torch.bfloat16, device=gpu)
+    t["q"] = both[1:].copy_(t["q"])
+    with pytest.raises(RuntimeError, match="out is written and lies where q does"):
+        paged_attention(**{k: G.T(x) for k, x in dict(t, out=both[:-1]).items()}).compile(target="hip_gfx950").execute()
+    wide = torch.full((rows, 8, 64), 7.0, dtype=torch.bfloat16, device=gpu)
+    t["q"], t["out"] = wide[:, :4].copy_(t["q"]), wide[:, 4:]
+    G.go(paged_attention(**{k: G.T(x) for k, x in t.items()}))
+    check(c, t, G._reference(c, 0.125, 0))
+
+    pool, x = np.zeros((3, 2, 2, 16, 64), np.int8), np.zeros((5, 2, 64), np.float32)
+    host = {"k": x, "v": x, "slots": np.arange(5, dtype=np.int32), "k_cache": pool[:, 0], "v_cache": pool[:, 1],
+            "k_scale": np.ones((3, 2), np.float32), "v_scale": np.ones((3, 2), np.float32)}
+    kinds = {np.dtype(np.float32): DType.F32, np.dtype(np.int32): DType.I32, np.dtype(np.int8): DType.I8}
+    w = paged_store(**{k: Tensor(data=a, shape=a.shape, dtype=kinds[a.dtype]) for k, a in host.items()})
+    with pytest.raises(RuntimeError, match="k_cache and v_cache are written and share host memory"):
+        w.compile(target="hip_gfx950").execute()
