@@ -291,10 +291,27 @@ int attend_nt(int64_t rows, int64_t batch, int64_t G, int64_t D, int type) {
     return type != 2 && D <= 128 && (G > 16 || each > 64) ? 2 : 1;
 }
 
+// The kernels of a call: of q [rows, q_heads, D] over the cache's [heads, page, D].
+struct AttendForm {
+    AttendShape s;
+    bool prompts;  // requests of more than `few` tokens go to the kernel for prompts
+    int few;
+};
+AttendForm attend_form(const std::vector<int64_t>& q, const std::vector<int64_t>& cache, int64_t batch, DType type, DType code, bool window, bool lse, bool vec) {
+    const int64_t rows = q[0], D = q[2];
+    AttendForm f;
+    f.s = AttendShape{static_cast<int>(D), static_cast<int>(cache[2]), static_cast<int>(q[1] / cache[1]), 1, type_id(type), code_id(code), window, lse, vec};
+    f.few = std::max(1, kFewRows / f.s.G);
+    // Launched if there can be such a request while every other one has a token.
+    f.prompts = rows - batch >= f.few && rows * q[1] > kFewInAll;
+    f.s.NT = attend_nt(f.prompts ? batch : rows, batch, f.s.G, D, f.s.type);
+    return f;
+}
+
 void run_attend(const Node& n, const std::vector<Operand>& o, const OperatorRun& run) {
     AttendArgs A{};
     const Operand &q = o[0], &out = o[8];
-    const int64_t rows = q.shape[0], D = q.shape[2], heads = o[1].shape[1], page = o[1].shape[2], batch = o[6].shape[0];
+    const int64_t rows = q.shape[0], D = q.shape[2], heads = o[1].shape[1], batch = o[6].shape[0];
     const bool lse = o.size() > 9 && o[9].shape.size() == 2;
     if (q.stride[2] != 1 || out.stride[2] != 1) stop(n, "q's and out's last dimensions must have stride 1");
     A.q = q.ptr, A.out = out.ptr;
@@ -318,18 +335,10 @@ void run_attend(const Node& n, const std::vector<Operand>& o, const OperatorRun&
     A.factor = static_cast<float>(n.op_floats.at("scale") * 1.4426950408889634);
     A.err = run.err;
     if (rows == 0 || batch == 0) return;
-    AttendShape s;
-    s.D = static_cast<int>(D), s.page = static_cast<int>(page), s.G = static_cast<int>(q.shape[1] / heads);
-    s.type = type_id(q.dtype);
-    s.NT = attend_nt(rows, batch, s.G, D, s.type);
-    s.code = code_id(o[1].dtype);
-    s.window = A.window > 0, s.lse = lse, s.vec = vectors(q) && vectors(out);
-    // Requests of more tokens than a few go to the kernel for prompts, launched
-    // if there can be one while every other request has a token.
-    const int few = std::max(1, kFewRows / s.G);
-    const bool prompts = rows - batch >= few && rows * q.shape[1] > kFewInAll;
-    A.few = prompts ? few : 0x7FFFFFFF;
-    if (prompts) s.NT = attend_nt(batch, batch, s.G, D, s.type);
+    const AttendForm form = attend_form(q.shape, o[1].shape, batch, q.dtype, o[1].dtype, A.window > 0, lse, vectors(q) && vectors(out));
+    const AttendShape& s = form.s;
+    const bool prompts = form.prompts;
+    A.few = prompts ? form.few : 0x7FFFFFFF;
     const int rb = 16 * s.NT, dp = (s.D + 63) / 64 * 64;
     const int64_t blocks = attend_waves(D) * static_cast<int64_t>(run.cus);
     auto whole = [](int64_t bytes) { return (static_cast<size_t>(bytes) + 255) / 256 * 256; };
@@ -533,17 +542,15 @@ const char* operator_error(int flag) {
     return nullptr;
 }
 
-std::vector<std::pair<std::string, std::string>> operator_sources(const Module& m, const Node& n) {
+std::pair<std::string, std::string> operator_source(const Module& m, const Node& n) {
     const Shapes s = shapes_of(m, n);
-    if (n.op == "paged_plan") return {{plan_source(), "ptowsp_paged_plan"}};
+    if (n.op == "paged_plan") return {plan_source(), "ptowsp_paged_plan"};
     const auto& c = s.of("k_cache");
     const int D = static_cast<int>(c[3]), page = static_cast<int>(c[2]), code = code_id(s.dtype[s.at("k_cache")]);
     if (n.op == "paged_store")
-        return {{store_source(D, page, type_id(s.dtype[0]), code, true, store_chunk(s.of("k")[0], c[1], c[2])), "ptowsp_paged_store"}};
-    const auto& q = s.of("q");
-    const int G = static_cast<int>(q[1] / c[1]);
-    const AttendShape t{D, page, G, attend_nt(q[0], s.of("lengths")[0], G, D, type_id(s.dtype[0])), type_id(s.dtype[0]), code, attr(n, "window") > 0, !s.of("lse").empty(), true};
-    return {{attend_source(t, false), "ptowsp_paged_attention"}, {attend_source(t, true), "ptowsp_paged_attention_prompts"}};
+        return {store_source(D, page, type_id(s.dtype[0]), code, true, store_chunk(s.of("k")[0], c[1], c[2])), "ptowsp_paged_store"};
+    const AttendForm f = attend_form(s.of("q"), c, s.of("lengths")[0], s.dtype[0], s.dtype[s.at("k_cache")], attr(n, "window") > 0, !s.of("lse").empty(), true);
+    return {attend_source(f.s, f.prompts), f.prompts ? "ptowsp_paged_attention_prompts" : "ptowsp_paged_attention"};
 }
 
 }  // namespace ptowsp

@@ -47,8 +47,8 @@ void run_operator(const Node& n, const std::vector<Operand>& operands, const Ope
 // The message of an error flag that an operator's kernel raised, or null.
 const char* operator_error(int flag);
 
-// Sources of the step's kernels for operands laid out one behind the other
-// (for builds without a GPU).
-std::vector<std::pair<std::string, std::string>> operator_sources(const Module& m, const Node& n);
+// The source of the kernels that a run of the step launches, for operands laid out
+// one behind the other, and its first entry (for builds without a GPU).
+std::pair<std::string, std::string> operator_source(const Module& m, const Node& n);
 
 }  // namespace ptowsp

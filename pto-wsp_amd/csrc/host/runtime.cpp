@@ -2619,11 +2619,11 @@ int ptowsp_hip_precompile(ptowsp_program* P, int index, int flags, const char** 
             if (static_cast<int>(li) == index) P->precompiled_source = ek.source;
         }
         size_t at = P->plan.launches.size();  // operator steps come after the launches
-        for (const Node* n : operator_nodes(P->m))
-            for (const auto& [text, entry] : operator_sources(P->m, *n)) {
-                (void)jit_compile(text);
-                if (static_cast<int>(at++) == index) P->precompiled_source = text;
-            }
+        for (const Node* n : operator_nodes(P->m)) {
+            const std::string text = operator_source(P->m, *n).first;
+            (void)jit_compile(text);
+            if (static_cast<int>(at++) == index) P->precompiled_source = text;
+        }
         if (source) *source = P->precompiled_source.c_str();
         return 0;
     } catch (const std::exception& e) {

@@ -64,7 +64,7 @@ def build(verbose: bool = False) -> str:
 
 
 def _operator_workloads():
-    """The paged operators, in types and shapes that between them reach every variant."""
+    """The paged operators, in types and shapes that between them reach every kernel."""
     from pto_wsp import DType, Tensor, paged_attention, paged_plan, paged_store
 
     def T(dtype, *shape):
@@ -73,8 +73,11 @@ def _operator_workloads():
     i32, f32 = DType.I32, DType.F32
     yield paged_plan(lengths=T(i32, 4), counts=T(i32, 4), page_table=T(i32, 4, 8), free_pages=T(i32, 9), used=T(i32, 1),
                      new_lengths=T(i32, 4), new_used=T(i32, 1), starts=T(i32, 5), slots=T(i32, 7), page_size=16)
+    bf16, f16, i8, e4m3 = DType.BF16, DType.F16, DType.I8, DType.F8E4M3
     for code, dt, heads, group, dim, page, rows, window in (
-            (DType.F8E4M3, DType.BF16, 8, 4, 128, 16, 4, 0), (DType.I8, DType.F16, 2, 7, 80, 8, 64, 9), (DType.I8, f32, 1, 40, 256, 64, 4, 0)):
+            # Few rows: 16 at a time and 32; prompts: tiles in bf16 and f16, rows one wave at a time.
+            (e4m3, bf16, 8, 4, 128, 16, 4, 0), (i8, f16, 2, 7, 80, 8, 64, 9), (i8, f32, 1, 40, 256, 64, 4, 0), (e4m3, bf16, 1, 24, 128, 16, 4, 9),
+            (e4m3, bf16, 8, 4, 128, 16, 1024, 0), (e4m3, f16, 2, 8, 64, 32, 1024, 9), (i8, bf16, 2, 4, 80, 24, 2048, 9), (i8, f32, 1, 40, 128, 16, 512, 0)):
         cache = {x + "_cache": T(code, 6, heads, page, dim) for x in "kv"} | {x + "_scale": T(f32, 6, heads) for x in "kv"}
         yield paged_store(k=T(dt, rows, heads, dim), v=T(dt, rows, heads, dim), slots=T(i32, rows), **cache)
         yield paged_attention(q=T(dt, rows, heads * group, dim), out=T(dt, rows, heads * group, dim), page_table=T(i32, 4, 3),
