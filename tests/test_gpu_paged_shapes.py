@@ -149,3 +149,37 @@ def test_operands_that_share_memory(gpu):
     w = paged_store(**{k: Tensor(data=a, shape=a.shape, dtype=kinds[a.dtype]) for k, a in host.items()})
     with pytest.raises(RuntimeError, match="k_cache and v_cache are written and share host memory"):
         w.compile(target="hip_gfx950").execute()
+
+
+# Windows shorter than a tile of 64 tokens, equal to it, beyond it and beyond every context; units of 4 * (32 / group) rows.
+@pytest.mark.parametrize("dt,kind,group,D,page,window", [
+    ("f16", "i8", 4, 128, 16, 100), ("f16", "e4m3", 5, 64, 32, 64), ("bf16", "i8", 5, 128, 64, 1), ("bf16", "e4m3", 4, 128, 16, 64),
+    ("bf16", "i8", 1, 64, 16, 33), ("f16", "i8", 12, 96, 48, 5000), ("bf16", "e4m3", 40, 64, 16, 200),
+])
+def test_windows_of_prompts(gpu, monkeypatch, dt, kind, group, D, page, window):
+    attend(gpu, monkeypatch, dt, kind, 2, group, D, page, [260, 60, 140, 400], [190, 1, 140, 77], window, True, window)
+
+
+@pytest.mark.parametrize("dt,kind,window", [("bf16", "e4m3", 3000), ("f16", "i8", 4500), ("bf16", "i8", 0)])
+def test_prompts_in_pieces(gpu, monkeypatch, dt, kind, window):
+    """Contexts so long that a unit is cut, whose pieces the last launch joins."""
+    attend(gpu, monkeypatch, dt, kind, 1, 4, 128, 16, [9000, 40], [130, 17], window, True, 5)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("window,context", [(25, 200), (0, 200), (3000, 6000)])
+def test_nan_in_prompts(gpu, monkeypatch, dt, window, context):
+    """A NaN among the values and one among the keys: rows whose window holds them, and those alone, have them."""
+    def change(c):
+        table, page = c["table"][0], c["codes"]["v"].shape[2]
+        for token, what in ((context - 60, "v"), (context - 40, "k")):
+            at, off = divmod(token, page)
+            c["codes"][what][table[at], 1, off, 5] = 0x7F
+
+    attend(gpu, monkeypatch, dt, "e4m3", 2, 4, 64, 16, [context, 30], [100, 1], window, True, context, change)
+
+
+@pytest.mark.parametrize("dt,kind,D,page", [("bf16", "e4m3", 128, 16), ("f16", "i8", 64, 8), ("f32", "i8", 80, 16)])
+def test_several_tokens_in_few_rows(gpu, monkeypatch, dt, kind, D, page):
+    """Up to 64 rows a key head: one unit or several, to the accuracy of single tokens."""
+    attend(gpu, monkeypatch, dt, kind, 2, 4, D, page, [300, 77, 16, 41], [16, 5, 16, 1], 0, False, D)
