@@ -1998,6 +1998,9 @@ void enqueue_operator(RunEnv& E, const Node& n, hipStream_t stream, uint64_t& la
     std::vector<Operand> operands(n.tensor_args.size());
     int dev = 0;
     check(hipGetDevice(&dev), "hipGetDevice");
+    if (!E.nscratch && E.P->res_dev != dev)
+        throw std::runtime_error(n.op + ": the program's workspace is on GPU " + std::to_string(E.P->res_dev) + ", the current one is " + std::to_string(dev) +
+                                 " (a program runs on one GPU)");
     for (size_t i = 0; i < operands.size(); ++i) {
         const TensorArg& t = n.tensor_args[i];
         const TensorState& T = E.ts[t.tid];

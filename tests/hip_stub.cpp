@@ -50,7 +50,9 @@ long long stub_coef(int i, int p, int v) { return log()[i].args.coef[p][v]; }
 
 const char* hipGetErrorString(hipError_t e) { return e == hipErrorInvalidValue ? "invalid argument" : "stub error"; }
 hipError_t hipGetLastError() { return hipSuccess; }
-hipError_t hipGetDevice(int* d) { return *d = 0, hipSuccess; }
+static int g_device = 0;  // the current GPU, and the one that any memory is on
+void stub_device(int d) { g_device = d; }
+hipError_t hipGetDevice(int* d) { return *d = g_device, hipSuccess; }
 hipError_t hipDeviceGetAttribute(int* v, hipDeviceAttribute_t a, int) {
     *v = a == hipDeviceAttributeMultiprocessorCount ? 256 : 160 * 1024;
     return hipSuccess;
@@ -79,7 +81,7 @@ hipError_t hipHostGetDevicePointer(void** d, void* h, unsigned) { return *d = h,
 hipError_t hipMemset(void* p, int v, size_t n) { return std::memset(p, v, n), hipSuccess; }
 hipError_t hipMemcpy(void* d, const void* s, size_t n, hipMemcpyKind) { return std::memcpy(d, s, n), hipSuccess; }
 hipError_t hipMemcpyAsync(void* d, const void* s, size_t n, hipMemcpyKind, hipStream_t) { return std::memcpy(d, s, n), hipSuccess; }
-hipError_t hipPointerGetAttributes(hipPointerAttribute_t* a, const void*) { return a->type = hipMemoryTypeDevice, hipSuccess; }
+hipError_t hipPointerGetAttributes(hipPointerAttribute_t* a, const void*) { return a->type = hipMemoryTypeDevice, a->device = g_device, hipSuccess; }
 // Memory that stub_allocation() names is one allocation; other memory is not known.
 static char* g_alloc = nullptr;
 static size_t g_alloc_bytes = 0;
