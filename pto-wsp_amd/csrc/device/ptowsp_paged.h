@@ -548,7 +548,7 @@ __device__ inline void store_rows(const StoreArgs& A) {
 // waves take 32 of every 128 tokens each, with a softmax of their own, and are
 // joined through LDS.  All tiles of all units make one line that the
 // workgroups cut into equal pieces, so a long request is shared by many of
-// them; the pieces of a unit that is cut meet in attend_join.
+// them; the pieces of a unit that is cut meet in join().
 //
 // Per 32 tokens a wave forms S^T = K q^T and O^T += V^T P^T with
 // v_mfma_f32_16x16x32: both operands' lanes hold what their loads deliver.
@@ -1246,9 +1246,9 @@ struct Attend {
     // ---- prompts ----
     // A unit is 4 * C tokens, C for each wave of a workgroup: the waves read the
     // same keys at about the same time, each for rows of its own, and need not
-    // meet.  attend_units lists the units, the longest first, those beyond a
-    // compute unit's share of the work in several pieces, which the
-    // last launch joins.
+    // meet.  list_units() lists the units, the longest first, those beyond 1.3 of
+    // a workgroup's share of the work in several pieces, which finish() joins in
+    // the launch behind.
     static constexpr int kUnitTokens = 4 * C;
 
     struct Span {
@@ -1649,7 +1649,9 @@ struct Attend {
     // False where the piece is to be done over.
     __device__ static bool tiles(const AttendArgs& A, const Part& p, Tiles& T) {
         constexpr int KS = DP / 16, DT = DP / 32;
-        const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5, wave = uniform(threadIdx.x >> 6);
+        // own_lane() keeps a few registers from scratch memory, which head sizes up to 64
+        // have to spare (8192-token prompts of 64: 112 us, and 120 with it).
+        const int lane = DP == 128 ? own_lane() : threadIdx.x & 63, n = lane & 31, h = lane >> 5, wave = uniform(threadIdx.x >> 6);
         const int row_i = n / GH, row_h = n - row_i * GH;
         const auto has_row = [&](int i, int hh) { return i < p.u.n && i < C && (HS == 1 || p.hs * RB + hh < G); };
         const bool valid = has_row(row_i, row_h);

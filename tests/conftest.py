@@ -4,6 +4,9 @@ import sys
 import pytest
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+if os.environ.get("PTO_WSP_TEST_WITHOUT_TORCH"):
+    sys.modules["torch"] = None  # as where torch is not installed: the system's libraries, its compiler among them
+
 for p in (os.path.join(ROOT, "pto-wsp_amd"), ROOT, os.path.join(ROOT, "tests")):
     if p not in sys.path:
         sys.path.insert(0, p)

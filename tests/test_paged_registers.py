@@ -6,6 +6,9 @@ Where only some lanes take a branch, the compiler may put a copy or a spill of a
 before the other lanes go on.  Those lanes then read what the register's new place held before."""
 
 import glob
+import os
+import subprocess
+import sys
 
 import pytest
 
@@ -66,6 +69,15 @@ def test_no_register_is_spilled(tmp_path, monkeypatch, dt, code, D, page, G, win
 @pytest.mark.parametrize("window", [9, 0])
 def test_float32(tmp_path, monkeypatch, code, D, page, window):
     _check(tmp_path, monkeypatch, "f32", code, D, page, 7, window, D == 80, page == 24 and window > 0)
+
+
+def test_the_system_compiler(tmp_path):
+    """The same of the kernels that hiprtc of ROCm itself makes; torch brings its own."""
+    if os.environ.get("PTO_WSP_TEST_WITHOUT_TORCH"):
+        pytest.skip("runs without torch already")
+    run = subprocess.run([sys.executable, "-m", "pytest", "-q", "-p", "no:cacheprovider", "--basetemp", str(tmp_path / "t"), "-k", "lanes_keep", __file__],
+                         env=dict(os.environ, PTO_WSP_TEST_WITHOUT_TORCH="1"), capture_output=True, text=True)
+    assert run.returncode == 0 and "15 passed" in run.stdout, run.stdout[-3000:]
 
 
 def test_the_search_finds_them():
