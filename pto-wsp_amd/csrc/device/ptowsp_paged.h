@@ -681,8 +681,11 @@ struct Attend {
     __device__ static pg_i64 pages_on(int id, long long stride) {
         return static_cast<pg_i64>(static_cast<pg_u64>(static_cast<pg_u32>(id)) * static_cast<pg_u32>(stride));
     }
-    // Elements before token `off` of a page, up to 4095 strides of 2^26; 16 of them have 32 bits.
-    __device__ static pg_i64 token_at(int off, long long stride) { return static_cast<pg_i64>(off) * static_cast<int>(stride); }
+    // Elements before token `off` of a page, up to 4095 strides of 2^26; 16 of them
+    // have 32 bits.  Neither is negative: as a signed product it takes more scalar
+    // registers, which the tile kernel beside it then lacks (8192-token prompts of
+    // head size 64: 120 us, so 112).
+    __device__ static pg_i64 token_at(int off, long long stride) { return pages_on(off, stride); }
 
     // Pages of the 32 tokens from `base` on.  Tokens outside the unit's
     // positions take the page of a neighbour inside; they are masked.

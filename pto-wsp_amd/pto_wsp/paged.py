@@ -57,7 +57,9 @@ def paged_plan(*, lengths: Tensor, counts: Tensor, page_table: Tensor, free_page
     * ``slots[T]``: page * page_size + offset of each row's token, -1 behind the last row.
 
     Where a length or count is negative, or the page table, the free pages or the ``T`` rows do not
-    suffice, ``synchronize()`` raises and nothing has been written.
+    suffice, ``synchronize()`` raises and nothing has been written.  Steps behind it in the same run take
+    ``starts`` and ``slots`` as they were: a plan that may run out of pages is synchronized before the
+    rows are stored.
     """
     return _operator("paged_plan", {"lengths": lengths, "counts": counts, "page_table": page_table, "free_pages": free_pages,
                                     "used": used, "new_lengths": new_lengths, "new_used": new_used, "starts": starts,
@@ -91,6 +93,11 @@ def paged_attention(*, q: Tensor, k_cache: Tensor, v_cache: Tensor, k_scale: Ten
     softmax's sum, -inf there.  ``scale`` defaults to 1 / sqrt(D) and may be negative; scales of the cache
     are not.  Rows behind the last request, and what lies in the cache beyond a request's tokens, are left
     alone.
+
+    Scores, maxima and sums are float32.  A weight is held to 2^-16 of itself for 16-bit queries and to 2^-24
+    for F32 ones.  In prompts of BF16 queries (requests of more than 64 rows a key head, in calls of more than
+    8192 query rows; head size up to 128, pages of a multiple of 16 tokens) weights, values and their scales
+    are f16, each off by at most 2^-11, an eighth of the output's own rounding.
     """
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1]) if isinstance(q, Tensor) and q.shape and q.shape[-1] > 0 else 1.0
