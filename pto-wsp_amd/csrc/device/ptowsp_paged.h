@@ -1652,9 +1652,7 @@ struct Attend {
     // False where the piece is to be done over.
     __device__ static bool tiles(const AttendArgs& A, const Part& p, Tiles& T) {
         constexpr int KS = DP / 16, DT = DP / 32;
-        // own_lane() keeps a few registers from scratch memory, which head sizes up to 64
-        // have to spare (8192-token prompts of 64: 112 us, and 120 with it).
-        const int lane = DP == 128 ? own_lane() : threadIdx.x & 63, n = lane & 31, h = lane >> 5, wave = uniform(threadIdx.x >> 6);
+        const int lane = own_lane(), n = lane & 31, h = lane >> 5, wave = uniform(threadIdx.x >> 6);
         const int row_i = n / GH, row_h = n - row_i * GH;
         const auto has_row = [&](int i, int hh) { return i < p.u.n && i < C && (HS == 1 || p.hs * RB + hh < G); };
         const bool valid = has_row(row_i, row_h);
