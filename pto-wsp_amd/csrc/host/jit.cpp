@@ -141,10 +141,12 @@ std::string jit_cache_dir() {
 
 std::vector<char> jit_compile(const std::string& source) {
     hiprtcProgram prog = nullptr;
-    const char* headers[] = {kDeviceHeader, kLaunchHeader, kPagedHeader, kPagedArgsHeader, kKernelAbi, kPtoisaBridge, kStdTypes, kStdTypes, kStdTypes, kStdTypes};
-    const char* names[] = {"ptowsp_device.h", "ptowsp_launch.h", "ptowsp_paged.h", "ptowsp_paged_args.h", "pto/wsp/codegen/abi/kernel_abi.hpp",
+    const char* headers[] = {kDeviceHeader, kLaunchHeader, kPagedHeader, kPagedArgsHeader, kNumbersHeader, kBlocksHeader, kBlocksArgsHeader, kRotateHeader,
+                             kKernelAbi, kPtoisaBridge, kStdTypes, kStdTypes, kStdTypes, kStdTypes};
+    const char* names[] = {"ptowsp_device.h", "ptowsp_launch.h", "ptowsp_paged.h", "ptowsp_paged_args.h", "ptowsp_numbers.h", "ptowsp_blocks.h",
+                           "ptowsp_blocks_args.h", "ptowsp_rotate.h", "pto/wsp/codegen/abi/kernel_abi.hpp",
                            "pto/wsp/codegen/abi/ptoisa_bridge.hpp", "cstdint", "cstddef", "stdint.h", "stddef.h"};
-    const int nh = source.rfind(kTuMarker, 0) == 0 ? 10 : 4;
+    const int nh = source.rfind(kTuMarker, 0) == 0 ? 14 : 8;
     if (hiprtcCreateProgram(&prog, source.c_str(), "ptowsp_kernel.hip", nh, headers, names) != HIPRTC_SUCCESS)
         throw CompileError("hiprtcCreateProgram failed");
     const int nopt = static_cast<int>(sizeof(kOptions) / sizeof(kOptions[0]));
@@ -168,7 +170,8 @@ std::vector<char> jit_compile(const std::string& source) {
 namespace {
 // The headers and options are hashed once: they are a hundred times a source.
 std::string source_key(const std::string& source) {
-    static const std::string fixed = hex64(fnv1a_64(options_key() + kDeviceHeader + kLaunchHeader + kPagedHeader + kPagedArgsHeader));
+    static const std::string fixed = hex64(fnv1a_64(options_key() + kDeviceHeader + kLaunchHeader + kPagedHeader + kPagedArgsHeader + kNumbersHeader +
+                                                     kBlocksHeader + kBlocksArgsHeader + kRotateHeader));
     static const std::string tu = hex64(fnv1a_64(std::string(kKernelAbi) + kPtoisaBridge + kStdTypes));
     return hex64(fnv1a_64(source + "\n" + fixed + (source.rfind(kTuMarker, 0) == 0 ? tu : "")));
 }

@@ -1,4 +1,4 @@
-#include "operators.hpp"
+#include "operators_shared.hpp"
 
 #include <algorithm>
 #include <cmath>
@@ -13,21 +13,6 @@ namespace ptowsp {
 namespace {
 
 constexpr int kPlanThreads = 1024, kPlanBatch = 4096;  // one workgroup's threads and requests
-
-enum Group { kIndex, kReal, kCode, kScale };  // I32; BF16, F16 or F32; I8 or F8E4M3; F32
-
-struct Param {
-    const char* name;
-    Group group;
-    int rank;
-    bool written;
-    bool optional;
-};
-
-struct Spec {
-    const char* op;
-    std::vector<Param> params;
-};
 
 const std::vector<Spec>& specs() {
     static const std::vector<Spec> all = {
@@ -48,45 +33,11 @@ const std::vector<Spec>& specs() {
 }
 
 const Spec& spec_of(const Node& n) {
-    for (const Spec& s : specs())
-        if (n.op == s.op) return s;
+    for (const std::vector<Spec>* all : {&specs(), &block_specs()})
+        for (const Spec& s : *all)
+            if (n.op == s.op) return s;
     throw CompileError("unknown operator '" + n.op + "'");
 }
-
-[[noreturn]] void refuse(const Node& n, const std::string& why) { throw CompileError(n.op + ": " + why); }
-[[noreturn]] void stop(const Node& n, const std::string& why) { throw std::runtime_error(n.op + ": " + why); }
-
-int64_t attr(const Node& n, const char* key) {
-    auto it = n.op_ints.find(key);
-    if (it == n.op_ints.end()) refuse(n, std::string("missing attribute ") + key);
-    return it->second;
-}
-
-std::string shape_text(const std::vector<int64_t>& s) {
-    std::string out = "[";
-    for (size_t i = 0; i < s.size(); ++i) out += (i ? ", " : "") + std::to_string(s[i]);
-    return out + "]";
-}
-
-// Operands in the order of the operator's parameters (null: left out).
-struct Shapes {
-    const Node& n;
-    const Spec& spec;
-    std::vector<std::vector<int64_t>> shape;
-    std::vector<DType> dtype;
-    size_t at(const char* name) const {
-        for (size_t i = 0; i < spec.params.size(); ++i)
-            if (!std::strcmp(spec.params[i].name, name)) return i;
-        throw CompileError(std::string("internal: no operand ") + name);
-    }
-    const std::vector<int64_t>& of(const char* name) const { return shape[at(name)]; }
-    void want(const char* name, const std::vector<int64_t>& s) const {
-        if (of(name) != s) refuse(n, std::string(name) + " has the shape " + shape_text(of(name)) + ", " + shape_text(s) + " is needed");
-    }
-    void same_type(const char* a, const char* b) const {
-        if (dtype[at(a)] != dtype[at(b)]) refuse(n, std::string(a) + " and " + b + " differ in type");
-    }
-};
 
 Shapes shapes_of(const Module& m, const Node& n) {
     const Spec& spec = spec_of(n);
@@ -106,10 +57,11 @@ Shapes shapes_of(const Module& m, const Node& n) {
         if (static_cast<int>(s.size()) != p.rank)
             refuse(n, std::string(p.name) + " has the shape " + shape_text(s) + ", rank " + std::to_string(p.rank) + " is needed");
         const DType d = ti.dtype;
-        const bool ok = p.group == kIndex   ? d == DType::I32
-                        : p.group == kScale ? d == DType::F32
-                        : p.group == kCode  ? d == DType::I8 || d == DType::F8E4M3
-                                            : d == DType::BF16 || d == DType::F16 || d == DType::F32;
+        const bool ok = p.group == kIndex       ? d == DType::I32
+                        : p.group == kScale     ? d == DType::F32
+                        : p.group == kCode      ? d == DType::I8 || d == DType::F8E4M3
+                        : p.group == kE4M3Code  ? d == DType::F8E4M3
+                                                : d == DType::BF16 || d == DType::F16 || d == DType::F32;
         if (!ok) refuse(n, std::string(p.name) + " has the unsupported type " + dtype_name(d));
         r.shape.push_back(std::move(s));
         r.dtype.push_back(d);
@@ -131,10 +83,6 @@ void check_cache(const Shapes& s) {
     if (page < 1 || page > 4096) refuse(s.n, "pages of " + std::to_string(page) + " tokens (1 to 4096 are supported)");
     if (D < 16 || D > 256 || D % 16) refuse(s.n, "head size " + std::to_string(D) + " (a multiple of 16 up to 256 is needed)");
 }
-
-int type_id(DType d) { return d == DType::BF16 ? 0 : d == DType::F16 ? 1 : 2; }
-int code_id(DType d) { return d == DType::F8E4M3 ? 0 : 1; }
-const char* flag(bool b) { return b ? "true" : "false"; }
 
 std::string entry_source(const std::string& entries) { return "#include \"ptowsp_paged.h\"\n" + entries; }
 
@@ -455,7 +403,9 @@ bool folds(const Operand& o) {
 
 void check_operator(const Module& m, const Node& n) {
     const Shapes s = shapes_of(m, n);
-    if (n.op == "paged_plan") {
+    if (is_block_operator(n)) {
+        check_block_operator(s);
+    } else if (n.op == "paged_plan") {
         const int64_t B = s.of("lengths")[0], page = attr(n, "page_size");
         s.want("counts", {B});
         if (s.of("page_table")[0] != B) refuse(n, "page_table has " + std::to_string(s.of("page_table")[0]) + " rows for " + std::to_string(B) + " requests");
@@ -521,13 +471,17 @@ void run_operator(const Node& n, const std::vector<Operand>& operands, const Ope
                 continue;
             }
             // Read by the thread that writes the same element, before it does.
-            const bool in_place = (a == "new_lengths" && b == "lengths") || (a == "new_used" && b == "used");
-            if (in_place && o.ptr == w.ptr && (w.shape[0] < 2 || o.stride[0] == w.stride[0])) continue;
+            const bool in_place = (a == "new_lengths" && b == "lengths") || (a == "new_used" && b == "used") || (a == "q_out" && b == "q") ||
+                                  (a == "k_out" && b == "k");
+            bool same = in_place && o.ptr == w.ptr;
+            for (size_t d = 0; same && d < w.shape.size(); ++d) same = w.shape[d] < 2 || o.stride[d] == w.stride[d];
+            if (same) continue;
             if (o.ptr == w.ptr || (meet(w, o) && run.allocated(w.ptr, static_cast<size_t>(extent(w))) && run.allocated(o.ptr, static_cast<size_t>(extent(o)))))
                 stop(n, a + " is written and lies where " + b + " does");
         }
     }
-    if (n.op == "paged_plan") run_plan(n, operands, run);
+    if (is_block_operator(n)) run_block_operator(n, operands, run);
+    else if (n.op == "paged_plan") run_plan(n, operands, run);
     else if (n.op == "paged_store") run_store(n, operands, run);
     else run_attend(n, operands, run);
 }
@@ -538,12 +492,14 @@ const char* operator_error(int flag) {
         case 5: return "paged_plan: a page number is negative or its slots exceed 32 bits (rows left out)";
         case 6: return "paged_store: a slot lies outside the cache (rows left out)";
         case 7: return "paged_attention: starts, a length or a page number is out of range";
+        case 8: return "paged_norm_rotate: starts or a position is out of range (rows left out)";
     }
     return nullptr;
 }
 
 std::pair<std::string, std::string> operator_source(const Module& m, const Node& n) {
     const Shapes s = shapes_of(m, n);
+    if (is_block_operator(n)) return block_operator_source(s);
     if (n.op == "paged_plan") return {plan_source(), "ptowsp_paged_plan"};
     const auto& c = s.of("k_cache");
     const int D = static_cast<int>(c[3]), page = static_cast<int>(c[2]), code = code_id(s.dtype[s.at("k_cache")]);

@@ -2048,7 +2048,7 @@ void enqueue_operator(RunEnv& E, const Node& n, hipStream_t stream, uint64_t& la
             LaunchArgs launch;
             char raw[sizeof(LaunchArgs)];
         } buffer;
-        static_assert(sizeof(AttendArgs) <= sizeof(LaunchArgs) && sizeof(StoreArgs) <= sizeof(LaunchArgs) && sizeof(PlanArgs) <= sizeof(LaunchArgs));
+        if (bytes > sizeof buffer) throw std::runtime_error(n.op + ": internal: kernel arguments too large");
         std::memcpy(buffer.raw, args, bytes);
         void* params[] = {buffer.raw};
         launch_kernel(E, jk->function, blocks, threads, 0, stream, params, entry);

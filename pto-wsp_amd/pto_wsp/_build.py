@@ -19,9 +19,10 @@ INCLUDE = os.path.join(os.path.dirname(ROOT), "include")
 BUILD_DIR = os.path.join(CSRC, "_build")
 LIB_PATH = os.path.join(PKG_DIR, "libptowsp_hip.so")
 
-HOST_SOURCES = ["module.cpp", "scalar.cpp", "analysis.cpp", "plan.cpp", "emit.cpp", "jit.cpp", "operators.cpp", "runtime.cpp", "noalloc.hip"]
+HOST_SOURCES = ["module.cpp", "scalar.cpp", "analysis.cpp", "plan.cpp", "emit.cpp", "jit.cpp", "operators.cpp", "blocks.cpp", "runtime.cpp", "noalloc.hip"]
 DEVICE_HEADERS = [("kDeviceHeader", "ptowsp_device.h"), ("kLaunchHeader", "ptowsp_launch.h"), ("kPagedHeader", "ptowsp_paged.h"),
-                  ("kPagedArgsHeader", "ptowsp_paged_args.h")]
+                  ("kPagedArgsHeader", "ptowsp_paged_args.h"), ("kNumbersHeader", "ptowsp_numbers.h"), ("kBlocksHeader", "ptowsp_blocks.h"),
+                  ("kBlocksArgsHeader", "ptowsp_blocks_args.h"), ("kRotateHeader", "ptowsp_rotate.h")]
 DELIM = "PTOWSP_HDR"
 
 

@@ -7,6 +7,7 @@ table names, ``page`` tokens each.  A serving step of requests with new tokens, 
 other into rows, is
 
 * ``paged_plan``       pages for the new tokens, where each row goes, where each request starts;
+* ``paged_norm_rotate`` norms of the rows' queries and keys, and their rotation by position;
 * ``paged_store``      the rows' keys and values into the cache;
 * ``paged_attention``  the rows' queries over their requests' tokens.
 
@@ -30,7 +31,7 @@ from typing import Any, Optional
 from pto_wsp.types import Tensor
 from pto_wsp.workload import Workload
 
-__all__ = ["paged_plan", "paged_store", "paged_attention"]
+__all__ = ["paged_plan", "paged_norm_rotate", "paged_store", "paged_attention"]
 
 
 def _operator(op: str, tensors: dict, attrs: dict) -> Workload:
@@ -64,6 +65,29 @@ def paged_plan(*, lengths: Tensor, counts: Tensor, page_table: Tensor, free_page
     return _operator("paged_plan", {"lengths": lengths, "counts": counts, "page_table": page_table, "free_pages": free_pages,
                                     "used": used, "new_lengths": new_lengths, "new_used": new_used, "starts": starts,
                                     "slots": slots}, {"page_size": int(page_size)})
+
+
+def paged_norm_rotate(*, q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, lengths: Tensor, starts: Tensor, q_out: Tensor, k_out: Tensor,
+                      q_weight: Optional[Tensor] = None, k_weight: Optional[Tensor] = None, offsets: Optional[Tensor] = None,
+                      eps: float = 1e-6, interleaved: bool = False) -> Workload:
+    """Norm and rotation of rows ``q [T, Hq, D]`` and ``k [T, Hk, D]`` (BF16, F16 or F32) in one pass.
+
+    Each head becomes ``x / sqrt(mean(x^2) + eps) * weight`` where its ``q_weight[D]`` or ``k_weight[D]`` (any of
+    the types) is given.  Then the first ``R = 2 * cos.shape[1]`` of its dims are rotated: pair i, which is dims
+    ``i`` and ``i + R / 2`` or, ``interleaved``, ``2 i`` and ``2 i + 1``, becomes ``(a c - b s, b c + a s)`` with
+    ``c, s = cos[p][i], sin[p][i]`` (``[positions, R / 2]``, F32).  Request b holds ``lengths[B]`` tokens, its rows
+    ``starts[b] .. starts[b + 1] - 1`` are its last ones; a token's position p is its place among them, plus
+    ``offsets[b]`` (the tokens of a shared prefix, say).  D is a multiple of 16 up to 256.
+
+    All is computed in float32 and rounded once, into ``q_out`` and ``k_out`` (as q and k, and each may be where it
+    comes from, with the same strides).  Rows of no request are left alone; positions outside the tables raise from
+    ``synchronize()``, their rows are left out.
+    """
+    tensors: dict[str, Any] = {"q": q, "k": k, "cos": cos, "sin": sin, "lengths": lengths, "starts": starts, "q_out": q_out, "k_out": k_out}
+    for name, t in (("q_weight", q_weight), ("k_weight", k_weight), ("offsets", offsets)):
+        if t is not None:
+            tensors[name] = t
+    return _operator("paged_norm_rotate", tensors, {"eps": float(eps), "interleaved": int(interleaved)})
 
 
 def paged_store(*, k: Tensor, v: Tensor, slots: Tensor, k_cache: Tensor, v_cache: Tensor, k_scale: Tensor,
