@@ -416,9 +416,24 @@ __device__ inline pg_i64 uniform64(pg_i64 x) {
     return static_cast<pg_i64>(static_cast<pg_u64>(hi) << 32 | lo);
 }
 
-template <int D_, int PAGE_, int G_, int NT_, int QT_, int CT_, bool WIN_, bool LSE_, bool VEC_, bool PROMPT_ = false>
+// The logarithm of a softmax's sum l, of scores times log2 e relative to m.
+__device__ inline float lse_of(float m, float l) {
+    return l == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f;
+}
+
+// What a call of the kernels is: paged_attention, or a part of
+// paged_prefix_attention (each request's rows over its own tokens; each group's
+// rows over their prefix), which leaves float32 results for merge_parts().
+constexpr int kWhole = 0, kOwnPart = 1, kPrefixPart = 2;
+
+template <int D_, int PAGE_, int G_, int NT_, int QT_, int CT_, bool WIN_, bool LSE_, bool VEC_, bool PROMPT_ = false, int PART_OF_ = kWhole>
 struct Attend {
     static constexpr bool PROMPT = PROMPT_;
+    static constexpr int PART_OF = PART_OF_;
+    static constexpr bool FULL = PART_OF == kPrefixPart;  // every row sees every token
+    static constexpr int OT = PART_OF == kWhole ? QT_ : kF32;
+    static constexpr bool OUT_VEC = VEC_ || PART_OF != kWhole;
+    static constexpr int kError = PART_OF == kWhole ? 7 : 9;
     static constexpr int D = D_, PAGE = PAGE_, G = G_, NT = NT_, QT = QT_, CT = CT_;
     static constexpr bool WIN = WIN_, LSE = LSE_, VEC = VEC_;
     static constexpr int RB = 16 * NT;
@@ -440,11 +455,21 @@ struct Attend {
     };
     __device__ static Request request(const AttendArgs& A, pg_i64 b, bool report) {
         Request r;
-        const int s0 = A.starts[b * A.s_starts], s1 = A.starts[(b + 1) * A.s_starts];
+        int s0, s1;
+        if constexpr (FULL) {
+            // The rows of requests members[b] .. members[b + 1] - 1.
+            const int m0 = A.members[b * A.s_members], m1 = A.members[(b + 1) * A.s_members];
+            const bool in = m0 >= 0 && m1 >= m0 && m1 <= A.requests;
+            s0 = A.starts[(in ? m0 : 0) * A.s_starts];
+            s1 = in ? A.starts[m1 * A.s_starts] : -1;
+        } else {
+            s0 = A.starts[b * A.s_starts];
+            s1 = A.starts[(b + 1) * A.s_starts];
+        }
         int length = A.lengths[b * A.s_lengths];
         const pg_i64 most = A.width * PAGE;
         const bool bad = s0 < 0 || s1 < s0 || s1 > A.rows || length < 0 || length > most;
-        if (bad && report) *A.err = 7;
+        if (bad && report) *A.err = kError;
         r.bad = bad;
         if (bad || (PROMPT ? s1 - s0 <= A.few : s1 - s0 > A.few)) {
             r.row = r.n = r.length = r.first = r.kt = r.units = 0;
@@ -524,6 +549,12 @@ struct Attend {
     // head size 64: 120 us, so 112).
     __device__ static pg_i64 token_at(int off, long long stride) { return pages_on(off, stride); }
 
+    // Position of a request's row i (a token), and the tokens that it sees behind those of row 0.
+    __device__ static int position(const Request& rq, int i) { return FULL ? rq.length - 1 : rq.length - rq.n + i; }
+    __device__ static constexpr int further(int i) { return FULL ? 0 : i; }
+    // Behind the last position that a unit's rows attend to.
+    __device__ static int end_of(int p0, int n) { return FULL ? p0 + 1 : p0 + n > 0 ? p0 + n : 0; }
+
     // Pages of the 32 tokens from `base` on.  Tokens outside the unit's
     // positions take the page of a neighbour inside; they are masked.
     static constexpr int IDS = PAGE % 32 == 0 ? 1 : 2;
@@ -532,7 +563,7 @@ struct Attend {
     };
     __device__ static int checked(const AttendArgs& A, int id) {
         const bool out = static_cast<pg_u32>(id) >= static_cast<pg_u32>(A.pages);
-        if (__ballot(out)) *A.err = 7;
+        if (__ballot(out)) *A.err = kError;
         return out ? 0 : id;
     }
 
@@ -744,7 +775,7 @@ struct Attend {
         pg_u32 seen[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            const int hi = u.p0 + (16 * t + n) / GH + 1, lo = WIN ? hi - A.window : 0;
+            const int hi = u.p0 + further((16 * t + n) / GH) + 1, lo = WIN ? hi - A.window : 0;
             seen[t] = 0;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -864,11 +895,11 @@ struct Attend {
         // o[q][i]: dim 64j + 16g + 4i + q.
         const int d = 64 * j + 16 * g;
         if (D % 64 != 0 && d >= D) return;
-        char* const p = A.out + (row * A.s_out[0] + head * A.s_out[1] + d) * elem_size(QT);
+        char* const p = A.out + (row * A.s_out[0] + head * A.s_out[1] + d) * elem_size(OT);
         float y[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) y[i] = o[i & 3][i >> 2] * f;
-        if constexpr (VEC && QT == kF32) {
+        if constexpr (OUT_VEC && OT == kF32) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) *reinterpret_cast<pg_f32x4*>(p + 16 * i) = pg_f32x4{y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]};
         } else if constexpr (VEC) {
@@ -885,7 +916,7 @@ struct Attend {
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) store_elem<QT>(p + i * elem_size(QT), y[i]);
+            for (int i = 0; i < 16; ++i) store_elem<OT>(p + i * elem_size(OT), y[i]);
         }
     }
 
@@ -957,8 +988,8 @@ struct Attend {
             u.table = A.table + b * A.s_table;
             u.aim(A, h);
             u.n = rq.n - tile * C < C ? rq.n - tile * C : C;
-            u.p0 = rq.length - rq.n + tile * C;
-            u.hi = u.p0 + u.n > 0 ? u.p0 + u.n : 0;
+            u.p0 = position(rq, tile * C);
+            u.hi = end_of(u.p0, u.n);
             u.lo = 0;
             if (WIN && u.p0 + 1 > A.window) u.lo = u.p0 + 1 - A.window;
             const int row = rq.row + tile * C, head = h * G + hs * RB;
@@ -1025,7 +1056,7 @@ struct Attend {
                         part[r] = m[t];
                         part[RB + r] = l[t];
                     } else if (LSE) {
-                        A.lse[(row + i) * A.s_lse[0] + (head + hh) * A.s_lse[1]] = lse_of(m[t], l[t]);
+                        put_sum(A, row + i, head + hh, m[t], l[t]);
                     }
                 }
             }
@@ -1046,8 +1077,11 @@ struct Attend {
         if (threadIdx.x == 0) span[0] = joined;
     }
 
-    __device__ static float lse_of(float m, float l) {
-        return l == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f;
+    // A row's maximum (of scores times log2 e) and sum: their logarithm, or as they are for merge_parts().
+    __device__ static void put_sum(const AttendArgs& A, int row, int head, float m, float l) {
+        float* const p = A.lse + (row * A.s_lse[0] + head * A.s_lse[1]);
+        if constexpr (PART_OF != kWhole) *reinterpret_cast<pg_f32x2*>(p) = pg_f32x2{m, l};
+        else *p = lse_of(m, l);
     }
 
     // This wave's steps of 32 tokens from `base` on, STRIDE tokens apart, below
@@ -1095,10 +1129,10 @@ struct Attend {
         int lo, hi;  // tokens of a unit's keys, lo a multiple of 32
     };
     __device__ static Span span_of(const AttendArgs& A, const Request& rq, int tile) {
-        const int p0 = rq.length - rq.n + tile * kUnitTokens;
+        const int p0 = position(rq, tile * kUnitTokens);
         const int n = rq.n - tile * kUnitTokens < kUnitTokens ? rq.n - tile * kUnitTokens : kUnitTokens;
         Span s;
-        s.hi = p0 + n > 0 ? p0 + n : 0;
+        s.hi = end_of(p0, n);
         s.lo = WIN && p0 + 1 > A.window ? (p0 + 1 - A.window) / 32 * 32 : 0;
         return s;
     }
@@ -1141,7 +1175,7 @@ struct Attend {
         if (total >= kBad) {
             if (threadIdx.x == 0) {
                 A.units[0] = 0;
-                *A.err = 7;
+                *A.err = kError;
             }
             return;
         }
@@ -1251,8 +1285,8 @@ struct Attend {
         p.u.table = A.table + p.b * A.s_table;
         p.u.h = p.h;
         p.u.n = p.rq.n - first < C ? p.rq.n - first : C;
-        p.u.p0 = p.rq.length - p.rq.n + first;
-        p.u.hi = p.u.n > 0 && p.u.p0 + p.u.n > 0 ? p.u.p0 + p.u.n : 0;
+        p.u.p0 = position(p.rq, first);
+        p.u.hi = p.u.n > 0 ? end_of(p.u.p0, p.u.n) : 0;
         p.u.lo = WIN && p.u.p0 + 1 > A.window ? p.u.p0 + 1 - A.window : 0;
     }
     __device__ static float* part_sums(const AttendArgs& A, const Part& p, int piece) {
@@ -1276,8 +1310,8 @@ struct Attend {
                 u.table = p.u.table;
                 u.aim(A, p.h);
                 u.n = p.u.n - i0 < C ? p.u.n - i0 : C;
-                u.p0 = p.u.p0 + i0;
-                u.hi = u.p0 + u.n > 0 ? u.p0 + u.n : 0;
+                u.p0 = p.u.p0 + further(i0);
+                u.hi = end_of(u.p0, u.n);
                 u.lo = WIN && u.p0 + 1 > A.window ? u.p0 + 1 - A.window : 0;
                 const int row = p.row + i0, head = p.head + h0;
                 State st;
@@ -1294,7 +1328,7 @@ struct Attend {
                         const float f = st.l[t] == 0.0f ? 0.0f : 1.0f / st.l[t];
 #pragma unroll
                         for (int j = 0; j < NK; ++j) write_row(A, row + i, head + hh, g, j, st.o[t][j], f);
-                        if (LSE && g == 0) A.lse[(row + i) * A.s_lse[0] + (head + hh) * A.s_lse[1]] = lse_of(st.m[t], st.l[t]);
+                        if (LSE && g == 0) put_sum(A, row + i, head + hh, st.m[t], st.l[t]);
                     } else {
                         const int at = W::place_of(i0 + i, h0 + hh);
                         if (g == 0) {
@@ -1357,13 +1391,17 @@ struct Attend {
             const float f = __shfl(inv, row, 64);
             if (!valid(row) || d >= D) continue;
             const int i = row / GH, hh = row - i * GH;
-            char* const q = A.out + ((p.row + i) * A.s_out[0] + (p.head + hh) * A.s_out[1] + d) * elem_size(QT);
+            char* const q = A.out + ((p.row + i) * A.s_out[0] + (p.head + hh) * A.s_out[1] + d) * elem_size(OT);
+            if constexpr (PART_OF != kWhole) {
+                *reinterpret_cast<pg_f32x4*>(q) = o[t] * f;
+            } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) store_elem<QT>(q + e * elem_size(QT), o[t][e] * f);
+                for (int e = 0; e < 4; ++e) store_elem<OT>(q + e * elem_size(OT), o[t][e] * f);
+            }
         }
         if (LSE && lane < RB && valid(r)) {
             const int i = r / GH, hh = r - i * GH;
-            A.lse[(p.row + i) * A.s_lse[0] + (p.head + hh) * A.s_lse[1]] = lse_of(m, l);
+            put_sum(A, p.row + i, p.head + hh, m, l);
         }
     }
 
@@ -1495,13 +1533,14 @@ struct Attend {
         const bool valid = has_row(row_i, row_h);
         // The lane's row attends to positions lo .. hi - 1; all the unit's rows to
         // those of every tile between `from` and `till`.
-        const int hi = p.u.p0 + row_i + 1 < p.end ? p.u.p0 + row_i + 1 : p.end;
+        const int hi = p.u.p0 + further(row_i) + 1 < p.end ? p.u.p0 + further(row_i) + 1 : p.end;
         const int lo = WIN ? p.u.p0 + row_i + 1 - A.window : 0;
-        const int first = p.rq.length - p.rq.n + p.tile * kUnitTokens;  // position of the unit's first row
+        const int first = position(p.rq, p.tile * kUnitTokens);  // position of the unit's first row
         const int ntok = p.rq.n - p.tile * kUnitTokens < kUnitTokens ? p.rq.n - p.tile * kUnitTokens : kUnitTokens;
         const int till = first + 1 < p.end ? first + 1 : p.end, from = WIN ? first + ntok - A.window : 0;
         Reach reach;
-        reach.hi = first + ntok < p.end ? first + ntok : p.end;
+        const int behind = FULL ? first + 1 : first + ntok;
+        reach.hi = behind < p.end ? behind : p.end;
         reach.lo = WIN && first + 1 > A.window ? first + 1 - A.window : 0;
         // q, with the sign of `factor`: scores are products with scales >= 0.
         const pg_u32 flip = A.factor < 0.0f ? 0x80008000u : 0u;
@@ -1712,14 +1751,16 @@ struct Attend {
         const int at = p.row + out_i, head = p.head + out_hh;
         if (p.pieces == 1) {
             const float f = l == 0.0f ? 0.0f : unit / l;
-            char* const op = A.out + (at * A.s_out[0] + head * A.s_out[1]) * 2;
+            char* const op = A.out + (at * A.s_out[0] + head * A.s_out[1]) * elem_size(OT);
 #pragma unroll
             for (int t = 0; t < DT; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int d = 32 * t + 8 * i + 4 * out_h;
                     if (D % 64 != 0 && d >= D) continue;
-                    if constexpr (VEC) {
+                    if constexpr (OT == kF32) {
+                        *reinterpret_cast<pg_f32x4*>(op + d * 4) = pg_f32x4{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]} * f;
+                    } else if constexpr (VEC) {
                         pg_u32x2 w;
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
@@ -1733,7 +1774,7 @@ struct Attend {
                         for (int e = 0; e < 4; ++e) store_elem<QT>(op + (d + e) * 2, o[t][4 * i + e] * f);
                     }
                 }
-            if (LSE && out_h == 0) A.lse[at * A.s_lse[0] + head * A.s_lse[1]] = lse_of(m, l);
+            if (LSE && out_h == 0) put_sum(A, at, head, m, l);
         } else {
             float* const part = part_sums(A, p, p.piece);
             if (out_h == 0) {
@@ -1751,7 +1792,7 @@ struct Attend {
     }
 
     // Narrow: the kernel for 16 rows a wave.
-    using Narrow = Attend<D, PAGE, G, 1, QT, CT, WIN, LSE, VEC, true>;
+    using Narrow = Attend<D, PAGE, G, 1, QT, CT, WIN, LSE, VEC, true, PART_OF>;
     __device__ static int* over(const AttendArgs& A) { return A.units + kUnitHead + A.room * kUnitInts + A.counters; }
     __device__ static int* cut(const AttendArgs& A) { return over(A) + A.room * A.heads; }
 
@@ -1877,13 +1918,46 @@ struct Attend {
             if (idx < pieces && d < D) {
                 const int i = pr / GH, hh = pr - i * GH;
                 const float s = sums[pr], f = s == 0.0f ? 0.0f : 1.0f / s;
-                char* const p = A.out + ((row + i) * A.s_out[0] + (head + hh) * A.s_out[1] + d) * elem_size(QT);
+                char* const p = A.out + ((row + i) * A.s_out[0] + (head + hh) * A.s_out[1] + d) * elem_size(OT);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) store_elem<QT>(p + e * elem_size(QT), o[e] * f);
-                if (LSE && d == 0) A.lse[(row + i) * A.s_lse[0] + (head + hh) * A.s_lse[1]] = lse_of(top[pr], s);
+                for (int e = 0; e < 4; ++e) store_elem<OT>(p + e * elem_size(OT), o[e] * f);
+                if (LSE && d == 0) put_sum(A, row + i, head + hh, top[pr], s);
             }
         }
     }
 };
+
+// paged_prefix_attention: the two parts of each row and head as one softmax.  A
+// part's result has been divided by its sum l; its weight is l * 2^(m - the larger
+// maximum) over those of both.  Four dims a thread.
+template <int D, int T, bool LSE>
+__device__ inline void merge_parts(const MergeArgs& A) {
+    constexpr int Q = D / 4;
+    const pg_i64 item = static_cast<pg_i64>(blockIdx.x) * blockDim.x + threadIdx.x, at = item / Q;
+    if (at >= A.rows * A.heads) return;
+    const int d = 4 * static_cast<int>(item - at * Q), row = static_cast<int>(at / A.heads), head = static_cast<int>(at - static_cast<pg_i64>(row) * A.heads);
+    auto first_row = [&](int request) { return A.starts[request * A.s_starts]; };
+    const int m0 = A.members[0], m1 = A.members[A.groups * A.s_members];
+    // Rows of no request are left alone; the groups' rows follow each other.
+    if (row < first_row(0) || row >= first_row(A.requests)) return;
+    const bool both = m0 >= 0 && m0 <= m1 && m1 <= A.requests && row >= first_row(m0) && row < first_row(m1);
+    const pg_f32x2 own = *reinterpret_cast<const pg_f32x2*>(A.sums[0] + 2 * at);
+    pg_f32x4 o = *reinterpret_cast<const pg_f32x4*>(A.parts[0] + at * D + d);
+    float m = own[0], l = own[1];
+    if (both) {
+        const pg_f32x2 shared = *reinterpret_cast<const pg_f32x2*>(A.sums[1] + 2 * at);
+        const pg_f32x4 p = *reinterpret_cast<const pg_f32x4*>(A.parts[1] + at * D + d);
+        m = fmaxf(own[0], shared[0]);
+        const float w0 = own[1] == 0.0f ? 0.0f : own[1] * __builtin_amdgcn_exp2f(own[0] - m), w1 = shared[1] == 0.0f ? 0.0f : shared[1] * __builtin_amdgcn_exp2f(shared[0] - m);
+        l = w0 + w1;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        // A part without positions is 0 and has no weight.
+        o = o * (w0 * inv) + p * (w1 * inv);
+    }
+    char* const out = A.out + (row * A.s_out[0] + head * A.s_out[1] + d) * elem_size(T);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) store_elem<T>(out + e * elem_size(T), o[e]);
+    if (LSE && d == 0) A.lse[row * A.s_lse[0] + head * A.s_lse[1]] = lse_of(m, l);
+}
 
 }  // namespace ptowsp

@@ -68,6 +68,22 @@ struct AttendArgs {
     int room, counters;  // entries and counters that `units` has room for
     int cus;             // workgroups that run at once
     int few;       // requests of at most so many rows are left to the kernel for few rows
+    // The prefixes' part of paged_prefix_attention: `batch` groups of requests.
+    const int* members;
+    long long s_members;
+    int requests;
+};
+
+struct MergeArgs {
+    const float* parts[2];  // results over own tokens and over prefixes, [row, head, D]
+    const float* sums[2];   // their maxima and sums, [row, head, 2]
+    const int* starts;
+    const int* members;
+    char* out;
+    float* lse;
+    long long s_starts, s_members, s_out[2], s_lse[2];
+    long long rows;
+    int heads, requests, groups;
 };
 
 }  // namespace ptowsp

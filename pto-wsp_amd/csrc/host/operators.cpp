@@ -28,6 +28,12 @@ const std::vector<Spec>& specs() {
          {{"q", kReal, 3, false, false}, {"k_cache", kCode, 4, false, false}, {"v_cache", kCode, 4, false, false},
           {"k_scale", kScale, 2, false, false}, {"v_scale", kScale, 2, false, false}, {"page_table", kIndex, 2, false, false},
           {"lengths", kIndex, 1, false, false}, {"starts", kIndex, 1, false, false}, {"out", kReal, 3, true, false},
+          {"lse", kScale, 2, true, true}}},
+        {"paged_prefix_attention",
+         {{"q", kReal, 3, false, false}, {"k_cache", kCode, 4, false, false}, {"v_cache", kCode, 4, false, false},
+          {"k_scale", kScale, 2, false, false}, {"v_scale", kScale, 2, false, false}, {"page_table", kIndex, 2, false, false},
+          {"lengths", kIndex, 1, false, false}, {"starts", kIndex, 1, false, false}, {"prefix_table", kIndex, 2, false, false},
+          {"prefix_lengths", kIndex, 1, false, false}, {"members", kIndex, 1, false, false}, {"out", kReal, 3, true, false},
           {"lse", kScale, 2, true, true}}}};
     return all;
 }
@@ -190,11 +196,12 @@ void run_store(const Node& n, const std::vector<Operand>& o, const OperatorRun& 
 struct AttendShape {
     int D, page, G, NT, type, code;
     bool window, lse, vec;
+    int part;  // 0: paged_attention; of paged_prefix_attention 1: own tokens, 2: prefixes
 };
 std::string attend_type(const AttendShape& s, int nt, bool prompt) {
     auto num = [](int v) { return std::to_string(v); };
     return "ptowsp::Attend<" + num(s.D) + ", " + num(s.page) + ", " + num(s.G) + ", " + num(nt) + ", " + num(s.type) + ", " + num(s.code) + ", " +
-           flag(s.window) + ", " + flag(s.lse) + ", " + flag(s.vec) + ", " + flag(prompt) + ">";
+           flag(s.window) + ", " + flag(s.lse) + ", " + flag(s.vec) + ", " + flag(prompt) + (s.part ? ", " + num(s.part) : "") + ">";
 }
 // Waves on a SIMD that the registers allow: 32 requests over 4096 tokens of head
 // size 256 take 101 us with one and 197, spilling, with two.
@@ -245,22 +252,22 @@ struct AttendForm {
     bool prompts;  // requests of more than `few` tokens go to the kernel for prompts
     int few;
 };
-AttendForm attend_form(const std::vector<int64_t>& q, const std::vector<int64_t>& cache, int64_t batch, DType type, DType code, bool window, bool lse, bool vec) {
+AttendForm attend_form(const std::vector<int64_t>& q, const std::vector<int64_t>& cache, int64_t batch, DType type, DType code, bool window, bool lse, bool vec,
+                       int part = 0) {
     const int64_t rows = q[0], D = q[2];
     AttendForm f;
-    f.s = AttendShape{static_cast<int>(D), static_cast<int>(cache[2]), static_cast<int>(q[1] / cache[1]), 1, type_id(type), code_id(code), window, lse, vec};
+    f.s = AttendShape{static_cast<int>(D), static_cast<int>(cache[2]), static_cast<int>(q[1] / cache[1]), 1, type_id(type), code_id(code), window, lse, vec, part};
     f.few = std::max(1, kFewRows / f.s.G);
     // Launched if there can be such a request while every other one has a token.
-    f.prompts = rows - batch >= f.few && rows * q[1] > kFewInAll;
+    f.prompts = rows - batch >= f.few && (rows * q[1] > kFewInAll || part == 2);
     f.s.NT = attend_nt(f.prompts ? batch : rows, batch, f.s.G, D, f.s.type);
     return f;
 }
 
-void run_attend(const Node& n, const std::vector<Operand>& o, const OperatorRun& run) {
+// The operands of attention that its calls have alike.
+AttendArgs attend_args(const Node& n, const std::vector<Operand>& o, const Operand& out, const OperatorRun& run) {
     AttendArgs A{};
-    const Operand &q = o[0], &out = o[8];
-    const int64_t rows = q.shape[0], D = q.shape[2], heads = o[1].shape[1], batch = o[6].shape[0];
-    const bool lse = o.size() > 9 && o[9].shape.size() == 2;
+    const Operand& q = o[0];
     if (q.stride[2] != 1 || out.stride[2] != 1) stop(n, "q's and out's last dimensions must have stride 1");
     A.q = q.ptr, A.out = out.ptr;
     for (int d = 0; d < 2; ++d) A.s_q[d] = q.stride[d], A.s_out[d] = out.stride[d];
@@ -273,52 +280,130 @@ void run_attend(const Node& n, const std::vector<Operand>& o, const OperatorRun&
     A.table = reinterpret_cast<const int*>(o[5].ptr), A.s_table = o[5].stride[0];
     A.lengths = reinterpret_cast<const int*>(o[6].ptr), A.s_lengths = o[6].stride[0];
     A.starts = reinterpret_cast<const int*>(o[7].ptr), A.s_starts = o[7].stride[0];
+    A.batch = o[6].shape[0], A.width = o[5].shape[1], A.pages = std::min<int64_t>(o[1].shape[0], int64_t(1) << 31), A.rows = q.shape[0];
+    A.heads = static_cast<int>(o[1].shape[1]);
+    A.factor = static_cast<float>(n.op_floats.at("scale") * 1.4426950408889634);
+    A.err = run.err;
+    return A;
+}
+
+size_t whole(int64_t bytes) { return (static_cast<size_t>(bytes) + 255) / 256 * 256; }
+
+// The workspace that a form's kernels need, and its places in it.
+struct AttendSpace {
+    size_t spans, few, units, need;  // bytes before the partial results of few rows, the units, the units' partial results; in all
+};
+AttendSpace attend_space(const Node& n, const AttendForm& form, AttendArgs& A, int cus) {
+    const AttendShape& s = form.s;
+    A.few = form.prompts ? form.few : 0x7FFFFFFF;
+    const int rb = 16 * s.NT, dp = (s.D + 63) / 64 * 64;
+    const int64_t blocks = attend_waves(s.D) * static_cast<int64_t>(cus);
+    A.blocks = static_cast<int>(blocks);
+    AttendSpace r{};
+    r.spans = whole(blocks * kSpanInts * 4);
+    r.few = r.spans + whole(2 * blocks * rb * (2 + dp) * 4);
+    r.units = r.need = r.few;
+    if (form.prompts) {
+        // Units, pieces and partial results as list_units makes them, at most.
+        const PromptShape p = prompt_shape(s);
+        const int prb = 16 * p.nt, c = s.G <= prb ? prb / s.G : 1, hs = s.G <= prb ? 1 : (s.G + prb - 1) / prb;
+        A.cus = cus * p.waves;
+        const int64_t entries = hs * (A.rows / (4 * c) + std::min<int64_t>(A.batch, A.rows / (A.few + 1))) + A.cus / A.heads + 1;
+        if (entries * A.heads >= (int64_t(1) << 24)) stop(n, "too many rows for one call");
+        A.room = static_cast<int>(entries), A.counters = 2 * A.cus;
+        r.units += whole((kUnitHead + entries * (kUnitInts + A.heads) + A.counters + A.cus / A.heads + 1) * 4);
+        r.need = r.units + whole(int64_t(2) * A.cus * 4 * prb * (2 + dp) * 4);
+    }
+    return r;
+}
+void attend_launch(const AttendForm& form, const AttendSpace& space, char* scratch, AttendArgs& A, const OperatorRun& run) {
+    A.spans = reinterpret_cast<int*>(scratch);
+    A.parts = reinterpret_cast<float*>(scratch + space.spans);
+    A.units = reinterpret_cast<int*>(scratch + space.few);
+    A.unit_parts = reinterpret_cast<float*>(scratch + space.units);
+    const std::string source = attend_source(form.s, form.prompts);
+    if (form.prompts) {
+        run.launch(source, "ptowsp_paged_attention_units", 1, 1024, &A, sizeof A);
+        run.launch(source, "ptowsp_paged_attention_prompts", static_cast<int64_t>(A.room) * A.heads + A.blocks, 256, &A, sizeof A);
+        run.launch(source, "ptowsp_paged_attention_finish", A.blocks, 256, &A, sizeof A);
+    } else {
+        run.launch(source, "ptowsp_paged_attention", A.blocks, 256, &A, sizeof A);
+        run.launch(source, "ptowsp_paged_attention_join", A.blocks, 256, &A, sizeof A);
+    }
+}
+
+void run_attend(const Node& n, const std::vector<Operand>& o, const OperatorRun& run) {
+    const Operand &q = o[0], &out = o[8];
+    const bool lse = o.size() > 9 && o[9].shape.size() == 2;
+    AttendArgs A = attend_args(n, o, out, run);
     if (lse) {
         A.lse = reinterpret_cast<float*>(o[9].ptr);
         for (int d = 0; d < 2; ++d) A.s_lse[d] = o[9].stride[d];
     }
-    A.batch = batch, A.width = o[5].shape[1], A.pages = std::min<int64_t>(o[1].shape[0], int64_t(1) << 31), A.rows = rows;
-    A.heads = static_cast<int>(heads);
     A.window = static_cast<int>(std::min<int64_t>(attr(n, "window"), 0x7FFFFFFF));
-    A.factor = static_cast<float>(n.op_floats.at("scale") * 1.4426950408889634);
-    A.err = run.err;
-    if (rows == 0 || batch == 0) return;
-    const AttendForm form = attend_form(q.shape, o[1].shape, batch, q.dtype, o[1].dtype, A.window > 0, lse, vectors(q) && vectors(out));
-    const AttendShape& s = form.s;
-    const bool prompts = form.prompts;
-    A.few = prompts ? form.few : 0x7FFFFFFF;
-    const int rb = 16 * s.NT, dp = (s.D + 63) / 64 * 64;
-    const int64_t blocks = attend_waves(D) * static_cast<int64_t>(run.cus);
-    auto whole = [](int64_t bytes) { return (static_cast<size_t>(bytes) + 255) / 256 * 256; };
-    const size_t span_bytes = whole(blocks * kSpanInts * 4), few_bytes = span_bytes + whole(2 * blocks * rb * (2 + dp) * 4);
-    size_t unit_bytes = 0, need = few_bytes;
-    int64_t entries = 0;
-    if (prompts) {
-        // Units, pieces and partial results as list_units makes them, at most.
-        const PromptShape p = prompt_shape(s);
-        const int prb = 16 * p.nt, c = s.G <= prb ? prb / s.G : 1, hs = s.G <= prb ? 1 : (s.G + prb - 1) / prb;
-        A.cus = run.cus * p.waves;
-        entries = hs * (rows / (4 * c) + std::min(batch, rows / (A.few + 1))) + A.cus / heads + 1;
-        if (entries * heads >= (int64_t(1) << 24)) stop(n, "too many rows for one call");
-        A.room = static_cast<int>(entries), A.counters = 2 * A.cus;
-        unit_bytes = whole((kUnitHead + entries * (kUnitInts + heads) + A.counters + A.cus / heads + 1) * 4);
-        need += unit_bytes + whole(int64_t(2) * A.cus * 4 * prb * (2 + dp) * 4);
+    if (A.rows == 0 || A.batch == 0) return;
+    const AttendForm form = attend_form(q.shape, o[1].shape, A.batch, q.dtype, o[1].dtype, A.window > 0, lse, vectors(q) && vectors(out));
+    const AttendSpace space = attend_space(n, form, A, run.cus);
+    attend_launch(form, space, run.scratch(space.need), A, run);
+}
+
+// ---- paged_prefix_attention ----
+std::string merge_source(int64_t D, int type, bool lse) {
+    return entry_source("extern \"C\" __global__ __launch_bounds__(256) void ptowsp_paged_prefix_merge(ptowsp::MergeArgs A) { ptowsp::merge_parts<" +
+                        std::to_string(D) + ", " + std::to_string(type) + ", " + flag(lse) + ">(A); }\n");
+}
+
+void run_prefix(const Node& n, const std::vector<Operand>& o, const OperatorRun& run) {
+    const Operand &q = o[0], &table = o[8], &lengths = o[9], &members = o[10], &out = o[11];
+    const bool lse = o.size() > 12 && o[12].shape.size() == 2;
+    AttendArgs own = attend_args(n, o, out, run), shared = own;
+    if (table.shape[1] > 1 && table.stride[1] != 1) stop(n, "prefix_table's last dimension must have stride 1");
+    shared.table = reinterpret_cast<const int*>(table.ptr), shared.s_table = table.stride[0], shared.width = table.shape[1];
+    shared.lengths = reinterpret_cast<const int*>(lengths.ptr), shared.s_lengths = lengths.stride[0], shared.batch = table.shape[0];
+    shared.members = reinterpret_cast<const int*>(members.ptr), shared.s_members = members.stride[0];
+    shared.requests = static_cast<int>(own.batch);
+    if (own.rows == 0 || own.batch == 0) return;
+    // Both parts leave results in float32, their maxima and sums.
+    const int64_t heads = q.shape[1], D = q.shape[2], all = own.rows * heads;
+    const size_t part_bytes = whole(all * D * 4), sum_bytes = whole(all * 8);
+    AttendArgs* const args[2] = {&own, &shared};
+    AttendForm form[2];
+    AttendSpace space[2];
+    const int many = shared.batch > 0 ? 2 : 1;
+    size_t need = 2 * (part_bytes + sum_bytes);
+    for (int i = 0; i < many; ++i) {
+        form[i] = attend_form(q.shape, o[1].shape, args[i]->batch, q.dtype, o[1].dtype, false, true, vectors(q), 1 + i);
+        space[i] = attend_space(n, form[i], *args[i], run.cus);
+        need += space[i].need;
     }
     char* const scratch = run.scratch(need);
-    A.spans = reinterpret_cast<int*>(scratch);
-    A.parts = reinterpret_cast<float*>(scratch + span_bytes);
-    A.units = reinterpret_cast<int*>(scratch + few_bytes);
-    A.unit_parts = reinterpret_cast<float*>(scratch + few_bytes + unit_bytes);
-    A.blocks = static_cast<int>(blocks);
-    const std::string source = attend_source(s, prompts);
-    if (prompts) {
-        run.launch(source, "ptowsp_paged_attention_units", 1, 1024, &A, sizeof A);
-        run.launch(source, "ptowsp_paged_attention_prompts", entries * heads + blocks, 256, &A, sizeof A);
-        run.launch(source, "ptowsp_paged_attention_finish", blocks, 256, &A, sizeof A);
-    } else {
-        run.launch(source, "ptowsp_paged_attention", blocks, 256, &A, sizeof A);
-        run.launch(source, "ptowsp_paged_attention_join", blocks, 256, &A, sizeof A);
+    MergeArgs M{};
+    char* at = scratch + 2 * (part_bytes + sum_bytes);
+    for (int i = 0; i < 2; ++i) {
+        char* const part = scratch + static_cast<size_t>(i) * (part_bytes + sum_bytes);
+        AttendArgs& A = *args[i];
+        A.out = part;
+        A.s_out[0] = heads * D, A.s_out[1] = D;
+        A.lse = reinterpret_cast<float*>(part + part_bytes);
+        A.s_lse[0] = 2 * heads, A.s_lse[1] = 2;
+        M.parts[i] = reinterpret_cast<const float*>(A.out);
+        M.sums[i] = A.lse;
+        if (i >= many) continue;
+        attend_launch(form[i], space[i], at, A, run);
+        at += space[i].need;
     }
+    M.starts = own.starts, M.s_starts = own.s_starts;
+    M.members = shared.members, M.s_members = shared.s_members;
+    M.out = out.ptr;
+    for (int d = 0; d < 2; ++d) M.s_out[d] = out.stride[d];
+    if (lse) {
+        M.lse = reinterpret_cast<float*>(o[12].ptr);
+        for (int d = 0; d < 2; ++d) M.s_lse[d] = o[12].stride[d];
+    }
+    M.rows = own.rows, M.heads = static_cast<int>(heads), M.requests = shared.requests, M.groups = static_cast<int>(shared.batch);
+    const int64_t groups = (all * (D / 4) + 255) / 256;
+    if (groups >= (int64_t(1) << 24)) stop(n, "too many rows for one call");
+    run.launch(merge_source(D, type_id(q.dtype), lse), "ptowsp_paged_prefix_merge", groups, 256, &M, sizeof M);
 }
 
 // ---- operands that share memory ----
@@ -437,7 +522,15 @@ void check_operator(const Module& m, const Node& n) {
         s.want("starts", {B + 1});
         if (!s.of("lse").empty()) s.want("lse", {q[0], q[1]});
         if (q[0] > (int64_t(1) << 31) - 1 || B > (1 << 24)) refuse(n, "too many rows or requests");
-        if (attr(n, "window") < 0) refuse(n, "a negative window");
+        if (n.op == "paged_attention") {
+            if (attr(n, "window") < 0) refuse(n, "a negative window");
+        } else {
+            const auto& p = s.of("prefix_table");
+            s.want("prefix_lengths", {p[0]});
+            s.want("members", {p[0] + 1});
+            if (p[0] > (1 << 24)) refuse(n, "too many groups");
+            if (p[1] > ((int64_t(1) << 31) - 4096) / c[2]) refuse(n, "the prefix table spans more than 2^31 tokens");
+        }
         auto it = n.op_floats.find("scale");
         if (it == n.op_floats.end() || !std::isfinite(it->second)) refuse(n, "missing attribute scale");
     }
@@ -483,7 +576,8 @@ void run_operator(const Node& n, const std::vector<Operand>& operands, const Ope
     if (is_block_operator(n)) run_block_operator(n, operands, run);
     else if (n.op == "paged_plan") run_plan(n, operands, run);
     else if (n.op == "paged_store") run_store(n, operands, run);
-    else run_attend(n, operands, run);
+    else if (n.op == "paged_attention") run_attend(n, operands, run);
+    else run_prefix(n, operands, run);
 }
 
 const char* operator_error(int flag) {
@@ -493,6 +587,7 @@ const char* operator_error(int flag) {
         case 6: return "paged_store: a slot lies outside the cache (rows left out)";
         case 7: return "paged_attention: starts, a length or a page number is out of range";
         case 8: return "paged_norm_rotate: starts or a position is out of range (rows left out)";
+        case 9: return "paged_prefix_attention: starts, members, a length or a page number is out of range";
     }
     return nullptr;
 }
@@ -505,6 +600,10 @@ std::pair<std::string, std::string> operator_source(const Module& m, const Node&
     const int D = static_cast<int>(c[3]), page = static_cast<int>(c[2]), code = code_id(s.dtype[s.at("k_cache")]);
     if (n.op == "paged_store")
         return {store_source(D, page, type_id(s.dtype[0]), code, true, store_chunk(s.of("k")[0], c[1], c[2])), "ptowsp_paged_store"};
+    if (n.op == "paged_prefix_attention") {
+        const AttendForm f = attend_form(s.of("q"), c, s.of("prefix_table")[0], s.dtype[0], s.dtype[s.at("k_cache")], false, true, true, 2);
+        return {attend_source(f.s, f.prompts), f.prompts ? "ptowsp_paged_attention_prompts" : "ptowsp_paged_attention"};
+    }
     const AttendForm f = attend_form(s.of("q"), c, s.of("lengths")[0], s.dtype[0], s.dtype[s.at("k_cache")], attr(n, "window") > 0, !s.of("lse").empty(), true);
     return {attend_source(f.s, f.prompts), f.prompts ? "ptowsp_paged_attention_prompts" : "ptowsp_paged_attention"};
 }

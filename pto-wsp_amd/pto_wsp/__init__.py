@@ -53,7 +53,7 @@ from pto_wsp.primitives import (
     slot_load_u64,
 )
 from pto_wsp.blocks import block_matmul, block_quantize
-from pto_wsp.paged import paged_plan, paged_store, paged_attention, paged_norm_rotate
+from pto_wsp.paged import paged_plan, paged_store, paged_attention, paged_norm_rotate, paged_prefix_attention
 from pto_wsp import scalar_expr
 from pto_wsp.ptoisa_jit import ptoisa, ptoisa_kernel
 
@@ -72,6 +72,6 @@ __all__ = [
     "KernelParam", "extract_kernel_params", "get_direction", "get_inner_type",
     "CompileError", "ExecutionError", "IRBridgeError", "PtoError",
     "parallel_for", "for_each", "select", "cond", "task", "combine", "sequential", "slot_set_u64", "slot_load_u64",
-    "paged_plan", "paged_store", "paged_attention", "paged_norm_rotate",
+    "paged_plan", "paged_store", "paged_attention", "paged_norm_rotate", "paged_prefix_attention",
     "block_quantize", "block_matmul", "scalar_expr",
 ]

@@ -9,7 +9,8 @@ other into rows, is
 * ``paged_plan``       pages for the new tokens, where each row goes, where each request starts;
 * ``paged_norm_rotate`` norms of the rows' queries and keys, and their rotation by position;
 * ``paged_store``      the rows' keys and values into the cache;
-* ``paged_attention``  the rows' queries over their requests' tokens.
+* ``paged_attention``  the rows' queries over their requests' tokens;
+* ``paged_prefix_attention`` the same where requests share a prefix, which is read once for all of them.
 
 Each call returns a ``Workload`` that compiles by itself, stands in ``sequential`` beside others, or,
 called inside a ``@workload``, is added to the loop around it; operands are tensors or views of them
@@ -31,7 +32,7 @@ from typing import Any, Optional
 from pto_wsp.types import Tensor
 from pto_wsp.workload import Workload
 
-__all__ = ["paged_plan", "paged_norm_rotate", "paged_store", "paged_attention"]
+__all__ = ["paged_plan", "paged_norm_rotate", "paged_store", "paged_attention", "paged_prefix_attention"]
 
 
 def _operator(op: str, tensors: dict, attrs: dict) -> Workload:
@@ -130,3 +131,28 @@ def paged_attention(*, q: Tensor, k_cache: Tensor, v_cache: Tensor, k_scale: Ten
     if lse is not None:
         tensors["lse"] = lse
     return _operator("paged_attention", tensors, {"window": int(window), "scale": float(scale)})
+
+
+def paged_prefix_attention(*, q: Tensor, k_cache: Tensor, v_cache: Tensor, k_scale: Tensor, v_scale: Tensor, prefix_table: Tensor,
+                           prefix_lengths: Tensor, members: Tensor, page_table: Tensor, lengths: Tensor, starts: Tensor, out: Tensor,
+                           scale: Optional[float] = None, lse: Optional[Tensor] = None) -> Workload:
+    """``paged_attention`` of requests in groups, each behind a prefix of its own that the group shares.
+
+    Group s is the requests ``members[s] .. members[s + 1] - 1`` (``members[S + 1]``, ascending); requests ahead of
+    the first group and behind the last one have no prefix.  Its prefix is ``prefix_lengths[S]`` tokens (0: none)
+    in the pages of ``prefix_table[S, W]``, of the same cache.  ``lengths[B]``, ``page_table[B, W]`` and
+    ``starts[B + 1]`` are of the requests' own tokens, as in ``paged_attention``, and a row attends to its group's
+    whole prefix and to the positions 0 .. p of its own: one softmax over both.  ``out`` and ``lse`` are as there.
+
+    A group's rows go over its prefix together, so that its pages are read once and not once a request.  Sums,
+    maxima and the results of both parts are float32; weights are held as there, and in groups of more than 64
+    rows a key head as in prompts there, in calls of any size.
+    """
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.shape[-1]) if isinstance(q, Tensor) and q.shape and q.shape[-1] > 0 else 1.0
+    tensors: dict[str, Any] = {"q": q, "k_cache": k_cache, "v_cache": v_cache, "k_scale": k_scale, "v_scale": v_scale, "page_table": page_table,
+                               "lengths": lengths, "starts": starts, "prefix_table": prefix_table, "prefix_lengths": prefix_lengths,
+                               "members": members, "out": out}
+    if lse is not None:
+        tensors["lse"] = lse
+    return _operator("paged_prefix_attention", tensors, {"scale": float(scale)})
