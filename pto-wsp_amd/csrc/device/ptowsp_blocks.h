@@ -232,102 +232,466 @@ __device__ inline pg_u32x4 codes16(const char* row, pg_i64 k, pg_i64 K) {
     return w;
 }
 
-template <int T>
-__device__ inline void put4(char* out, pg_i64 n, pg_i64 N, pg_f32x4 y) {
+// Columns n .. of a row of N results.
+template <int T, bool INSIDE, int MANY>
+__device__ inline void put_row(char* out, pg_i64 n, pg_i64 N, const float (&y)[MANY]) {
     char* const p = out + n * elem_size(T);
-    if (n + 4 <= N) {
+    if (INSIDE || n + MANY <= N) {
         if constexpr (T == kF32) {
-            __builtin_memcpy(p, &y, 16);
-        } else if constexpr (T == kF16) {
-            const pg_h2 w[2] = {{static_cast<_Float16>(y[0]), static_cast<_Float16>(y[1])}, {static_cast<_Float16>(y[2]), static_cast<_Float16>(y[3])}};
-            __builtin_memcpy(p, w, 8);
+            __builtin_memcpy(p, y, 4 * MANY);
         } else {
-            const pg_bf2 w[2] = {__builtin_convertvector((pg_f32x2{y[0], y[1]}), pg_bf2), __builtin_convertvector((pg_f32x2{y[2], y[3]}), pg_bf2)};
-            __builtin_memcpy(p, w, 8);
+            pg_u32 w[MANY / 2];
+#pragma unroll
+            for (int i = 0; i < MANY / 2; ++i) {
+                if constexpr (T == kF16) w[i] = __builtin_bit_cast(pg_u32, (pg_h2{static_cast<_Float16>(y[2 * i]), static_cast<_Float16>(y[2 * i + 1])}));
+                else w[i] = __builtin_bit_cast(pg_u32, __builtin_convertvector((pg_f32x2{y[2 * i], y[2 * i + 1]}), pg_bf2));
+            }
+            __builtin_memcpy(p, w, 2 * MANY);
         }
         return;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < MANY; ++i)
         if (n + i < N) store_elem<T>(p + i * elem_size(T), y[i]);
 }
+template <int T, bool INSIDE>
+__device__ inline void put4(char* out, pg_i64 n, pg_i64 N, pg_f32x4 x) {
+    put_row<T, INSIDE, 4>(out, n, N, {x[0], x[1], x[2], x[3]});
+}
+template <int T, bool INSIDE>
+__device__ inline void put8(char* out, pg_i64 n, pg_i64 N, pg_f32x4 x, pg_f32x4 y) {
+    put_row<T, INSIDE, 8>(out, n, N, {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]});
+}
 
-template <int BM, int BN, int WM, int WN, int T>
+// Raw buffer descriptor for p (no range check: offsets are bounded on the host).
+__device__ inline pg_u32x4 buffer_at(const void* p) {
+    const pg_u64 a = reinterpret_cast<pg_u64>(p);
+    return pg_u32x4{static_cast<pg_u32>(__builtin_amdgcn_readfirstlane(static_cast<int>(a))),
+                    static_cast<pg_u32>(__builtin_amdgcn_readfirstlane(static_cast<int>(a >> 32))) & 0xFFFFu, 0xFFFFFFFFu, 0x00020000u};
+}
+// 16 (or 4) bytes per lane from a buffer into LDS at `lds` + 16 (or 4) * lane.
+// In inline asm: the compiler would wait for it ahead of every LDS read.  The
+// caller waits with landed_and_read() and a barrier before it reads them.
+__device__ inline void to_lds16(pg_u32x4 buffer, int voff, int soff, pg_u32 lds) {
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
+                 :
+                 : "v"(voff), "s"(buffer), "s"(soff), "s"(lds)
+                 : "memory", "m0");
+}
+__device__ inline void to_lds4(pg_u32x4 buffer, int voff, int soff, pg_u32 lds) {
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dword %0, %1, %2 offen lds"
+                 :
+                 : "v"(voff), "s"(buffer), "s"(soff), "s"(lds)
+                 : "memory", "m0");
+}
+// All but this wave's last N loads have landed, and its reads of LDS have ended.
+template <int N>
+__device__ inline void landed_and_read() {
+    static_assert(N < 64);
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+// The same but for the last `many` stages, MOST at most, of LOADS loads each (the
+// last of MOST: LAST).
+template <int MOST, int LOADS, int LAST = LOADS>
+__device__ inline void landed_of(int many) {
+    if constexpr (MOST == 0) {
+        landed_and_read<0>();
+    } else {
+        if (many >= MOST) landed_and_read<(MOST - 1) * LOADS + LAST>();
+        else landed_of<MOST - 1, LOADS>(many);
+    }
+}
+__device__ inline void meet() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+template <int V>
+struct Int {
+    static constexpr int value = V;
+};
+
+// BM x BN results for a workgroup of WM x WN waves; a ring of NS stages of K in LDS.
+// DIRECT: rows, their distances and K are multiples of 16 bytes, and codes go from
+// memory straight to LDS; otherwise through registers, at any address.
+template <int BM, int BN, int WM, int WN, int NS, bool DIRECT, int T>
 struct BlockGemm {
-    static constexpr int THREADS = 64 * WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
     static constexpr bool F16 = T == kF32;
-    static constexpr int PIECES = (BM + BN) * 8 / THREADS;  // 16-byte pieces of a stage that a thread loads
-    static_assert(kScaleBlock % TN == 0 && (BM + BN) * 8 % THREADS == 0 && THREADS % 8 == 0);
+    static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES, TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
+    static constexpr int PIECES = (BM + BN) * 8 / THREADS, AP = BM * 8 / THREADS;  // 16-byte pieces of a stage that a thread loads, and of a's
+    static constexpr bool PAIRS = TN % 32 == 0;
+    static constexpr int SM = BM < 64 ? 64 : BM, SLOADS = (SM / 64 + WAVES - 1) / WAVES, LOADS = PIECES + SLOADS;
+    static constexpr int STAGE = (BM + BN) * 128 + SM * 4;
+    static_assert(kScaleBlock % TN == 0 && (BM + BN) * 8 % THREADS == 0 && BM * 8 % THREADS == 0);
 
-    // Rows of 128 codes, those of `a` first.  Piece c of row r lies at c ^ (r & 7):
-    // the 16 rows of an operand's read meet in no bank.
+    // Of each stage rows of 128 codes, those of `a` first, then the scales of a's
+    // rows.  Piece c of row r lies at c ^ key(r): the rows of an operand's read meet
+    // in no bank.
     struct Shared {
-        alignas(1024) char bytes[(BM + BN) * 128];
-        float scales[BM];
+        alignas(1024) char bytes[(DIRECT ? NS : 1) * STAGE];
     };
+
+    __device__ static int key_a(int r) { return r & 7; }
+    __device__ static int key_b(int r) { return PAIRS ? (r & 3) | (r >> 1 & 4) : r & 7; }
+
+    struct Place {
+        pg_i64 m0, n0;
+        int split;
+    };
+    // Workgroups take turns on the 8 XCDs: each gets a run of neighbouring tiles, 8
+    // rows of tiles deep.
+    __device__ static Place place(const MatmulArgs& A) {
+        const int all = A.tiles_m * A.tiles_n, split = blockIdx.x / all, id = blockIdx.x - split * all, xcd = id & 7;
+        const int t = (all >> 3) * xcd + (xcd < (all & 7) ? xcd : all & 7) + (id >> 3);
+        const int deep = 8 * A.tiles_n, strip = t / deep, in = t - strip * deep, rows = A.tiles_m - 8 * strip < 8 ? A.tiles_m - 8 * strip : 8;
+        const int n = in / rows;
+        return Place{static_cast<pg_i64>(8 * strip + in - n * rows) * BM, static_cast<pg_i64>(n) * BN, split};
+    }
 
     __device__ static void run(const MatmulArgs& A, Shared& sh) {
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave - wm * WN;
         const int c = lane & 15, g = lane >> 4;
-        const int tile_n = blockIdx.x / A.tiles_m, tile_m = blockIdx.x - tile_n * A.tiles_m;
-        const pg_i64 m0 = static_cast<pg_i64>(tile_m) * BM, n0 = static_cast<pg_i64>(tile_n) * BN;
+        const Place at = place(A);
+        const int rows = A.M - at.m0 < BM ? static_cast<int>(A.M - at.m0) : BM, cols = A.N - at.n0 < BN ? static_cast<int>(A.N - at.n0) : BN;
         pg_f32x4 acc[FM][FN];
 #pragma unroll
         for (int i = 0; i < FM; ++i)
 #pragma unroll
             for (int j = 0; j < FN; ++j) acc[i][j] = pg_f32x4{0, 0, 0, 0};
-        const char* from[PIECES];
-        pg_i64 at[PIECES];
+        const pg_i64 strip = (at.n0 + wn * TN) / kScaleBlock, strips = (A.N + kScaleBlock - 1) / kScaleBlock;
+        // The split's stages, and its codes of a row.
+        const int first = static_cast<int>(static_cast<pg_i64>(A.stages) * at.split / A.splits);
+        const int stages = static_cast<int>(static_cast<pg_i64>(A.stages) * (at.split + 1) / A.splits) - first;
+        const pg_i64 k0 = static_cast<pg_i64>(first) * kScaleBlock, K = A.K - k0 < static_cast<pg_i64>(stages) * kScaleBlock ? A.K - k0 : static_cast<pg_i64>(stages) * kScaleBlock;
+        const char* const a0 = A.a + at.m0 * A.s_a + k0;
+        const char* const b0 = A.b + at.n0 * A.s_b + k0;
+        const float* const as0 = A.a_scale + at.m0 * A.s_as[0] + first * A.s_as[1];
+        const pg_u32x4 buf_a = buffer_at(a0), buf_b = buffer_at(b0), buf_s = buffer_at(as0);
+        const pg_u32 lds = static_cast<pg_u32>(reinterpret_cast<pg_u64>((const __attribute__((address_space(3))) void*)sh.bytes));
+        const int tail = static_cast<int>(K - static_cast<pg_i64>(stages - 1) * kScaleBlock);  // codes of the last stage
+        // A thread's pieces: slot i & 7 of row i >> 3 holds the piece (i ^ row) & 7.
+        int voff[PIECES], soff_s[SLOADS];
+        pg_i64 far[PIECES];  // the same without a limit
+        auto piece_row = [&](int p) { return static_cast<int>(threadIdx.x + THREADS * p) >> 3; };
+        const int slot = static_cast<int>(threadIdx.x) & 7, row8 = static_cast<int>(threadIdx.x) >> 3;
+        const int col[2] = {(slot ^ key_a(row8)) * 16, (slot ^ key_b(row8)) * 16};  // first codes of its pieces of a, of b
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
-            const int i = threadIdx.x + THREADS * p, r = i >> 3;
-            const pg_i64 m = m0 + r < A.M ? m0 + r : A.M - 1, n = n0 + r - BM < A.N ? n0 + r - BM : A.N - 1;
-            from[p] = r < BM ? A.a + m * A.s_a : A.b + n * A.s_b;
-            at[p] = (i & 7) * 16;
+            const int r = piece_row(p);
+            // Rows behind the last one repeat it; their results are not stored.
+            far[p] = r < BM ? (r < rows ? r : rows - 1) * A.s_a : (r - BM < cols ? r - BM : cols - 1) * A.s_b;
+            voff[p] = static_cast<int>(far[p]) + col[p >= AP];
         }
-        const pg_i64 strip = (n0 + wn * TN) / kScaleBlock, strips = (A.N + kScaleBlock - 1) / kScaleBlock;
-        const float* const bs = A.b_scale + (strip < strips ? strip : strips - 1) * A.s_bs[0];
-        for (int s = 0; s < A.stages; ++s) {
+#pragma unroll
+        for (int p = 0; p < SLOADS; ++p) {
+            const int r = (wave + WAVES * p) % (SM / 64) * 64 + lane;
+            soff_s[p] = static_cast<int>((r < rows ? r : rows - 1) * A.s_as[0]) * 4;
+        }
+        // The p-th of a wave's loads of stage s, into a place of the ring.
+        auto load = [&](int s, int slot, int p, const int (&back)[2]) {
+            const pg_u32 base = lds + slot * STAGE;
+            if (p < PIECES) {
+                to_lds16(p < AP ? buf_a : buf_b, voff[p < PIECES ? p : 0] - back[p >= AP], s * kScaleBlock, base + (wave * 64 + THREADS * p) * 16);
+            } else {
+                const int q = p - PIECES;
+                to_lds4(buf_s, soff_s[q], static_cast<int>(s * A.s_as[1]) * 4, base + (BM + BN) * 128 + (wave + WAVES * q) % (SM / 64) * 256);
+            }
+        };
+        // The scale of the weights' block, one stage ahead, through the scalar cache.
+        const auto* const bs = reinterpret_cast<const __attribute__((address_space(4))) float*>(
+            reinterpret_cast<pg_u64>(A.b_scale + (strip < strips ? strip : strips - 1) * A.s_bs[0] + first * A.s_bs[1]));
+        auto weight_scale = [&](int s) { return bs[(s < stages ? s : stages - 1) * A.s_bs[1]]; };
+        // Where this lane's pieces of a row lie, in every 16 rows alike.  Its four numbers
+        // of columns 16j .. and of 16 (j + 1) .. shall be neighbours in the result, so the
+        // MFMAs' rows 4g + e of both are columns 8g + e and 8g + 4 + e.
+        const int rb = PAIRS ? 8 * (c >> 2) + (c & 3) : c;
+        int piece_a[2], piece_b[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            piece_a[h] = c * 128 + ((g + 4 * h) ^ key_a(c)) * 16;
+            piece_b[h] = rb * 128 + ((g + 4 * h) ^ key_b(rb)) * 16;
+        }
+        auto column = [](int j) { return PAIRS ? 32 * (j >> 1) + 4 * (j & 1) : 16 * j; };
+        const int arow = wm * TM * 128, brow = (BM + wn * TN) * 128, srow = (BM + BN) * 128 + (wm * TM + c) * 4;
+        // What the wave has read of a stage: its columns, and the next 16 rows.
+        Codes32<F16> b[FN];
+        pg_u32x4 raw[2];
+        float raw_scale;
+        auto read = [&](const char* p) { return *reinterpret_cast<const pg_u32x4*>(p); };
+        auto read_rows = [&](const char* stage, int i) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) raw[h] = read(stage + arow + i * 2048 + piece_a[h]);
+            raw_scale = *reinterpret_cast<const float*>(stage + srow + 64 * i);
+        };
+        auto read_column = [&](const char* stage, int j, int limit) {
+            pg_u32x4 w[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                w[h] = read(stage + brow + column(j) * 128 + piece_b[h]);
+                if (limit) {  // the stage's codes
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[h][e] = 64 * h + 16 * g < limit ? w[h][e] : 0;
+                }
+            }
+            b[j] = Codes32<F16>(w[0], w[1]);
+        };
+        // The MFMAs of stage s, of which the columns and the first rows have been read.
+        // A sum is used two MFMAs later.  At POINT the stage's last rows have been read,
+        // and the workgroup meets: the next stage has landed, and this one's place is
+        // free.  Its columns follow those of this stage as their last MFMAs begin.  The
+        // loads are spread among the MFMAs, since each holds up the wave until it has
+        // left: EARLY of them behind POINT, a stage ahead of the others.  The order is
+        // kept as it stands here.
+        // KIND: 3 all stages up to s + NS are there to load; 2 none behind s + NS - 1; 1
+        // nothing is left to load; 0 the last stage.
+        constexpr int MANY = FM * FN, LAG = MANY > 2 ? 2 : MANY - 1;
+        constexpr int POINT = FM > 1 ? (FM - 2) * FN + FN / 2 : 0, EARLY = FM > 1 ? LOADS * (MANY - POINT) / MANY : 0;
+        int s = 0, ring = 0;
+        auto body = [&](auto kind, float sb, const int (&back1)[2], const int (&back2)[2]) {
+            constexpr int KIND = decltype(kind)::value;
+            const int after = ring == NS - 1 ? 0 : ring + 1, before = ring == 0 ? NS - 1 : ring - 1;
+            const char* const stage = sh.bytes + ring * STAGE;
+            const char* const behind = sh.bytes + after * STAGE;
+            const int limit = KIND == 3 ? 0 : s + 2 == stages ? tail : kScaleBlock;
+            pg_f32x4 y[LAG + 1];
+            float f[2];
+            Codes32<F16> a;
+            auto add = [&](int k) {
+                const int i = k / FN, j = k - i * FN;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(y[k % (LAG + 1)][e], f[i & 1], acc[i][j][e]);
+            };
+#pragma unroll
+            for (int k = 0; k < MANY; ++k) {
+                const int i = k / FN, j = k - i * FN;
+                if (j == 0) {
+                    a = Codes32<F16>(raw[0], raw[1]);
+                    f[i & 1] = raw_scale * sb;
+                    if (i + 1 < FM) read_rows(stage, i + 1);
+                    else if (KIND > 0 && FM > 1) read_rows(behind, 0);
+                }
+                y[k % (LAG + 1)] = stage_sum<F16>(b[j], a);
+                if constexpr (KIND > 0) {
+                    if (KIND > 1 && k < POINT) {
+#pragma unroll
+                        for (int p = EARLY + k * (LOADS - EARLY) / POINT; p < EARLY + (k + 1) * (LOADS - EARLY) / POINT; ++p) load(s + NS - 1, before, p, back1);
+                    }
+                    if (k == POINT) {
+                        if (KIND > 1 && POINT == 0) {
+#pragma unroll
+                            for (int p = EARLY; p < LOADS; ++p) load(s + NS - 1, before, p, back1);
+                        }
+                        if (KIND > 1 || NS == 2) landed_and_read<(NS - 2) * LOADS>();
+                        else landed_of<NS - 2, LOADS>(stages - s - 2);
+                        meet();
+                    }
+                    if (KIND > 2 && k >= POINT) {
+#pragma unroll
+                        for (int p = (k - POINT) * EARLY / (MANY - POINT); p < (k - POINT + 1) * EARLY / (MANY - POINT); ++p) load(s + NS, ring, p, back2);
+                    }
+                    if (FM > 1 && i == FM - 1) read_column(behind, j, limit);
+                }
+                if (k >= LAG) add(k - LAG);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if constexpr (KIND > 0 && FM == 1) {
+#pragma unroll
+                for (int j = 0; j < FN; ++j) read_column(behind, j, limit);
+                read_rows(behind, 0);
+            }
+#pragma unroll
+            for (int k = MANY - LAG; k < MANY; ++k) add(k);
+            __builtin_amdgcn_sched_barrier(0);
+            ring = after;
+            ++s;
+        };
+        auto begin = [&](int limit) {
+            read_rows(sh.bytes, 0);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) read_column(sh.bytes, j, limit);
+        };
+        if constexpr (DIRECT) {
+            // Pieces behind K repeat the row's last one; their weights are cleared where
+            // they are read.
+            const int none[2] = {0, 0}, back[2] = {col[0] > tail - 16 ? col[0] - (tail - 16) : 0, col[1] > tail - 16 ? col[1] - (tail - 16) : 0};
+            auto back_of = [&](int stage, int (&x)[2]) {
+                x[0] = stage == stages - 1 ? back[0] : 0;
+                x[1] = stage == stages - 1 ? back[1] : 0;
+            };
+            int now[2];
+#pragma unroll
+            for (int q = 0; q < NS; ++q) {
+                back_of(q, now);
+                if (q < stages)
+#pragma unroll
+                    for (int p = 0; p < (q < NS - 1 ? LOADS : EARLY); ++p) load(q, q, p, now);
+            }
+            landed_of<NS - 1, LOADS, EARLY>(stages - 1);
+            meet();
+            begin(stages == 1 ? tail : kScaleBlock);
+            float sb = weight_scale(0), next;
+            while (s + NS < stages) {
+                next = weight_scale(s + 1);
+                back_of(s + NS, now);
+                body(Int<3>(), sb, none, now);
+                sb = next;
+            }
+            if (s + NS == stages) {
+                next = weight_scale(s + 1);
+                body(Int<2>(), sb, back, none);
+                sb = next;
+            }
+            while (s + 1 < stages) {
+                next = weight_scale(s + 1);
+                body(Int<1>(), sb, none, none);
+                sb = next;
+            }
+            body(Int<0>(), sb, none, none);
+        } else {
             pg_u32x4 w[PIECES];
+            auto fetch = [&](int s) {
 #pragma unroll
-            for (int p = 0; p < PIECES; ++p) w[p] = codes16(from[p], static_cast<pg_i64>(s) * kScaleBlock + at[p], A.K);
-            __syncthreads();
+                for (int p = 0; p < PIECES; ++p)
+                    w[p] = codes16((p < AP ? a0 : b0) + far[p], static_cast<pg_i64>(s) * kScaleBlock + col[p >= AP], K);
+            };
+            fetch(0);
+            for (int t = 0; t < stages; ++t) {
+                __syncthreads();
 #pragma unroll
-            for (int p = 0; p < PIECES; ++p) {
-                const int i = threadIdx.x + THREADS * p, r = i >> 3;
-                *reinterpret_cast<pg_u32x4*>(sh.bytes + r * 128 + ((i & 7) ^ (r & 7)) * 16) = w[p];
+                for (int p = 0; p < PIECES; ++p) *reinterpret_cast<pg_u32x4*>(sh.bytes + (threadIdx.x + THREADS * p) * 16) = w[p];
+                for (int r = threadIdx.x; r < BM; r += THREADS)
+                    reinterpret_cast<float*>(sh.bytes + (BM + BN) * 128)[r] = as0[(r < rows ? r : rows - 1) * A.s_as[0] + t * A.s_as[1]];
+                __syncthreads();
+                if (t + 1 < stages) fetch(t + 1);
+                const int none[2] = {0, 0};
+                begin(0);
+                body(Int<0>(), weight_scale(t), none, none);
+                ring = 0;
             }
-            for (int r = threadIdx.x; r < BM; r += THREADS) {
-                const pg_i64 m = m0 + r < A.M ? m0 + r : A.M - 1;
-                sh.scales[r] = A.a_scale[m * A.s_as[0] + s * A.s_as[1]];
-            }
-            __syncthreads();
-            const float sb = bs[s * A.s_bs[1]];
-            auto frag = [&](int r, int half) { return *reinterpret_cast<const pg_u32x4*>(sh.bytes + r * 128 + ((g + 4 * half) ^ (r & 7)) * 16); };
-            Codes32<F16> b[FN];
-#pragma unroll
-            for (int j = 0; j < FN; ++j) b[j] = Codes32<F16>(frag(BM + wn * TN + 16 * j + c, 0), frag(BM + wn * TN + 16 * j + c, 1));
+        }
+        auto store = [&](auto whole, auto type, char* to, pg_i64 stride) {
+            constexpr bool INSIDE = decltype(whole)::value;
+            constexpr int OT = decltype(type)::value;
 #pragma unroll
             for (int i = 0; i < FM; ++i) {
                 const int r = wm * TM + 16 * i + c;
-                const Codes32<F16> a(frag(r, 0), frag(r, 1));
-                const float f = sh.scales[r] * sb;
+                if (!INSIDE && r >= rows) continue;
+                char* const out = to + (at.m0 + r) * stride * elem_size(OT);
 #pragma unroll
                 for (int j = 0; j < FN; ++j) {
-                    const pg_f32x4 y = stage_sum<F16>(b[j], a);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(y[e], f, acc[i][j][e]);
+                    if constexpr (PAIRS) {
+                        if (j % 2 == 0) put8<OT, INSIDE>(out, at.n0 + wn * TN + 16 * j + 8 * g, A.N, acc[i][j], acc[i][j + 1]);
+                    } else {
+                        put4<OT, INSIDE>(out, at.n0 + wn * TN + 16 * j + 4 * g, A.N, acc[i][j]);
+                    }
                 }
             }
-        }
-#pragma unroll
-        for (int i = 0; i < FM; ++i) {
-            const pg_i64 m = m0 + wm * TM + 16 * i + c;
-            if (m >= A.M) continue;
-#pragma unroll
-            for (int j = 0; j < FN; ++j) put4<T>(A.out + m * A.s_out * elem_size(T), n0 + wn * TN + 16 * j + 4 * g, A.N, acc[i][j]);
-        }
+        };
+        if (A.splits > 1) store(Flag<false>(), Int<kF32>(), reinterpret_cast<char*>(A.parts + at.split * A.M * A.N), A.N);
+        else if (rows == BM && cols == BN) store(Flag<true>(), Int<T>(), A.out, A.s_out);
+        else store(Flag<false>(), Int<T>(), A.out, A.s_out);
     }
 };
+
+// Up to 16 rows of a: the weights are the work, and each is used once, so that they
+// go from memory straight to the MFMAs' registers.  A workgroup has 16 columns; its
+// waves share the stages of K, and their sums are added in LDS, in order.
+template <int WAVES, bool DIRECT, int T>
+struct BlockStream {
+    static constexpr bool F16 = T == kF32;
+    struct Shared {
+        pg_f32x4 sums[WAVES][64];
+    };
+    struct Stage {
+        pg_u32x4 a[2], b[2];
+        float scale, weight;
+    };
+
+    __device__ static void run(const MatmulArgs& A, Shared& sh) {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+        const int split = blockIdx.x / A.tiles_n, tile = blockIdx.x - split * A.tiles_n;
+        const pg_i64 n0 = static_cast<pg_i64>(tile) * 16;
+        const int shares = A.splits * WAVES, share = split * WAVES + wave;
+        int s = static_cast<int>(static_cast<pg_i64>(A.stages) * share / shares);
+        const int end = static_cast<int>(static_cast<pg_i64>(A.stages) * (share + 1) / shares);
+        // Rows and columns behind the last one repeat it; their results are not stored.
+        const pg_i64 row = c < A.M ? c : A.M - 1, col = n0 + c < A.N ? n0 + c : A.N - 1;
+        const char* const a = A.a + row * A.s_a;
+        const char* const b = A.b + col * A.s_b;
+        const float* const as = A.a_scale + row * A.s_as[0];
+        const float* const bs = A.b_scale + n0 / kScaleBlock * A.s_bs[0];
+        auto load = [&](int t, Stage& x) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const pg_i64 k = static_cast<pg_i64>(t) * kScaleBlock + 64 * h + 16 * g;
+                if constexpr (DIRECT) {
+                    // Pieces behind K repeat the row's last one; their weights are cleared in add().
+                    const pg_i64 at = k < A.K ? k : A.K - 16;
+                    x.a[h] = *reinterpret_cast<const pg_u32x4*>(a + at);
+                    x.b[h] = *reinterpret_cast<const pg_u32x4*>(b + at);
+                } else {
+                    x.a[h] = codes16(a, k, A.K);
+                    x.b[h] = codes16(b, k, A.K);
+                }
+            }
+            x.scale = as[t * A.s_as[1]];
+            x.weight = bs[t * A.s_bs[1]];
+        };
+        pg_f32x4 acc = {0, 0, 0, 0};
+        auto add = [&](int t, Stage& x) {
+            if (DIRECT && static_cast<pg_i64>(t + 1) * kScaleBlock > A.K) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const bool in = static_cast<pg_i64>(t) * kScaleBlock + 64 * h + 16 * g < A.K;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x.b[h][e] = in ? x.b[h][e] : 0;
+                }
+            }
+            const pg_f32x4 y = stage_sum<F16>(Codes32<F16>(x.b[0], x.b[1]), Codes32<F16>(x.a[0], x.a[1]));
+            const float f = x.scale * x.weight;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(y[e], f, acc[e]);
+        };
+        // The stages ahead are under way during one.
+        constexpr int AHEAD = 4;
+        Stage x[AHEAD];
+#pragma unroll
+        for (int q = 0; q < AHEAD - 1; ++q)
+            if (s + q < end) load(s + q, x[q]);
+        while (s < end) {
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q) {
+                if (s + AHEAD - 1 < end) load(s + AHEAD - 1, x[(q + AHEAD - 1) % AHEAD]);
+                if (s < end) add(s, x[q]);
+                ++s;
+            }
+        }
+        sh.sums[wave][lane] = acc;
+        __syncthreads();
+        if (wave > 0) return;
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) acc += sh.sums[w][lane];
+        if (c >= A.M) return;
+        if (A.splits == 1) put4<T, false>(A.out + c * A.s_out * elem_size(T), n0 + 4 * g, A.N, acc);
+        else put4<kF32, false>(reinterpret_cast<char*>(A.parts + (split * A.M + c) * A.N), n0 + 4 * g, A.N, acc);
+    }
+};
+
+// The sums of the splits, in order.  Four columns a thread.
+template <int T>
+__device__ inline void join_splits(const MatmulArgs& A) {
+    const pg_i64 fours = (A.N + 3) / 4, item = static_cast<pg_i64>(blockIdx.x) * blockDim.x + threadIdx.x, m = item / fours, n = 4 * (item - m * fours);
+    if (m >= A.M) return;
+    float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < A.splits; ++s) {
+        const float* const p = A.parts + (s * A.M + m) * A.N + n;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] += p[n + e < A.N ? e : 0];
+    }
+    put_row<T, false, 4>(A.out + m * A.s_out * elem_size(T), n, A.N, y);
+}
 
 }  // namespace ptowsp

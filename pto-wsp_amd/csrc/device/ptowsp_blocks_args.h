@@ -29,6 +29,8 @@ struct MatmulArgs {
     long long M, N, K;
     int stages;                        // blocks of K
     int tiles_m, tiles_n;
+    int splits;                        // workgroups that share a tile's stages
+    float* parts;                      // their sums, [split, M, N], if they are several
 };
 
 struct RotateArgs {

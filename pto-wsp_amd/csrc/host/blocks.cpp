@@ -69,15 +69,73 @@ void run_quantize(const Node& n, const std::vector<Operand>& o, const OperatorRu
 }
 
 // ---- block_matmul ----
+// Tiles of results, and the us that a stage of K takes where a compute unit has one
+// of them, and where it has as many as it holds.
+struct MatmulTile {
+    int bm, bn, wm, wn, ring, per_cu;
+    double alone, shared;
+};
+// Fitted to 2900 timings of 42 shapes, from 1 x 82 x 128 to 8192 x 6144 x 4096, each
+// with every tile and 1 to 8 splits of K, weights from memory: the choice costs 4%
+// over the fastest on average.  64 rows of 6144 x 4096 take 12.5 us in tiles of 32 x
+// 64, 16.5 in 64 x 64 and 60 in 256 x 256; 512 rows 47, 37 and 75, and 29 in 128 x
+// 128; 8192 rows 341 in 128 x 128 and 224 in 256 x 256.
+constexpr MatmulTile kTiles[] = {
+    {16, 16, 1, 1, 0, 8, 0.13, 0.65},  // BlockStream
+    {32, 64, 1, 4, 6, 2, 0.33, 0.45}, {64, 64, 2, 2, 4, 2, 0.41, 0.70}, {64, 128, 1, 4, 3, 2, 0.63, 0.95},
+    {128, 128, 2, 2, 4, 1, 0.84, 0.94}, {256, 256, 4, 2, 2, 1, 2.3, 2.2},
+};
+constexpr int kStreamWaves = 4;
 struct MatmulForm {
     std::string source;
-    int bm, bn, threads;
+    MatmulTile tile;
+    int splits, threads;
+    int64_t tiles_m, tiles_n;
 };
-MatmulForm matmul_form(DType type) {
-    MatmulForm f{"", 128, 128, 256};
-    const std::string t = "ptowsp::BlockGemm<128, 128, 2, 2, " + num(type_id(type)) + ">";
+MatmulForm matmul_form(int64_t M, int64_t N, int64_t K, DType type, bool direct, int cus) {
+    const double stages = static_cast<double>(scale_blocks(K));
+    MatmulForm f{};
+    double best = 0.0;
+    for (const MatmulTile& t : kTiles) {
+        if (!t.ring && M > t.bm) continue;
+        // Float32 results take twice the registers for codes; other addresses need some for pieces under way.
+        if (t.bm == 256 && (type == DType::F32 || !direct)) continue;
+        const double tiles = static_cast<double>(parts(M, t.bm)) * static_cast<double>(parts(N, t.bn));
+        for (const int splits : {1, 2, 3, 4, 6, 8}) {
+            if (splits > stages) break;
+            const double each = tiles * splits / cus, room = t.per_cu;
+            const double stage = each <= 1.0    ? t.alone * (0.6 + 0.4 * each)
+                                 : each <= room ? t.alone + (t.shared - t.alone) * (each - 1.0) / (room - 1.0)
+                                                : t.shared * 0.5 * (std::ceil(each / room) + each / room);
+            double us = 3.4 + stage * (std::ceil(stages / splits) + 1.0);
+            if (splits > 1) us += 3.7 + splits * 8.0 * static_cast<double>(M) * static_cast<double>(N) / 4.5e6;
+            if (best > 0.0 && us >= best) continue;
+            best = us;
+            f.tile = t;
+            f.splits = splits;
+        }
+    }
+    f.tiles_m = parts(M, f.tile.bm), f.tiles_n = parts(N, f.tile.bn);
+    const std::string out = num(type_id(type));
+    std::string t;
+    if (f.tile.ring) {
+        f.threads = 64 * f.tile.wm * f.tile.wn;
+        t = "ptowsp::BlockGemm<" + num(f.tile.bm) + ", " + num(f.tile.bn) + ", " + num(f.tile.wm) + ", " + num(f.tile.wn) + ", " + num(f.tile.ring) + ", " + flag(direct) +
+            ", " + out + ">";
+    } else {
+        f.threads = 64 * kStreamWaves;
+        t = "ptowsp::BlockStream<" + num(kStreamWaves) + ", " + std::string(flag(direct)) + ", " + out + ">";
+    }
     f.source = entry("ptowsp_blocks.h", f.threads, "ptowsp_block_matmul", "MatmulArgs", "__shared__ " + t + "::Shared lds; " + t + "::run(A, lds)");
+    if (f.splits > 1) f.source += "extern \"C\" __global__ __launch_bounds__(256) void ptowsp_block_matmul_join(ptowsp::MatmulArgs A) { ptowsp::join_splits<" + out + ">(A); }\n";
     return f;
+}
+
+// Whether rows can go straight to LDS: 16-byte pieces, offsets within a tile in 31 bits.
+bool direct_rows(const Operand& x, const Operand& scale, int64_t K) {
+    constexpr int64_t kMost = int64_t(1) << 31;
+    return K % 16 == 0 && (x.shape[0] < 2 || x.stride[0] % 16 == 0) && reinterpret_cast<uintptr_t>(x.ptr) % 16 == 0 && 256 * x.stride[0] + K < kMost &&
+           4 * (256 * scale.stride[0] + scale_blocks(K) * scale.stride[1]) < kMost;
 }
 
 void run_matmul(const Node& n, const std::vector<Operand>& o, const OperatorRun& run) {
@@ -90,11 +148,12 @@ void run_matmul(const Node& n, const std::vector<Operand>& o, const OperatorRun&
     A.M = a.shape[0], A.N = b.shape[0], A.K = a.shape[1];
     A.stages = static_cast<int>(scale_blocks(A.K));
     if (A.M == 0) return;
-    const MatmulForm f = matmul_form(out.dtype);
-    const int64_t tm = parts(A.M, f.bm), tn = parts(A.N, f.bn);
-    if (tm * tn >= (int64_t(1) << 23)) stop(n, "too many rows and columns for one call");
-    A.tiles_m = static_cast<int>(tm), A.tiles_n = static_cast<int>(tn);
-    run.launch(f.source, "ptowsp_block_matmul", tm * tn, f.threads, &A, sizeof A);
+    const MatmulForm f = matmul_form(A.M, A.N, A.K, out.dtype, direct_rows(a, as, A.K) && direct_rows(b, bs, A.K), run.cus);
+    if (f.tiles_m * f.tiles_n * f.splits >= (int64_t(1) << 22)) stop(n, "too many rows and columns for one call");
+    A.tiles_m = static_cast<int>(f.tiles_m), A.tiles_n = static_cast<int>(f.tiles_n), A.splits = f.splits;
+    if (f.splits > 1) A.parts = reinterpret_cast<float*>(run.scratch(static_cast<size_t>(f.splits * A.M * A.N) * 4));
+    run.launch(f.source, "ptowsp_block_matmul", f.tiles_m * f.tiles_n * f.splits, f.threads, &A, sizeof A);
+    if (f.splits > 1) run.launch(f.source, "ptowsp_block_matmul_join", parts(A.M * parts(A.N, 4), 256), 256, &A, sizeof A);
 }
 
 // ---- paged_norm_rotate ----
@@ -227,7 +286,8 @@ void run_block_operator(const Node& n, const std::vector<Operand>& operands, con
 std::pair<std::string, std::string> block_operator_source(const Shapes& s) {
     const Node& n = s.n;
     if (n.op == "block_quantize") return {quantize_form(s.of("x")[0], s.of("x")[1], attr(n, "rows"), s.dtype[s.at("x")]).source, "ptowsp_block_quantize"};
-    if (n.op == "block_matmul") return {matmul_form(s.dtype[s.at("out")]).source, "ptowsp_block_matmul"};
+    // For the 256 compute units of the target.
+    if (n.op == "block_matmul") return {matmul_form(s.of("a")[0], s.of("b")[0], s.of("a")[1], s.dtype[s.at("out")], s.of("a")[1] % 16 == 0, 256).source, "ptowsp_block_matmul"};
     const bool qn = !s.of("q_weight").empty(), kn = !s.of("k_weight").empty();
     return {rotate_form(s.of("q"), s.of("k")[1], 2 * s.of("cos")[1], s.dtype[s.at("q")], s.dtype[s.at(qn ? "q_weight" : "k_weight")], qn, kn,
                         attr(n, "interleaved") != 0)
