@@ -416,6 +416,16 @@ __device__ inline pg_i64 uniform64(pg_i64 x) {
     return static_cast<pg_i64>(static_cast<pg_u64>(hi) << 32 | lo);
 }
 
+// One of the two AttendArgs of a kernel whose only argument is a PrefixArgs: what is loaded or
+// computed of them for one kind of workgroup is not moved ahead of the choice, where
+// every kind would carry it.
+__device__ inline const AttendArgs& args_of(bool shared) {
+    auto p = (const __attribute__((address_space(4))) char*)__builtin_amdgcn_kernarg_segment_ptr() +
+             (shared ? __builtin_offsetof(PrefixArgs, shared) : __builtin_offsetof(PrefixArgs, own));
+    asm volatile("" : "+s"(p));
+    return *(const AttendArgs*)(const __attribute__((address_space(4))) AttendArgs*)p;
+}
+
 // The logarithm of a softmax's sum l, of scores times log2 e relative to m.
 __device__ inline float lse_of(float m, float l) {
     return l == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f;
@@ -425,6 +435,8 @@ __device__ inline float lse_of(float m, float l) {
 // paged_prefix_attention (each request's rows over its own tokens; each group's
 // rows over their prefix), which leaves float32 results for merge_parts().
 constexpr int kWhole = 0, kOwnPart = 1, kPrefixPart = 2;
+constexpr int kLeastTiles = 4;      // of a piece of line(): its beginning costs about as much
+constexpr int kFromLine = 1 << 15;  // of a row's entry (put_pieces): the pieces are those of line()
 
 template <int D_, int PAGE_, int G_, int NT_, int QT_, int CT_, bool WIN_, bool LSE_, bool VEC_, bool PROMPT_ = false, int PART_OF_ = kWhole>
 struct Attend {
@@ -1060,6 +1072,14 @@ struct Attend {
                     }
                 }
             }
+            if constexpr (PART_OF != kWhole) {
+                if (opens && !closes && wave == 0 && lane < RB) {
+                    const int i = lane / GH, hh = lane - i * GH;
+                    const pg_i64 end = xb + (unit + 1) * rq.kt;
+                    if (i < u.n && (HS == 1 || hs * RB + hh < G))
+                        put_pieces(A, row + i, head + hh, static_cast<int>(w), static_cast<int>((end * pieces - 1) / total), lane);
+                }
+            }
             if (opens && !closes) {
                 joined = 1;
                 if (threadIdx.x == 0) {
@@ -1080,8 +1100,13 @@ struct Attend {
     // A row's maximum (of scores times log2 e) and sum: their logarithm, or as they are for merge_parts().
     __device__ static void put_sum(const AttendArgs& A, int row, int head, float m, float l) {
         float* const p = A.lse + (row * A.s_lse[0] + head * A.s_lse[1]);
-        if constexpr (PART_OF != kWhole) *reinterpret_cast<pg_f32x2*>(p) = pg_f32x2{m, l};
+        if constexpr (PART_OF != kWhole) *reinterpret_cast<pg_f32x4*>(p) = pg_f32x4{m, l, 0.0f, 0.0f};
         else *p = lse_of(m, l);
+    }
+    // A row of a unit that workgroups `first` .. `last` share: its place in their partial results.
+    __device__ static void put_pieces(const AttendArgs& A, int row, int head, int first, int last, int place) {
+        const int many = (last - first + 1) | (PROMPT ? kFromLine : 0) | place << 16;
+        *reinterpret_cast<pg_f32x4*>(A.lse + (row * A.s_lse[0] + head * A.s_lse[1])) = pg_f32x4{0.0f, 0.0f, __int_as_float(first), __int_as_float(many)};
     }
 
     // This wave's steps of 32 tokens from `base` on, STRIDE tokens apart, below
@@ -1291,6 +1316,7 @@ struct Attend {
     }
     __device__ static float* part_sums(const AttendArgs& A, const Part& p, int piece) {
         const int wave = uniform(threadIdx.x >> 6);
+        if constexpr (FULL) return A.unit_parts + (static_cast<pg_i64>(p.slot + piece) * 4 + wave) * PART;
         return A.unit_parts + ((static_cast<pg_i64>(p.slot + piece) * A.heads + p.h) * 4 + wave) * PART;
     }
 
@@ -1744,7 +1770,9 @@ struct Attend {
                 }
             }
         }
-        if (!done) return false;
+        // The waves agree; where another branch follows, the compiler is told, so that it
+        // keeps no sums for it.
+        if (FULL ? uniform(done) == 0 : !done) return false;
         l += __shfl_xor(l, 32, 64);
         const int out_lane = own_lane(), out_n = out_lane & 31, out_h = out_lane >> 5, out_i = out_n / GH, out_hh = out_n - out_i * GH;
         if (!has_row(out_i, out_hh)) return true;
@@ -1796,14 +1824,14 @@ struct Attend {
     __device__ static int* over(const AttendArgs& A) { return A.units + kUnitHead + A.room * kUnitInts + A.counters; }
     __device__ static int* cut(const AttendArgs& A) { return over(A) + A.room * A.heads; }
 
-    __device__ static void prompt(const AttendArgs& A, Tiles& T) {
-        const int entry = static_cast<int>(blockIdx.x / A.heads), h = static_cast<int>(blockIdx.x) - entry * A.heads;
+    __device__ static void prompt(const AttendArgs& A, Tiles& T, int workgroup) {
+        const int entry = workgroup / A.heads, h = workgroup - entry * A.heads;
         if (entry >= A.units[0]) return;
         Part p;
         part_of(A, entry, h, p);
         if constexpr (TILES) {
             if (!tiles(A, p, T) && threadIdx.x == 0) {
-                over(A)[atomicAdd(A.units + 1, 1)] = static_cast<int>(blockIdx.x);
+                over(A)[atomicAdd(A.units + 1, 1)] = workgroup;
                 if (p.pieces > 1) atomicAdd(counter(A, p), 1);
             }
         } else {
@@ -1818,8 +1846,112 @@ struct Attend {
         constexpr size_t few = sizeof(typename F::Shared), mine = TILES ? sizeof(Tiles) : 0;
         __shared__ __attribute__((aligned(1024))) char lds[few > mine ? few : mine];
         const int units = static_cast<int>(gridDim.x) - A.blocks;
-        if (static_cast<int>(blockIdx.x) < units) prompt(A, *reinterpret_cast<Tiles*>(lds));
+        if (static_cast<int>(blockIdx.x) < units) prompt(A, *reinterpret_cast<Tiles*>(lds), static_cast<int>(blockIdx.x));
         else F::run(A, static_cast<int>(blockIdx.x) - units, *reinterpret_cast<typename F::Shared*>(lds));
+    }
+
+    // ---- prefixes of many rows ----
+    // A unit's tiles are cut into equal pieces of `limit` tiles at most, one for a
+    // workgroup; every workgroup finds its own.  With few units the pieces are as many
+    // as run at once, with more they are as short as keeps the workgroups alike.
+    __device__ static int units_of(const Request& r) { return (r.n + kUnitTokens - 1) / kUnitTokens * HS; }
+    __device__ static int tiles_of(const Request& r) { return r.length > kTile ? static_cast<int>((static_cast<pg_u32>(r.length) + (kTile - 1)) / kTile) : 1; }
+    __device__ static int pieces_of(const Request& r, int limit) { return (tiles_of(r) + limit - 1) / limit; }
+    __device__ static bool line_part(const AttendArgs& A, int workgroup, Part& p) {
+        __shared__ pg_i64 scan[4], begin[3];
+        const int wave = uniform(threadIdx.x >> 6);
+        const pg_i64 per = (A.batch + kAttendThreads - 1) / kAttendThreads, b0 = threadIdx.x * per;
+        const pg_i64 b1 = b0 + per < A.batch ? b0 + per : A.batch;
+        // Units and tiles of a key head, then pieces and those of units in several.
+        pg_i64 units = 0, tiles_here = 0, pieces = 0, cut = 0;
+        for (pg_i64 b = b0; b < b1; ++b) {
+            const Request r = request(A, b, workgroup == 0);
+            units += units_of(r);
+            tiles_here += static_cast<pg_i64>(units_of(r)) * tiles_of(r);
+        }
+        pg_i64 all_units, all_tiles, all;
+        block_scan<kAttendThreads>(units, all_units, scan);
+        block_scan<kAttendThreads>(tiles_here, all_tiles, scan);
+        all_units *= A.heads;
+        all_tiles *= A.heads;
+        const pg_i64 room = 2 * all_units <= A.cus ? A.cus - all_units : A.cus + A.cus / 3;
+        const pg_i64 share = (all_tiles + room - 1) / room;
+        const int limit = share < kLeastTiles ? kLeastTiles : static_cast<int>(share);
+        for (pg_i64 b = b0; b < b1; ++b) {
+            const Request r = request(A, b, false);
+            const int k = pieces_of(r, limit);
+            pieces += static_cast<pg_i64>(units_of(r)) * k;
+            cut += k > 1 ? static_cast<pg_i64>(units_of(r)) * k : 0;
+        }
+        const pg_i64 before = block_scan<kAttendThreads>(pieces, all, scan) * A.heads;
+        pg_i64 all_cut;
+        const pg_i64 cut_before = block_scan<kAttendThreads>(cut, all_cut, scan) * A.heads;
+        if (workgroup >= all * A.heads) return false;
+        if (workgroup >= before && workgroup < before + pieces * A.heads) {
+            pg_i64 at = before, slot = cut_before;
+            for (pg_i64 b = b0; b < b1; ++b) {
+                const Request r = request(A, b, false);
+                const int k = pieces_of(r, limit);
+                const pg_i64 here = static_cast<pg_i64>(A.heads) * units_of(r) * k;
+                if (workgroup < at + here) {
+                    begin[0] = b;
+                    begin[1] = at;
+                    begin[2] = slot;
+                    break;
+                }
+                at += here;
+                if (k > 1) slot += here;
+            }
+        }
+        __syncthreads();
+        // The piece: units side by side, so that workgroups beside each other read the same tiles.
+        p.b = uniform(static_cast<int>(begin[0]));
+        const int item = uniform(workgroup - static_cast<int>(begin[1]));
+        p.rq = request(A, p.b, false);
+        p.rq.row = uniform(p.rq.row);
+        p.rq.n = uniform(p.rq.n);
+        p.rq.length = uniform(p.rq.length);
+        const int kt = tiles_of(p.rq), many = units_of(p.rq);
+        p.pieces = uniform(pieces_of(p.rq, limit));
+        p.piece = uniform(item / (A.heads * many));
+        const int unit = item - p.piece * (A.heads * many);
+        p.h = uniform(unit / many);
+        const int in = unit - p.h * many;
+        p.tile = uniform(in / HS);
+        p.hs = in - p.tile * HS;
+        p.slot = uniform(static_cast<int>(begin[2])) + unit * p.pieces;
+        p.base = uniform(static_cast<int>(static_cast<pg_i64>(kt) * p.piece / p.pieces)) * kTile;
+        p.end = uniform(static_cast<int>(static_cast<pg_i64>(kt) * (p.piece + 1) / p.pieces)) * kTile;
+        if (p.end > p.rq.length) p.end = p.rq.length;
+        const int first = p.tile * kUnitTokens + wave * C;
+        p.row = p.rq.row + first;
+        p.head = p.h * G + p.hs * RB;
+        p.u.table = A.table + p.b * A.s_table;
+        p.u.h = p.h;
+        p.u.n = p.rq.n - first < C ? p.rq.n - first : C;
+        p.u.p0 = position(p.rq, first);
+        p.u.hi = p.u.n > 0 ? end_of(p.u.p0, p.u.n) : 0;
+        p.u.lo = 0;
+        return true;
+    }
+    __device__ static void line(const AttendArgs& A, int workgroup, Tiles& T) {
+        Part p;
+        if (!line_part(A, workgroup, p)) return;
+        if (p.pieces > 1 && p.piece == 0) {
+            const int wave = uniform(threadIdx.x >> 6), lane = own_lane(), i = lane / GH, hh = lane - i * GH;
+            if (lane < RB && i < p.u.n && i < C && (HS == 1 || p.hs * RB + hh < G))
+                put_pieces(A, p.row + i, p.head + hh, p.slot, p.slot + p.pieces - 1, wave * RB + lane);
+        }
+        if constexpr (TILES) {
+            if (tiles(A, p, T)) return;
+            // What that leaves to bf16 parts is done by the same waves, which find their
+            // piece again: what they would keep takes registers from the tiles.
+            const AttendArgs& again = args_of(true);
+            asm volatile("" : "+s"(workgroup));
+            if (line_part(again, workgroup, p)) Narrow::template rows<Attend>(again, p);
+        } else {
+            Narrow::template rows<Attend>(A, p);
+        }
     }
 
     // What remains: units that the workgroups for few rows left open, units in
@@ -1927,37 +2059,133 @@ struct Attend {
     }
 };
 
-// paged_prefix_attention: the two parts of each row and head as one softmax.  A
-// part's result has been divided by its sum l; its weight is l * 2^(m - the larger
-// maximum) over those of both.  Four dims a thread.
-template <int D, int T, bool LSE>
-__device__ inline void merge_parts(const MergeArgs& A) {
-    constexpr int Q = D / 4;
-    const pg_i64 item = static_cast<pg_i64>(blockIdx.x) * blockDim.x + threadIdx.x, at = item / Q;
-    if (at >= A.rows * A.heads) return;
-    const int d = 4 * static_cast<int>(item - at * Q), row = static_cast<int>(at / A.heads), head = static_cast<int>(at - static_cast<pg_i64>(row) * A.heads);
-    auto first_row = [&](int request) { return A.starts[request * A.s_starts]; };
-    const int m0 = A.members[0], m1 = A.members[A.groups * A.s_members];
-    // Rows of no request are left alone; the groups' rows follow each other.
-    if (row < first_row(0) || row >= first_row(A.requests)) return;
-    const bool both = m0 >= 0 && m0 <= m1 && m1 <= A.requests && row >= first_row(m0) && row < first_row(m1);
-    const pg_f32x2 own = *reinterpret_cast<const pg_f32x2*>(A.sums[0] + 2 * at);
-    pg_f32x4 o = *reinterpret_cast<const pg_f32x4*>(A.parts[0] + at * D + d);
-    float m = own[0], l = own[1];
-    if (both) {
-        const pg_f32x2 shared = *reinterpret_cast<const pg_f32x2*>(A.sums[1] + 2 * at);
-        const pg_f32x4 p = *reinterpret_cast<const pg_f32x4*>(A.parts[1] + at * D + d);
-        m = fmaxf(own[0], shared[0]);
-        const float w0 = own[1] == 0.0f ? 0.0f : own[1] * __builtin_amdgcn_exp2f(own[0] - m), w1 = shared[1] == 0.0f ? 0.0f : shared[1] * __builtin_amdgcn_exp2f(shared[0] - m);
-        l = w0 + w1;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        // A part without positions is 0 and has no weight.
-        o = o * (w0 * inv) + p * (w1 * inv);
+// ---------------------------------------------------------------------------
+// paged_prefix_attention
+//
+// A row's softmax over its prefix and its own tokens is that over each of both,
+// joined by their maxima and sums.  The first launch has workgroups of four kinds:
+// prefixes of groups with many rows, cut into equal pieces (line); prefixes of few
+// rows and own tokens of few rows (run); own tokens of prompts, whose list is made in
+// a launch ahead and whose pieces are joined in one behind.  Each leaves float32
+// results: of a unit that one workgroup had in the row's place, of the others in
+// pieces.  The last launch joins what there is of a row.
+// ---------------------------------------------------------------------------
+
+// LP: the line's kernels; FP, FO: few rows over prefixes and own tokens; UO: prompts over own tokens.
+template <class LP, class FP, class FO, class UO, bool LINE, bool PROMPTS>
+__device__ inline void prefix_parts(const PrefixArgs& A) {
+    constexpr size_t few = sizeof(typename FP::Shared) > sizeof(typename FO::Shared) ? sizeof(typename FP::Shared) : sizeof(typename FO::Shared);
+    constexpr size_t lines = LINE && LP::TILES ? sizeof(typename LP::Tiles) : 0, prompts = PROMPTS && UO::TILES ? sizeof(typename UO::Tiles) : 0;
+    constexpr size_t tiles = lines > prompts ? lines : prompts;
+    __shared__ __attribute__((aligned(1024))) char lds[few > tiles ? few : tiles];
+    int w = blockIdx.x;
+    if constexpr (LINE) {
+        if (w < A.lines) {
+            [[clang::always_inline]] LP::line(args_of(true), w, *reinterpret_cast<typename LP::Tiles*>(lds));
+            return;
+        }
+        w -= A.lines;
     }
-    char* const out = A.out + (row * A.s_out[0] + head * A.s_out[1] + d) * elem_size(T);
+    if (w < A.few_prefixes) {
+        [[clang::always_inline]] FP::run(args_of(true), w, *reinterpret_cast<typename FP::Shared*>(lds));
+        return;
+    }
+    w -= A.few_prefixes;
+    if (w < A.own.blocks) {
+        [[clang::always_inline]] FO::run(args_of(false), w, *reinterpret_cast<typename FO::Shared*>(lds));
+        return;
+    }
+    if constexpr (PROMPTS) [[clang::always_inline]] UO::prompt(args_of(false), *reinterpret_cast<typename UO::Tiles*>(lds), w - A.own.blocks);
+}
+
+// What there is of a row: maximum, sum and a lane's four dims.
+struct Joined {
+    float m, l;
+    pg_f32x4 o;
+};
+
+// LANES lanes a row, four dims each.  RBF, RBL: rows of a partial result of run(), of a wave of line().
+template <int DP, int LANES>
+__device__ inline Joined join_part(const AttendArgs& A, int rbf, int rbl, pg_i64 row, int head, int d, int D) {
+    Joined r;
+    const pg_f32x4 entry = *reinterpret_cast<const pg_f32x4*>(A.lse + row * A.s_lse[0] + head * A.s_lse[1]);
+    // Entries of requests out of range, which no kernel has written, may be anything.
+    const int code = __float_as_int(entry[3]), many = code & (kFromLine - 1), first = __float_as_int(entry[2]);
+    const bool line = code & kFromLine;
+    if (many == 0 || first < 0 || first > (line ? A.room : A.blocks) - many) {
+        // The result has been divided by its sum: a sum of 1 and the sum in the weight.
+        r.m = entry[0];
+        r.l = entry[1];
+        r.o = *reinterpret_cast<const pg_f32x4*>(A.out + (row * A.s_out[0] + head * A.s_out[1] + (d < D ? d : 0)) * 4) * r.l;
+        if (r.l == 0.0f) r.o = pg_f32x4{0, 0, 0, 0};
+        return r;
+    }
+    const int rb = line ? rbl : rbf, place = static_cast<int>(static_cast<pg_u32>(code) >> 16) & (line ? 4 * rb - 1 : rb - 1), at = place & (rb - 1);
+    const pg_i64 part = static_cast<pg_i64>(rb) * (2 + DP);
+    const float* const base = line ? A.unit_parts + place / rb * part : A.parts;
+    const pg_i64 slot = line ? 4 * part : part;
+    auto piece = [&](int k) { return base + (line ? first + k : 2 * (first + k) + (k == 0 ? 1 : 0)) * slot; };
+    const int l0 = threadIdx.x & (LANES - 1);
+    float m = -__builtin_inff();
+    for (int k = l0; k < many; k += LANES) m = fmaxf(m, piece(k)[at]);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) store_elem<T>(out + e * elem_size(T), o[e]);
-    if (LSE && d == 0) A.lse[row * A.s_lse[0] + head * A.s_lse[1]] = lse_of(m, l);
+    for (int x = LANES / 2; x >= 1; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, LANES));
+    r.m = m;
+    r.l = 0.0f;
+    r.o = pg_f32x4{0, 0, 0, 0};
+    for (int k0 = 0; k0 < many; k0 += LANES) {
+        float weight = 0.0f;
+        if (k0 + l0 < many) {
+            const float* const p = piece(k0 + l0);
+            weight = p[at] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(p[at] - m);
+            r.l += weight * p[rb + at];
+        }
+        const int n = many - k0 < LANES ? many - k0 : LANES;
+        for (int k = 0; k < n; k += 8) {
+            pg_f32x4 x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = *reinterpret_cast<const pg_f32x4*>(piece(k0 + (k + e < n ? k + e : n - 1)) + 2 * rb + at * DP + d);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float f = __shfl(weight, k + e, LANES);
+                if (k + e < n) r.o += f * x[e];
+            }
+        }
+    }
+#pragma unroll
+    for (int x = LANES / 2; x >= 1; x >>= 1) r.l += __shfl_xor(r.l, x, LANES);
+    return r;
+}
+
+template <int D, int RBP, int RBL, int RBO, int T, bool LSE>
+__device__ inline void merge_parts(const PrefixArgs& A) {
+    constexpr int DP = (D + 63) / 64 * 64, LANES = DP / 4 < 64 ? DP / 4 == 48 ? 64 : DP / 4 : 64;
+    const pg_i64 item = (static_cast<pg_i64>(blockIdx.x) * blockDim.x + threadIdx.x) / LANES;
+    const int heads = A.q_heads, lane = threadIdx.x & (LANES - 1), d = 4 * lane < DP ? 4 * lane : 0;
+    const pg_i64 row = item / heads;
+    const int head = static_cast<int>(item - row * heads);
+    const AttendArgs &own = A.own, &shared = A.shared;
+    auto first_row = [&](int request) { return own.starts[request * own.s_starts]; };
+    const int requests = static_cast<int>(own.batch), m0 = shared.members[0], m1 = shared.members[shared.batch * shared.s_members];
+    // Rows of no request are left alone; the groups' rows follow each other.
+    if (row >= own.rows || row < first_row(0) || row >= first_row(requests)) return;
+    const bool both = m0 >= 0 && m0 <= m1 && m1 <= requests && row >= first_row(m0) && row < first_row(m1);
+    Joined r = join_part<DP, LANES>(own, RBO, RBO, row, head, d, D);
+    if (both) {
+        const Joined p = join_part<DP, LANES>(shared, RBP, RBL, row, head, d, D);
+        const float m = fmaxf(r.m, p.m);
+        const float w0 = r.l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(r.m - m), w1 = p.l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(p.m - m);
+        r.o = r.o * w0 + p.o * w1;
+        r.l = r.l * w0 + p.l * w1;
+        r.m = m;
+    }
+    const float f = r.l == 0.0f ? 0.0f : 1.0f / r.l;
+    if (4 * lane < D) {
+        char* const out = A.out + (row * A.s_out[0] + head * A.s_out[1] + d) * elem_size(T);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) store_elem<T>(out + e * elem_size(T), r.o[e] * f);
+    }
+    if (LSE && lane == 0) A.lse[row * A.s_lse[0] + head * A.s_lse[1]] = lse_of(r.m, r.l);
 }
 
 }  // namespace ptowsp

@@ -74,16 +74,17 @@ struct AttendArgs {
     int requests;
 };
 
-struct MergeArgs {
-    const float* parts[2];  // results over own tokens and over prefixes, [row, head, D]
-    const float* sums[2];   // their maxima and sums, [row, head, 2]
-    const int* starts;
-    const int* members;
+struct PrefixArgs {
+    // Results of both parts in float32, [row, head, D], and an entry for each row and
+    // head (`lse`): its maximum and sum, or where its pieces lie.  `room` of the
+    // prefixes: pieces of line() that there is room for.
+    AttendArgs own, shared;
+    int lines;         // workgroups for prefixes of many rows
+    int few_prefixes;  // workgroups for prefixes of few
+    int q_heads;
     char* out;
     float* lse;
-    long long s_starts, s_members, s_out[2], s_lse[2];
-    long long rows;
-    int heads, requests, groups;
+    long long s_out[2], s_lse[2];
 };
 
 }  // namespace ptowsp

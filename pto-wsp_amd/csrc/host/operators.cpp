@@ -259,7 +259,7 @@ AttendForm attend_form(const std::vector<int64_t>& q, const std::vector<int64_t>
     f.s = AttendShape{static_cast<int>(D), static_cast<int>(cache[2]), static_cast<int>(q[1] / cache[1]), 1, type_id(type), code_id(code), window, lse, vec, part};
     f.few = std::max(1, kFewRows / f.s.G);
     // Launched if there can be such a request while every other one has a token.
-    f.prompts = rows - batch >= f.few && (rows * q[1] > kFewInAll || part == 2);
+    f.prompts = part == 2 ? rows > f.few : rows - batch >= f.few && rows * q[1] > kFewInAll;
     f.s.NT = attend_nt(f.prompts ? batch : rows, batch, f.s.G, D, f.s.type);
     return f;
 }
@@ -308,6 +308,12 @@ AttendSpace attend_space(const Node& n, const AttendForm& form, AttendArgs& A, i
         const PromptShape p = prompt_shape(s);
         const int prb = 16 * p.nt, c = s.G <= prb ? prb / s.G : 1, hs = s.G <= prb ? 1 : (s.G + prb - 1) / prb;
         A.cus = cus * p.waves;
+        if (s.part == 2) {
+            // Pieces of units in several, as line() makes them: A.cus, or twice what 4 / 3 of them share.
+            A.room = 8 * A.cus / 3 + 1;
+            r.need = r.units + whole(static_cast<int64_t>(A.room) * 4 * prb * (2 + dp) * 4);
+            return r;
+        }
         const int64_t entries = hs * (A.rows / (4 * c) + std::min<int64_t>(A.batch, A.rows / (A.few + 1))) + A.cus / A.heads + 1;
         if (entries * A.heads >= (int64_t(1) << 24)) stop(n, "too many rows for one call");
         A.room = static_cast<int>(entries), A.counters = 2 * A.cus;
@@ -316,11 +322,14 @@ AttendSpace attend_space(const Node& n, const AttendForm& form, AttendArgs& A, i
     }
     return r;
 }
-void attend_launch(const AttendForm& form, const AttendSpace& space, char* scratch, AttendArgs& A, const OperatorRun& run) {
+void attend_place(const AttendSpace& space, char* scratch, AttendArgs& A) {
     A.spans = reinterpret_cast<int*>(scratch);
     A.parts = reinterpret_cast<float*>(scratch + space.spans);
     A.units = reinterpret_cast<int*>(scratch + space.few);
     A.unit_parts = reinterpret_cast<float*>(scratch + space.units);
+}
+void attend_launch(const AttendForm& form, const AttendSpace& space, char* scratch, AttendArgs& A, const OperatorRun& run) {
+    attend_place(space, scratch, A);
     const std::string source = attend_source(form.s, form.prompts);
     if (form.prompts) {
         run.launch(source, "ptowsp_paged_attention_units", 1, 1024, &A, sizeof A);
@@ -348,62 +357,76 @@ void run_attend(const Node& n, const std::vector<Operand>& o, const OperatorRun&
 }
 
 // ---- paged_prefix_attention ----
-std::string merge_source(int64_t D, int type, bool lse) {
-    return entry_source("extern \"C\" __global__ __launch_bounds__(256) void ptowsp_paged_prefix_merge(ptowsp::MergeArgs A) { ptowsp::merge_parts<" +
-                        std::to_string(D) + ", " + std::to_string(type) + ", " + flag(lse) + ">(A); }\n");
+// own: the requests' own tokens; shared: the groups' prefixes.
+std::string prefix_source(const AttendForm& own, const AttendForm& shared, int type, bool lse) {
+    const std::string w = std::to_string(attend_waves(own.s.D)), bounds = "256, " + w;
+    const std::string lp = attend_type(shared.s, prompt_shape(shared.s).nt, true), fp = attend_type(shared.s, shared.s.NT, false);
+    const std::string uo = attend_type(own.s, prompt_shape(own.s).nt, true), fo = attend_type(own.s, own.s.NT, false);
+    auto entry_of = [](const std::string& bounds, const char* name, const char* args, const std::string& body) {
+        return "extern \"C\" __global__ __launch_bounds__(" + bounds + ") void ptowsp_paged_prefix" + name + "(ptowsp::" + args + " A) { " + body + "; }\n";
+    };
+    std::string source = entry_source(entry_of(bounds, "_parts", "PrefixArgs", "ptowsp::prefix_parts<" + lp + ", " + fp + ", " + fo + ", " + uo + ", " + flag(shared.prompts) + ", " + flag(own.prompts) + ">(A)"));
+    source += entry_of("256", "_merge", "PrefixArgs", "ptowsp::merge_parts<" + std::to_string(own.s.D) + ", " + fp + "::RB, " + lp + "::RB, " + fo + "::RB, " + std::to_string(type) + ", " + flag(lse) + ">(A)");
+    if (own.prompts) source += entry_of("1024", "_units", "AttendArgs", uo + "::list_units<1024>(A)") + entry_of(bounds, "_finish", "AttendArgs", uo + "::finish<" + fo + ">(A)");
+    return source;
 }
 
 void run_prefix(const Node& n, const std::vector<Operand>& o, const OperatorRun& run) {
     const Operand &q = o[0], &table = o[8], &lengths = o[9], &members = o[10], &out = o[11];
     const bool lse = o.size() > 12 && o[12].shape.size() == 2;
-    AttendArgs own = attend_args(n, o, out, run), shared = own;
+    PrefixArgs P{};
+    AttendArgs &own = P.own, &shared = P.shared;
+    own = attend_args(n, o, out, run);
+    shared = own;
     if (table.shape[1] > 1 && table.stride[1] != 1) stop(n, "prefix_table's last dimension must have stride 1");
     shared.table = reinterpret_cast<const int*>(table.ptr), shared.s_table = table.stride[0], shared.width = table.shape[1];
     shared.lengths = reinterpret_cast<const int*>(lengths.ptr), shared.s_lengths = lengths.stride[0], shared.batch = table.shape[0];
     shared.members = reinterpret_cast<const int*>(members.ptr), shared.s_members = members.stride[0];
     shared.requests = static_cast<int>(own.batch);
     if (own.rows == 0 || own.batch == 0) return;
-    // Both parts leave results in float32, their maxima and sums.
     const int64_t heads = q.shape[1], D = q.shape[2], all = own.rows * heads;
-    const size_t part_bytes = whole(all * D * 4), sum_bytes = whole(all * 8);
-    AttendArgs* const args[2] = {&own, &shared};
-    AttendForm form[2];
-    AttendSpace space[2];
-    const int many = shared.batch > 0 ? 2 : 1;
-    size_t need = 2 * (part_bytes + sum_bytes);
-    for (int i = 0; i < many; ++i) {
-        form[i] = attend_form(q.shape, o[1].shape, args[i]->batch, q.dtype, o[1].dtype, false, true, vectors(q), 1 + i);
-        space[i] = attend_space(n, form[i], *args[i], run.cus);
-        need += space[i].need;
-    }
-    char* const scratch = run.scratch(need);
-    MergeArgs M{};
-    char* at = scratch + 2 * (part_bytes + sum_bytes);
+    const AttendForm mine = attend_form(q.shape, o[1].shape, own.batch, q.dtype, o[1].dtype, false, true, vectors(q), 1);
+    const AttendForm theirs = attend_form(q.shape, o[1].shape, shared.batch, q.dtype, o[1].dtype, false, true, vectors(q), 2);
+    const AttendSpace spaces[2] = {attend_space(n, mine, own, run.cus), attend_space(n, theirs, shared, run.cus)};
+    // Both parts' results, [row, head, D], and their entries, [row, head, 4].
+    const size_t part_bytes = whole(all * D * 4), entry_bytes = whole(all * 16);
+    char* at = run.scratch(2 * (part_bytes + entry_bytes) + spaces[0].need + spaces[1].need);
     for (int i = 0; i < 2; ++i) {
-        char* const part = scratch + static_cast<size_t>(i) * (part_bytes + sum_bytes);
-        AttendArgs& A = *args[i];
-        A.out = part;
+        AttendArgs& A = i ? shared : own;
+        A.out = at;
         A.s_out[0] = heads * D, A.s_out[1] = D;
-        A.lse = reinterpret_cast<float*>(part + part_bytes);
-        A.s_lse[0] = 2 * heads, A.s_lse[1] = 2;
-        M.parts[i] = reinterpret_cast<const float*>(A.out);
-        M.sums[i] = A.lse;
-        if (i >= many) continue;
-        attend_launch(form[i], space[i], at, A, run);
-        at += space[i].need;
+        A.lse = reinterpret_cast<float*>(at + part_bytes);
+        A.s_lse[0] = 4 * heads, A.s_lse[1] = 4;
+        attend_place(spaces[i], at + part_bytes + entry_bytes, A);
+        at += part_bytes + entry_bytes + spaces[i].need;
     }
-    M.starts = own.starts, M.s_starts = own.s_starts;
-    M.members = shared.members, M.s_members = shared.s_members;
-    M.out = out.ptr;
-    for (int d = 0; d < 2; ++d) M.s_out[d] = out.stride[d];
+    P.few_prefixes = shared.batch > 0 ? shared.blocks : 0;
+    const bool line = theirs.prompts && shared.batch > 0;
+    if (line) {
+        // Units, and pieces beyond them, at most.
+        const int prb = 16 * prompt_shape(theirs.s).nt, c = theirs.s.G <= prb ? prb / theirs.s.G : 1, hs = theirs.s.G <= prb ? 1 : (theirs.s.G + prb - 1) / prb;
+        const int64_t units = hs * (own.rows / (4 * c) + std::min<int64_t>(shared.batch, own.rows / (shared.few + 1))) * shared.heads;
+        if (units >= (int64_t(1) << 22)) stop(n, "too many rows for one call");
+        P.lines = static_cast<int>(units) + shared.cus + shared.cus / 3;
+    }
+    P.q_heads = static_cast<int>(heads);
+    P.out = out.ptr;
+    for (int d = 0; d < 2; ++d) P.s_out[d] = out.stride[d];
     if (lse) {
-        M.lse = reinterpret_cast<float*>(o[12].ptr);
-        for (int d = 0; d < 2; ++d) M.s_lse[d] = o[12].stride[d];
+        P.lse = reinterpret_cast<float*>(o[12].ptr);
+        for (int d = 0; d < 2; ++d) P.s_lse[d] = o[12].stride[d];
     }
-    M.rows = own.rows, M.heads = static_cast<int>(heads), M.requests = shared.requests, M.groups = static_cast<int>(shared.batch);
-    const int64_t groups = (all * (D / 4) + 255) / 256;
+    const int lanes = D <= 64 ? 16 : D <= 128 ? 32 : 64;
+    const int64_t groups = (all * lanes + 255) / 256;
     if (groups >= (int64_t(1) << 24)) stop(n, "too many rows for one call");
-    run.launch(merge_source(D, type_id(q.dtype), lse), "ptowsp_paged_prefix_merge", groups, 256, &M, sizeof M);
+    AttendForm shared_form = theirs;
+    shared_form.prompts = line;
+    const std::string source = prefix_source(mine, shared_form, type_id(q.dtype), lse);
+    if (mine.prompts) run.launch(source, "ptowsp_paged_prefix_units", 1, 1024, &own, sizeof own);
+    const int64_t prompts = mine.prompts ? static_cast<int64_t>(own.room) * own.heads : 0;
+    run.launch(source, "ptowsp_paged_prefix_parts", P.lines + P.few_prefixes + own.blocks + prompts, 256, &P, sizeof P);
+    if (mine.prompts) run.launch(source, "ptowsp_paged_prefix_finish", own.blocks, 256, &own, sizeof own);
+    run.launch(source, "ptowsp_paged_prefix_merge", groups, 256, &P, sizeof P);
 }
 
 // ---- operands that share memory ----
@@ -601,8 +624,12 @@ std::pair<std::string, std::string> operator_source(const Module& m, const Node&
     if (n.op == "paged_store")
         return {store_source(D, page, type_id(s.dtype[0]), code, true, store_chunk(s.of("k")[0], c[1], c[2])), "ptowsp_paged_store"};
     if (n.op == "paged_prefix_attention") {
-        const AttendForm f = attend_form(s.of("q"), c, s.of("prefix_table")[0], s.dtype[0], s.dtype[s.at("k_cache")], false, true, true, 2);
-        return {attend_source(f.s, f.prompts), f.prompts ? "ptowsp_paged_attention_prompts" : "ptowsp_paged_attention"};
+        const DType type = s.dtype[0], code_type = s.dtype[s.at("k_cache")];
+        const int64_t groups = s.of("prefix_table")[0];
+        AttendForm shared = attend_form(s.of("q"), c, groups, type, code_type, false, true, true, 2);
+        shared.prompts = shared.prompts && groups > 0;
+        return {prefix_source(attend_form(s.of("q"), c, s.of("lengths")[0], type, code_type, false, true, true, 1), shared, type_id(type), !s.of("lse").empty()),
+                "ptowsp_paged_prefix_parts"};
     }
     const AttendForm f = attend_form(s.of("q"), c, s.of("lengths")[0], s.dtype[0], s.dtype[s.at("k_cache")], attr(n, "window") > 0, !s.of("lse").empty(), true);
     return {attend_source(f.s, f.prompts), f.prompts ? "ptowsp_paged_attention_prompts" : "ptowsp_paged_attention"};
