@@ -1857,56 +1857,68 @@ struct Attend {
     __device__ static int units_of(const Request& r) { return (r.n + kUnitTokens - 1) / kUnitTokens * HS; }
     __device__ static int tiles_of(const Request& r) { return r.length > kTile ? static_cast<int>((static_cast<pg_u32>(r.length) + (kTile - 1)) / kTile) : 1; }
     __device__ static int pieces_of(const Request& r, int limit) { return (tiles_of(r) + limit - 1) / limit; }
+    __device__ static int line_limit(const AttendArgs& A, pg_i64 units, pg_i64 tiles) {
+        units *= A.heads;
+        tiles *= A.heads;
+        const pg_i64 room = 2 * units <= A.cus ? A.cus - units : A.cus + A.cus / 3, share = (tiles + room - 1) / room;
+        return share < kLeastTiles ? kLeastTiles : static_cast<int>(share);
+    }
     __device__ static bool line_part(const AttendArgs& A, int workgroup, Part& p) {
-        __shared__ pg_i64 scan[4], begin[3];
         const int wave = uniform(threadIdx.x >> 6);
-        const pg_i64 per = (A.batch + kAttendThreads - 1) / kAttendThreads, b0 = threadIdx.x * per;
-        const pg_i64 b1 = b0 + per < A.batch ? b0 + per : A.batch;
-        // Units and tiles of a key head, then pieces and those of units in several.
-        pg_i64 units = 0, tiles_here = 0, pieces = 0, cut = 0;
-        for (pg_i64 b = b0; b < b1; ++b) {
-            const Request r = request(A, b, workgroup == 0);
-            units += units_of(r);
-            tiles_here += static_cast<pg_i64>(units_of(r)) * tiles_of(r);
-        }
-        pg_i64 all_units, all_tiles, all;
-        block_scan<kAttendThreads>(units, all_units, scan);
-        block_scan<kAttendThreads>(tiles_here, all_tiles, scan);
-        all_units *= A.heads;
-        all_tiles *= A.heads;
-        const pg_i64 room = 2 * all_units <= A.cus ? A.cus - all_units : A.cus + A.cus / 3;
-        const pg_i64 share = (all_tiles + room - 1) / room;
-        const int limit = share < kLeastTiles ? kLeastTiles : static_cast<int>(share);
-        for (pg_i64 b = b0; b < b1; ++b) {
-            const Request r = request(A, b, false);
-            const int k = pieces_of(r, limit);
-            pieces += static_cast<pg_i64>(units_of(r)) * k;
-            cut += k > 1 ? static_cast<pg_i64>(units_of(r)) * k : 0;
-        }
-        const pg_i64 before = block_scan<kAttendThreads>(pieces, all, scan) * A.heads;
-        pg_i64 all_cut;
-        const pg_i64 cut_before = block_scan<kAttendThreads>(cut, all_cut, scan) * A.heads;
-        if (workgroup >= all * A.heads) return false;
-        if (workgroup >= before && workgroup < before + pieces * A.heads) {
-            pg_i64 at = before, slot = cut_before;
+        int limit, item;
+        p.b = 0;
+        p.slot = 0;
+        if (A.batch == 1) {
+            const Request r = request(A, 0, workgroup == 0);
+            limit = line_limit(A, units_of(r), static_cast<pg_i64>(units_of(r)) * tiles_of(r));
+            if (workgroup >= static_cast<pg_i64>(A.heads) * units_of(r) * pieces_of(r, limit)) return false;
+            item = workgroup;
+        } else {
+            __shared__ pg_i64 scan[4], begin[3];
+            const pg_i64 per = (A.batch + kAttendThreads - 1) / kAttendThreads, b0 = threadIdx.x * per;
+            const pg_i64 b1 = b0 + per < A.batch ? b0 + per : A.batch;
+            // Units and tiles of a key head, then pieces and those of units in several.
+            pg_i64 units = 0, tiles_here = 0, pieces = 0, cut = 0;
+            for (pg_i64 b = b0; b < b1; ++b) {
+                const Request r = request(A, b, workgroup == 0);
+                units += units_of(r);
+                tiles_here += static_cast<pg_i64>(units_of(r)) * tiles_of(r);
+            }
+            pg_i64 all_units, all_tiles, all, all_cut;
+            block_scan<kAttendThreads>(units, all_units, scan);
+            block_scan<kAttendThreads>(tiles_here, all_tiles, scan);
+            limit = line_limit(A, all_units, all_tiles);
             for (pg_i64 b = b0; b < b1; ++b) {
                 const Request r = request(A, b, false);
                 const int k = pieces_of(r, limit);
-                const pg_i64 here = static_cast<pg_i64>(A.heads) * units_of(r) * k;
-                if (workgroup < at + here) {
-                    begin[0] = b;
-                    begin[1] = at;
-                    begin[2] = slot;
-                    break;
-                }
-                at += here;
-                if (k > 1) slot += here;
+                pieces += static_cast<pg_i64>(units_of(r)) * k;
+                cut += k > 1 ? static_cast<pg_i64>(units_of(r)) * k : 0;
             }
+            const pg_i64 before = block_scan<kAttendThreads>(pieces, all, scan) * A.heads;
+            const pg_i64 cut_before = block_scan<kAttendThreads>(cut, all_cut, scan) * A.heads;
+            if (workgroup >= all * A.heads) return false;
+            if (workgroup >= before && workgroup < before + pieces * A.heads) {
+                pg_i64 at = before, slot = cut_before;
+                for (pg_i64 b = b0; b < b1; ++b) {
+                    const Request r = request(A, b, false);
+                    const int k = pieces_of(r, limit);
+                    const pg_i64 here = static_cast<pg_i64>(A.heads) * units_of(r) * k;
+                    if (workgroup < at + here) {
+                        begin[0] = b;
+                        begin[1] = at;
+                        begin[2] = slot;
+                        break;
+                    }
+                    at += here;
+                    if (k > 1) slot += here;
+                }
+            }
+            __syncthreads();
+            p.b = uniform(static_cast<int>(begin[0]));
+            item = workgroup - uniform(static_cast<int>(begin[1]));
+            p.slot = uniform(static_cast<int>(begin[2]));
         }
-        __syncthreads();
         // The piece: units side by side, so that workgroups beside each other read the same tiles.
-        p.b = uniform(static_cast<int>(begin[0]));
-        const int item = uniform(workgroup - static_cast<int>(begin[1]));
         p.rq = request(A, p.b, false);
         p.rq.row = uniform(p.rq.row);
         p.rq.n = uniform(p.rq.n);
@@ -1919,7 +1931,7 @@ struct Attend {
         const int in = unit - p.h * many;
         p.tile = uniform(in / HS);
         p.hs = in - p.tile * HS;
-        p.slot = uniform(static_cast<int>(begin[2])) + unit * p.pieces;
+        p.slot += unit * p.pieces;
         p.base = uniform(static_cast<int>(static_cast<pg_i64>(kt) * p.piece / p.pieces)) * kTile;
         p.end = uniform(static_cast<int>(static_cast<pg_i64>(kt) * (p.piece + 1) / p.pieces)) * kTile;
         if (p.end > p.rq.length) p.end = p.rq.length;
@@ -2078,6 +2090,9 @@ __device__ inline void prefix_parts(const PrefixArgs& A) {
     constexpr size_t lines = LINE && LP::TILES ? sizeof(typename LP::Tiles) : 0, prompts = PROMPTS && UO::TILES ? sizeof(typename UO::Tiles) : 0;
     constexpr size_t tiles = lines > prompts ? lines : prompts;
     __shared__ __attribute__((aligned(1024))) char lds[few > tiles ? few : tiles];
+    // The line's workgroups first: they fill the chip, and what they leave of it at the
+    // end the shorter ones take.  In turns with those for own tokens, 8 by 8, 64
+    // requests behind 16384 tokens take 78 us, so 68.
     int w = blockIdx.x;
     if constexpr (LINE) {
         if (w < A.lines) {
@@ -2086,16 +2101,19 @@ __device__ inline void prefix_parts(const PrefixArgs& A) {
         }
         w -= A.lines;
     }
-    if (w < A.few_prefixes) {
-        [[clang::always_inline]] FP::run(args_of(true), w, *reinterpret_cast<typename FP::Shared*>(lds));
-        return;
+    if constexpr (PROMPTS) {
+        const int prompts = A.own.room * A.own.heads;
+        if (w < prompts) {
+            [[clang::always_inline]] UO::prompt(args_of(false), *reinterpret_cast<typename UO::Tiles*>(lds), w);
+            return;
+        }
+        w -= prompts;
     }
-    w -= A.few_prefixes;
     if (w < A.own.blocks) {
         [[clang::always_inline]] FO::run(args_of(false), w, *reinterpret_cast<typename FO::Shared*>(lds));
         return;
     }
-    if constexpr (PROMPTS) [[clang::always_inline]] UO::prompt(args_of(false), *reinterpret_cast<typename UO::Tiles*>(lds), w - A.own.blocks);
+    [[clang::always_inline]] FP::run(args_of(true), w - A.own.blocks, *reinterpret_cast<typename FP::Shared*>(lds));
 }
 
 // What there is of a row: maximum, sum and a lane's four dims.
@@ -2125,35 +2143,47 @@ __device__ inline Joined join_part(const AttendArgs& A, int rbf, int rbl, pg_i64
     const float* const base = line ? A.unit_parts + place / rb * part : A.parts;
     const pg_i64 slot = line ? 4 * part : part;
     auto piece = [&](int k) { return base + (line ? first + k : 2 * (first + k) + (k == 0 ? 1 : 0)) * slot; };
-    const int l0 = threadIdx.x & (LANES - 1);
-    float m = -__builtin_inff();
-    for (int k = l0; k < many; k += LANES) m = fmaxf(m, piece(k)[at]);
+    // The first pieces' numbers are under way while their weights are found.
+    constexpr int AHEAD = 8;
+    pg_f32x4 x[AHEAD];
+    auto fetch = [&](int k0) {
 #pragma unroll
-    for (int x = LANES / 2; x >= 1; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, LANES));
+        for (int e = 0; e < AHEAD; ++e)
+            if (k0 + e < many) x[e] = *reinterpret_cast<const pg_f32x4*>(piece(k0 + e) + 2 * rb + at * DP + d);
+    };
+    fetch(0);
+    const int l0 = threadIdx.x & (LANES - 1);
+    float m = -__builtin_inff(), own_m = m, own_l = 0.0f;  // of piece l0
+    if (l0 < many) {
+        own_m = piece(l0)[at];
+        own_l = piece(l0)[rb + at];
+    }
+    m = own_m;
+    for (int k = l0 + LANES; k < many; k += LANES) m = fmaxf(m, piece(k)[at]);
+#pragma unroll
+    for (int z = LANES / 2; z >= 1; z >>= 1) m = fmaxf(m, __shfl_xor(m, z, LANES));
     r.m = m;
     r.l = 0.0f;
     r.o = pg_f32x4{0, 0, 0, 0};
     for (int k0 = 0; k0 < many; k0 += LANES) {
-        float weight = 0.0f;
-        if (k0 + l0 < many) {
-            const float* const p = piece(k0 + l0);
-            weight = p[at] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(p[at] - m);
-            r.l += weight * p[rb + at];
+        if (k0 > 0 && k0 + l0 < many) {
+            own_m = piece(k0 + l0)[at];
+            own_l = piece(k0 + l0)[rb + at];
         }
+        const float weight = k0 + l0 >= many || own_m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(own_m - m);
+        r.l += weight * own_l;
         const int n = many - k0 < LANES ? many - k0 : LANES;
-        for (int k = 0; k < n; k += 8) {
-            pg_f32x4 x[8];
+        for (int k = 0; k < n; k += AHEAD) {
+            if (k0 + k > 0) fetch(k0 + k);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = *reinterpret_cast<const pg_f32x4*>(piece(k0 + (k + e < n ? k + e : n - 1)) + 2 * rb + at * DP + d);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float f = __shfl(weight, k + e, LANES);
+            for (int e = 0; e < AHEAD; ++e) {
+                const float f = __shfl(weight, k + e < LANES ? k + e : 0, LANES);
                 if (k + e < n) r.o += f * x[e];
             }
         }
     }
 #pragma unroll
-    for (int x = LANES / 2; x >= 1; x >>= 1) r.l += __shfl_xor(r.l, x, LANES);
+    for (int z = LANES / 2; z >= 1; z >>= 1) r.l += __shfl_xor(r.l, z, LANES);
     return r;
 }
 
