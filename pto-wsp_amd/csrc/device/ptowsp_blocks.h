@@ -15,7 +15,9 @@ namespace ptowsp {
 // finite |x| among them, the scale, the codes.  Weights' blocks have 128 rows as
 // well, which a workgroup's 16 groups of lanes share.  A code is the product
 // with 1 / scale, rounded as float32 values are.  Infinities and NaN are met
-// only where the block's largest bits say so.
+// only where the block's largest bits say so.  Bound by HBM: 16384 rows of 4096 in
+// bf16 (203 MB) 32 us, 6.4 TB/s; with NaN tests and clamps on every number 41 us.
+// 128-row blocks of the same 37 us, 5.4 TB/s.
 // ---------------------------------------------------------------------------
 
 // Columns c .. c + 7 of a row of K; what lies behind K counts as 0.
@@ -69,14 +71,16 @@ __device__ inline pg_u32 most_bits(pg_u32 x) {
     return x;
 }
 
-template <int T>
+// FINITE: all numbers of the block are, and none is beyond the largest code by more
+// than a few roundings of float32, which round away again.
+template <int T, bool FINITE>
 __device__ inline pg_u32 codes8(const Eight<T>& x, float inverse, pg_u32& hi) {
     float y[8];
     values8<T>(x, y);
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] *= inverse;
-    hi = encode4<kE4M3, false>(y + 4);
-    return encode4<kE4M3, false>(y);
+    hi = encode4<kE4M3, FINITE>(y + 4);
+    return encode4<kE4M3, FINITE>(y);
 }
 
 __device__ inline void put8(char* row, pg_i64 c, pg_i64 K, pg_u32 lo, pg_u32 hi) {
@@ -115,10 +119,12 @@ __device__ inline void quantize_rows(const QuantizeArgs& A) {
         if constexpr (T != kF32) bits = (bits & 0xFFFFu) > bits >> 16 ? bits & 0xFFFFu : bits >> 16;
         bits = most_bits<16>(bits);
         float most = number_of<T>(bits);
-        if (__ballot(bits >= kInf)) most = __uint_as_float(most_bits<16>(__float_as_uint(finite8<T>(x[u], 0.0f))));
+        const bool finite = __ballot(bits >= kInf) == 0;
+        if (!finite) most = __uint_as_float(most_bits<16>(__float_as_uint(finite8<T>(x[u], 0.0f))));
         const float scale = fmaxf(most / 448.0f, 0x1p-126f), inverse = 1.0f / scale;
-        pg_u32 hi;
-        const pg_u32 lo = codes8<T>(x[u], inverse, hi);
+        pg_u32 lo, hi;
+        if (finite) lo = codes8<T, true>(x[u], inverse, hi);
+        else lo = codes8<T, false>(x[u], inverse, hi);
         if (in[u]) {
             put8(A.codes + row[u] * A.s_codes, block[u] * kScaleBlock + 8 * l, A.cols, lo, hi);
             if (l == 0) A.scales[row[u] * A.s_scales[0] + block[u] * A.s_scales[1]] = scale;
@@ -157,7 +163,7 @@ __device__ inline void quantize_squares(const QuantizeArgs& A) {
     for (int u = 0; u < 8; ++u) {
         const pg_i64 r = r0 + g + 16 * u;
         pg_u32 hi;
-        const pg_u32 lo = codes8<T>(x[u], inverse, hi);
+        const pg_u32 lo = codes8<T, false>(x[u], inverse, hi);
         if (r < A.rows) put8(A.codes + r * A.s_codes, c, A.cols, lo, hi);
     }
     if (threadIdx.x == 0) A.scales[strip * A.s_scales[0] + block * A.s_scales[1]] = scale;

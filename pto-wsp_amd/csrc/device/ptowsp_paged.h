@@ -1936,12 +1936,15 @@ struct Attend {
         p.end = uniform(static_cast<int>(static_cast<pg_i64>(kt) * (p.piece + 1) / p.pieces)) * kTile;
         if (p.end > p.rq.length) p.end = p.rq.length;
         const int first = p.tile * kUnitTokens + wave * C;
-        p.row = p.rq.row + first;
-        p.head = p.h * G + p.hs * RB;
+        p.row = uniform(p.rq.row + first);
+        p.head = uniform(p.h * G + p.hs * RB);
+        p.slot = uniform(p.slot);
+        p.base = uniform(p.base);
+        p.end = uniform(p.end);
         p.u.table = A.table + p.b * A.s_table;
         p.u.h = p.h;
-        p.u.n = p.rq.n - first < C ? p.rq.n - first : C;
-        p.u.p0 = position(p.rq, first);
+        p.u.n = uniform(p.rq.n - first < C ? p.rq.n - first : C);
+        p.u.p0 = uniform(position(p.rq, first));
         p.u.hi = p.u.n > 0 ? end_of(p.u.p0, p.u.n) : 0;
         p.u.lo = 0;
         return true;

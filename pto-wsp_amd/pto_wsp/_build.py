@@ -65,8 +65,8 @@ def build(verbose: bool = False) -> str:
 
 
 def _operator_workloads():
-    """The paged operators, in types and shapes that between them reach every kernel."""
-    from pto_wsp import DType, Tensor, paged_attention, paged_plan, paged_store
+    """The operators, in types and shapes that between them reach every kernel."""
+    from pto_wsp import DType, Tensor, block_matmul, block_quantize, paged_attention, paged_norm_rotate, paged_plan, paged_prefix_attention, paged_store
 
     def T(dtype, *shape):
         return Tensor(data=None, shape=shape, dtype=dtype)
@@ -83,6 +83,19 @@ def _operator_workloads():
         yield paged_store(k=T(dt, rows, heads, dim), v=T(dt, rows, heads, dim), slots=T(i32, rows), **cache)
         yield paged_attention(q=T(dt, rows, heads * group, dim), out=T(dt, rows, heads * group, dim), page_table=T(i32, 4, 3),
                               lengths=T(i32, 4), starts=T(i32, 5), window=window, lse=T(f32, rows, heads * group) if window else None, **cache)
+        yield paged_prefix_attention(q=T(dt, rows, heads * group, dim), out=T(dt, rows, heads * group, dim), page_table=T(i32, 4, 3), lengths=T(i32, 4),
+                                     starts=T(i32, 5), prefix_table=T(i32, 2, 3), prefix_lengths=T(i32, 2), members=T(i32, 3),
+                                     lse=T(f32, rows, heads * group) if window else None, **cache)
+    for dt in (bf16, f16, f32):
+        for m, k, n in ((1, 4096, 6144), (64, 4096, 6144), (128, 4096, 6144), (256, 4096, 6144), (512, 4096, 6144), (8192, 4096, 6144), (300, 1160, 1000)):
+            blocks = -(-k // 128)
+            for rows in (1, 128):
+                yield block_quantize(x=T(dt, m, k), codes=T(e4m3, m, k), scales=T(f32, -(-m // rows), blocks), rows=rows)
+            yield block_matmul(a=T(e4m3, m, k), a_scale=T(f32, m, blocks), b=T(e4m3, n, k), b_scale=T(f32, -(-n // 128), blocks), out=T(dt, m, n))
+        for dim, turned, interleaved, weights in ((128, 128, False, "qk"), (80, 32, True, ""), (256, 2, False, "q"), (96, 50, True, "k")):
+            yield paged_norm_rotate(q=T(dt, 9, 4, dim), k=T(dt, 9, 2, dim), q_out=T(dt, 9, 4, dim), k_out=T(dt, 9, 2, dim), cos=T(f32, 9, turned // 2),
+                                    sin=T(f32, 9, turned // 2), lengths=T(i32, 4), starts=T(i32, 5), interleaved=interleaved,
+                                    **{x + "_weight": T(dt, dim) for x in weights})
 
 
 def check_device_templates() -> None:
