@@ -252,7 +252,8 @@ void check_block_operator(const Shapes& s) {
         if (x[1] < 1) refuse(n, "x has no columns");
         s.want("codes", x);
         s.want("scales", {parts(x[0], rows), scale_blocks(x[1])});
-        if (x[0] > kMost || x[1] > kMost || x[0] * scale_blocks(x[1]) > (int64_t(1) << 27)) refuse(n, "x has too many blocks for one call");
+        if (x[0] > kMost || x[1] > kMost || x[0] * scale_blocks(x[1]) > (int64_t(1) << 27) || parts(x[0], rows) * scale_blocks(x[1]) > (int64_t(1) << (rows == 1 ? 27 : 23)))
+            refuse(n, "x has too many blocks for one call");
     } else if (n.op == "block_matmul") {
         const auto &a = s.of("a"), &b = s.of("b");
         if (a[1] != b[1]) refuse(n, "a has " + num(a[1]) + " columns, b " + num(b[1]));

@@ -48,6 +48,7 @@ def prefix(rows=5, heads=2, G=4, D=64, batch=3, groups=2, dt=BF16, c=None, **oth
     (lambda: quantize(rows=128, scales=T(F32, 5, 3)), "scales has the shape"),
     (lambda: quantize(scales=T(BF16, 5, 3)), "unsupported type bf16"),
     (lambda: quantize(M=1 << 24, K=2048), "too many blocks"),
+    (lambda: quantize(M=1, K=(1 << 30) + 1, rows=128), "too many blocks"),
     (lambda: quantize(x=T(BF16, 5, 300, 1)), "rank 2 is needed"),
     (lambda: matmul(b=T(E4M3, 200, 305)), "a has 304 columns, b 305"),
     (lambda: matmul(a=T(I8, 5, 304)), "unsupported type i8"),
