@@ -1,7 +1,8 @@
 // Operators over a paged KV cache held in 8 bits, hand-written for gfx950:
-// block tables and slot maps (plan), quantising writes (store) and causal
-// grouped-query attention (attend).  The host library compiles one entry per
-// combination of types, head size, page size and group.
+// block tables and slot maps (plan), quantising writes (store), causal
+// grouped-query attention (attend) and the same for requests that share prefixes.
+// The host library compiles one entry per combination of types, head size, page
+// size and group.
 #pragma once
 
 #include "ptowsp_numbers.h"
@@ -1857,11 +1858,27 @@ struct Attend {
     __device__ static int units_of(const Request& r) { return (r.n + kUnitTokens - 1) / kUnitTokens * HS; }
     __device__ static int tiles_of(const Request& r) { return r.length > kTile ? static_cast<int>((static_cast<pg_u32>(r.length) + (kTile - 1)) / kTile) : 1; }
     __device__ static int pieces_of(const Request& r, int limit) { return (tiles_of(r) + limit - 1) / limit; }
+    // Few units and two workgroups a compute unit: pieces for both of them, or for one. A
+    // tile then takes 1.65 us and not 2.35, half the results are written, and the other
+    // place is for the workgroups of own tokens, whose time is latency; it is not known
+    // here, and their number stands for it.  The whole call with pieces for both and for
+    // one, 8 x 4 heads of 128, 64 requests of 64 to 1024 own tokens: behind 16384 shared
+    // ones 81 and 69 us, 24576 91 and 80, 32768 104 and 102, 49152 125 and 139; 1024 to
+    // 4096 behind 49152 182 and 153, 1 behind 24576 71 and 74; 256 requests behind 8192
+    // 161 and 141, behind 16384 205 and 211.  As many pieces as there are compute units
+    // take 74 us where these take 71: some are left to the own tokens.
     __device__ static int line_limit(const AttendArgs& A, pg_i64 units, pg_i64 tiles) {
         units *= A.heads;
         tiles *= A.heads;
-        const pg_i64 room = 2 * units <= A.cus ? A.cus - units : A.cus + A.cus / 3, share = (tiles + room - 1) / room;
-        return share < kLeastTiles ? kLeastTiles : static_cast<int>(share);
+        const auto share = [&](pg_i64 room) {
+            const pg_i64 each = (tiles + room - 1) / room;
+            return each < kLeastTiles ? kLeastTiles : static_cast<int>(each);
+        };
+        if (2 * units > A.cus) return share(A.cus + A.cus / 3);
+        const int two = share(A.cus - units);
+        if (!TILES || 4 * units > A.cus) return two;
+        const int one = share(A.cus / 2 - units), own = A.requests < 4 * A.cus / A.heads ? A.requests * A.heads / A.cus : 4;
+        return 7 * one <= 10 * two + 40 + 45 * own ? one : two;
     }
     __device__ static bool line_part(const AttendArgs& A, int workgroup, Part& p) {
         const int wave = uniform(threadIdx.x >> 6);
@@ -1869,9 +1886,9 @@ struct Attend {
         p.b = 0;
         p.slot = 0;
         if (A.batch == 1) {
-            const Request r = request(A, 0, workgroup == 0);
-            limit = line_limit(A, units_of(r), static_cast<pg_i64>(units_of(r)) * tiles_of(r));
-            if (workgroup >= static_cast<pg_i64>(A.heads) * units_of(r) * pieces_of(r, limit)) return false;
+            p.rq = request(A, 0, workgroup == 0);
+            limit = line_limit(A, units_of(p.rq), static_cast<pg_i64>(units_of(p.rq)) * tiles_of(p.rq));
+            if (workgroup >= static_cast<pg_i64>(A.heads) * units_of(p.rq) * pieces_of(p.rq, limit)) return false;
             item = workgroup;
         } else {
             __shared__ pg_i64 scan[4], begin[3];
@@ -1917,9 +1934,9 @@ struct Attend {
             p.b = uniform(static_cast<int>(begin[0]));
             item = workgroup - uniform(static_cast<int>(begin[1]));
             p.slot = uniform(static_cast<int>(begin[2]));
+            p.rq = request(A, p.b, false);
         }
         // The piece: units side by side, so that workgroups beside each other read the same tiles.
-        p.rq = request(A, p.b, false);
         p.rq.row = uniform(p.rq.row);
         p.rq.n = uniform(p.rq.n);
         p.rq.length = uniform(p.rq.length);
@@ -2084,6 +2101,15 @@ struct Attend {
 // a launch ahead and whose pieces are joined in one behind.  Each leaves float32
 // results: of a unit that one workgroup had in the row's place, of the others in
 // pieces.  The last launch joins what there is of a row.
+//
+// A group's rows read a prefix's pages together: 64 requests' tokens of 8 x 4 heads
+// of 128 behind 16384 shared tokens and 64 to 1024 of their own take 57 us and 10 for
+// the join.  A workgroup of the line has its first scores after 7 us, four loads one
+// behind the other, then takes 1.65 us a tile and 3 to write; one of own tokens takes
+// 18 us, 9 of them for a single token; about 6 are empty workgroups.  Prompts of 256
+// tokens, 16 of two groups: 295 to 302 us, 680 TFLOP/s, bound as paged_attention's
+// prompts are, and 26 for the join, by HBM.  Four requests: 10 and 6 us, the latency of
+// two launches.
 // ---------------------------------------------------------------------------
 
 // LP: the line's kernels; FP, FO: few rows over prefixes and own tokens; UO: prompts over own tokens.
@@ -2093,9 +2119,10 @@ __device__ inline void prefix_parts(const PrefixArgs& A) {
     constexpr size_t lines = LINE && LP::TILES ? sizeof(typename LP::Tiles) : 0, prompts = PROMPTS && UO::TILES ? sizeof(typename UO::Tiles) : 0;
     constexpr size_t tiles = lines > prompts ? lines : prompts;
     __shared__ __attribute__((aligned(1024))) char lds[few > tiles ? few : tiles];
-    // The line's workgroups first: they fill the chip, and what they leave of it at the
-    // end the shorter ones take.  In turns with those for own tokens, 8 by 8, 64
-    // requests behind 16384 tokens take 78 us, so 68.
+    // The line's workgroups first: they fill the chip, or a place of each compute unit,
+    // and what they leave of it the shorter ones take.  In turns with those for own
+    // tokens, 8 by 8, or the line's second half behind them, calls whose line fills the
+    // chip take 10% longer.
     int w = blockIdx.x;
     if constexpr (LINE) {
         if (w < A.lines) {

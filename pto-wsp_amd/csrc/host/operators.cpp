@@ -403,11 +403,11 @@ void run_prefix(const Node& n, const std::vector<Operand>& o, const OperatorRun&
     P.few_prefixes = shared.batch > 0 ? shared.blocks : 0;
     const bool line = theirs.prompts && shared.batch > 0;
     if (line) {
-        // Units, and pieces beyond them, at most.
+        // Pieces, at most: line_limit() makes no more than A.cus of few units.
         const int prb = 16 * prompt_shape(theirs.s).nt, c = theirs.s.G <= prb ? prb / theirs.s.G : 1, hs = theirs.s.G <= prb ? 1 : (theirs.s.G + prb - 1) / prb;
         const int64_t units = hs * (own.rows / (4 * c) + std::min<int64_t>(shared.batch, own.rows / (shared.few + 1))) * shared.heads;
         if (units >= (int64_t(1) << 22)) stop(n, "too many rows for one call");
-        P.lines = static_cast<int>(units) + shared.cus + shared.cus / 3;
+        P.lines = 2 * units <= shared.cus ? shared.cus : static_cast<int>(units) + shared.cus + shared.cus / 3;
     }
     P.q_heads = static_cast<int>(heads);
     P.out = out.ptr;

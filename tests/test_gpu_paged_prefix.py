@@ -217,6 +217,14 @@ def test_prefix_shared_by_many(gpu):
     attend(gpu, case(rng, "bf16", "e4m3", 2, 8, 128, 16, [900, 17, 2500], [0, 60, 92, 95], [c + 3 for c in counts], counts), lse=False)
 
 
+@pytest.mark.parametrize("many", [2, 40, 69])
+@pytest.mark.parametrize("groups", [1, 2])
+def test_prefix_pieces_by_units(gpu, many, groups):
+    """Units of a group's rows few (pieces for one workgroup a compute unit), more (for two) and many (beyond that)."""
+    members = [0, many // 2, many] if groups == 2 else [0, many]
+    attend(gpu, case(np.random.default_rng(11), "bf16", "e4m3", 8, 4, 64, 16, [1500, 777][:groups], members, [20] * many, [16] * many))
+
+
 def test_prefix_layouts(gpu):
     """Strided queries, results, tables and counts."""
     torch = _torch()
