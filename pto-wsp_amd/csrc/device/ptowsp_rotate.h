@@ -17,24 +17,39 @@ namespace ptowsp {
 // crosses lanes; LANES lanes hold a head, a wave as many heads of one token as
 // fit, and goes on with the token's next ones under the same sines.  Its request is
 // found 64 steps at a time: two dependent loads for 4096 requests.  Bound by HBM:
-// 16384 tokens of 32 + 8 heads of 128 in bf16 (344 MB) 60 us, 5.7 TB/s; 64 tokens by
+// 16384 tokens of 32 + 8 heads of 128 in bf16 (344 MB) 52 us, 6.6 TB/s; 64 tokens by
 // latency, 3.9 us.
 // ---------------------------------------------------------------------------
 
 constexpr int rotate_piece(int R) { return R % 16 == 0 ? 8 : R % 8 == 0 ? 4 : R % 4 == 0 ? 2 : 1; }
 
-template <int T, int P>
+// ONCE: bytes that the call reads once.  16 of them (a head's dims, side by side in
+// a wave) are read without a place in the caches: 16384 tokens of inputs from memory
+// take 71 us so and 76 otherwise, of inputs in the caches 52 both.  Other pieces are
+// parts of cache lines that another load needs too: float32 heads took 21 us so and 19
+// otherwise.
+typedef pg_u32 pg_any_u32x4 __attribute__((ext_vector_type(4), aligned(2)));
+template <int BYTES, bool ONCE>
+__device__ inline void read(void* to, const char* p) {
+    if constexpr (ONCE && BYTES == 16) {
+        const pg_any_u32x4 w = __builtin_nontemporal_load(reinterpret_cast<const pg_any_u32x4*>(p));
+        __builtin_memcpy(to, &w, 16);
+    } else {
+        __builtin_memcpy(to, p, BYTES);
+    }
+}
+template <int T, int P, bool ONCE = false>
 __device__ inline void load_piece(const char* p, float (&y)[P]) {
     if constexpr (T == kF32) {
-        __builtin_memcpy(y, p, 4 * P);
+        read<4 * P, ONCE>(y, p);
     } else if constexpr (T == kF16) {
         _Float16 h[P];
-        __builtin_memcpy(h, p, 2 * P);
+        read<2 * P, ONCE>(h, p);
 #pragma unroll
         for (int i = 0; i < P; ++i) y[i] = static_cast<float>(h[i]);
     } else {
         pg_u16 h[P];
-        __builtin_memcpy(h, p, 2 * P);
+        read<2 * P, ONCE>(h, p);
 #pragma unroll
         for (int i = 0; i < P; ++i) y[i] = __uint_as_float(static_cast<pg_u32>(h[i]) << 16);
     }
@@ -122,8 +137,8 @@ struct Rotate {
             for (int e = 0; e < EACH; ++e) {
                 const bool in = l + LANES * e < GROUPS;
                 const int i = in ? l + LANES * e : GROUPS - 1;
-                load_piece<T, P>(x + low(i) * elem_size(T), y[e][0]);
-                load_piece<T, P>(x + high(i) * elem_size(T), y[e][1]);
+                load_piece<T, P, true>(x + low(i) * elem_size(T), y[e][0]);
+                load_piece<T, P, true>(x + high(i) * elem_size(T), y[e][1]);
                 float part = 0.0f;
 #pragma unroll
                 for (int k = 0; k < P; ++k) part = __builtin_fmaf(y[e][0][k], y[e][0][k], __builtin_fmaf(y[e][1][k], y[e][1][k], part));
