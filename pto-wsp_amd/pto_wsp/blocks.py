@@ -36,7 +36,8 @@ def block_matmul(*, a: Tensor, a_scale: Tensor, b: Tensor, b_scale: Tensor, out:
     ``out[m, n]`` is the sum over blocks j of ``a_scale[m, j] * b_scale[n // 128, j]`` times the sum of the block's
     products of codes.  Sums are float32, rounded once at the end.  For BF16 and F16 results the matrix instruction
     cuts each product at 2^-13 of the largest of the eight that it adds at once, which costs 1.5e-5 of a typical
-    result; for F32 results products are exact.  Rows of a and b may lie at any distance; where a row's codes, its
-    distance and K are multiples of 16 bytes they are loaded straight into shared memory.
+    result; for F32 results products are exact.  Scales may be any, also such that their product lies beyond float32
+    where the result does not.  Rows of a and b may lie at any distance; where a row's codes, its distance and K are
+    multiples of 16 bytes they are loaded straight into shared memory.
     """
     return _operator("block_matmul", {"a": a, "a_scale": a_scale, "b": b, "b_scale": b_scale, "out": out}, {})
