@@ -2152,15 +2152,18 @@ struct Joined {
     pg_f32x4 o;
 };
 
-// LANES lanes a row, four dims each.  RBF, RBL: rows of a partial result of run(), of a wave of line().
-template <int DP, int LANES>
+// LANES lanes a row, four dims each.  rbf, rbl: rows of a partial result of run(), of a wave of line(); LINE: whether
+// that may have had a part in it.
+template <int DP, int LANES, bool LINE>
 __device__ inline Joined join_part(const AttendArgs& A, int rbf, int rbl, pg_i64 row, int head, int d, int D) {
     Joined r;
     const pg_f32x4 entry = *reinterpret_cast<const pg_f32x4*>(A.lse + row * A.s_lse[0] + head * A.s_lse[1]);
-    // Entries of requests out of range, which no kernel has written, may be anything.
+    // Entries of requests out of range, which no kernel has written, may be anything, what
+    // an earlier call left there among it.  Of own tokens `room` counts units, of which the
+    // workspace holds no results, so that an entry of the line names no pieces there.
     const int code = __float_as_int(entry[3]), many = code & (kFromLine - 1), first = __float_as_int(entry[2]);
     const bool line = code & kFromLine;
-    if (many == 0 || first < 0 || first > (line ? A.room : A.blocks) - many) {
+    if (many == 0 || (line && !LINE) || first < 0 || first > (line ? A.room : A.blocks) - many) {
         // The result has been divided by its sum: a sum of 1 and the sum in the weight.
         r.m = entry[0];
         r.l = entry[1];
@@ -2230,9 +2233,9 @@ __device__ inline void merge_parts(const PrefixArgs& A) {
     // Rows of no request are left alone; the groups' rows follow each other.
     if (row >= own.rows || row < first_row(0) || row >= first_row(requests)) return;
     const bool both = m0 >= 0 && m0 <= m1 && m1 <= requests && row >= first_row(m0) && row < first_row(m1);
-    Joined r = join_part<DP, LANES>(own, RBO, RBO, row, head, d, D);
+    Joined r = join_part<DP, LANES, false>(own, RBO, RBO, row, head, d, D);
     if (both) {
-        const Joined p = join_part<DP, LANES>(shared, RBP, RBL, row, head, d, D);
+        const Joined p = join_part<DP, LANES, true>(shared, RBP, RBL, row, head, d, D);
         const float m = fmaxf(r.m, p.m);
         const float w0 = r.l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(r.m - m), w1 = p.l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(p.m - m);
         r.o = r.o * w0 + p.o * w1;
