@@ -106,8 +106,9 @@ struct Rotate {
         const pg_i64 b = request_of(A, row);
         const int s0 = A.starts[b * A.s_starts], s1 = A.starts[(b + 1) * A.s_starts];
         if (row < s0 || row >= s1) return;
-        const pg_i64 pos = static_cast<pg_i64>(A.lengths[b * A.s_lengths]) - (s1 - row) + (A.offsets ? A.offsets[b * A.s_offsets] : 0);
-        if (s1 > A.rows || s0 < 0 || pos < 0 || pos >= A.positions) {
+        // The token's place among its request's, and its position.
+        const pg_i64 place = static_cast<pg_i64>(A.lengths[b * A.s_lengths]) - (s1 - row), pos = place + (A.offsets ? A.offsets[b * A.s_offsets] : 0);
+        if (s1 > A.rows || s0 < 0 || place < 0 || pos < 0 || pos >= A.positions) {
             *A.err = 8;
             return;
         }
