@@ -86,6 +86,19 @@ __device__ inline pg_i64 request_of(const RotateArgs& A, pg_i64 row) {
     return lo;
 }
 
+// Where one of a wave's 64 requests starts, and where the next one does.  The search
+// takes requests in order and may not meet one that is not, so the first waves look at
+// all of them, by loads ahead of the search's; ahead of their own token's the check takes
+// 7% of a call of 16384 tokens.
+struct Starts {
+    int from, to;
+    __device__ bool bad(const RotateArgs& A) const { return from < 0 || to < from || to > A.rows; }
+};
+__device__ inline Starts starts_of(const RotateArgs& A, pg_i64 wave) {
+    const pg_i64 b = 64 * wave + (threadIdx.x & 63), at = b < A.batch ? b : A.batch - 1;
+    return Starts{A.starts[at * A.s_starts], A.starts[(at + 1) * A.s_starts]};
+}
+
 // WT: the type of the weights; QN, KN: whether queries and keys are normalised.
 template <int D, int R, int T, int WT, bool QN, bool KN, bool INTER>
 struct Rotate {
@@ -101,8 +114,20 @@ struct Rotate {
     __device__ static int low(int i) { return INTER || i >= TURN ? 2 * P * i : P * i; }
     __device__ static int high(int i) { return INTER || i >= TURN ? 2 * P * i + P : R / 2 + P * i; }
 
-    // Heads first, first + step, ... of the token in `row`.
+    // Heads first, first + step, ... of the token in `row`, and the order of requests.
     __device__ static void run(const RotateArgs& A, pg_i64 row, int first, int step) {
+        const pg_i64 wave = row * step + first;
+        const bool looks = 64 * wave < A.batch;
+        Starts mine = {0, 0};
+        if (looks) mine = starts_of(A, wave);
+        turn(A, row, first, step);
+        if (looks) {
+            bool bad = mine.bad(A);
+            for (pg_i64 w = wave + A.rows * step; 64 * w < A.batch; w += A.rows * step) bad |= starts_of(A, w).bad(A);
+            if (__ballot(bad)) *A.err = 8;
+        }
+    }
+    __device__ static void turn(const RotateArgs& A, pg_i64 row, int first, int step) {
         const pg_i64 b = request_of(A, row);
         const int s0 = A.starts[b * A.s_starts], s1 = A.starts[(b + 1) * A.s_starts];
         if (row < s0 || row >= s1) return;

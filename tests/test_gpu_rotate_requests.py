@@ -28,3 +28,27 @@ def test_places_ahead_of_a_request(gpu, D):
     t["lengths"] = ints(gpu, [5, 3, 6])
     go(rotate(t))
     check_rotate(t, "f32")
+
+
+@pytest.mark.parametrize("batch,where", [(4, 2), (3, 2), (64, 40), (65, 63), (300, 130), (5000, 4500)])
+@pytest.mark.parametrize("what", ["down", "beyond", "below"])
+def test_starts_out_of_order(gpu, batch, where, what):
+    """One start that goes down, lies beyond the rows or below 0, behind any number of others; fewer waves than requests
+    have 64 among them, too."""
+    counts = np.zeros(batch, int)
+    counts[[0, -1]] = 2, 1
+    t = rotate_case(gpu, counts, np.full(batch, 3), 2, 1, 64, 16, "f32", batch, spare=1)
+    t["starts"][where] = {"down": 1 if where < batch - 1 else 0, "beyond": len(t["q"]) + 1, "below": -1}[what]
+    raises(t)
+
+
+@pytest.mark.parametrize("batch", [64, 129, 5000])
+def test_starts_beyond_the_rows(gpu, batch):
+    """All rows are of requests in order; one behind them has rows that there are none of."""
+    counts = np.zeros(batch, int)
+    counts[3] = 4
+    t = rotate_case(gpu, counts, np.full(batch, 3), 2, 1, 64, 16, "f32", batch, spare=0)
+    go(rotate(t))
+    check_rotate(t, "f32")
+    t["starts"][-1] += 1
+    raises(t)
