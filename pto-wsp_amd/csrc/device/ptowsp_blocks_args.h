@@ -43,7 +43,7 @@ struct RotateArgs {
     const int* starts;
     const int* offsets;  // null: none
     long long s_x[2][2], s_out[2][2];  // row, head
-    long long s_weight[2], s_cos, s_sin, s_lengths, s_starts, s_offsets;
+    long long s_cos, s_sin, s_lengths, s_starts, s_offsets;
     long long batch, rows, positions;
     int heads[2];
     float eps;

@@ -79,8 +79,7 @@ struct PrefixArgs {
     // head (`lse`): its maximum and sum, or where its pieces lie.  `room` of the
     // prefixes: pieces of line() that there is room for.
     AttendArgs own, shared;
-    int lines;         // workgroups for prefixes of many rows
-    int few_prefixes;  // workgroups for prefixes of few
+    int lines;  // workgroups for prefixes of many rows
     int q_heads;
     char* out;
     float* lse;

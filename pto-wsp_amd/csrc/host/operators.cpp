@@ -400,7 +400,7 @@ void run_prefix(const Node& n, const std::vector<Operand>& o, const OperatorRun&
         attend_place(spaces[i], at + part_bytes + entry_bytes, A);
         at += part_bytes + entry_bytes + spaces[i].need;
     }
-    P.few_prefixes = shared.batch > 0 ? shared.blocks : 0;
+    const int few_prefixes = shared.batch > 0 ? shared.blocks : 0;  // workgroups for prefixes of few rows
     const bool line = theirs.prompts && shared.batch > 0;
     if (line) {
         // Pieces, at most: line_limit() makes no more than A.cus of few units.
@@ -424,7 +424,7 @@ void run_prefix(const Node& n, const std::vector<Operand>& o, const OperatorRun&
     const std::string source = prefix_source(mine, shared_form, type_id(q.dtype), lse);
     if (mine.prompts) run.launch(source, "ptowsp_paged_prefix_units", 1, 1024, &own, sizeof own);
     const int64_t prompts = mine.prompts ? static_cast<int64_t>(own.room) * own.heads : 0;
-    run.launch(source, "ptowsp_paged_prefix_parts", P.lines + P.few_prefixes + own.blocks + prompts, 256, &P, sizeof P);
+    run.launch(source, "ptowsp_paged_prefix_parts", P.lines + few_prefixes + own.blocks + prompts, 256, &P, sizeof P);
     if (mine.prompts) run.launch(source, "ptowsp_paged_prefix_finish", own.blocks, 256, &own, sizeof own);
     run.launch(source, "ptowsp_paged_prefix_merge", groups, 256, &P, sizeof P);
 }

@@ -20,6 +20,7 @@
 #include <string>
 #include <vector>
 
+#include "../device/ptowsp_blocks_args.h"
 #include "../device/ptowsp_launch.h"
 #include "../device/ptowsp_paged_args.h"
 #include "analysis.hpp"
@@ -2048,6 +2049,9 @@ void enqueue_operator(RunEnv& E, const Node& n, hipStream_t stream, uint64_t& la
             LaunchArgs launch;
             char raw[sizeof(LaunchArgs)];
         } buffer;
+        constexpr size_t kLargest = std::max({sizeof(PlanArgs), sizeof(StoreArgs), sizeof(AttendArgs), sizeof(PrefixArgs), sizeof(QuantizeArgs), sizeof(MatmulArgs),
+                                              sizeof(RotateArgs)});
+        static_assert(kLargest <= sizeof(LaunchArgs));
         if (bytes > sizeof buffer) throw std::runtime_error(n.op + ": internal: kernel arguments too large");
         std::memcpy(buffer.raw, args, bytes);
         void* params[] = {buffer.raw};
