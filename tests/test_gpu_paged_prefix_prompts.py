@@ -128,3 +128,16 @@ def test_prompts_captured(gpu):
                 prog.synchronize()
             check(c, t, ref)
             assert torch.equal(first, t["out"])
+
+
+def test_more_groups_than_threads(gpu):
+    """300 groups with more rows than the kernel for few takes, of one request or two, some without a prefix and some
+    without rows: each workgroup finds its piece among them."""
+    rng = np.random.default_rng(11)
+    counts = rng.integers(17, 24, size=400)
+    counts[rng.permutation(400)[:40]] = 0
+    counts[7] = 90
+    members = np.concatenate([[0], np.cumsum(np.arange(300) % 3 == 0) + np.arange(1, 301)])
+    prefix = rng.integers(0, 200, size=300)
+    prefix[rng.permutation(300)[:30]] = 0
+    attend(gpu, case(rng, "bf16", "e4m3", 1, 4, 64, 16, prefix, members, counts + rng.integers(0, 60, size=400), counts))
