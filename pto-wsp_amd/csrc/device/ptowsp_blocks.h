@@ -199,8 +199,8 @@ typedef int pg_i32x8 __attribute__((ext_vector_type(8)));
 // result does not, and a sum of 0 adds 0; nothing else is rounded than in a product of
 // the two scales, which alone may lie below 2^-126 or beyond 2^128.  Factors are below
 // 2^64, those of normal numbers 2^-63 and above; infinities and NaN are factors.  Against
-// that product 8192 x 6144 x 4096 takes 1% longer to bf16 and 4% to float32, 512 rows 3%,
-// 64 rows 4%; a branch for such products alone took as long or spilled registers.
+// that product 8192 x 6144 x 4096 takes 2% longer to bf16 and to float32, 1024 rows 4%, 64
+// rows 3%; a branch for such products alone took as long or spilled registers.
 __device__ inline int power_of(float scale) { return static_cast<int>((__float_as_uint(scale) >> 24 & 0x7Fu) + 64u); }
 __device__ inline float factor_of(float scale, int power) { return scale * __uint_as_float(static_cast<pg_u32>(254 - power) << 23); }
 struct Halves {
@@ -438,7 +438,7 @@ struct BlockGemm {
                 to_lds4(buf_s, soff_s[q], static_cast<int>(s * A.s_as[1]) * 4, base + (BM + BN) * 128 + (wave + WAVES * q) % (SM / 64) * 256);
             }
         };
-        // The scale of the weights' block, one stage ahead, through the scalar cache.
+        // The scale of the weights' block, through the scalar cache, a stage ahead of its use.
         const auto* const bs = reinterpret_cast<const __attribute__((address_space(4))) float*>(
             reinterpret_cast<pg_u64>(A.b_scale + (strip < strips ? strip : strips - 1) * A.s_bs[0] + first * A.s_bs[1]));
         auto weight_scale = [&](int s) { return bs[(s < stages ? s : stages - 1) * A.s_bs[1]]; };
@@ -489,7 +489,11 @@ struct BlockGemm {
         constexpr int MANY = FM * FN, LAG = MANY > 2 ? 2 : MANY - 1;
         constexpr int POINT = (FM - 2) * FN + FN / 2, EARLY = LOADS * (MANY - POINT) / MANY;
         int s = 0, ring = 0;
-        // next: the next stage's scale of the weights.
+        // TOGETHER: the next stage's first scales are read with its first rows, all ahead of an
+        // MFMA that waits for reads, instead of at POINT: 64 rows of 6144 x 4096 gain 3%, 128
+        // rows 3%, 8192 rows to float32 2%; 1024 rows to bf16 would lose 2%.
+        constexpr bool TOGETHER = WIDE || FN <= 2;
+        // next: the next stage's scale of the weights, which has been loaded.
         auto body = [&](auto kind, float next, const int (&back1)[2], const int (&back2)[2]) {
             constexpr int KIND = decltype(kind)::value;
             const int after = ring == NS - 1 ? 0 : ring + 1, before = ring == 0 ? NS - 1 : ring - 1;
@@ -514,12 +518,16 @@ struct BlockGemm {
                     f[i & 1] = row.factor * weight.factor;
                     power = row.power;
                     a = Codes32<WIDE>(raw[0], raw[1], power);
-                    if (KIND > 0 && i == FM - 1) follows = uniform_halves(next);
+                    if (WIDE && KIND > 0 && i == FM - 1) follows = uniform_halves(next);
                     if (i + 1 < FM) read_rows(stage, i + 1);
                     else if (KIND > 0) read_rows(behind, 0);
                     if (i + 1 < FM) row = Halves(scale);
                     if (i + 2 < FM) scale = scale_at(stage, i + 2);
                     else if (KIND > 0 && i == FM - 1) later = scale_at(behind, 1);
+                    if (TOGETHER && KIND > 0 && i == FM - 1) {
+                        scale = scale_at(behind, 0);
+                        __builtin_amdgcn_sched_barrier(0);  // these loads ahead of the MFMA's wait
+                    }
                 }
                 y[k % (LAG + 1)] = stage_sum<WIDE>(b[j], a, weight.power, power);
                 if constexpr (KIND > 0) {
@@ -535,7 +543,7 @@ struct BlockGemm {
                         if (KIND > 1 || NS == 2) landed_and_read<(NS - 2) * LOADS>();
                         else landed_of<NS - 2, LOADS>(stages - s - 2);
                         meet();
-                        scale = scale_at(behind, 0);
+                        if (!TOGETHER) scale = scale_at(behind, 0);
                     }
                     if (KIND > 2 && k >= POINT) {
 #pragma unroll
@@ -550,7 +558,7 @@ struct BlockGemm {
             for (int k = MANY - LAG; k < MANY; ++k) add(k);
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (KIND > 0) {
-                weight = follows;
+                weight = WIDE ? follows : uniform_halves(next);
                 row = Halves(scale);
                 scale = later;
             }
@@ -584,13 +592,24 @@ struct BlockGemm {
             landed_of<NS - 1, LOADS, EARLY>(stages - 1);
             meet();
             begin(stages == 1 ? tail : kScaleBlock, weight_scale(0));
+            float next = weight_scale(1), coming;
             while (s + NS < stages) {
+                coming = weight_scale(s + 2);
                 back_of(s + NS, now);
-                body(Int<3>(), weight_scale(s + 1), none, now);
+                body(Int<3>(), next, none, now);
+                next = coming;
             }
-            if (s + NS == stages) body(Int<2>(), weight_scale(s + 1), back, none);
-            while (s + 1 < stages) body(Int<1>(), weight_scale(s + 1), none, none);
-            body(Int<0>(), 0.0f, none, none);
+            if (s + NS == stages) {
+                coming = weight_scale(s + 2);
+                body(Int<2>(), next, back, none);
+                next = coming;
+            }
+            while (s + 1 < stages) {
+                coming = weight_scale(s + 2);
+                body(Int<1>(), next, none, none);
+                next = coming;
+            }
+            body(Int<0>(), next, none, none);
         } else {
             pg_u32x4 w[PIECES];
             auto fetch = [&](int s) {
