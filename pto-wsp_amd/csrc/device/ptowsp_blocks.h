@@ -184,11 +184,11 @@ __device__ inline void quantize_squares(const QuantizeArgs& A) {
 //
 // The host chooses the tile and the shares of K by a fitted cost (BlockStream for up
 // to 16 rows).  Many rows are bound by the clock that the card's power leaves and by
-// instructions beside the MFMAs: 8192 x 6144 x 4096 to bf16 225 us, 1.83 PFLOP/s; 183
-// with all codes zero, 186 without the loads, 214 without the stores.  Few rows by the
-// way of the weights through the ring, 32 stages one behind the other: 64 x 6144 x
-// 4096 (27 MB) 12.6 us, 2.1 TB/s; deeper rings, wider tiles, shares of K and an order
-// of stages of its own for each workgroup gain nothing.
+// instructions beside the MFMAs: 8192 x 6144 x 4096 to bf16 220 us, 1.87 PFLOP/s (10%
+// less with all codes zero).  Few rows by the way of the weights through the ring, 32
+// stages one behind the other: 64 x 6144 x 4096 (27 MB) 13.3 us, 2.0 TB/s; deeper rings,
+// wider tiles, shares of K and an order of stages of its own for each workgroup gain
+// nothing.  The stream takes 8.5 us for one row of these weights, 12.4 for 16.
 // ---------------------------------------------------------------------------
 
 typedef int pg_i32x8 __attribute__((ext_vector_type(8)));

@@ -21,6 +21,9 @@ namespace ptowsp {
 // latency, 3.9 us.
 // ---------------------------------------------------------------------------
 
+// Dims of a lane's piece: a pair's halves shall lie in one lane, so that R's divisors set
+// it for the dims that do not turn too.  16384 tokens as above, from memory: R = 128 71 us,
+// 96 or 64 78, 36 or 20 132, 4 or 2 117 to 121.
 constexpr int rotate_piece(int R) { return R % 16 == 0 ? 8 : R % 8 == 0 ? 4 : R % 4 == 0 ? 2 : 1; }
 
 // ONCE: bytes that the call reads once.  16 of them (a head's dims, side by side in

@@ -82,8 +82,9 @@ struct MatmulTile {
     double alone, shared;
 };
 // Fitted to 2900 timings of 42 shapes, from 1 x 82 x 128 to 8192 x 6144 x 4096, each
-// with every tile and 1 to 8 splits of K, weights from memory: the choice costs 4%
-// over the fastest on average.  64 rows of 6144 x 4096 take 12.5 us in tiles of 32 x
+// with every tile and 1 to 8 splits of K, weights from memory, to bf16 and with rows that
+// go straight to LDS: there the choice cost 4% over the fastest on average.  Scales were
+// multiplied with each other then; their halves take every tile 1 to 5% longer.  64 rows of 6144 x 4096 take 12.5 us in tiles of 32 x
 // 64, 16.5 in 64 x 64 and 60 in 256 x 256; 512 rows 47, 37 and 75, and 29 in 128 x
 // 128; 8192 rows 341 in 128 x 128 and 224 in 256 x 256.
 constexpr MatmulTile kTiles[] = {
