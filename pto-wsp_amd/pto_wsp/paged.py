@@ -80,10 +80,10 @@ def paged_norm_rotate(*, q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, lengths
     ``starts[b] .. starts[b + 1] - 1`` are its last ones; a token's position p is its place among them, plus
     ``offsets[b]`` (the tokens of a shared prefix, say).  D is a multiple of 16 up to 256.
 
-    All is computed in float32 and rounded once, into ``q_out`` and ``k_out`` (as q and k, and each may be where it
-    comes from, with the same strides).  Rows of no request are left alone; positions outside the tables, and rows of a
-    request beyond its ``lengths[b]`` tokens, raise from ``synchronize()`` and are left out; starts that go down, or lie
-    beyond the rows, raise too.
+    All is computed in float32 (heads whose squares add up to more than it holds become 0) and rounded once, into
+    ``q_out`` and ``k_out`` (as q and k, and each may be where it comes from, with the same strides).  Rows of no
+    request are left alone; positions outside the tables, and rows of a request beyond its ``lengths[b]`` tokens, raise
+    from ``synchronize()`` and are left out; starts that go down, or lie beyond the rows, raise too.
     """
     tensors: dict[str, Any] = {"q": q, "k": k, "cos": cos, "sin": sin, "lengths": lengths, "starts": starts, "q_out": q_out, "k_out": k_out}
     for name, t in (("q_weight", q_weight), ("k_weight", k_weight), ("offsets", offsets)):

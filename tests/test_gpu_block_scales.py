@@ -70,3 +70,25 @@ def test_scales_at_the_ends(gpu, M, N, K, dt):
     t = {"a": e4m3(gpu, a), "a_scale": torch.from_numpy(sa).to(gpu), "b": e4m3(gpu, b), "b_scale": torch.from_numpy(sb).to(gpu)}
     go(block_matmul(**{k: T(x) for k, x in t.items()}, out=T(out)))
     assert np.isnan(f64(out)[M - 1]).all() and np.array_equal(f64(out)[:M - 1], got[:M - 1])
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("M,N,K", [(5, 200, 1024), (64, 512, 1024), (300, 384, 512), (37, 70, 333)])
+def test_scales_of_any_sign_and_not_finite(gpu, M, N, K, dt):
+    """Negative scales; infinite and NaN ones of weights reach their 128 columns, and no others."""
+    torch = _torch()
+    a, sa, b, sb = operands(M, N, K, M + N, 0x20, 0x70, 3, -3)
+    rng = np.random.default_rng(2)
+    sa, sb = (s * rng.choice(np.float32([-1, 1]), size=s.shape) for s in (sa, sb))
+    got = check_matmul(gpu, a, sa, b, sb, dt)
+    assert (got < 0).any() and (got > 0).any()
+    sb[0, 1], sb[-1, 2] = np.inf, np.nan
+    t = {"a": e4m3(gpu, a), "a_scale": torch.from_numpy(sa).to(gpu), "b": e4m3(gpu, b), "b_scale": torch.from_numpy(sb).to(gpu)}
+    out = torch.zeros((M, N), dtype=_dt(dt), device=gpu)
+    go(block_matmul(**{k: T(x) for k, x in t.items()}, out=T(out)))
+    want = B.matmul(a, sa, b, sb)[0]
+    now = f64(out)
+    assert np.array_equal(np.isnan(now), np.isnan(want)) and np.array_equal(np.isinf(now), np.isinf(want))
+    assert (np.sign(now) == np.sign(want))[np.isinf(want)].all()
+    fine = np.isfinite(want)
+    assert np.array_equal(now[fine], got[fine])
